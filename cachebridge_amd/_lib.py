@@ -34,6 +34,9 @@ CB_MAX_WINDOW_CLASSES = 4
 CB_MAX_SUPPORT = 16
 CB_NOALLOC_WORKSPACE_BYTES = 16777216
 CB_NOALLOC_MAX_TOKENS = 1398080
+CB_ERROR_CACHE_ROW = 1
+CB_ERROR_TARGET_ROW = 2
+CB_ERROR_REQUEST = 4
 
 _c_void_p = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -125,6 +128,42 @@ class CbPlanInfo(ctypes.Structure):
     ]
 
 
+class CbQueryBatch(ctypes.Structure):
+    _fields_ = [
+        ("cache", CbRows),
+        ("index_entries", _i64),
+        ("query_start", _c_void_p),
+        ("lengths", _c_void_p),
+        ("offsets", _c_void_p),
+        ("request_stride", _i64),
+        ("num_requests", _i32),
+        ("num_tokens", _i32),
+        ("max_query", _i32),
+        ("max_length", _i32),
+    ]
+
+
+class CbHeads(ctypes.Structure):
+    _fields_ = [
+        ("data", _c_void_p),
+        ("token_stride", _i64),
+        ("head_stride", _i64),
+        ("heads", _i32),
+        ("reserved", _i32),
+    ]
+
+
+class CbScores(ctypes.Structure):
+    _fields_ = [
+        ("scale", ctypes.c_float),
+        ("cap", ctypes.c_float),
+        ("window", _i32),
+        ("causal", _i32),
+        ("slopes", _c_void_p),
+        ("prefix_lengths", _c_void_p),
+    ]
+
+
 # Every symbol the header declares, with (restype, argtypes).
 SIGNATURES = {
     "cb_last_error": (ctypes.c_char_p, []),
@@ -155,6 +194,31 @@ SIGNATURES = {
         ctypes.c_int,
         [_i32, _i64, _i32, _i32, _i32, _i32, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64,
          _c_void_p, _i64, _c_void_p],
+    ),
+    "cb_install_tokens": (
+        ctypes.c_int,
+        [ctypes.POINTER(CbQueryBatch), _i32, _i32, _i32, ctypes.POINTER(CbHeads), ctypes.POINTER(CbHeads),
+         ctypes.POINTER(CbHeads), ctypes.POINTER(CbHeads), _c_void_p, _i32, _i32, ctypes.c_float, _c_void_p,
+         _i32, _c_void_p, _c_void_p],
+    ),
+    "cb_attention_workspace_bytes": (
+        ctypes.c_int,
+        [ctypes.POINTER(CbQueryBatch), _i32, _i32, ctypes.POINTER(CbScores), _i32, ctypes.POINTER(_i64)],
+    ),
+    "cb_paged_attention": (
+        ctypes.c_int,
+        [ctypes.POINTER(CbQueryBatch), _i32, _i32, _i32, ctypes.POINTER(CbScores), ctypes.POINTER(CbHeads),
+         ctypes.POINTER(CbHeads), _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
+    ),
+    "cb_add_key_weights": (
+        ctypes.c_int,
+        [ctypes.POINTER(CbQueryBatch), _i32, _i32, _i32, ctypes.POINTER(CbScores), ctypes.POINTER(CbHeads),
+         _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
+    ),
+    "cb_evict_tokens": (
+        ctypes.c_int,
+        [ctypes.POINTER(CbQueryBatch), ctypes.POINTER(CbQueryBatch), _i32, _i32, _c_void_p, _i64, _i32, _i32,
+         _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
     ),
 }
 

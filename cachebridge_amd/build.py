@@ -9,10 +9,11 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
-SOURCES = [PACKAGE / "csrc" / "cb_handoff.hip"]
+SOURCES = [PACKAGE / "csrc" / "cb_handoff.hip", PACKAGE / "csrc" / "cb_queries.hip"]
 OUTPUT = PACKAGE / "libcachebridge_hip.so"
 ARCH = os.environ.get("CACHEBRIDGE_OFFLOAD_ARCH", "gfx950")
 
@@ -21,7 +22,6 @@ FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     # Keep the compiler from emitting packed fp32 VALU ops on this target.
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall",
@@ -37,14 +37,21 @@ def hipcc() -> str:
 
 
 def build_library(verbose: bool = False) -> Path:
-    """Compile every HIP source into the package's shared library."""
+    """Compile every HIP source (at the same time) and link the package's shared library."""
     tmp = OUTPUT.with_suffix(".so.tmp")
-    cmd = [hipcc(), *FLAGS, *map(str, SOURCES), "-o", str(tmp)]
-    result = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or result.returncode:
-        sys.stderr.write(result.stdout + result.stderr)
-    if result.returncode:
-        raise RuntimeError(f"hipcc failed ({result.returncode}): {' '.join(cmd)}")
+    with tempfile.TemporaryDirectory() as work:
+        objects = [Path(work) / f"{source.stem}.o" for source in SOURCES]
+        steps = [[[hipcc(), *FLAGS, "-c", str(source), "-o", str(obj)] for source, obj in zip(SOURCES, objects)],
+                 [[hipcc(), *FLAGS, "-shared", *map(str, objects), "-o", str(tmp)]]]
+        for commands in steps:
+            running = [subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+                       for cmd in commands]
+            output = [process.communicate()[0] for process in running]
+            for cmd, process, text in zip(commands, running, output):
+                if verbose or process.returncode:
+                    sys.stderr.write(text)
+                if process.returncode:
+                    raise RuntimeError(f"hipcc failed ({process.returncode}): {' '.join(cmd)}")
     os.replace(tmp, OUTPUT)
     return OUTPUT
 

@@ -1,0 +1,1273 @@
+// Queries on an installed prefix for MI355X (gfx950): new tokens rotated and
+// stored into a paged cache, attention over it, the attention each cached
+// token got, and eviction by it. The C ABI is in include/cachebridge_hip.h.
+//
+// Layout shared by the score kernels. A request's new tokens and the G query
+// heads of one KV head form rows r = i * G + g of one matrix (i: new token),
+// so that K and V are read once per KV head whatever the number of heads and
+// new tokens. Scores are computed transposed, S^T = K Q^T: an MFMA result
+// holds one query row per lane and several keys per lane, so the softmax
+// statistics of a row stay in its lane (plus one exchange among the lanes that
+// share the row), and P^T is the next product's second operand as it stands:
+// O^T += V^T P^T sums over keys, whose order within a step is free as long as
+// both operands use the same one.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/cachebridge_hip.h"
+#include "cb_common.h"
+
+namespace {
+
+typedef __bf16 io_bf16;
+typedef _Float16 io_f16;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNegInf = -INFINITY;
+
+// ---------------------------------------------------------------------------
+// Requests, their cached tokens and their rows
+// ---------------------------------------------------------------------------
+
+struct QBatch {
+  const int32_t* query_start;
+  const int32_t* lengths;
+  const int64_t* offsets;
+  int64_t request_stride;
+  int64_t index_offset;
+  int64_t entries;
+  const void* index;
+  int64_t rows;
+  int64_t row_stride_b;
+  int32_t kind;
+  int32_t page_size;
+  int32_t page_shift;  // log2(page_size), or -1
+  int32_t requests;
+  int32_t tokens;
+  int32_t max_query;
+  int32_t max_length;
+  int32_t* err;
+};
+
+struct Request {
+  int q0;        // first token row
+  int n;         // new tokens
+  int length;    // cached tokens, the new ones included
+  int64_t first; // index entry of cached token 0 (block tables: its page's)
+  uint32_t rem;  // block tables: cached token 0's slot in its page
+  bool ok;
+};
+
+__device__ inline void flag(int32_t* err, int bits) {
+  if (err) atomicOr(err, bits);
+}
+
+// The request's index position alone (eviction: no new tokens involved).
+__device__ inline void place_request(const QBatch& B, int b, Request& r) {
+  const int64_t start = (B.offsets ? B.offsets[b] : b * B.request_stride);
+  r.ok = start >= 0 && start <= (int64_t{1} << 61);
+  const int64_t u = r.ok ? start + B.index_offset : 0;
+  r.first = u;
+  r.rem = 0;
+  if (B.kind == CB_INDEX_BLOCK_TABLE) {
+    r.first = B.page_shift >= 0 ? u >> B.page_shift : u / B.page_size;
+    r.rem = static_cast<uint32_t>(u - r.first * B.page_size);
+  }
+}
+
+__device__ inline Request load_request(const QBatch& B, int b) {
+  Request r;
+  place_request(B, b, r);
+  const int64_t q0 = B.query_start[b], q1 = B.query_start[b + 1];
+  const int length = B.lengths[b];
+  r.ok = r.ok && q0 >= 0 && q1 >= q0 && q1 <= B.tokens && q1 - q0 <= B.max_query && length <= B.max_length &&
+         q1 - q0 <= length;
+  r.q0 = static_cast<int>(q0);
+  r.n = r.ok ? static_cast<int>(q1 - q0) : 0;
+  r.length = r.ok ? length : 0;
+  return r;
+}
+
+// Pool row of cached token j, or -1 where its index entry or the row it names
+// is out of range. The arithmetic within a request is 32 bits wide (at most
+// 2^30 tokens); the request's own start is 64.
+__device__ inline int64_t cache_row(const QBatch& B, const Request& r, int j) {
+  int64_t row;
+  if (B.kind == CB_INDEX_BLOCK_TABLE) {
+    const uint32_t x = r.rem + static_cast<uint32_t>(j);
+    const uint32_t page = B.page_shift >= 0 ? x >> B.page_shift : x / static_cast<uint32_t>(B.page_size);
+    const int64_t e = r.first + page;
+    if (e >= B.entries) return -1;
+    const int64_t p = reinterpret_cast<const CB_GLOBAL int32_t*>(as_global(B.index))[e];
+    row = p * B.page_size + static_cast<int64_t>(x - page * static_cast<uint32_t>(B.page_size));
+    if (p < 0) return -1;
+  } else {
+    const int64_t e = r.first + j;
+    if (B.kind == CB_INDEX_IDENTITY) {
+      row = e;
+    } else {
+      if (e >= B.entries) return -1;
+      row = B.kind == CB_INDEX_I32 ? reinterpret_cast<const CB_GLOBAL int32_t*>(as_global(B.index))[e]
+                                   : reinterpret_cast<const CB_GLOBAL int64_t*>(as_global(B.index))[e];
+    }
+  }
+  return row >= 0 && row < B.rows ? row : -1;
+}
+
+// The request that token row t belongs to, or `requests` if none does: a wave
+// counts the requests that end at or before t, 64 at a time.
+__device__ inline int request_of_token(const QBatch& B, int t) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int b = 0;
+  for (int i = 0; i < B.requests; i += kWave) {
+    const bool past = i + lane < B.requests && B.query_start[i + lane + 1] <= t;
+    const int c = __popcll(__ballot(past));
+    b += c;
+    if (c < kWave) break;
+  }
+  return b;
+}
+
+// ---------------------------------------------------------------------------
+// Elements
+// ---------------------------------------------------------------------------
+
+template <typename IO>
+__device__ inline float to_f32(IO x) {
+  return static_cast<float>(x);
+}
+template <typename IO>
+__device__ inline IO from_f32(float x) {
+  return static_cast<IO>(x);  // round to nearest even
+}
+template <typename IO>
+__device__ inline IO load_elem(const char* p) {
+  return gload<IO>(as_global(static_cast<const void*>(p)));
+}
+template <typename IO>
+__device__ inline void store_elem(char* p, IO v) {
+  gstore<IO>(as_global(static_cast<void*>(p)), v);
+}
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
+
+// ---------------------------------------------------------------------------
+// New tokens: rotation and store
+// ---------------------------------------------------------------------------
+
+struct Strided {
+  char* data;
+  int64_t token_b, head_b;
+};
+
+struct InstallArgs {
+  QBatch batch;
+  DevRows cache;
+  int32_t layer;
+  int32_t head_dim, rotary_dim, interleaved;
+  int32_t q_heads, kv_heads;
+  int32_t slices;  // waves per token
+  Strided q, q_out, k, v;
+  const double* inv_freq;
+  const void* positions;
+  int32_t positions_kind;
+  float magnitude;
+};
+
+constexpr int kInstallWaves = 4;
+constexpr int kMaxPairs = 256;  // head_dim <= 512
+
+// sin and cos of `turns` revolutions. The angle is reduced to an eighth of a
+// turn either side of a quarter's multiple in 64 bits (positions times a
+// frequency reach thousands of radians, where 32 bits leave no digits of the
+// phase), then both are Taylor polynomials in fp32: |x| <= pi/4, first
+// terms left out x^11/11! and x^12/12! below 2^-29.
+__device__ inline void sincos_turns(double turns, float* sn, float* cs) {
+  const double q = __builtin_rint(turns * 4.0);
+  const float x = static_cast<float>((turns - q * 0.25) * 6.283185307179586476925);
+  const int quadrant = static_cast<int>(static_cast<int64_t>(q) & 3);
+  const float y = x * x;
+  const float s = x + x * y * (-1.0f / 6 + y * (1.0f / 120 + y * (-1.0f / 5040 + y * (1.0f / 362880))));
+  const float c = 1.0f + y * (-0.5f + y * (1.0f / 24 + y * (-1.0f / 720 + y * (1.0f / 40320 + y * (-1.0f / 3628800)))));
+  const float a = (quadrant & 1) ? c : s, b = (quadrant & 1) ? s : c;
+  *sn = (quadrant & 2) ? -a : a;
+  *cs = (quadrant == 1 || quadrant == 2) ? -b : b;
+}
+
+// V elements as one access where V * sizeof(IO) is 16, else element by element.
+template <typename IO, int V>
+__device__ inline void load_vec(const char* p, float* out) {
+  if constexpr (V * sizeof(IO) == 16) {
+    typedef IO vec __attribute__((ext_vector_type(V)));
+    const vec x = gload<vec>(as_global(static_cast<const void*>(p)));
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = static_cast<float>(x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = to_f32(load_elem<IO>(p + i * sizeof(IO)));
+  }
+}
+template <typename IO, int V>
+__device__ inline void store_vec(char* p, const float* in) {
+  if constexpr (V * sizeof(IO) == 16) {
+    typedef IO vec __attribute__((ext_vector_type(V)));
+    vec x;
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = from_f32<IO>(in[i]);
+    gstore<vec>(as_global(static_cast<void*>(p)), x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) store_elem<IO>(p + i * sizeof(IO), from_f32<IO>(in[i]));
+  }
+}
+
+// One wave per (token, slice of its heads' elements). Lanes compute the
+// token's angles once into LDS, then each item is V pairs of a head (two
+// vectors) or V elements that are copied. Bound by memory: every element is
+// read once and written once.
+template <typename IO, int V>
+__global__ __launch_bounds__(kInstallWaves * kWave) void install_tokens_kernel(InstallArgs a) {
+  __shared__ float2 turn[kInstallWaves][kMaxPairs];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kInstallWaves + wave;
+  const int t = static_cast<int>(unit / a.slices), slice = static_cast<int>(unit % a.slices);
+  if (t >= a.batch.tokens) return;
+  const int b = request_of_token(a.batch, t);
+  if (b >= a.batch.requests) return;
+  const Request r = load_request(a.batch, b);
+  if (!r.ok) {
+    if (lane == 0) flag(a.batch.err, CB_ERROR_REQUEST);
+    return;
+  }
+  if (t < r.q0 || t >= r.q0 + r.n) return;
+  const int p = r.length - r.n + (t - r.q0);
+  const int64_t row = cache_row(a.batch, r, p);
+  if (row < 0 && lane == 0) flag(a.batch.err, CB_ERROR_TARGET_ROW);
+  int64_t pos = p;
+  if (a.positions)
+    pos = a.positions_kind == CB_INDEX_I64 ? static_cast<const int64_t*>(a.positions)[t]
+                                           : static_cast<const int32_t*>(a.positions)[t];
+  const int pairs = a.rotary_dim / 2;
+  for (int i = lane; i < pairs; i += kWave) {
+    float s, c;
+    sincos_turns(static_cast<double>(pos) * a.inv_freq[i] * 0.15915494309189533577, &s, &c);
+    turn[wave][i] = make_float2(c * a.magnitude, s * a.magnitude);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const int rot_items = pairs / V, pass_items = (a.head_dim - a.rotary_dim) / V, head_items = rot_items + pass_items;
+  const int v_items = a.head_dim / V;
+  const int turned = (a.q_heads + a.kv_heads) * head_items;
+  const int total = turned + a.kv_heads * v_items;
+  const int per = (total + a.slices - 1) / a.slices;
+  const int stop = min(total, (slice + 1) * per);
+  char* krow = const_cast<char*>((const char*)layer_base(a.cache, 0, a.layer)) + row * a.cache.row_stride_b;
+  char* vrow = const_cast<char*>((const char*)layer_base(a.cache, 1, a.layer)) + row * a.cache.row_stride_b;
+  constexpr int E = sizeof(IO);
+  for (int idx = slice * per + lane; idx < stop; idx += kWave) {
+    const char* src;
+    char* dst;
+    int item;
+    if (idx < turned) {
+      const int head = idx / head_items;
+      item = idx - head * head_items;
+      if (head < a.q_heads) {
+        src = a.q.data + t * a.q.token_b + head * a.q.head_b;
+        dst = a.q_out.data + t * a.q_out.token_b + head * a.q_out.head_b;
+      } else {
+        src = a.k.data + t * a.k.token_b + (head - a.q_heads) * a.k.head_b;
+        dst = krow + static_cast<int64_t>(head - a.q_heads) * a.head_dim * E;
+        if (row < 0) continue;
+      }
+    } else {
+      if (row < 0) continue;
+      const int head = (idx - turned) / v_items;
+      const int off = (idx - turned - head * v_items) * V;
+      float x[V];
+      load_vec<IO, V>(a.v.data + t * a.v.token_b + head * a.v.head_b + off * E, x);
+      store_vec<IO, V>(vrow + (static_cast<int64_t>(head) * a.head_dim + off) * E, x);
+      continue;
+    }
+    if (item >= rot_items) {
+      const int off = a.rotary_dim + (item - rot_items) * V;
+      float x[V];
+      load_vec<IO, V>(src + off * E, x);
+      store_vec<IO, V>(dst + off * E, x);
+      continue;
+    }
+    const int first = item * V;
+    const int oa = a.interleaved ? 2 * first : first, ob = a.interleaved ? oa + V : first + pairs;
+    float x[2 * V], y[2 * V];
+    load_vec<IO, V>(src + oa * E, x);
+    load_vec<IO, V>(src + ob * E, x + V);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 cs = turn[wave][first + i];
+      if (a.interleaved) {
+        y[2 * i] = x[2 * i] * cs.x - x[2 * i + 1] * cs.y;
+        y[2 * i + 1] = x[2 * i + 1] * cs.x + x[2 * i] * cs.y;
+      } else {
+        y[i] = x[i] * cs.x - x[i + V] * cs.y;
+        y[i + V] = x[i + V] * cs.x + x[i] * cs.y;
+      }
+    }
+    store_vec<IO, V>(dst + oa * E, y);
+    store_vec<IO, V>(dst + ob * E, y + V);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Scores: tiles of query rows, the cached tokens they see
+// ---------------------------------------------------------------------------
+
+struct ScoreArgs {
+  QBatch batch;
+  DevRows cache;
+  int32_t layer;
+  int32_t head_dim, q_heads, kv_heads, group;
+  Strided q;
+  float scale, cap;
+  int32_t window, causal;
+  const float* slopes;
+  const int32_t* prefix;
+};
+
+struct AttendArgs {
+  ScoreArgs s;
+  Strided out;
+  float* lse;
+  float* part_out;   // [splits][tokens * q_heads][head_dim], each normalised
+  float* part_lse;   // [splits][tokens * q_heads], log2
+  int32_t tile_slots;     // query tiles launched per KV head
+  int32_t request_slots;  // tiles per request if tiles are laid out by request, else 0
+  int32_t splits;
+  int32_t tiles_per_split;
+};
+
+// Tile `i` of the launch: its request, and which of the request's tiles (the
+// last first: under a causal mask it has the most keys). Returns false if
+// there is none.
+__device__ inline bool find_tile(const AttendArgs& a, int i, int rows_per_tile, Request& r, int& b, int& tile) {
+  const QBatch& B = a.s.batch;
+  const int G = a.s.group;
+  if (a.request_slots > 0) {
+    b = i / a.request_slots;
+    r = load_request(B, b);
+    const int tiles = static_cast<int>((static_cast<int64_t>(r.n) * G + rows_per_tile - 1) / rows_per_tile);
+    tile = tiles - 1 - (i - b * a.request_slots);
+    if (!r.ok && threadIdx.x == 0 && i == b * a.request_slots) flag(B.err, CB_ERROR_REQUEST);
+    return tile >= 0;
+  }
+  const int lane = threadIdx.x & (kWave - 1);
+  int64_t before = 0;
+  for (int b0 = 0; b0 < B.requests; b0 += kWave) {
+    int64_t c = 0;
+    if (b0 + lane < B.requests) {
+      const Request m = load_request(B, b0 + lane);
+      c = (static_cast<int64_t>(m.n) * G + rows_per_tile - 1) / rows_per_tile;
+      if (!m.ok && i == 0 && threadIdx.x < kWave) flag(B.err, CB_ERROR_REQUEST);
+    }
+    int64_t sum = c;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int64_t up = __shfl_up(sum, d);
+      if (lane >= d) sum += up;
+    }
+    const uint64_t hit = __ballot(before + sum > i);
+    if (hit) {
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(hit)) - 1);
+      b = b0 + l;
+      r = load_request(B, b);
+      const int64_t end = before + __shfl(sum, l);
+      tile = static_cast<int>(end - 1 - i);
+      return true;
+    }
+    before += __shfl(sum, kWave - 1);
+  }
+  return false;
+}
+
+// Cached tokens that query rows [row0, row1] of a request may see: [0, na) if
+// a prefix stands apart from the window, then [lb, hb). They are walked in
+// tiles of KT keys, those of the prefix first.
+struct KeyRange {
+  int na, lb, hb;
+  int ta, tiles;
+  int np;      // prefix length within the cache
+  int p0, p1;  // cached token of the first and last row
+};
+
+template <int KT>
+__device__ inline KeyRange key_range(const ScoreArgs& s, const Request& r, int b, int row0, int row1) {
+  KeyRange k;
+  k.np = s.prefix ? max(0, min(s.prefix[b], r.length)) : 0;
+  k.p0 = r.length - r.n + row0 / s.group;
+  k.p1 = r.length - r.n + row1 / s.group;
+  const int lo = s.window > 0 ? max(0, k.p0 - s.window + 1) : 0;
+  const int hi = s.causal ? k.p1 + 1 : r.length;
+  k.na = s.window > 0 ? min(k.np, lo) : 0;
+  k.lb = lo;
+  k.hb = max(hi, k.np);
+  if (k.np < lo) k.hb = hi;
+  k.ta = (k.na + KT - 1) / KT;
+  k.tiles = k.ta + (k.hb - k.lb + KT - 1) / KT;
+  return k;
+}
+
+template <int KT>
+__device__ inline int tile_start(const KeyRange& k, int t) {
+  return t < k.ta ? t * KT : k.lb + (t - k.ta) * KT;
+}
+__device__ inline int tile_end(const KeyRange& k, int t) { return t < k.ta ? k.na : k.hb; }
+
+// Whether every row of the tile sees every key of [start, start + KT).
+template <int KT>
+__device__ inline bool sees_all(const ScoreArgs& s, const KeyRange& k, int start, int end) {
+  if (start + KT > end) return false;
+  if (start + KT <= k.np) return true;
+  return (!s.causal || start + KT <= k.p0 + 1) && (s.window == 0 || start > k.p1 - s.window);
+}
+
+// Without branches (bitwise operators): lanes differ in p and j.
+__device__ inline bool sees(const ScoreArgs& s, const KeyRange& k, int p, int j) {
+  const int above = s.window > 0 ? p - s.window : -1, below = s.causal ? p : 0x7fffffff;
+  return (j < k.np) | ((j <= below) & (j > above));
+}
+
+// cap * tanh(x / cap), tanh y = (1 - e) / (1 + e) with e = exp(-2|y|).
+__device__ inline float capped(float x, float cap) {
+  const float e = exp2_fast(-2.0f * kLog2e * fabsf(x) / cap);
+  return copysignf(cap * (1.0f - e) / (1.0f + e), x);
+}
+
+// A raw product's score, in natural units.
+template <bool MOD>
+__device__ inline float natural_score(const ScoreArgs& s, float dot, float slope, int p, int j) {
+  float x = dot * s.scale;
+  if constexpr (MOD) {
+    if (s.cap > 0) x = capped(x, s.cap);
+    x -= slope * fabsf(static_cast<float>(p - j));
+  }
+  return x;
+}
+
+// ---------------------------------------------------------------------------
+// General attention: any even head_dim up to 512, any type, fp32 products
+// (16x16x4 MFMA: lane l holds A[l % 16][l / 16] and B[l / 16][l % 16], its
+// result rows 4 (l / 16) + e of column l % 16). A workgroup's four waves share
+// tiles of 16 keys in LDS, 16 query rows each.
+// ---------------------------------------------------------------------------
+
+constexpr int kAnyWaves = 4;
+constexpr int kAnyRows = 16 * kAnyWaves;
+constexpr int kAnyKeys = 16;
+
+__device__ inline f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+__device__ inline bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
+
+template <typename IO, int DP, bool MOD>
+__global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(AttendArgs a) {
+  constexpr int KT = kAnyKeys, LD = DP + 4, NB = DP / 16;
+  __shared__ float lk[KT * LD], lv[KT * LD];
+  const ScoreArgs& s = a.s;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int c = lane & 15, g = lane >> 4;
+  const int head = blockIdx.x % s.kv_heads;
+  const int rest = blockIdx.x / s.kv_heads;
+  const int split = rest % a.splits;
+  Request r;
+  int b, tile;
+  if (!find_tile(a, rest / a.splits, kAnyRows, r, b, tile)) return;
+  const int rows = r.n * s.group;
+  const int row0 = tile * kAnyRows, row1 = min(rows, row0 + kAnyRows) - 1;
+  const KeyRange kr = key_range<KT>(s, r, b, row0, row1);
+  const int t0 = split * a.tiles_per_split, t1 = min(kr.tiles, t0 + a.tiles_per_split);
+  if (a.splits > 1 && t0 >= t1) return;
+
+  const int row = row0 + 16 * wave + c;  // this lane's query row
+  const bool live = row < rows;
+  const int i = min(row, rows - 1) / s.group;
+  const int qh = head * s.group + min(row, rows - 1) % s.group;
+  const int p = r.length - r.n + i;
+  const int D = s.head_dim;
+  const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
+  float q[DP / 4];
+#pragma unroll
+  for (int e = 0; e < DP / 4; ++e)
+    q[e] = 4 * e + g < D ? to_f32(load_elem<IO>(qp + (4 * e + g) * static_cast<int>(sizeof(IO)))) : 0.0f;
+  float slope = 0;
+  if constexpr (MOD) slope = s.slopes ? s.slopes[qh] : 0.0f;
+
+  const char* kbase = (const char*)layer_base(s.cache, 0, s.layer) + static_cast<int64_t>(head) * D * sizeof(IO);
+  const char* vbase = (const char*)layer_base(s.cache, 1, s.layer) + static_cast<int64_t>(head) * D * sizeof(IO);
+  f32x4 o[NB];
+#pragma unroll
+  for (int d = 0; d < NB; ++d) o[d] = f32x4{0, 0, 0, 0};
+  float m = kNegInf, l = 0;
+  for (int t = t0; t < t1; ++t) {
+    const int start = tile_start<KT>(kr, t), end = tile_end(kr, t);
+    __syncthreads();
+    bool missing = false;
+#pragma unroll
+    for (int u = 0; u < KT / kAnyWaves; ++u) {
+      const int key = wave * (KT / kAnyWaves) + u, j = start + key;
+      const int64_t kvrow = j < end ? cache_row(s.batch, r, j) : -1;
+      if (j < end && kvrow < 0) {
+        missing = true;
+        if (lane == 0) flag(s.batch.err, CB_ERROR_CACHE_ROW);
+      }
+      for (int d = lane; d < DP; d += kWave) {
+        const bool in = kvrow >= 0 && d < D;
+        const int64_t off = kvrow * s.cache.row_stride_b + d * static_cast<int>(sizeof(IO));
+        lk[key * LD + d] = in ? to_f32(load_elem<IO>(kbase + off)) : 0.0f;
+        lv[key * LD + d] = in ? to_f32(load_elem<IO>(vbase + off)) : 0.0f;
+      }
+      if (lane == 0) lk[key * LD + DP] = kvrow >= 0 ? 1.0f : 0.0f;  // whether the key has a row
+    }
+    const bool any_missing = __syncthreads_or(missing);
+    f32x4 st = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < DP / 4; ++e) st = mfma4(lk[c * LD + 4 * e + g], q[e], st);
+    const bool whole = !any_missing && sees_all<KT>(s, kr, start, end);
+    float x[4], top = kNegInf;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int j = start + 4 * g + e;
+      x[e] = natural_score<MOD>(s, st[e], slope, p, j) * kLog2e;
+      const bool in = whole | ((j < end) & sees(s, kr, p, j) & (lk[(4 * g + e) * LD + DP] != 0.0f));
+      x[e] = in ? x[e] : kNegInf;
+      top = fmaxf(top, x[e]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float m1 = fmaxf(m, top);
+    const float mu = m1 == kNegInf ? 0.0f : m1;
+    const float alpha = exp2_fast(m - mu);
+    m = m1;
+    float pr[4];
+    l *= alpha;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      pr[e] = exp2_fast(x[e] - mu);
+      l += pr[e];
+    }
+#pragma unroll
+    for (int d = 0; d < NB; ++d) {
+      o[d] *= alpha;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = lv[(4 * g + e) * LD + 16 * d + c];
+        if (!whole && __any(not_finite(v))) {
+          // Zero weights times infinities would be NaN in rows that do not
+          // see them: such values go in by what they do to a sum instead.
+          const float vis = pr[e] != 0.0f ? 1.0f : 0.0f;
+          const bool nan = v != v;
+          const f32x4 z = {0, 0, 0, 0};
+          const f32x4 up = mfma4(nan || v == INFINITY ? 1.0f : 0.0f, vis, z);
+          const f32x4 dn = mfma4(nan || v == kNegInf ? 1.0f : 0.0f, vis, z);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if (up[w] > 0) o[d][w] += INFINITY;
+            if (dn[w] > 0) o[d][w] += kNegInf;
+          }
+          v = not_finite(v) ? 0.0f : v;
+        }
+        o[d] = mfma4(v, pr[e], o[d]);
+      }
+    }
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (!live) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float lse2 = l == 0.0f ? kNegInf : m + log2_fast(l);
+  const int64_t at = static_cast<int64_t>(r.q0 + i) * s.q_heads + qh;
+  if (a.splits > 1) {
+    const int64_t slot = static_cast<int64_t>(split) * s.batch.tokens * s.q_heads + at;
+    float* po = a.part_out + slot * D;
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (16 * d + 4 * g + e < D) po[16 * d + 4 * g + e] = o[d][e] * inv;
+    if (g == 0) a.part_lse[slot] = lse2;
+    return;
+  }
+  char* op = a.out.data + static_cast<int64_t>(r.q0 + i) * a.out.token_b + qh * a.out.head_b;
+#pragma unroll
+  for (int d = 0; d < NB; ++d)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (16 * d + 4 * g + e < D)
+        store_elem<IO>(op + (16 * d + 4 * g + e) * static_cast<int>(sizeof(IO)), from_f32<IO>(o[d][e] * inv));
+  if (a.lse && g == 0) a.lse[at] = lse2 * kLn2;
+}
+
+// Joins the splits of one (token, head) per wave: out = sum 2^(lse_z - lse) out_z.
+template <typename IO, int KT>
+__global__ __launch_bounds__(256) void join_splits_kernel(AttendArgs a, int rows_per_tile) {
+  const ScoreArgs& s = a.s;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+  const int t = static_cast<int>(at / s.q_heads), qh = static_cast<int>(at % s.q_heads);
+  if (t >= s.batch.tokens) return;
+  const int b = request_of_token(s.batch, t);
+  if (b >= s.batch.requests) return;
+  const Request r = load_request(s.batch, b);
+  if (!r.ok || t < r.q0 || t >= r.q0 + r.n) return;
+  const int row = (t - r.q0) * s.group + qh % s.group;
+  const int row0 = row / rows_per_tile * rows_per_tile;
+  const KeyRange kr = key_range<KT>(s, r, b, row0, min(r.n * s.group, row0 + rows_per_tile) - 1);
+  const int n = min(a.splits, (kr.tiles + a.tiles_per_split - 1) / a.tiles_per_split);
+  const int64_t step = static_cast<int64_t>(s.batch.tokens) * s.q_heads;
+  float top = kNegInf;
+  for (int z = 0; z < n; ++z) top = fmaxf(top, a.part_lse[z * step + at]);
+  const float mu = top == kNegInf ? 0.0f : top;
+  float total = 0;
+  for (int z = 0; z < n; ++z) total += exp2_fast(a.part_lse[z * step + at] - mu);
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  char* op = a.out.data + static_cast<int64_t>(t) * a.out.token_b + qh * a.out.head_b;
+  for (int d = lane; d < s.head_dim; d += kWave) {
+    float o = 0;
+    for (int z = 0; z < n; ++z) {
+      const float w = exp2_fast(a.part_lse[z * step + at] - mu) * inv;
+      if (w != 0.0f) o += w * a.part_out[(z * step + at) * s.head_dim + d];
+    }
+    store_elem<IO>(op + d * static_cast<int>(sizeof(IO)), from_f32<IO>(o));
+  }
+  if (a.lse && lane == 0) a.lse[at] = total == 0.0f ? kNegInf : (top + log2_fast(total)) * kLn2;
+}
+
+// ---------------------------------------------------------------------------
+// Weights of cached tokens
+// ---------------------------------------------------------------------------
+
+struct WeightArgs {
+  ScoreArgs s;
+  const float* lse;
+  float* weights;
+  int64_t weights_stride;
+  int32_t key_slots;  // key tiles launched per request
+};
+
+// The new tokens of a request that may see any of the cached tokens
+// [start, start + keys): all below a prefix, else those between.
+__device__ inline void query_range(const ScoreArgs& s, const Request& r, int np, int start, int keys, int* i0, int* i1) {
+  *i0 = 0;
+  *i1 = r.n;
+  if (start < np) return;
+  const int first = r.length - r.n;
+  if (s.causal) *i0 = min(r.n, max(0, start - first));
+  if (s.window > 0) *i1 = max(*i0, static_cast<int>(min(static_cast<int64_t>(r.n), static_cast<int64_t>(start) + keys - 1 + s.window - first)));
+}
+
+// General form: a workgroup owns 16 keys of a request, its waves take every
+// fourth block of 16 query rows of each KV head; partial sums meet in LDS in
+// wave order.
+template <typename IO, int DP, bool MOD>
+__global__ __launch_bounds__(kAnyWaves * kWave, 1) void key_weights_any_kernel(WeightArgs a) {
+  __shared__ float sums[kAnyWaves][16];
+  const ScoreArgs& s = a.s;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int c = lane & 15, g = lane >> 4;
+  const int b = blockIdx.x / a.key_slots, start = (blockIdx.x % a.key_slots) * 16;
+  const Request r = load_request(s.batch, b);
+  if (!r.ok && start == 0 && threadIdx.x == 0) flag(s.batch.err, CB_ERROR_REQUEST);
+  if (start >= r.length) return;
+  const int np = s.prefix ? max(0, min(s.prefix[b], r.length)) : 0;
+  KeyRange kr{};
+  kr.np = np;
+  int i0, i1;
+  query_range(s, r, np, start, 16, &i0, &i1);
+  const int D = s.head_dim;
+  const int64_t mine = start + c < r.length ? cache_row(s.batch, r, start + c) : -1;
+  if (start + c < r.length && mine < 0 && wave == 0 && g == 0) flag(s.batch.err, CB_ERROR_CACHE_ROW);
+  const uint64_t rows_ok = __ballot(mine >= 0);
+  float sum[4] = {0, 0, 0, 0};
+  for (int head = 0; head < s.kv_heads; ++head) {
+    const char* kp = (const char*)layer_base(s.cache, 0, s.layer) + static_cast<int64_t>(head) * D * sizeof(IO) + mine * s.cache.row_stride_b;
+    float k[DP / 4];
+#pragma unroll
+    for (int e = 0; e < DP / 4; ++e)
+      k[e] = mine >= 0 && 4 * e + g < D ? to_f32(load_elem<IO>(kp + (4 * e + g) * static_cast<int>(sizeof(IO)))) : 0.0f;
+    for (int row0 = i0 * s.group + 16 * wave; row0 < i1 * s.group; row0 += kAnyRows) {
+      const int row = min(row0 + c, i1 * s.group - 1);
+      const int i = row / s.group, qh = head * s.group + row % s.group, p = r.length - r.n + i;
+      const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
+      f32x4 st = {0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < DP / 4; ++e)
+        st = mfma4(k[e], 4 * e + g < D ? to_f32(load_elem<IO>(qp + (4 * e + g) * static_cast<int>(sizeof(IO)))) : 0.0f, st);
+      const float lse = a.lse[static_cast<int64_t>(r.q0 + i) * s.q_heads + qh];
+      float slope = 0;
+      if constexpr (MOD) slope = s.slopes ? s.slopes[qh] : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = start + 4 * g + e;
+        const bool in = (row0 + c < i1 * s.group) & (lse != kNegInf) & sees(s, kr, p, j);
+        // The difference first: what is near the row's maximum keeps its bits.
+        const float w = exp2_fast((natural_score<MOD>(s, st[e], slope, p, j) - lse) * kLog2e);
+        sum[e] += in ? w : 0.0f;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) sum[e] += __shfl_xor(sum[e], d);
+    if (c == 0) sums[wave][4 * g + e] = sum[e];
+  }
+  __syncthreads();
+  if (threadIdx.x < 16 && start + static_cast<int>(threadIdx.x) < r.length && ((rows_ok >> threadIdx.x) & 1)) {
+    float add = 0;
+#pragma unroll
+    for (int w = 0; w < kAnyWaves; ++w) add += sums[w][threadIdx.x];
+    a.weights[b * a.weights_stride + start + threadIdx.x] += add;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Eviction
+// ---------------------------------------------------------------------------
+
+struct EvictArgs {
+  QBatch batch, target;
+  const float* weights;
+  int64_t weights_stride;
+  int32_t budget, first, last;
+  int32_t* kept;
+  int32_t* kept_lengths;
+  float* kept_weights;
+  int2* rows;  // [requests][budget] source and target row of each kept token, -1 for none
+};
+
+constexpr int kSelectWaves = 16;
+constexpr int kSelectThreads = kSelectWaves * kWave;
+
+// Orders fp32 as unsigned integers; both zeros are one value, every NaN the largest.
+__device__ inline uint32_t rank_of(float w) {
+  if (w != w) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(w == 0.0f ? 0.0f : w);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ inline void keep_token(const EvictArgs& a, int b, const Request& src, const Request& dst, int at, int j, float w) {
+  const int64_t slot = static_cast<int64_t>(b) * a.budget + at;
+  a.kept[slot] = j;
+  a.kept_weights[slot] = w;
+  const int64_t from = cache_row(a.batch, src, j);
+  const int64_t to = dst.ok ? cache_row(a.target, dst, at) : -1;
+  if (from < 0) flag(a.batch.err, CB_ERROR_CACHE_ROW);
+  if (to < 0) flag(a.batch.err, CB_ERROR_TARGET_ROW);
+  a.rows[slot] = from >= 0 && to >= 0 ? make_int2(static_cast<int>(from), static_cast<int>(to)) : make_int2(-1, -1);
+}
+
+// One workgroup per request. The weights between the first and last tokens
+// are searched for the smallest rank that is still kept, two bits a step from
+// the top: each step counts, by ballots, the ranks at or above three
+// thresholds. No atomics, so no order to depend on.
+__global__ __launch_bounds__(kSelectThreads) void select_tokens_kernel(EvictArgs a) {
+  __shared__ int counts[2][3][kSelectWaves];
+  const int b = blockIdx.x;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  Request src, dst;
+  place_request(a.batch, b, src);
+  place_request(a.target, b, dst);
+  const int length = a.batch.lengths[b];
+  src.ok = src.ok && length >= 0 && length <= a.batch.max_length;
+  if (threadIdx.x == 0 && !src.ok) flag(a.batch.err, CB_ERROR_REQUEST);
+  const int64_t slot0 = static_cast<int64_t>(b) * a.budget;
+  if (!src.ok) {  // its outputs stay as they were; nothing is copied
+    for (int j = threadIdx.x; j < a.budget; j += kSelectThreads) a.rows[slot0 + j] = make_int2(-1, -1);
+    return;
+  }
+  const float* w = a.weights + b * a.weights_stride;
+  const int n = min(length, a.budget);
+  if (threadIdx.x == 0) a.kept_lengths[b] = n;
+  for (int j = n + threadIdx.x; j < a.budget; j += kSelectThreads) {
+    a.kept[slot0 + j] = -1;
+    a.kept_weights[slot0 + j] = 0.0f;
+    a.rows[slot0 + j] = make_int2(-1, -1);
+  }
+  if (length <= a.budget) {
+    for (int j = threadIdx.x; j < length; j += kSelectThreads) keep_token(a, b, src, dst, j, j, w[j]);
+    return;
+  }
+  for (int j = threadIdx.x; j < a.first; j += kSelectThreads) keep_token(a, b, src, dst, j, j, w[j]);
+  for (int j = threadIdx.x; j < a.last; j += kSelectThreads)
+    keep_token(a, b, src, dst, n - a.last + j, length - a.last + j, w[length - a.last + j]);
+  const int need = n - a.first - a.last;
+  if (need == 0) return;
+  // Wave v's share of the middle: 64-token groups in order.
+  const int mid = length - a.first - a.last;
+  const int groups = (mid + kWave - 1) / kWave;
+  const int per = (groups + kSelectWaves - 1) / kSelectWaves;
+  const int g0 = wave * per, g1 = min(groups, g0 + per);
+  const float* wm = w + a.first;
+  uint32_t base = 0;  // the largest value found so far with at least `need` ranks at or above it
+  int step = 0;
+  for (int shift = 30; shift >= 0; shift -= 2, ++step) {
+    int c[3] = {0, 0, 0};
+    for (int g = g0; g < g1; ++g) {
+      const int j = g * kWave + lane;
+      const bool in = j < mid;
+      const uint32_t k = in ? rank_of(wm[j]) : 0;
+#pragma unroll
+      for (int u = 0; u < 3; ++u) c[u] += __popcll(__ballot(in && k >= base + (static_cast<uint32_t>(u + 1) << shift)));
+    }
+    if (lane == 0)
+      for (int u = 0; u < 3; ++u) counts[step & 1][u][wave] = c[u];
+    __syncthreads();
+    uint32_t up = 0;
+#pragma unroll
+    for (int u = 0; u < 3; ++u) {
+      int total = 0;
+#pragma unroll
+      for (int v = 0; v < kSelectWaves; ++v) total += counts[step & 1][u][v];
+      if (total >= need) up = u + 1;
+    }
+    base += up << shift;
+  }
+  // Ranks above `base` are kept, and of those equal to it the first ones.
+  int above = 0, equal = 0;
+  for (int g = g0; g < g1; ++g) {
+    const int j = g * kWave + lane;
+    const bool in = j < mid;
+    const uint32_t k = in ? rank_of(wm[j]) : 0;
+    above += __popcll(__ballot(in && k > base));
+    equal += __popcll(__ballot(in && k == base));
+  }
+  __syncthreads();
+  if (lane == 0) {
+    counts[0][0][wave] = above;
+    counts[0][1][wave] = equal;
+  }
+  __syncthreads();
+  int above_before = 0, equal_before = 0, all_above = 0;
+  for (int v = 0; v < kSelectWaves; ++v) {
+    if (v < wave) {
+      above_before += counts[0][0][v];
+      equal_before += counts[0][1][v];
+    }
+    all_above += counts[0][0][v];
+  }
+  const int ties = need - all_above;
+  const uint64_t below = (uint64_t{1} << lane) - 1;
+  for (int g = g0; g < g1; ++g) {
+    const int j = g * kWave + lane;
+    const bool in = j < mid;
+    const float x = in ? wm[j] : 0.0f;
+    const uint32_t k = rank_of(x);
+    const uint64_t ma = __ballot(in && k > base), me = __ballot(in && k == base);
+    const int ea = equal_before + __popcll(me & below);
+    const bool keep = in && (k > base || (k == base && ea < ties));
+    const int at = a.first + above_before + __popcll(ma & below) + min(ea, ties);
+    if (keep) keep_token(a, b, src, dst, at, a.first + j, x);
+    above_before += __popcll(ma);
+    equal_before += __popcll(me);
+  }
+}
+
+struct MoveArgs {
+  DevRows src, dst;
+  const int2* rows;
+  int64_t count;
+  int32_t chunks_per_row;
+  int32_t tokens_per_block;
+};
+
+// Every layer's K and V rows of the kept tokens; a thread keeps four chunks in
+// flight, as copy_rows_kernel.
+template <typename V>
+__global__ __launch_bounds__(256) void move_rows_kernel(MoveArgs a) {
+  constexpr int U = 4;
+  const int layer = blockIdx.y >> 1, kind = blockIdx.y & 1;
+  gcptr sbase = layer_base(a.src, kind, layer);
+  gptr dbase = const_cast<gptr>(layer_base(a.dst, kind, layer));
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens_per_block;
+  const int total = static_cast<int>(min(static_cast<int64_t>(a.tokens_per_block), a.count - t0)) * a.chunks_per_row;
+  for (int base = threadIdx.x; base < total; base += blockDim.x * U) {
+    int64_t so[U], to[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int idx = base + u * blockDim.x;
+      so[u] = to[u] = -1;
+      if (idx < total) {
+        const int2 rw = a.rows[t0 + idx / a.chunks_per_row];
+        const int64_t off = (idx % a.chunks_per_row) * static_cast<int>(sizeof(V));
+        if (rw.x >= 0) {
+          so[u] = rw.x * a.src.row_stride_b + off;
+          to[u] = rw.y * a.dst.row_stride_b + off;
+        }
+      }
+    }
+    V v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (so[u] >= 0) v[u] = gload<V>(sbase + so[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (to[u] >= 0) gstore<V>(dbase + to[u], v[u]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+int elem_bytes(int32_t dtype) {
+  return dtype == CB_DTYPE_F32 ? 4 : dtype == CB_DTYPE_BF16 || dtype == CB_DTYPE_F16 ? 2 : 0;
+}
+
+int check_batch(const cb_query_batch* batch, int32_t dtype, int32_t head_dim, int32_t* err, bool queries, QBatch* B,
+                DevRows* rows) {
+  if (!batch) return fail(CB_EINVAL, "null batch");
+  const int eb = elem_bytes(dtype);
+  if (!eb) return fail(CB_EINVAL, "bad dtype");
+  if (head_dim < 2 || head_dim > 512 || head_dim % 2) return fail(CB_EINVAL, "head_dim must be even, 2 to 512");
+  int rc;
+  if ((rc = to_dev_rows(batch->cache, eb, rows, eb))) return rc;
+  const cb_rows& c = batch->cache;
+  if (c.heads < 1) return fail(CB_EINVAL, "the cache needs KV heads");
+  if (c.head_offset != 0) return fail(CB_EINVAL, "the cache's head_offset must be 0");
+  if (c.row_stride < static_cast<int64_t>(c.heads) * head_dim)
+    return fail(CB_EINVAL, "the cache's rows are shorter than heads * head_dim");
+  if (c.rows > 0x7fffffff) return fail(CB_EINVAL, "more than 2^31 - 1 cache rows");
+  if (c.index_kind == CB_INDEX_BLOCK_TABLE && c.page_size > (1 << 20)) return fail(CB_EINVAL, "page_size above 2^20");
+  if (c.index_kind != CB_INDEX_IDENTITY && batch->index_entries < 0) return fail(CB_EINVAL, "negative index_entries");
+  if (batch->num_requests < 0 || batch->num_tokens < 0) return fail(CB_EINVAL, "negative batch size");
+  if (batch->request_stride < 0) return fail(CB_EINVAL, "negative request_stride");
+  if (batch->request_stride > (int64_t{1} << 31)) return fail(CB_EINVAL, "request_stride above 2^31");
+  if (batch->max_length < 0 || batch->max_length > (1 << 30)) return fail(CB_EINVAL, "max_length must be 0 to 2^30");
+  if (batch->num_requests > 0 && (!batch->lengths || (queries && !batch->query_start)))
+    return fail(CB_EINVAL, "null query_start or lengths");
+  if (queries && (batch->max_query < 0 || batch->max_query > batch->num_tokens))
+    return fail(CB_EINVAL, "max_query must be 0 to num_tokens");
+  B->query_start = batch->query_start;
+  B->lengths = batch->lengths;
+  B->offsets = batch->offsets;
+  B->request_stride = batch->request_stride;
+  B->index_offset = c.index_offset;
+  B->entries = batch->index_entries;
+  B->index = c.index;
+  B->rows = c.rows;
+  B->row_stride_b = rows->row_stride_b;
+  B->kind = c.index_kind;
+  B->page_size = c.index_kind == CB_INDEX_BLOCK_TABLE ? c.page_size : 1;
+  B->page_shift = (B->page_size & (B->page_size - 1)) ? -1 : __builtin_ctz(static_cast<unsigned>(B->page_size));
+  B->requests = batch->num_requests;
+  B->tokens = batch->num_tokens;
+  B->max_query = batch->max_query;
+  B->max_length = batch->max_length;
+  B->err = err;
+  return CB_OK;
+}
+
+int check_heads(const char* name, const cb_heads* h, int32_t heads, int eb, int32_t tokens, Strided* out) {
+  if (!h) return fail(CB_EINVAL, "null %s", name);
+  if (h->heads != heads) return fail(CB_EINVAL, "%s has %d heads, %d expected", name, h->heads, heads);
+  if (tokens > 0 && !h->data) return fail(CB_EINVAL, "null %s data", name);
+  if (h->token_stride < 0 || h->head_stride < 0) return fail(CB_EINVAL, "negative stride of %s", name);
+  if (reinterpret_cast<uintptr_t>(h->data) % eb) return fail(CB_EINVAL, "%s is not aligned to its elements", name);
+  *out = Strided{static_cast<char*>(h->data), h->token_stride * eb, h->head_stride * eb};
+  return CB_OK;
+}
+
+bool aligned16(const Strided& s) {
+  return (reinterpret_cast<uintptr_t>(s.data) | static_cast<uintptr_t>(s.token_b) | static_cast<uintptr_t>(s.head_b)) % 16 == 0;
+}
+
+// Pools of one buffer per layer hold allocations of their own, which are
+// 16-byte aligned; a stacked pool's bases and layer stride are checked.
+bool rows_aligned16(const DevRows& r, int head_bytes) {
+  if (r.row_stride_b % 16 || head_bytes % 16) return false;
+  if (r.k_layers) return true;
+  return (reinterpret_cast<uintptr_t>(r.k_base) | reinterpret_cast<uintptr_t>(r.v_base) | static_cast<uintptr_t>(r.layer_stride_b)) % 16 == 0;
+}
+
+int check_scores(const cb_query_batch* batch, int32_t layer, int32_t dtype, int32_t head_dim, const cb_scores* sc,
+                 int32_t q_heads, int32_t* err, ScoreArgs* s) {
+  int rc;
+  if ((rc = check_batch(batch, dtype, head_dim, err, true, &s->batch, &s->cache))) return rc;
+  if (!sc) return fail(CB_EINVAL, "null scores");
+  if (layer < 0 || layer >= batch->cache.num_layers) return fail(CB_EINVAL, "layer %d outside the cache", layer);
+  const int kv = batch->cache.heads;
+  if (q_heads < 1 || q_heads % kv) return fail(CB_EINVAL, "query heads must be a positive multiple of the KV heads");
+  if (!std::isfinite(sc->scale)) return fail(CB_EINVAL, "scale must be finite");
+  if (!std::isfinite(sc->cap) || sc->cap < 0) return fail(CB_EINVAL, "cap must be finite and not negative");
+  if (sc->window < 0) return fail(CB_EINVAL, "negative window");
+  if (static_cast<int64_t>(batch->max_query) * (q_heads / kv) > 0x3fffffff) return fail(CB_EINVAL, "too many query rows");
+  s->layer = layer;
+  s->head_dim = head_dim;
+  s->q_heads = q_heads;
+  s->kv_heads = kv;
+  s->group = q_heads / kv;
+  s->scale = sc->scale;
+  s->cap = sc->cap;
+  s->window = sc->window;
+  s->causal = sc->causal != 0;
+  s->slopes = sc->slopes;
+  s->prefix = sc->prefix_lengths;
+  return CB_OK;
+}
+
+int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
+
+constexpr int kTargetGroups = 512;  // workgroups that fill the 256 CUs twice
+
+// How the launch is cut: query tiles, and key splits where the tiles alone
+// would leave CUs idle.
+struct AttendShape {
+  int rows_per_tile, keys_per_tile;
+  int tile_slots, request_slots, splits, tiles_per_split;
+};
+
+AttendShape attend_shape(const ScoreArgs& s) {
+  AttendShape h{};
+  h.rows_per_tile = kAnyRows;
+  h.keys_per_tile = kAnyKeys;
+  const QBatch& B = s.batch;
+  const int per_request = std::max(1, ceil_div(static_cast<int64_t>(B.max_query) * s.group, h.rows_per_tile));
+  const int64_t by_request = static_cast<int64_t>(per_request) * B.requests;
+  const int64_t packed = ceil_div(static_cast<int64_t>(B.tokens) * s.group, h.rows_per_tile) + static_cast<int64_t>(B.requests);
+  h.request_slots = by_request <= packed ? per_request : 0;
+  h.tile_slots = static_cast<int>(std::min(by_request, packed));
+  int64_t keys = B.max_length;
+  if (s.window > 0 && s.causal && !s.prefix) keys = std::min<int64_t>(keys, static_cast<int64_t>(s.window) + std::min<int64_t>(B.max_query, h.rows_per_tile / s.group + 2));
+  const int key_tiles = std::max(1, ceil_div(keys, h.keys_per_tile) + (s.prefix ? 1 : 0));
+  const int64_t groups = static_cast<int64_t>(h.tile_slots) * s.kv_heads;
+  int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kTargetGroups / std::max<int64_t>(1, groups), key_tiles / 8)));
+  h.tiles_per_split = ceil_div(key_tiles, splits);
+  h.splits = ceil_div(key_tiles, h.tiles_per_split);
+  if (h.splits == 1) h.tiles_per_split = 0x7fffffff;  // one split takes whatever there is
+  return h;
+}
+
+int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
+
+int64_t attend_workspace(const ScoreArgs& s, const AttendShape& h) {
+  if (h.splits <= 1) return 0;
+  const int64_t rows = static_cast<int64_t>(h.splits) * s.batch.tokens * s.q_heads;
+  return round256(rows * s.head_dim * 4) + round256(rows * 4);
+}
+
+template <typename IO, int DP>
+void launch_any(const AttendArgs& a, bool mod, unsigned grid, hipStream_t st) {
+  if (mod) hipLaunchKernelGGL((attend_any_kernel<IO, DP, true>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
+  else hipLaunchKernelGGL((attend_any_kernel<IO, DP, false>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
+}
+template <typename IO>
+void launch_attend(const AttendArgs& a, const AttendShape& h, bool mod, unsigned grid, hipStream_t st) {
+  const int d = a.s.head_dim;
+  if (d <= 64) launch_any<IO, 64>(a, mod, grid, st);
+  else if (d <= 128) launch_any<IO, 128>(a, mod, grid, st);
+  else if (d <= 256) launch_any<IO, 256>(a, mod, grid, st);
+  else launch_any<IO, 512>(a, mod, grid, st);
+  if (h.splits > 1) {
+    const unsigned joins = static_cast<unsigned>((static_cast<int64_t>(a.s.batch.tokens) * a.s.q_heads + 3) / 4);
+    hipLaunchKernelGGL((join_splits_kernel<IO, kAnyKeys>), dim3(joins), dim3(256), 0, st, a, h.rows_per_tile);
+  }
+}
+
+template <typename IO, int DP>
+void launch_weights_any(const WeightArgs& a, bool mod, unsigned grid, hipStream_t st) {
+  if (mod) hipLaunchKernelGGL((key_weights_any_kernel<IO, DP, true>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
+  else hipLaunchKernelGGL((key_weights_any_kernel<IO, DP, false>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
+}
+template <typename IO>
+void launch_weights(const WeightArgs& a, bool mod, unsigned grid, hipStream_t st) {
+  const int d = a.s.head_dim;
+  if (d <= 64) launch_weights_any<IO, 64>(a, mod, grid, st);
+  else if (d <= 128) launch_weights_any<IO, 128>(a, mod, grid, st);
+  else if (d <= 256) launch_weights_any<IO, 256>(a, mod, grid, st);
+  else launch_weights_any<IO, 512>(a, mod, grid, st);
+}
+
+template <typename IO>
+void launch_install(const InstallArgs& a, bool wide, unsigned grid, hipStream_t st) {
+  if (wide) hipLaunchKernelGGL((install_tokens_kernel<IO, 16 / sizeof(IO)>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, a);
+  else hipLaunchKernelGGL((install_tokens_kernel<IO, 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int cb_install_tokens(const cb_query_batch* batch, int32_t layer, int32_t dtype, int32_t head_dim, const cb_heads* q,
+                      const cb_heads* q_out, const cb_heads* k, const cb_heads* v, const double* inv_freq,
+                      int32_t rotary_dim, int32_t interleaved, float magnitude, const void* positions,
+                      int32_t positions_kind, int32_t* d_error_flag, void* stream) {
+  InstallArgs a{};
+  int rc;
+  if ((rc = check_batch(batch, dtype, head_dim, d_error_flag, true, &a.batch, &a.cache))) return rc;
+  if (layer < 0 || layer >= batch->cache.num_layers) return fail(CB_EINVAL, "layer %d outside the cache", layer);
+  if (!q) return fail(CB_EINVAL, "null q");
+  const int eb = elem_bytes(dtype), kv = batch->cache.heads, n = batch->num_tokens;
+  if (q->heads < 1 || q->heads > (1 << 16)) return fail(CB_EINVAL, "q needs 1 to 65536 heads");
+  if ((rc = check_heads("q", q, q->heads, eb, n, &a.q)) || (rc = check_heads("q_out", q_out, q->heads, eb, n, &a.q_out)) ||
+      (rc = check_heads("k", k, kv, eb, n, &a.k)) || (rc = check_heads("v", v, kv, eb, n, &a.v)))
+    return rc;
+  if (rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2)
+    return fail(CB_EINVAL, "rotary_dim must be even, 2 to head_dim");
+  if (!inv_freq) return fail(CB_EINVAL, "null inv_freq");
+  if (!std::isfinite(magnitude)) return fail(CB_EINVAL, "magnitude must be finite");
+  if (positions && positions_kind != CB_INDEX_I32 && positions_kind != CB_INDEX_I64)
+    return fail(CB_EINVAL, "positions must be int32 or int64");
+  if (n == 0 || batch->num_requests == 0) return CB_OK;
+  a.layer = layer;
+  a.head_dim = head_dim;
+  a.rotary_dim = rotary_dim;
+  a.interleaved = interleaved != 0;
+  a.q_heads = q->heads;
+  a.kv_heads = kv;
+  a.inv_freq = inv_freq;
+  a.positions = positions;
+  a.positions_kind = positions_kind;
+  a.magnitude = magnitude;
+  const int vec = 16 / eb;
+  const bool wide = (rotary_dim / 2) % vec == 0 && head_dim % vec == 0 && aligned16(a.q) && aligned16(a.q_out) &&
+                    aligned16(a.k) && aligned16(a.v) && rows_aligned16(a.cache, head_dim * eb);
+  const int items = (q->heads + kv) * (head_dim - rotary_dim / 2) / (wide ? vec : 1) + kv * head_dim / (wide ? vec : 1);
+  a.slices = std::max(1, std::min(64, items / (4 * kWave)));
+  const int64_t grid = (static_cast<int64_t>(n) * a.slices + kInstallWaves - 1) / kInstallWaves;
+  if (grid > 0x7fffffff) return fail(CB_EINVAL, "too many tokens");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == CB_DTYPE_BF16) launch_install<io_bf16>(a, wide, static_cast<unsigned>(grid), st);
+  else if (dtype == CB_DTYPE_F16) launch_install<io_f16>(a, wide, static_cast<unsigned>(grid), st);
+  else launch_install<float>(a, wide, static_cast<unsigned>(grid), st);
+  CB_HIP(hipGetLastError());
+  return CB_OK;
+}
+
+int cb_attention_workspace_bytes(const cb_query_batch* batch, int32_t dtype, int32_t head_dim, const cb_scores* scores,
+                                 int32_t query_heads, int64_t* bytes) {
+  if (!bytes) return fail(CB_EINVAL, "null bytes");
+  ScoreArgs s{};
+  int rc;
+  if ((rc = check_scores(batch, 0, dtype, head_dim, scores, query_heads, nullptr, &s))) return rc;
+  *bytes = s.batch.tokens && s.batch.requests ? attend_workspace(s, attend_shape(s)) : 0;
+  return CB_OK;
+}
+
+int cb_paged_attention(const cb_query_batch* batch, int32_t layer, int32_t dtype, int32_t head_dim,
+                       const cb_scores* scores, const cb_heads* q, const cb_heads* out, float* lse, void* d_workspace,
+                       int64_t workspace_bytes, int32_t* d_error_flag, void* stream) {
+  if (!q) return fail(CB_EINVAL, "null q");
+  AttendArgs a{};
+  int rc;
+  if ((rc = check_scores(batch, layer, dtype, head_dim, scores, q->heads, d_error_flag, &a.s))) return rc;
+  const int eb = elem_bytes(dtype), n = batch->num_tokens;
+  if ((rc = check_heads("q", q, q->heads, eb, n, &a.s.q)) || (rc = check_heads("out", out, q->heads, eb, n, &a.out))) return rc;
+  if (n == 0 || batch->num_requests == 0) return CB_OK;
+  const AttendShape h = attend_shape(a.s);
+  const int64_t need = attend_workspace(a.s, h);
+  if (need > 0 && (!d_workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(d_workspace) % 256))
+    return fail(CB_EINVAL, "attention needs a 256-byte aligned workspace of %lld bytes", static_cast<long long>(need));
+  a.lse = lse;
+  a.tile_slots = h.tile_slots;
+  a.request_slots = h.request_slots;
+  a.splits = h.splits;
+  a.tiles_per_split = h.tiles_per_split;
+  if (need > 0) {
+    a.part_out = static_cast<float*>(d_workspace);
+    a.part_lse = reinterpret_cast<float*>(static_cast<char*>(d_workspace) +
+                                          round256(static_cast<int64_t>(h.splits) * n * q->heads * head_dim * 4));
+  }
+  const int64_t grid = static_cast<int64_t>(h.tile_slots) * h.splits * a.s.kv_heads;
+  if (grid > 0x7fffffff) return fail(CB_EINVAL, "too many query tiles");
+  const bool mod = a.s.cap > 0 || a.s.slopes;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == CB_DTYPE_BF16) launch_attend<io_bf16>(a, h, mod, static_cast<unsigned>(grid), st);
+  else if (dtype == CB_DTYPE_F16) launch_attend<io_f16>(a, h, mod, static_cast<unsigned>(grid), st);
+  else launch_attend<float>(a, h, mod, static_cast<unsigned>(grid), st);
+  CB_HIP(hipGetLastError());
+  return CB_OK;
+}
+
+int cb_add_key_weights(const cb_query_batch* batch, int32_t layer, int32_t dtype, int32_t head_dim,
+                       const cb_scores* scores, const cb_heads* q, const float* lse, float* weights,
+                       int64_t weights_stride, int32_t* d_error_flag, void* stream) {
+  if (!q) return fail(CB_EINVAL, "null q");
+  WeightArgs a{};
+  int rc;
+  if ((rc = check_scores(batch, layer, dtype, head_dim, scores, q->heads, d_error_flag, &a.s))) return rc;
+  const int eb = elem_bytes(dtype), n = batch->num_tokens;
+  if ((rc = check_heads("q", q, q->heads, eb, n, &a.s.q))) return rc;
+  if (weights_stride < batch->max_length) return fail(CB_EINVAL, "weights rows are shorter than max_length");
+  if (n == 0 || batch->num_requests == 0 || batch->max_length == 0) return CB_OK;
+  if (!lse || !weights) return fail(CB_EINVAL, "null lse or weights");
+  a.lse = lse;
+  a.weights = weights;
+  a.weights_stride = weights_stride;
+  a.key_slots = ceil_div(batch->max_length, 16);
+  const int64_t grid = static_cast<int64_t>(a.key_slots) * batch->num_requests;
+  if (grid > 0x7fffffff) return fail(CB_EINVAL, "too many cached tokens");
+  const bool mod = a.s.cap > 0 || a.s.slopes;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == CB_DTYPE_BF16) launch_weights<io_bf16>(a, mod, static_cast<unsigned>(grid), st);
+  else if (dtype == CB_DTYPE_F16) launch_weights<io_f16>(a, mod, static_cast<unsigned>(grid), st);
+  else launch_weights<float>(a, mod, static_cast<unsigned>(grid), st);
+  CB_HIP(hipGetLastError());
+  return CB_OK;
+}
+
+int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, int32_t dtype, int32_t head_dim,
+                    const float* weights, int64_t weights_stride, int32_t budget, int32_t first, int32_t last,
+                    int32_t* kept, int32_t* kept_lengths, float* kept_weights, void* d_workspace,
+                    int64_t workspace_bytes, int32_t* d_error_flag, void* stream) {
+  EvictArgs a{};
+  MoveArgs m{};
+  int rc;
+  if ((rc = check_batch(batch, dtype, head_dim, d_error_flag, false, &a.batch, &m.src)) ||
+      (rc = check_batch(target, dtype, head_dim, d_error_flag, false, &a.target, &m.dst)))
+    return rc;
+  if (target->num_requests != batch->num_requests) return fail(CB_EINVAL, "batch and target differ in requests");
+  if (target->cache.heads != batch->cache.heads || target->cache.num_layers != batch->cache.num_layers)
+    return fail(CB_EINVAL, "batch and target differ in layers or KV heads");
+  if (budget < 1 || budget > (1 << 30)) return fail(CB_EINVAL, "budget must be 1 to 2^30");
+  if (first < 0 || last < 0 || static_cast<int64_t>(first) + last > budget)
+    return fail(CB_EINVAL, "first + last must be within the budget");
+  if (weights_stride < batch->max_length) return fail(CB_EINVAL, "weights rows are shorter than max_length");
+  if (batch->num_requests == 0) return CB_OK;
+  if ((!weights && batch->max_length > 0) || !kept || !kept_lengths || !kept_weights) return fail(CB_EINVAL, "null weights or kept");
+  const int64_t slots = static_cast<int64_t>(batch->num_requests) * budget;
+  if (!d_workspace || workspace_bytes < slots * 8 || reinterpret_cast<uintptr_t>(d_workspace) % 8)
+    return fail(CB_EINVAL, "eviction needs an 8-byte aligned workspace of %lld bytes", static_cast<long long>(slots * 8));
+  const int eb = elem_bytes(dtype);
+  const int64_t row_bytes = static_cast<int64_t>(batch->cache.heads) * head_dim * eb;
+  if (row_bytes > (1 << 24)) return fail(CB_EINVAL, "rows above 16 MB");
+  a.weights = weights;
+  a.weights_stride = weights_stride;
+  a.budget = budget;
+  a.first = first;
+  a.last = last;
+  a.kept = kept;
+  a.kept_lengths = kept_lengths;
+  a.kept_weights = kept_weights;
+  a.rows = static_cast<int2*>(d_workspace);
+  const bool wide = row_bytes % 16 == 0 && rows_aligned16(m.src, 16) && rows_aligned16(m.dst, 16);
+  const int chunk = wide ? 16 : eb;
+  m.rows = a.rows;
+  m.count = slots;
+  m.chunks_per_row = static_cast<int32_t>(row_bytes / chunk);
+  m.tokens_per_block = std::max(1, 1024 / m.chunks_per_row);
+  const int64_t blocks = (slots + m.tokens_per_block - 1) / m.tokens_per_block;
+  if (blocks > 0x7fffffff || batch->cache.num_layers > 32767) return fail(CB_EINVAL, "eviction too large");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(select_tokens_kernel, dim3(static_cast<unsigned>(batch->num_requests)), dim3(kSelectThreads), 0, st, a);
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(2 * batch->cache.num_layers));
+  if (wide) hipLaunchKernelGGL(move_rows_kernel<uint4>, grid, dim3(256), 0, st, m);
+  else if (eb == 4) hipLaunchKernelGGL(move_rows_kernel<uint32_t>, grid, dim3(256), 0, st, m);
+  else hipLaunchKernelGGL(move_rows_kernel<uint16_t>, grid, dim3(256), 0, st, m);
+  CB_HIP(hipGetLastError());
+  return CB_OK;
+}
+
+}  // extern "C"

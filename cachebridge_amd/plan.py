@@ -48,6 +48,7 @@ class Rows:
     device: torch.device
     keep: list = field(default_factory=list)
     owned: list = field(default_factory=list)
+    index_entries: int = 0
 
     @property
     def num_layers(self) -> int:
@@ -142,7 +143,8 @@ def rows_from_layers(k_layers: Sequence[torch.Tensor], v_layers: Sequence[torch.
     c.index = idx_ptr
     c.index_offset = index_offset
     c.page_size = page_size or 0
-    return Rows(c, first.dtype, first.device, [ptrs, *keep, *k_layers, *v_layers], owned=[ptrs])
+    return Rows(c, first.dtype, first.device, [ptrs, *keep, *k_layers, *v_layers], owned=[ptrs],
+                index_entries=keep[0].numel() if keep else 0)
 
 
 def rows_from_stacked(k: torch.Tensor, v: torch.Tensor, *, index=None, block_table=None,
@@ -157,7 +159,7 @@ def rows_from_stacked(k: torch.Tensor, v: torch.Tensor, *, index=None, block_tab
     kind, idx_ptr, keep = _index_fields(index, block_table, page_size, index_offset, tokens)
     c = _lib.CbRows(None, None, k.data_ptr(), v.data_ptr(), rows * heads * dim, heads * dim, rows, layers, head_offset,
                     heads, kind, idx_ptr, index_offset, page_size or 0)
-    return Rows(c, k.dtype, k.device, [k, v, *keep])
+    return Rows(c, k.dtype, k.device, [k, v, *keep], index_entries=keep[0].numel() if keep else 0)
 
 
 @dataclass(frozen=True)

@@ -52,6 +52,46 @@ def _inverse_frequency(head_dim: int, theta: float, scaling: dict | None):
     return inv, (0.1 * math.log(factor) + 1.0) * attn
 
 
+def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None):
+    """``(inv_freq, magnitude)``: radians per position of each rotated pair, in float64.
+
+    ``scaling`` is None or a dictionary with ``rope_type`` ``"linear"`` (every
+    frequency divided by ``factor``), ``"yarn"`` (the blend of
+    ``_inverse_frequency``) or ``"llama3"`` (slow turns divided by ``factor``,
+    fast ones kept, blended between the two wavelengths).
+    """
+    if type(rotary_dim) is not int or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("RoPE head dimension must be even")
+    inv = float(theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    kind = "none" if scaling is None else scaling.get("rope_type", scaling.get("type"))
+    if kind == "none":
+        return inv, 1.0
+    if kind not in ("linear", "yarn", "llama3"):
+        raise ValueError(f"unsupported RoPE scaling type: {kind!r}")
+    factor = float(scaling["factor"])
+    if kind == "linear":
+        if factor <= 0:
+            raise ValueError("linear RoPE factor must be positive")
+        return inv / factor, 1.0
+    original = float(scaling["original_max_position_embeddings"])
+    if factor <= 1 or original <= 0:
+        raise ValueError(f"{kind} factor must exceed one and original window must be positive")
+    if kind == "llama3":
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if not 0 < low < high:
+            raise ValueError("llama3 frequency factors must satisfy 0 < low < high")
+        turns = original * inv / (2 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0, 1)
+        return inv / factor * (1 - keep) + inv * keep, 1.0
+    bounds = [rotary_dim * math.log(original / (float(scaling.get(name, default)) * 2 * math.pi))
+              / (2 * math.log(theta)) for name, default in (("beta_fast", 32), ("beta_slow", 1))]
+    first, stop = max(math.floor(bounds[0]), 0), min(math.ceil(bounds[1]), rotary_dim - 1)
+    ramp = (torch.arange(rotary_dim // 2, dtype=torch.float64) - first) / (stop - first if stop != first else 0.001)
+    keep = (1 - ramp.clamp(0, 1)) * float(scaling.get("extrapolation_factor", 1))
+    magnitude = (0.1 * math.log(factor) + 1.0) * float(scaling.get("attn_factor", 1))
+    return inv / factor * (1 - keep) + inv * keep, magnitude
+
+
 def rope_tables(head_dim: int, theta: float, scaling: dict | None, positions: int):
     """``(cos, sin)`` of shape ``[positions, head_dim // 2]`` fp32 on the CPU."""
     if positions < 1:

@@ -292,6 +292,124 @@ int cb_delta_state_transform(int32_t dtype, int64_t batch, int32_t k, int32_t v,
    their pair: they set bit 3. */
 int cb_plan_read_errors(cb_plan* plan, int32_t* flags, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Queries on an installed prefix: new tokens of a batch of requests over one
+ * paged pool. Request b's new tokens are rows query_start[b] ..
+ * query_start[b + 1] - 1 of the token tensors; they are the last of its
+ * lengths[b] cached tokens (their K/V rows are part of the cache, see
+ * cb_install_tokens). Its cached token j is at index entry u = start + j of
+ * the cache's index (the cb_rows rules, index_offset included), with
+ * start = offsets[b], or b * request_stride without offsets. The arrays are
+ * device memory and are read by the kernels, so a captured graph follows
+ * their values; max_query and max_length are the host's upper bounds of new
+ * and cached tokens per request.
+ *
+ * A request that breaks these bounds (query_start falling or past
+ * num_tokens, more new tokens than max_query or than cached ones, a length
+ * above max_length, a negative start) is left out whole: its rows of every
+ * output stay as they were. A cached token whose index entry lies outside
+ * the index or names a row outside the pool is left out by itself. Both are
+ * flagged in *d_error_flag (bits CB_ERROR_*) where it is not NULL; it is
+ * never cleared. Rows of no request stay as they were.
+ * No counterpart in the reference, whose target engine answers the queries.
+ */
+#define CB_ERROR_CACHE_ROW 1 /* a cached token without a valid row */
+#define CB_ERROR_TARGET_ROW 2 /* a token whose row to write is not valid */
+#define CB_ERROR_REQUEST 4    /* a request outside the batch's bounds */
+
+typedef struct cb_query_batch {
+  cb_rows cache;         /* heads: KV heads; head_offset 0; buffers of k_layers / v_layers
+                            16-byte aligned */
+  int64_t index_entries; /* entries of cache.index (not read for CB_INDEX_IDENTITY) */
+  const int32_t* query_start; /* [num_requests + 1] */
+  const int32_t* lengths;     /* [num_requests] */
+  const int64_t* offsets;     /* [num_requests] or NULL */
+  int64_t request_stride;
+  int32_t num_requests;
+  int32_t num_tokens; /* rows of the token tensors */
+  int32_t max_query;
+  int32_t max_length; /* at most 2^30 */
+} cb_query_batch;
+
+/* A token tensor [num_tokens][heads][head_dim], head_dim contiguous; strides
+   in elements. */
+typedef struct cb_heads {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+  int32_t heads;
+  int32_t reserved;
+} cb_heads;
+
+/* How a score becomes a weight. New token i of a request is its cached token
+   p = length - new + i; it sees cached token j if j < prefix_lengths[b], or
+   if (j <= p or not causal) and (j > p - window or window is 0). Its score is
+   x = scale * (q . k), then cap * tanh(x / cap) if cap > 0, then minus
+   slopes[h] * |p - j|. */
+typedef struct cb_scores {
+  float scale;
+  float cap;
+  int32_t window;
+  int32_t causal;
+  const float* slopes;           /* device, one per query head, or NULL */
+  const int32_t* prefix_lengths; /* device, one per request, or NULL */
+} cb_scores;
+
+/* Rotate the new tokens' queries and keys to their positions and store their
+   K/V rows into the cache, one launch. Pair i of the first rotary_dim
+   elements of a head (elements i and i + rotary_dim / 2, or 2i and 2i + 1 if
+   interleaved) turns by position * inv_freq[i] radians (device doubles,
+   rotary_dim / 2 of them; the angle is reduced in 64 bits) and is scaled by
+   magnitude. positions (CB_INDEX_I32 or CB_INDEX_I64 entries, one per token
+   row) replaces p where it is not NULL. q_out may be q itself. Rotated values
+   are computed in fp32 and rounded once. Asynchronous. */
+int cb_install_tokens(const cb_query_batch* batch, int32_t layer, int32_t dtype, int32_t head_dim,
+                      const cb_heads* q, const cb_heads* q_out, const cb_heads* k,
+                      const cb_heads* v, const double* inv_freq, int32_t rotary_dim,
+                      int32_t interleaved, float magnitude, const void* positions,
+                      int32_t positions_kind, int32_t* d_error_flag, void* stream);
+
+/* Device workspace bytes of cb_paged_attention for this batch (0: none). */
+int cb_attention_workspace_bytes(const cb_query_batch* batch, int32_t dtype, int32_t head_dim,
+                                 const cb_scores* scores, int32_t query_heads, int64_t* bytes);
+
+/* out[t][h] = sum over the cached tokens that new token t sees of
+   softmax(score) * v. Query head h reads KV head h / (query heads / KV heads).
+   lse (fp32 [num_tokens][query heads], or NULL) gets ln(sum exp(score)). A
+   token that sees nothing gets zeros, and -infinity in lse. What a token does
+   not see never reaches its row, NaN and infinities included. Statistics and
+   sums are fp32. d_workspace is 256-byte aligned device memory that no other
+   launch may use until this one completes. Asynchronous. */
+int cb_paged_attention(const cb_query_batch* batch, int32_t layer, int32_t dtype, int32_t head_dim,
+                       const cb_scores* scores, const cb_heads* q, const cb_heads* out, float* lse,
+                       void* d_workspace, int64_t workspace_bytes, int32_t* d_error_flag,
+                       void* stream);
+
+/* weights[b][j] += sum over request b's new tokens and query heads of
+   exp(score - lse), for the cached tokens j that they see; lse as
+   cb_paged_attention gives it (a row with lse -infinity adds nothing).
+   weights is fp32, rows weights_stride elements apart. One workgroup owns a
+   weight, in a fixed order: the same call gives the same bits. Asynchronous. */
+int cb_add_key_weights(const cb_query_batch* batch, int32_t layer, int32_t dtype, int32_t head_dim,
+                       const cb_scores* scores, const cb_heads* q, const float* lse, float* weights,
+                       int64_t weights_stride, int32_t* d_error_flag, void* stream);
+
+/* Keep at most `budget` cached tokens of each request: its first `first`, its
+   last `last` and, of the rest, those of the largest weights (equal weights:
+   the lowest index first; NaN above every number), and copy their rows of
+   every layer, in order, to tokens 0, 1, ... of the same request of `target`
+   (another pool, or pages of this one that no kept token is read from).
+   kept [requests][budget] gets the cached token of each, then -1;
+   kept_lengths [requests] their count; kept_weights [requests][budget] their
+   weights, then 0. Of `target` the cache, index, offsets and request_stride
+   are read. d_workspace is 8 * num_requests * budget bytes of device memory.
+   Asynchronous. */
+int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, int32_t dtype,
+                    int32_t head_dim, const float* weights, int64_t weights_stride, int32_t budget,
+                    int32_t first, int32_t last, int32_t* kept, int32_t* kept_lengths,
+                    float* kept_weights, void* d_workspace, int64_t workspace_bytes,
+                    int32_t* d_error_flag, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
