@@ -336,6 +336,7 @@ struct ScoreArgs {
   int32_t window, causal;
   const float* slopes;
   const int32_t* prefix;
+  int32_t mod;  // scores are more than a product times a positive scale
 };
 
 struct AttendArgs {
@@ -426,12 +427,10 @@ __device__ inline int tile_start(const KeyRange& k, int t) {
 }
 __device__ inline int tile_end(const KeyRange& k, int t) { return t < k.ta ? k.na : k.hb; }
 
-// Whether every row of the tile sees every key of [start, start + KT).
-template <int KT>
-__device__ inline bool sees_all(const ScoreArgs& s, const KeyRange& k, int start, int end) {
-  if (start + KT > end) return false;
-  if (start + KT <= k.np) return true;
-  return (!s.causal || start + KT <= k.p0 + 1) && (s.window == 0 || start > k.p1 - s.window);
+// Whether every row of the tile sees every key of [start, stop).
+__device__ inline bool sees_all(const ScoreArgs& s, const KeyRange& k, int start, int stop) {
+  if (stop <= k.np) return true;
+  return (!s.causal || stop <= k.p0 + 1) && (s.window == 0 || start > k.p1 - s.window);
 }
 
 // Without branches (bitwise operators): lanes differ in p and j.
@@ -535,7 +534,7 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(Attend
     f32x4 st = {0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < DP / 4; ++e) st = mfma4(lk[c * LD + 4 * e + g], q[e], st);
-    const bool whole = !any_missing && sees_all<KT>(s, kr, start, end);
+    const bool whole = !any_missing && start + KT <= end && sees_all(s, kr, start, start + KT);
     float x[4], top = kNegInf;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -643,6 +642,506 @@ __global__ __launch_bounds__(256) void join_splits_kernel(AttendArgs a, int rows
     store_elem<IO>(op + d * static_cast<int>(sizeof(IO)), from_f32<IO>(o));
   }
   if (a.lse && lane == 0) a.lse[at] = total == 0.0f ? kNegInf : (top + log2_fast(total)) * kLn2;
+}
+
+// ---------------------------------------------------------------------------
+// Attention in 16-bit types, head_dim a multiple of 8 up to 256 (padded with
+// zeros to DP = 64, 128 or 256).
+//
+// One wave computes 32 query rows against tiles of KT keys with
+// v_mfma_f32_32x32x16 (result register e of lane l: row 8 (e / 4) + 4 (l / 32)
+// + e % 4, column l % 32): S^T = K Q^T has a query row per lane pair, so a
+// lane sees half of its row's keys of a tile. Packed in register order, eight
+// of its weights are the second operand of a step of 16 keys, in the key order
+// {4h .. 4h+3, 8+4h .. 8+4h+3} (h = l / 32); V^T is read in the same order by
+// transposing LDS reads, so weights never leave their lane.
+//
+// K and V rows come through LDS by DMA (global_load_lds_dwordx4: the LDS side
+// is 16 bytes a lane in lane order, the global side any address a lane, which
+// gathers rows of pages for free). A row's 16-byte chunks sit at positions
+// chunk ^ f(key): the readers' lanes then hit distinct banks (K: 16 rows of
+// one chunk; V: 4 rows of 4 chunks).
+// ---------------------------------------------------------------------------
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+#define CB_LDS_SPACE __attribute__((address_space(3)))
+
+// An LDS address as the byte offset that DMA takes.
+template <typename T>
+__device__ inline CB_LDS_SPACE T* lds_at(uint32_t offset) {
+  return (CB_LDS_SPACE T*)static_cast<uintptr_t>(offset);
+}
+
+template <typename IO>
+struct Half;
+template <>
+struct Half<io_bf16> {
+  typedef io_bf16 x8 __attribute__((ext_vector_type(8)));
+  static constexpr uint32_t kExponent = 0x7f807f80u, kCarry = 0x00800080u, kInf = 0x7f80u;
+  static __device__ inline f32x16 mul(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+  }
+  static __device__ inline uint32_t pack(float a, float b) { return pack_bf16(a, b); }
+};
+template <>
+struct Half<io_f16> {
+  typedef io_f16 x8 __attribute__((ext_vector_type(8)));
+  typedef io_f16 x2 __attribute__((ext_vector_type(2)));
+  static constexpr uint32_t kExponent = 0x7c007c00u, kCarry = 0x04000400u, kInf = 0x7c00u;
+  static __device__ inline f32x16 mul(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+  }
+  static __device__ inline uint32_t pack(float a, float b) {
+    const f32x2 f = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, x2));  // round to nearest even
+  }
+};
+
+// What the DMA reads for keys without a row and elements past head_dim.
+__device__ const uint4 g_zeros[1] = {};
+
+constexpr int kMaxDp = 256;
+
+template <int DP>
+__device__ inline int swizzle_k(int key) {
+  return DP == 64 ? (key >> 1) & 7 : key & 15;
+}
+template <int DP>
+__device__ inline int swizzle_v(int key) {
+  return DP == 64 ? ((key >> 1) & 1) << 2 : (key & 3) << 2;
+}
+
+__device__ inline void dma16(gcptr src, uint32_t lds) {
+  const uint32_t la = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :: "v"(reinterpret_cast<uint64_t>(src)), "s"(la) : "memory", "m0");
+}
+
+// s_waitcnt operands (gfx9 layout): everything, or the LDS DMA alone.
+constexpr int kWaitAll = 0x0070;     // vmcnt 0, expcnt 7, lgkmcnt 0
+__device__ inline void wait_and_meet() {
+  __builtin_amdgcn_s_waitcnt(kWaitAll);
+  asm volatile("s_barrier" ::: "memory");
+}
+__device__ inline void wait_own() {
+  __builtin_amdgcn_s_waitcnt(kWaitAll);
+  asm volatile("" ::: "memory");
+}
+
+// One lane's part of staging tiles of KT keys: N DMA instructions for K and as
+// many for V, instruction u of this wave covering bytes [(first + u) * 1024,
+// + 1024) of a tile. Index entries are fetched a tile ahead of the rows they
+// name, rows a tile ahead of the products.
+template <typename IO, int DP, int KT, int N>
+struct Stager {
+  static constexpr int C = DP / 8;  // 16-byte chunks a row
+  int64_t entry[N];                 // what the index holds (identity: the row)
+  gcptr kbase, vbase;
+
+  __device__ inline int key(int first, int u) const { return (first + u) * (kWave / C) + (threadIdx.x & (kWave - 1)) / C; }
+
+  __device__ inline void init(const ScoreArgs& s, int head) {
+    const int64_t off = static_cast<int64_t>(head) * s.head_dim * 2;
+    kbase = layer_base(s.cache, 0, s.layer) + off;
+    vbase = layer_base(s.cache, 1, s.layer) + off;
+  }
+  __device__ inline void fetch(const QBatch& B, const Request& r, int first, int start, int end) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int j = start + key(first, u);
+      int64_t e = r.first + j;
+      if (B.kind == CB_INDEX_IDENTITY) {
+        entry[u] = j < end ? e : -1;
+        continue;
+      }
+      if (B.kind == CB_INDEX_BLOCK_TABLE) {
+        const uint32_t x = r.rem + static_cast<uint32_t>(j);
+        e = r.first + (B.page_shift >= 0 ? x >> B.page_shift : x / static_cast<uint32_t>(B.page_size));
+      }
+      const bool in = (j < end) & (e < B.entries);
+      const int64_t at = in ? e : 0;
+      if (B.entries <= 0) entry[u] = -1;
+      else if (B.kind == CB_INDEX_I64) entry[u] = reinterpret_cast<const CB_GLOBAL int64_t*>(as_global(B.index))[at];
+      else entry[u] = reinterpret_cast<const CB_GLOBAL int32_t*>(as_global(B.index))[at];
+      entry[u] = in ? entry[u] : -1;
+    }
+  }
+  // Issues the DMA of the tile whose entries were fetched. Returns the lanes'
+  // keys below `end` that have no row (a wave's ballots, per instruction).
+  __device__ inline void issue(const ScoreArgs& s, const Request& r, int first, int start, int end, uint32_t lk, uint32_t lv,
+                               uint32_t* bad) {
+    const QBatch& B = s.batch;
+    const int lane = threadIdx.x & (kWave - 1), pos = lane % C;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int k = key(first, u), j = start + k;
+      int64_t row = entry[u];
+      if (B.kind == CB_INDEX_BLOCK_TABLE) {
+        const uint32_t x = r.rem + static_cast<uint32_t>(j), ps = static_cast<uint32_t>(B.page_size);
+        const uint32_t in_page = B.page_shift >= 0 ? x & (ps - 1) : x % ps;
+        row = row < 0 ? -1 : row * ps + in_page;
+      }
+      const bool ok = (row >= 0) & (row < B.rows);
+      if (__any(!ok & (j < end))) {
+        if (!ok & (j < end) & (pos == 0)) {
+          flag(B.err, CB_ERROR_CACHE_ROW);
+          atomicOr(bad + (k >> 5), 1u << (k & 31));
+        }
+      }
+      const int ck = pos ^ swizzle_k<DP>(k), cv = pos ^ swizzle_v<DP>(k);
+      gcptr zero = as_global(static_cast<const void*>(g_zeros));
+      gcptr ka = (ok & (ck * 8 < s.head_dim)) ? kbase + row * B.row_stride_b + ck * 16 : zero;
+      gcptr va = (ok & (cv * 8 < s.head_dim)) ? vbase + row * B.row_stride_b + cv * 16 : zero;
+      dma16(ka, lk + (first + u) * 1024);
+      dma16(va, lv + (first + u) * 1024);
+    }
+  }
+};
+
+// 32 query rows of one wave: their operands, statistics and sums.
+template <typename IO, int DP, int KT, bool MOD>
+struct RowBlock {
+  typedef Half<IO> H;
+  static constexpr int KB = KT / 32, DB = DP / 32, KS = DP / 16;
+  u32x4 q[KS];
+  f32x16 o[DB];
+  float m, l;
+  float slope;
+  int row, i, qh, p;  // this lane's query row
+  bool live;
+
+  __device__ inline void init(const ScoreArgs& s, const Request& r, int head, int row0, bool vector) {
+    const int lane = threadIdx.x & (kWave - 1), h = lane >> 5;
+    const int rows = r.n * s.group;
+    row = row0 + (lane & 31);
+    live = row < rows;
+    const int at = min(row, rows - 1);
+    i = at / s.group;
+    qh = head * s.group + at - i * s.group;
+    p = r.length - r.n + i;
+    const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int d = 16 * k + 8 * h;
+      u32x4 x = {0, 0, 0, 0};
+      if (d < s.head_dim) {
+        if (vector) {
+          x = gload<u32x4>(as_global(static_cast<const void*>(qp + 2 * d)));
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            x[w] = load_elem<uint16_t>(qp + 2 * d + 4 * w) | static_cast<uint32_t>(load_elem<uint16_t>(qp + 2 * d + 4 * w + 2)) << 16;
+        }
+      }
+      q[k] = x;
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = 0;
+    m = kNegInf;
+    l = 0;
+    slope = 0;
+    if constexpr (MOD) slope = s.slopes ? s.slopes[qh] : 0.0f;
+  }
+
+  // LDS addresses within a tile that depend on the lane alone.
+  struct Lanes {
+    uint32_t k[DP == 64 ? 4 : 8];  // K chunk 2 ks + h of row l % 32; ks + 8: 256 bytes on
+    uint32_t v[DP == 64 ? 2 : 4];  // V rows 4h + (l % 16) / 4, block db; db + 4: 256 bytes on
+  };
+  static __device__ inline Lanes lanes() {
+    Lanes a;
+    const int lane = threadIdx.x & (kWave - 1), h = lane >> 5, c = lane & 31;
+#pragma unroll
+    for (int ks = 0; ks < (DP == 64 ? 4 : 8); ++ks) a.k[ks] = c * DP * 2 + ((2 * ks + h) ^ swizzle_k<DP>(c)) * 16;
+    const int l16 = lane & 15, key = 4 * h + (l16 >> 2);
+#pragma unroll
+    for (int db = 0; db < (DP == 64 ? 2 : 4); ++db)
+      a.v[db] = key * DP * 2 + ((db * 4 + ((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1)) ^ swizzle_v<DP>(key)) * 16 + (l16 & 1) * 8;
+    return a;
+  }
+
+  static __device__ inline u32x4 k_frag(const Lanes& a, uint32_t base, int kb, int ks) {
+    return *lds_at<const u32x4>(a.k[ks & 7] + base + kb * 32 * DP * 2 + (ks >> 3) * 256);
+  }
+  static __device__ inline u32x4 v_frag(const Lanes& a, uint32_t base, int step, int db) {
+    const uint32_t at = a.v[db & 3] + base + step * 16 * DP * 2 + (db >> 2) * 256;
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(at));
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(at + 8 * DP * 2));
+    const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
+    return u32x4{x.x, x.y, y.x, y.y};
+  }
+
+  // One tile of KT keys that starts at cached token `start`. `whole`: every
+  // row sees every key. `bad`: keys without a row, 32 a word.
+  __device__ __attribute__((always_inline)) void step(const ScoreArgs& s, const KeyRange& kr, const Lanes& a, uint32_t lk,
+                                                      uint32_t lv, int start, int end, bool whole, const uint32_t* bad,
+                                                      float scale2) {
+    const int h = (threadIdx.x & (kWave - 1)) >> 5;
+    f32x16 st[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      f32x16 z;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) z[e] = 0;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) z = H::mul(k_frag(a, lk, kb, ks), q[ks], z);
+      st[kb] = z;
+    }
+    // Scores times scale2 are in the log2 domain (MOD: scale2 is 1 and they
+    // are put there at once).
+    if constexpr (MOD) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          st[kb][e] = natural_score<true>(s, st[kb][e], slope, p, start + 32 * kb + 8 * (e >> 2) + 4 * h + (e & 3)) * kLog2e;
+    }
+    if (!whole) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const uint32_t gone = bad[kb];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int k = 8 * (e >> 2) + 4 * h + (e & 3), j = start + 32 * kb + k;
+          const bool in = (j < end) & sees(s, kr, p, j) & !((gone >> k) & 1);
+          st[kb][e] = in ? st[kb][e] : kNegInf;
+        }
+      }
+    }
+    float top = kNegInf;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, st[kb][e]);
+    top *= scale2;
+    // The maximum may lag by 2^8: weights up to 256 lose no digits in fp32
+    // sums or in 16 bits, and the sums are scaled again only when a row's
+    // maximum has really grown.
+    if (__any(top > m + 8.0f)) {
+      const float both = fmaxf(top, __shfl_xor(top, 32));
+      const float m1 = fmaxf(m, both);
+      const float alpha = m1 == kNegInf ? 1.0f : exp2_fast(m - m1);
+      m = m1;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= alpha;
+    }
+    const float mu = m == kNegInf ? 0.0f : m;
+    u32x4 w[KB][2];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float x = exp2_fast(__builtin_fmaf(st[kb][e], scale2, -mu)), y = exp2_fast(__builtin_fmaf(st[kb][e + 1], scale2, -mu));
+        l += x + y;
+        w[kb][e >> 3][(e & 7) >> 1] = H::pack(x, y);
+      }
+#pragma unroll
+    for (int t = 0; t < 2 * KB; ++t)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] = H::mul(v_frag(a, lv, t, d), w[t >> 1][t & 1], o[d]);
+  }
+
+  // Adds the infinities that were taken out of V tiles (see mark_not_finite).
+  __device__ inline void add_marks(const uint32_t* up, const uint32_t* down) {
+    const int lane = threadIdx.x & (kWave - 1), h = lane >> 5;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const uint32_t u = up[(lane & 31) * DB + d], w = down[(lane & 31) * DB + d];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int bit = 8 * (e >> 2) + 4 * h + (e & 3);
+        o[d][e] += (u >> bit) & 1 ? INFINITY : 0.0f;
+        o[d][e] += (w >> bit) & 1 ? kNegInf : 0.0f;
+      }
+    }
+  }
+
+  __device__ inline void finish(const AttendArgs& a, const Request& r, int split, bool vector) {
+    const ScoreArgs& s = a.s;
+    const int h = (threadIdx.x & (kWave - 1)) >> 5;
+    l += __shfl_xor(l, 32);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float lse2 = l == 0.0f ? kNegInf : m + log2_fast(l);
+    if (!live) return;
+    const int64_t at = static_cast<int64_t>(r.q0 + i) * s.q_heads + qh;
+    if (a.splits > 1) {
+      const int64_t slot = static_cast<int64_t>(split) * s.batch.tokens * s.q_heads + at;
+      gptr po = as_global(static_cast<void*>(a.part_out + slot * s.head_dim));
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (32 * d + 8 * g < s.head_dim)
+            gstore<f32x4>(po + (32 * d + 8 * g + 4 * h) * 4,
+                          f32x4{o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv});
+      if (h == 0) a.part_lse[slot] = lse2;
+      return;
+    }
+    char* op = a.out.data + static_cast<int64_t>(r.q0 + i) * a.out.token_b + qh * a.out.head_b;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (32 * d + 8 * g < s.head_dim) {
+          char* to = op + (32 * d + 8 * g + 4 * h) * 2;
+          const uint2 x = make_uint2(H::pack(o[d][4 * g] * inv, o[d][4 * g + 1] * inv), H::pack(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
+          if (vector) {
+            gstore<uint2>(as_global(static_cast<void*>(to)), x);
+          } else {
+            store_elem<uint16_t>(to, static_cast<uint16_t>(x.x));
+            store_elem<uint16_t>(to + 2, static_cast<uint16_t>(x.x >> 16));
+            store_elem<uint16_t>(to + 4, static_cast<uint16_t>(x.y));
+            store_elem<uint16_t>(to + 6, static_cast<uint16_t>(x.y >> 16));
+          }
+        }
+    if (a.lse && h == 0) a.lse[at] = lse2 * kLn2;
+  }
+};
+
+// A tile that some rows see and others do not: a weight of zero times an
+// infinity would be NaN in rows that do not see the value. Such values are
+// taken out of the tile and noted, a bit per (row, element), for the rows that
+// see their key; the sums get them at the end (+inf, -inf, both for NaN).
+
+// Whether a 16-byte chunk holds an infinity or NaN.
+template <typename IO>
+__device__ inline bool has_not_finite(u32x4 x) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) any |= ((x[u] & Half<IO>::kExponent) + Half<IO>::kCarry) & 0x80008000u;
+  return any != 0;
+}
+
+// One wave notes, for its 32 rows (marks [32][DP / 32], lane l < 32 owns row
+// l's words), every such value of the V tile at lv.
+template <typename IO, int DP, int KT>
+__device__ __attribute__((always_inline)) inline void mark_not_finite(uint32_t lv, int np, int below, int above, int start, int end,
+                                                          CB_LDS_SPACE uint32_t* up, CB_LDS_SPACE uint32_t* down) {
+  constexpr int C = DP / 8;
+  const int lane = threadIdx.x & (kWave - 1);
+  for (int n = 0; n < KT * C / kWave; ++n) {
+    const u32x4 x = *lds_at<const u32x4>(lv + (n * kWave + lane) * 16);
+    uint64_t hits = __ballot(has_not_finite<IO>(x));
+    while (hits) {
+      const int at = __ffsll(static_cast<unsigned long long>(hits)) - 1;
+      hits &= hits - 1;
+      const int chunk = n * kWave + at, key = chunk / C, d0 = ((chunk % C) ^ swizzle_v<DP>(key)) * 8, j = start + key;
+      const bool seen = (j < end) & ((j < np) | ((j <= below) & (j > above)));
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t word = __shfl(e < 4 ? (e < 2 ? x[0] : x[1]) : (e < 6 ? x[2] : x[3]), at);
+        const uint32_t v = (word >> (16 * (e & 1))) & 0xffffu, mag = v & 0x7fffu;
+        const bool nan = mag > Half<IO>::kInf, inf = mag == Half<IO>::kInf;
+        const uint32_t bit = 1u << ((d0 + e) & 31);
+        const int w = (lane & 31) * (DP / 32) + ((d0 + e) >> 5);
+        if (seen & (lane < 32) & (nan | (inf & (v < 0x8000u)))) up[w] |= bit;
+        if (seen & (lane < 32) & (nan | (inf & (v >= 0x8000u)))) down[w] |= bit;
+      }
+    }
+  }
+}
+
+// Zeros in place of the values of this thread's chunk that are not finite.
+template <typename IO>
+__device__ inline u32x4 finite_part(u32x4 x) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const uint32_t c = ((x[u] & Half<IO>::kExponent) + Half<IO>::kCarry) & 0x80008000u;
+    x[u] &= ~((c & 0x8000u ? 0xffffu : 0u) | (c & 0x80000000u ? 0xffff0000u : 0u));
+  }
+  return x;
+}
+
+// Many query rows: a workgroup's NW waves hold 32 rows each and share K and V
+// tiles, double buffered: while a tile is used the next one arrives.
+template <typename IO, int DP, int KT, int NW, bool MOD>
+__global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_kernel(AttendArgs a, int vector) {
+  constexpr int kTile = KT * DP * 2, N = kTile / 1024 / NW;
+  static_assert(N >= 1 && kTile % (1024 * NW) == 0, "a tile is whole DMA instructions of every wave");
+  __shared__ __align__(1024) char tiles[4 * kTile];  // K, V of one buffer, K, V of the other
+  __shared__ uint32_t bad[3][KT / 32];
+  __shared__ uint32_t marks[2][NW][32 * (DP / 32)];
+  __shared__ uint32_t odd[2];  // this tile holds values that are not finite; some tile did
+  const ScoreArgs& s = a.s;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int head = blockIdx.x % s.kv_heads, rest = blockIdx.x / s.kv_heads;
+  const int split = rest % a.splits;
+  Request r;
+  int b, tile;
+  if (!find_tile(a, rest / a.splits, 32 * NW, r, b, tile)) return;
+  const int rows = r.n * s.group, row0 = tile * 32 * NW;
+  const KeyRange kr = key_range<KT>(s, r, b, row0, min(rows, row0 + 32 * NW) - 1);
+  const int t0 = split * a.tiles_per_split, t1 = a.splits > 1 ? min(kr.tiles, t0 + a.tiles_per_split) : kr.tiles;
+  if (a.splits > 1 && t0 >= t1) return;
+
+  typedef RowBlock<IO, DP, KT, MOD> Block;
+  Block blk;
+  blk.init(s, r, head, row0 + 32 * wave, vector);
+  const typename Block::Lanes lanes = Block::lanes();
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((CB_LDS_SPACE char*)tiles));
+  const float scale2 = MOD ? 1.0f : s.scale * kLog2e;
+  Stager<IO, DP, KT, N> stage;
+  stage.init(s, head);
+  const int first = wave * N;
+  if (threadIdx.x < 3 * (KT / 32)) (&bad[0][0])[threadIdx.x] = 0;
+  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+  for (int w = threadIdx.x; w < 2 * NW * DP; w += NW * kWave) (&marks[0][0][0])[w] = 0;
+  __syncthreads();
+  if (t0 < t1) {
+    stage.fetch(s.batch, r, first, tile_start<KT>(kr, t0), tile_end(kr, t0));
+    stage.issue(s, r, first, tile_start<KT>(kr, t0), tile_end(kr, t0), lds, lds + kTile, bad[0]);
+    if (t0 + 1 < t1) stage.fetch(s.batch, r, first, tile_start<KT>(kr, t0 + 1), tile_end(kr, t0 + 1));
+  }
+  uint32_t buf = 0;
+  int slot = 0;
+  for (int t = t0; t < t1; ++t) {
+    wait_and_meet();
+    const int next = slot == 2 ? 0 : slot + 1;
+    if (threadIdx.x < KT / 32) bad[next == 2 ? 0 : next + 1][threadIdx.x] = 0;
+    if (t + 1 < t1) {
+      const int start = tile_start<KT>(kr, t + 1), end = tile_end(kr, t + 1);
+      const uint32_t to = lds + (buf ^ (2 * kTile));
+      stage.issue(s, r, first, start, end, to, to + kTile, bad[next]);
+      if (t + 2 < t1) stage.fetch(s.batch, r, first, tile_start<KT>(kr, t + 2), tile_end(kr, t + 2));
+    }
+    const int start = tile_start<KT>(kr, t), end = tile_end(kr, t);
+    uint32_t gone[KT / 32], some = 0;
+#pragma unroll
+    for (int k = 0; k < KT / 32; ++k) some |= gone[k] = bad[slot][k];
+    const bool all = sees_all(s, kr, start, min(end, start + KT));
+    const bool whole = all && __builtin_amdgcn_readfirstlane(some) == 0 && start + KT <= end;
+    if (!all) {
+      const uint32_t lv = lds + buf + kTile + (threadIdx.x & (kWave - 1)) * 16;
+      bool strange = false;
+#pragma unroll
+      for (int u = 0; u < N; ++u) strange |= has_not_finite<IO>(*lds_at<const u32x4>(lv + (first + u) * 1024));
+      if (strange) odd[0] = odd[1] = 1;
+      __syncthreads();
+      if (odd[0]) {
+        mark_not_finite<IO, DP, KT>(lds + buf + kTile, kr.np, s.causal ? blk.p : 0x7fffffff, s.window > 0 ? blk.p - s.window : -1,
+                                    start, end, (CB_LDS_SPACE uint32_t*)marks[0][wave], (CB_LDS_SPACE uint32_t*)marks[1][wave]);
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          CB_LDS_SPACE u32x4* at = lds_at<u32x4>(lv + (first + u) * 1024);
+          *at = finite_part<IO>(*at);
+        }
+        if (threadIdx.x == 0) odd[0] = 0;
+        __syncthreads();
+      }
+    }
+    blk.step(s, kr, lanes, lds + buf, lds + buf + kTile, start, end, whole, gone, scale2);
+    buf ^= 2 * kTile;
+    slot = next;
+  }
+  __syncthreads();
+  if (odd[1]) blk.add_marks(marks[0][wave], marks[1][wave]);
+  blk.finish(a, r, split, vector);
 }
 
 // ---------------------------------------------------------------------------
@@ -1015,6 +1514,8 @@ int check_scores(const cb_query_batch* batch, int32_t layer, int32_t dtype, int3
   s->causal = sc->causal != 0;
   s->slopes = sc->slopes;
   s->prefix = sc->prefix_lengths;
+  // The plain form takes a row's maximum before the scale: that needs one above zero.
+  s->mod = s->cap > 0 || s->slopes || !(s->scale > 0);
   return CB_OK;
 }
 
@@ -1025,14 +1526,18 @@ constexpr int kTargetGroups = 512;  // workgroups that fill the 256 CUs twice
 // How the launch is cut: query tiles, and key splits where the tiles alone
 // would leave CUs idle.
 struct AttendShape {
+  bool half;  // the 16-bit kernels
   int rows_per_tile, keys_per_tile;
   int tile_slots, request_slots, splits, tiles_per_split;
 };
 
-AttendShape attend_shape(const ScoreArgs& s) {
+constexpr int kTileWaves = 4;
+
+AttendShape attend_shape(const ScoreArgs& s, int32_t dtype) {
   AttendShape h{};
-  h.rows_per_tile = kAnyRows;
-  h.keys_per_tile = kAnyKeys;
+  h.half = dtype != CB_DTYPE_F32 && s.head_dim % 8 == 0 && s.head_dim <= kMaxDp && rows_aligned16(s.cache, s.head_dim * 2);
+  h.rows_per_tile = h.half ? 32 * kTileWaves : kAnyRows;
+  h.keys_per_tile = !h.half ? kAnyKeys : s.head_dim <= (s.mod ? 64 : 128) ? 64 : 32;
   const QBatch& B = s.batch;
   const int per_request = std::max(1, ceil_div(static_cast<int64_t>(B.max_query) * s.group, h.rows_per_tile));
   const int64_t by_request = static_cast<int64_t>(per_request) * B.requests;
@@ -1063,9 +1568,32 @@ void launch_any(const AttendArgs& a, bool mod, unsigned grid, hipStream_t st) {
   if (mod) hipLaunchKernelGGL((attend_any_kernel<IO, DP, true>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
   else hipLaunchKernelGGL((attend_any_kernel<IO, DP, false>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
 }
+template <typename IO, int DP, int KT, bool MOD>
+void launch_half(const AttendArgs& a, const AttendShape& h, unsigned grid, hipStream_t st) {
+  const int vector = aligned16(a.s.q) && aligned16(a.out);
+  hipLaunchKernelGGL((attend_tile_kernel<IO, DP, KT, kTileWaves, MOD>), dim3(grid), dim3(kTileWaves * kWave), 0, st, a, vector);
+  if (h.splits > 1) {
+    const unsigned joins = static_cast<unsigned>((static_cast<int64_t>(a.s.batch.tokens) * a.s.q_heads + 3) / 4);
+    hipLaunchKernelGGL((join_splits_kernel<IO, KT>), dim3(joins), dim3(256), 0, st, a, h.rows_per_tile);
+  }
+}
 template <typename IO>
 void launch_attend(const AttendArgs& a, const AttendShape& h, bool mod, unsigned grid, hipStream_t st) {
   const int d = a.s.head_dim;
+  if constexpr (sizeof(IO) == 2) {
+    if (h.half) {
+      if (mod) {
+        if (d <= 64) launch_half<IO, 64, 64, true>(a, h, grid, st);
+        else if (d <= 128) launch_half<IO, 128, 32, true>(a, h, grid, st);
+        else launch_half<IO, 256, 32, true>(a, h, grid, st);
+      } else {
+        if (d <= 64) launch_half<IO, 64, 64, false>(a, h, grid, st);
+        else if (d <= 128) launch_half<IO, 128, 64, false>(a, h, grid, st);
+        else launch_half<IO, 256, 32, false>(a, h, grid, st);
+      }
+      return;
+    }
+  }
   if (d <= 64) launch_any<IO, 64>(a, mod, grid, st);
   else if (d <= 128) launch_any<IO, 128>(a, mod, grid, st);
   else if (d <= 256) launch_any<IO, 256>(a, mod, grid, st);
@@ -1152,7 +1680,7 @@ int cb_attention_workspace_bytes(const cb_query_batch* batch, int32_t dtype, int
   ScoreArgs s{};
   int rc;
   if ((rc = check_scores(batch, 0, dtype, head_dim, scores, query_heads, nullptr, &s))) return rc;
-  *bytes = s.batch.tokens && s.batch.requests ? attend_workspace(s, attend_shape(s)) : 0;
+  *bytes = s.batch.tokens && s.batch.requests ? attend_workspace(s, attend_shape(s, dtype)) : 0;
   return CB_OK;
 }
 
@@ -1166,7 +1694,7 @@ int cb_paged_attention(const cb_query_batch* batch, int32_t layer, int32_t dtype
   const int eb = elem_bytes(dtype), n = batch->num_tokens;
   if ((rc = check_heads("q", q, q->heads, eb, n, &a.s.q)) || (rc = check_heads("out", out, q->heads, eb, n, &a.out))) return rc;
   if (n == 0 || batch->num_requests == 0) return CB_OK;
-  const AttendShape h = attend_shape(a.s);
+  const AttendShape h = attend_shape(a.s, dtype);
   const int64_t need = attend_workspace(a.s, h);
   if (need > 0 && (!d_workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(d_workspace) % 256))
     return fail(CB_EINVAL, "attention needs a 256-byte aligned workspace of %lld bytes", static_cast<long long>(need));
@@ -1182,7 +1710,7 @@ int cb_paged_attention(const cb_query_batch* batch, int32_t layer, int32_t dtype
   }
   const int64_t grid = static_cast<int64_t>(h.tile_slots) * h.splits * a.s.kv_heads;
   if (grid > 0x7fffffff) return fail(CB_EINVAL, "too many query tiles");
-  const bool mod = a.s.cap > 0 || a.s.slopes;
+  const bool mod = a.s.mod;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == CB_DTYPE_BF16) launch_attend<io_bf16>(a, h, mod, static_cast<unsigned>(grid), st);
   else if (dtype == CB_DTYPE_F16) launch_attend<io_f16>(a, h, mod, static_cast<unsigned>(grid), st);
@@ -1209,7 +1737,7 @@ int cb_add_key_weights(const cb_query_batch* batch, int32_t layer, int32_t dtype
   a.key_slots = ceil_div(batch->max_length, 16);
   const int64_t grid = static_cast<int64_t>(a.key_slots) * batch->num_requests;
   if (grid > 0x7fffffff) return fail(CB_EINVAL, "too many cached tokens");
-  const bool mod = a.s.cap > 0 || a.s.slopes;
+  const bool mod = a.s.mod;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == CB_DTYPE_BF16) launch_weights<io_bf16>(a, mod, static_cast<unsigned>(grid), st);
   else if (dtype == CB_DTYPE_F16) launch_weights<io_f16>(a, mod, static_cast<unsigned>(grid), st);
