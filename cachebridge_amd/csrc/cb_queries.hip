@@ -609,14 +609,20 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(Attend
   if (a.lse && g == 0) a.lse[at] = lse2 * kLn2;
 }
 
-// Joins the splits of one (token, head) per wave: out = sum 2^(lse_z - lse) out_z.
-template <typename IO, int KT>
-__global__ __launch_bounds__(256) void join_splits_kernel(AttendArgs a, int rows_per_tile) {
+// Joins the splits of one (token, head) a workgroup: out = sum 2^(lse_z - lse)
+// out_z. Threads of one group of LANES hold four elements each of a
+// split's row, the groups take splits in turn and meet in LDS in group order.
+constexpr int kJoinThreads = 256;
+
+template <typename IO, int KT, int LANES>
+__global__ __launch_bounds__(kJoinThreads) void join_splits_kernel(AttendArgs a, int rows_per_tile) {
+  constexpr int GROUPS = kJoinThreads / LANES;
+  __shared__ float red[2][kJoinThreads / kWave];
+  __shared__ f32x4 sums[GROUPS][LANES];
   const ScoreArgs& s = a.s;
-  const int lane = threadIdx.x & (kWave - 1);
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int64_t at = blockIdx.x;
   const int t = static_cast<int>(at / s.q_heads), qh = static_cast<int>(at % s.q_heads);
-  if (t >= s.batch.tokens) return;
   const int b = request_of_token(s.batch, t);
   if (b >= s.batch.requests) return;
   const Request r = load_request(s.batch, b);
@@ -626,22 +632,51 @@ __global__ __launch_bounds__(256) void join_splits_kernel(AttendArgs a, int rows
   const KeyRange kr = key_range<KT>(s, r, b, row0, min(r.n * s.group, row0 + rows_per_tile) - 1);
   const int n = min(a.splits, (kr.tiles + a.tiles_per_split - 1) / a.tiles_per_split);
   const int64_t step = static_cast<int64_t>(s.batch.tokens) * s.q_heads;
+  const float* lse = a.part_lse + at;
   float top = kNegInf;
-  for (int z = 0; z < n; ++z) top = fmaxf(top, a.part_lse[z * step + at]);
+  for (int z = threadIdx.x; z < n; z += kJoinThreads) top = fmaxf(top, lse[z * step]);
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if (lane == 0) red[0][wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / kWave; ++w) top = fmaxf(top, red[0][w]);
   const float mu = top == kNegInf ? 0.0f : top;
   float total = 0;
-  for (int z = 0; z < n; ++z) total += exp2_fast(a.part_lse[z * step + at] - mu);
+  for (int z = threadIdx.x; z < n; z += kJoinThreads) total += exp2_fast(lse[z * step] - mu);
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) total += __shfl_xor(total, d);
+  if (lane == 0) red[1][wave] = total;
+  const int g = threadIdx.x / LANES, x = threadIdx.x % LANES;
+  const int D = s.head_dim;
+  f32x4 o = {0, 0, 0, 0};
+  const bool vector = D % 4 == 0;
+  for (int z = g; z < n; z += GROUPS) {
+    const float w = exp2_fast(lse[z * step] - mu);
+    if (w == 0.0f || 4 * x >= D) continue;
+    const float* from = a.part_out + (z * step + at) * D + 4 * x;
+    if (vector) {
+      o += w * *reinterpret_cast<const f32x4*>(from);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (4 * x + e < D) o[e] += w * from[e];
+    }
+  }
+  sums[g][x] = o;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / kWave; ++w) total += red[1][w];
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   char* op = a.out.data + static_cast<int64_t>(t) * a.out.token_b + qh * a.out.head_b;
-  for (int d = lane; d < s.head_dim; d += kWave) {
-    float o = 0;
-    for (int z = 0; z < n; ++z) {
-      const float w = exp2_fast(a.part_lse[z * step + at] - mu) * inv;
-      if (w != 0.0f) o += w * a.part_out[(z * step + at) * s.head_dim + d];
-    }
-    store_elem<IO>(op + d * static_cast<int>(sizeof(IO)), from_f32<IO>(o));
+  for (int d = threadIdx.x; d < D; d += kJoinThreads) {
+    float sum = 0;
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) sum += sums[k][d / 4][d & 3];
+    store_elem<IO>(op + d * static_cast<int>(sizeof(IO)), from_f32<IO>(sum * inv));
   }
-  if (a.lse && lane == 0) a.lse[at] = total == 0.0f ? kNegInf : (top + log2_fast(total)) * kLn2;
+  if (a.lse && threadIdx.x == 0) a.lse[at] = total == 0.0f ? kNegInf : (top + log2_fast(total)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------
@@ -876,13 +911,8 @@ struct RowBlock {
     return u32x4{x.x, x.y, y.x, y.y};
   }
 
-  // One tile of KT keys that starts at cached token `start`. `whole`: every
-  // row sees every key. `bad`: keys without a row, 32 a word.
-  __device__ __attribute__((always_inline)) void step(const ScoreArgs& s, const KeyRange& kr, const Lanes& a, uint32_t lk,
-                                                      uint32_t lv, int start, int end, bool whole, const uint32_t* bad,
-                                                      float scale2) {
-    const int h = (threadIdx.x & (kWave - 1)) >> 5;
-    f32x16 st[KB];
+  // Raw products of the rows with a tile of KT keys.
+  __device__ __attribute__((always_inline)) void products(const Lanes& a, uint32_t lk, f32x16 (&st)[KB]) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       f32x16 z;
@@ -892,6 +922,14 @@ struct RowBlock {
       for (int ks = 0; ks < KS; ++ks) z = H::mul(k_frag(a, lk, kb, ks), q[ks], z);
       st[kb] = z;
     }
+  }
+
+  // Their weights, of the tile that starts at cached token `start`. `whole`:
+  // every row sees every key. `bad`: keys without a row, 32 a word.
+  __device__ __attribute__((always_inline)) void weigh(const ScoreArgs& s, const KeyRange& kr, f32x16 (&st)[KB], int start,
+                                                       int end, bool whole, const uint32_t* bad, float scale2,
+                                                       u32x4 (&w)[KB][2]) {
+    const int h = (threadIdx.x & (kWave - 1)) >> 5;
     // Scores times scale2 are in the log2 domain (MOD: scale2 is 1 and they
     // are put there at once).
     if constexpr (MOD) {
@@ -932,7 +970,6 @@ struct RowBlock {
       for (int d = 0; d < DB; ++d) o[d] *= alpha;
     }
     const float mu = m == kNegInf ? 0.0f : m;
-    u32x4 w[KB][2];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -941,6 +978,9 @@ struct RowBlock {
         l += x + y;
         w[kb][e >> 3][(e & 7) >> 1] = H::pack(x, y);
       }
+  }
+
+  __device__ __attribute__((always_inline)) void add_values(const Lanes& a, uint32_t lv, const u32x4 (&w)[KB][2]) {
 #pragma unroll
     for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
@@ -1135,13 +1175,192 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_ker
         __syncthreads();
       }
     }
-    blk.step(s, kr, lanes, lds + buf, lds + buf + kTile, start, end, whole, gone, scale2);
+    f32x16 st[KT / 32];
+    u32x4 w[KT / 32][2];
+    blk.products(lanes, lds + buf, st);
+    blk.weigh(s, kr, st, start, end, whole, gone, scale2, w);
+    blk.add_values(lanes, lds + buf + kTile, w);
     buf ^= 2 * kTile;
     slot = next;
   }
   __syncthreads();
   if (odd[1]) blk.add_marks(marks[0][wave], marks[1][wave]);
   blk.finish(a, r, split, vector);
+}
+
+// Few query rows (a decoding step): one block of 32 rows, whose keys the NW
+// waves of a workgroup and the splits divide. Bound by memory, so each wave
+// streams tiles of 32 keys through LDS of its own without barriers: two tiles
+// of K and V are in flight, the next K is asked for as soon as the products
+// have read its place, the next V after its sums. The rows that the index
+// names are resolved into LDS first, so that the loop's only vector memory
+// operations are the DMA, whose count tells what has arrived.
+constexpr int kStepTiles = 64;  // tiles a split holds at most
+
+constexpr int wait_vm(int n) { return (n & 15) | 0x70 | 0xf00 | ((n >> 4) << 14); }
+
+template <typename IO, int DP, int NW, bool MOD>
+__global__ __launch_bounds__(NW * kWave, 1) void attend_step_kernel(AttendArgs a, int vector) {
+  constexpr int KT = 32, kTile = KT * DP * 2, N = kTile / 1024, C = DP / 8, LD = DP + 4;
+  static_assert(4 * kTile >= 32 * LD * 4, "a wave's sums fit its tiles");
+  __shared__ __align__(1024) char tiles[NW * 4 * kTile];  // a wave's K, K, V, V
+  __shared__ int key_rows[kStepTiles * KT];
+  __shared__ uint32_t marks[2][NW][32 * (DP / 32)];
+  __shared__ float stats[2][NW][32];
+  const ScoreArgs& s = a.s;
+  const QBatch& B = s.batch;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int head = blockIdx.x % s.kv_heads, rest = blockIdx.x / s.kv_heads;
+  const int split = rest % a.splits;
+  Request r;
+  int b, tile;
+  if (!find_tile(a, rest / a.splits, 32, r, b, tile)) return;
+  const int rows = r.n * s.group, row0 = tile * 32;
+  const KeyRange kr = key_range<KT>(s, r, b, row0, min(rows, row0 + 32) - 1);
+  const int t0 = split * a.tiles_per_split, t1 = min(kr.tiles, t0 + min(a.tiles_per_split, kStepTiles));
+  if (a.splits > 1 && t0 >= t1) return;
+
+  for (int k = threadIdx.x; k < (t1 - t0) * KT; k += NW * kWave) {
+    const int t = t0 + k / KT, j = tile_start<KT>(kr, t) + k % KT;
+    int64_t row = -1;
+    if (j < tile_end(kr, t)) {
+      row = cache_row(B, r, j);
+      if (row < 0) flag(B.err, CB_ERROR_CACHE_ROW);
+    }
+    key_rows[k] = static_cast<int>(row);
+  }
+  for (int w = threadIdx.x; w < 2 * NW * DP; w += NW * kWave) (&marks[0][0][0])[w] = 0;
+  typedef RowBlock<IO, DP, KT, MOD> Block;
+  Block blk;
+  blk.init(s, r, head, row0, vector);
+  const typename Block::Lanes lanes = Block::lanes();
+  const float scale2 = MOD ? 1.0f : s.scale * kLog2e;
+  const int64_t off = static_cast<int64_t>(head) * s.head_dim * 2;
+  gcptr kbase = layer_base(s.cache, 0, s.layer) + off, vbase = layer_base(s.cache, 1, s.layer) + off;
+  gcptr zero = as_global(static_cast<const void*>(g_zeros));
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((CB_LDS_SPACE char*)tiles)) + wave * 4 * kTile;
+  wait_and_meet();
+
+  const int n = t1 - t0 > wave ? (t1 - t0 - wave + NW - 1) / NW : 0;  // this wave's tiles: t0 + wave, + NW, ...
+  auto request = [&](int i, gcptr base, uint32_t to, bool value) __attribute__((always_inline)) {
+    const int at = (wave + i * NW) * KT;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int k = u * (kWave / C) + lane / C;
+      const int row = key_rows[at + k];
+      const int c = (lane % C) ^ (value ? swizzle_v<DP>(k) : swizzle_k<DP>(k));
+      gcptr from = ((row >= 0) & (c * 8 < s.head_dim)) ? base + row * B.row_stride_b + c * 16 : zero;
+      dma16(from, to + u * 1024);
+    }
+  };
+  bool some_mark = false;
+  if (n > 0) {
+    request(0, kbase, lds, false);
+    request(0, vbase, lds + 2 * kTile, true);
+  }
+  if (n > 1) {
+    request(1, kbase, lds + kTile, false);
+    request(1, vbase, lds + 3 * kTile, true);
+  }
+  uint32_t buf = 0;
+  for (int i = 0; i < n; ++i) {
+    const int t = t0 + wave + i * NW, start = tile_start<KT>(kr, t), end = tile_end(kr, t);
+    const uint32_t gone = static_cast<uint32_t>(__ballot(key_rows[(t - t0) * KT + (lane & 31)] < 0));
+    if (i + 1 < n) __builtin_amdgcn_s_waitcnt(wait_vm(3 * N));
+    else __builtin_amdgcn_s_waitcnt(wait_vm(N));
+    asm volatile("" ::: "memory");
+    f32x16 st[1];
+    u32x4 w[1][2];
+    blk.products(lanes, lds + buf, st);
+    if (i + 2 < n) {
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // the products' LDS reads
+      request(i + 2, kbase, lds + buf, false);
+    }
+    const bool all = sees_all(s, kr, start, min(end, start + KT));
+    blk.weigh(s, kr, st, start, end, all & (gone == 0), &gone, scale2, w);
+    if (i + 2 < n) __builtin_amdgcn_s_waitcnt(wait_vm(3 * N));
+    else if (i + 1 < n) __builtin_amdgcn_s_waitcnt(wait_vm(2 * N));
+    else __builtin_amdgcn_s_waitcnt(wait_vm(0));
+    asm volatile("" ::: "memory");
+    const uint32_t lv = lds + 2 * kTile + buf;
+    if (!all) {
+      bool strange = false;
+#pragma unroll
+      for (int u = 0; u < N; ++u) strange |= has_not_finite<IO>(*lds_at<const u32x4>(lv + u * 1024 + lane * 16));
+      if (__any(strange)) {
+        some_mark = true;
+        mark_not_finite<IO, DP, KT>(lv, kr.np, s.causal ? blk.p : 0x7fffffff, s.window > 0 ? blk.p - s.window : -1, start, end,
+                                    (CB_LDS_SPACE uint32_t*)marks[0][wave], (CB_LDS_SPACE uint32_t*)marks[1][wave]);
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          CB_LDS_SPACE u32x4* at = lds_at<u32x4>(lv + u * 1024 + lane * 16);
+          *at = finite_part<IO>(*at);
+        }
+      }
+    }
+    blk.add_values(lanes, lv, w);
+    if (i + 2 < n) {
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      request(i + 2, vbase, lv, true);
+    }
+    buf ^= kTile;
+  }
+  if (some_mark) blk.add_marks(marks[0][wave], marks[1][wave]);
+
+  // The waves' sums meet in LDS, each wave's in its own tiles.
+  blk.l += __shfl_xor(blk.l, 32);
+  const int c = lane & 31, h = lane >> 5;
+  float* mine = reinterpret_cast<float*>(tiles + wave * 4 * kTile) + c * LD;
+  if (blk.live) {
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(mine + 32 * d + 8 * g + 4 * h) =
+            f32x4{blk.o[d][4 * g], blk.o[d][4 * g + 1], blk.o[d][4 * g + 2], blk.o[d][4 * g + 3]};
+  }
+  if (h == 0) {
+    stats[0][wave][c] = blk.m;
+    stats[1][wave][c] = blk.l;
+  }
+  __syncthreads();
+  const int D = s.head_dim, live = min(32, rows - row0), pairs = D / 2;
+  for (int x = threadIdx.x; x < live * pairs; x += NW * kWave) {
+    const int y = x / pairs, d = 2 * (x - y * pairs);
+    float m = kNegInf;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, stats[0][w][y]);
+    const float mu = m == kNegInf ? 0.0f : m;
+    float l = 0, o0 = 0, o1 = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = exp2_fast(stats[0][w][y] - mu);
+      const float* from = reinterpret_cast<const float*>(tiles + w * 4 * kTile) + y * LD + d;
+      l += f * stats[1][w][y];
+      // A wave that saw nothing of this row has nothing to add.
+      o0 += f != 0.0f ? f * from[0] : 0.0f;
+      o1 += f != 0.0f ? f * from[1] : 0.0f;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float lse2 = l == 0.0f ? kNegInf : m + log2_fast(l);
+    const int row = row0 + y, i = row / s.group, qh = head * s.group + row - i * s.group;
+    const int64_t at = static_cast<int64_t>(r.q0 + i) * s.q_heads + qh;
+    if (a.splits > 1) {
+      const int64_t slot = static_cast<int64_t>(split) * B.tokens * s.q_heads + at;
+      *reinterpret_cast<float2*>(a.part_out + slot * D + d) = make_float2(o0 * inv, o1 * inv);
+      if (d == 0) a.part_lse[slot] = lse2;
+    } else {
+      char* op = a.out.data + static_cast<int64_t>(r.q0 + i) * a.out.token_b + qh * a.out.head_b + d * 2;
+      const uint32_t packed = Half<IO>::pack(o0 * inv, o1 * inv);
+      if (vector) {
+        gstore<uint32_t>(as_global(static_cast<void*>(op)), packed);
+      } else {
+        store_elem<uint16_t>(op, static_cast<uint16_t>(packed));
+        store_elem<uint16_t>(op + 2, static_cast<uint16_t>(packed >> 16));
+      }
+      if (a.lse && d == 0) a.lse[at] = lse2 * kLn2;
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1153,7 +1372,8 @@ struct WeightArgs {
   const float* lse;
   float* weights;
   int64_t weights_stride;
-  int32_t key_slots;  // key tiles launched per request
+  int32_t key_slots;        // workgroups launched per request
+  int32_t waves_per_block;  // 16-bit kernel: waves that share a block of 32 keys (1, 2 or 4)
 };
 
 // The new tokens of a request that may see any of the cached tokens
@@ -1229,6 +1449,115 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void key_weights_any_kernel(W
 #pragma unroll
     for (int w = 0; w < kAnyWaves; ++w) add += sums[w][threadIdx.x];
     a.weights[b * a.weights_stride + start + threadIdx.x] += add;
+  }
+}
+
+// 16-bit form: a wave holds 32 keys of one KV head as MFMA operands in
+// registers and walks blocks of 32 query rows, whose operands come straight
+// from memory (the few rows of a batch stay in cache); S^T keeps a row a lane
+// pair, so a key's sum over rows is a sum over lanes, made once at the end.
+// The waves that share a block of keys (4 if there are 4 or more blocks of
+// rows to walk, else fewer, so that none idles) meet in LDS in wave order.
+constexpr int kWeightWaves = 4;
+
+template <typename IO, int DP, bool MOD>
+__global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 2 : 4) void key_weights_kernel(WeightArgs a, int vector) {
+  typedef Half<IO> H;
+  constexpr int KS = DP / 16;
+  __shared__ float sums[kWeightWaves][32];
+  const ScoreArgs& s = a.s;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int h = lane >> 5, c = lane & 31;
+  const int b = blockIdx.x / a.key_slots;
+  const int share = a.waves_per_block, sub = wave % share;
+  const int wide = 32 * (kWeightWaves / share);  // keys of the workgroup
+  const int first_key = (blockIdx.x % a.key_slots) * wide, start = first_key + 32 * (wave / share);
+  const Request r = load_request(s.batch, b);
+  if (!r.ok && first_key == 0 && threadIdx.x == 0) flag(s.batch.err, CB_ERROR_REQUEST);
+  if (first_key >= r.length) return;
+  KeyRange kr{};
+  kr.np = s.prefix ? max(0, min(s.prefix[b], r.length)) : 0;
+  int i0 = 0, i1 = 0;
+  if (start < r.length) query_range(s, r, kr.np, start, 32, &i0, &i1);
+  const int j = start + c;
+  const int64_t mine = j < r.length ? cache_row(s.batch, r, j) : -1;
+  if ((j < r.length) & (mine < 0) & (sub == 0) & (h == 0)) flag(s.batch.err, CB_ERROR_CACHE_ROW);
+  const uint32_t there = static_cast<uint32_t>(__ballot(mine >= 0));
+  const int D = s.head_dim;
+  const int low = i0 * s.group, high = i1 * s.group, blocks = (high - low + 31) / 32;
+  float sum[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sum[e] = 0;
+  int held = -1;
+  u32x4 k[KS];
+  for (int item = sub; item < s.kv_heads * blocks; item += share) {
+    const int head = item / blocks, row0 = low + (item - head * blocks) * 32;
+    if (head != held) {
+      held = head;
+      gcptr kp = layer_base(s.cache, 0, s.layer) + static_cast<int64_t>(head) * D * 2 + mine * s.batch.row_stride_b;
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        const int d = 16 * x + 8 * h;
+        k[x] = u32x4{0, 0, 0, 0};
+        if ((mine >= 0) & (d < D)) k[x] = gload<u32x4>(kp + 2 * d);
+      }
+    }
+    const int row = row0 + c, at = min(row, high - 1), i = at / s.group, qh = head * s.group + at - i * s.group;
+    const int p = r.length - r.n + i;
+    const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
+    float lse = a.lse[static_cast<int64_t>(r.q0 + i) * s.q_heads + qh];
+    // Nothing is added by lanes past the last row and rows that see nothing.
+    lse = (row >= high) | (lse == kNegInf) ? INFINITY : lse;
+    float slope = 0;
+    if constexpr (MOD) slope = s.slopes ? s.slopes[qh] : 0.0f;
+    f32x16 st;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) st[e] = 0;
+#pragma unroll
+    for (int x = 0; x < KS; ++x) {
+      const int d = 16 * x + 8 * h;
+      u32x4 q = {0, 0, 0, 0};
+      if (d < D) {
+        if (vector) {
+          q = gload<u32x4>(as_global(static_cast<const void*>(qp + 2 * d)));
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            q[w] = load_elem<uint16_t>(qp + 2 * d + 4 * w) | static_cast<uint32_t>(load_elem<uint16_t>(qp + 2 * d + 4 * w + 2)) << 16;
+        }
+      }
+      st = H::mul(k[x], q, st);
+    }
+    kr.p0 = r.length - r.n + row0 / s.group;
+    kr.p1 = r.length - r.n + min(row0 + 31, high - 1) / s.group;
+    const bool whole = sees_all(s, kr, start, start + 32);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int key = start + 8 * (e >> 2) + 4 * h + (e & 3);
+      // The difference first: what is near the row's maximum keeps its bits.
+      const float w = exp2_fast((natural_score<MOD>(s, st[e], slope, p, key) - lse) * kLog2e);
+      sum[e] += (whole | sees(s, kr, p, key)) ? w : 0.0f;
+    }
+  }
+  // Sums over the 32 lanes of a half: each exchange halves what a lane holds.
+#pragma unroll
+  for (int n = 8, d = 16; n >= 1; n >>= 1, d >>= 1) {
+    const bool up = (lane & d) != 0;
+#pragma unroll
+    for (int e = 0; e < n; ++e) {
+      const float keep = up ? sum[e + n] : sum[e], give = up ? sum[e] : sum[e + n];
+      sum[e] = keep + __shfl_xor(give, d);
+    }
+  }
+  sum[0] += __shfl_xor(sum[0], 1);
+  // Lane bits 4, 3, 2, 1 chose register bits 3, 2, 1, 0.
+  const int e = (lane >> 1) & 15;
+  if ((lane & 1) == 0) sums[wave][8 * (e >> 2) + 4 * h + (e & 3)] = sum[0];
+  __syncthreads();
+  if (sub == 0 && h == 0 && j < r.length && ((there >> c) & 1)) {
+    float add = 0;
+    for (int w = 0; w < share; ++w) add += sums[wave + w][c];
+    a.weights[b * a.weights_stride + j] += add;
   }
 }
 
@@ -1527,18 +1856,28 @@ constexpr int kTargetGroups = 512;  // workgroups that fill the 256 CUs twice
 // would leave CUs idle.
 struct AttendShape {
   bool half;  // the 16-bit kernels
+  bool step;  // of these, the one for few rows
   int rows_per_tile, keys_per_tile;
   int tile_slots, request_slots, splits, tiles_per_split;
 };
 
+// Whether the 16-bit kernels take the call: whole 16-byte chunks of rows.
+bool takes_half(const ScoreArgs& s, int32_t dtype) {
+  return dtype != CB_DTYPE_F32 && s.head_dim % 8 == 0 && s.head_dim <= kMaxDp && rows_aligned16(s.cache, s.head_dim * 2);
+}
+
 constexpr int kTileWaves = 4;
+constexpr int kStepRows = 32;  // query rows per KV head up to which attend_step_kernel is taken
+constexpr int kStepGroups = 1024;
+constexpr int kStepWaves = 2;
 
 AttendShape attend_shape(const ScoreArgs& s, int32_t dtype) {
   AttendShape h{};
-  h.half = dtype != CB_DTYPE_F32 && s.head_dim % 8 == 0 && s.head_dim <= kMaxDp && rows_aligned16(s.cache, s.head_dim * 2);
-  h.rows_per_tile = h.half ? 32 * kTileWaves : kAnyRows;
-  h.keys_per_tile = !h.half ? kAnyKeys : s.head_dim <= (s.mod ? 64 : 128) ? 64 : 32;
+  h.half = takes_half(s, dtype);
   const QBatch& B = s.batch;
+  h.step = h.half && static_cast<int64_t>(B.max_query) * s.group <= kStepRows;
+  h.rows_per_tile = h.step ? 32 : h.half ? 32 * kTileWaves : kAnyRows;
+  h.keys_per_tile = !h.half ? kAnyKeys : !h.step && s.head_dim <= (s.mod ? 64 : 128) ? 64 : 32;
   const int per_request = std::max(1, ceil_div(static_cast<int64_t>(B.max_query) * s.group, h.rows_per_tile));
   const int64_t by_request = static_cast<int64_t>(per_request) * B.requests;
   const int64_t packed = ceil_div(static_cast<int64_t>(B.tokens) * s.group, h.rows_per_tile) + static_cast<int64_t>(B.requests);
@@ -1548,10 +1887,12 @@ AttendShape attend_shape(const ScoreArgs& s, int32_t dtype) {
   if (s.window > 0 && s.causal && !s.prefix) keys = std::min<int64_t>(keys, static_cast<int64_t>(s.window) + std::min<int64_t>(B.max_query, h.rows_per_tile / s.group + 2));
   const int key_tiles = std::max(1, ceil_div(keys, h.keys_per_tile) + (s.prefix ? 1 : 0));
   const int64_t groups = static_cast<int64_t>(h.tile_slots) * s.kv_heads;
-  int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kTargetGroups / std::max<int64_t>(1, groups), key_tiles / 8)));
+  const int64_t target = h.step ? kStepGroups : kTargetGroups;
+  int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(1, groups), key_tiles / 8)));
+  if (h.step) splits = std::max(splits, ceil_div(key_tiles, kStepTiles));
   h.tiles_per_split = ceil_div(key_tiles, splits);
   h.splits = ceil_div(key_tiles, h.tiles_per_split);
-  if (h.splits == 1) h.tiles_per_split = 0x7fffffff;  // one split takes whatever there is
+  if (h.splits == 1 && !h.step) h.tiles_per_split = 0x7fffffff;  // one split takes whatever there is
   return h;
 }
 
@@ -1563,6 +1904,14 @@ int64_t attend_workspace(const ScoreArgs& s, const AttendShape& h) {
   return round256(rows * s.head_dim * 4) + round256(rows * 4);
 }
 
+template <typename IO, int KT>
+void launch_join(const AttendArgs& a, const AttendShape& h, hipStream_t st) {
+  if (h.splits <= 1) return;
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.s.batch.tokens) * a.s.q_heads));
+  if (a.s.head_dim <= 128) hipLaunchKernelGGL((join_splits_kernel<IO, KT, 32>), grid, dim3(kJoinThreads), 0, st, a, h.rows_per_tile);
+  else hipLaunchKernelGGL((join_splits_kernel<IO, KT, 128>), grid, dim3(kJoinThreads), 0, st, a, h.rows_per_tile);
+}
+
 template <typename IO, int DP>
 void launch_any(const AttendArgs& a, bool mod, unsigned grid, hipStream_t st) {
   if (mod) hipLaunchKernelGGL((attend_any_kernel<IO, DP, true>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
@@ -1571,11 +1920,10 @@ void launch_any(const AttendArgs& a, bool mod, unsigned grid, hipStream_t st) {
 template <typename IO, int DP, int KT, bool MOD>
 void launch_half(const AttendArgs& a, const AttendShape& h, unsigned grid, hipStream_t st) {
   const int vector = aligned16(a.s.q) && aligned16(a.out);
-  hipLaunchKernelGGL((attend_tile_kernel<IO, DP, KT, kTileWaves, MOD>), dim3(grid), dim3(kTileWaves * kWave), 0, st, a, vector);
-  if (h.splits > 1) {
-    const unsigned joins = static_cast<unsigned>((static_cast<int64_t>(a.s.batch.tokens) * a.s.q_heads + 3) / 4);
-    hipLaunchKernelGGL((join_splits_kernel<IO, KT>), dim3(joins), dim3(256), 0, st, a, h.rows_per_tile);
-  }
+  if (h.step) hipLaunchKernelGGL((attend_step_kernel<IO, DP, kStepWaves, MOD>), dim3(grid), dim3(kStepWaves * kWave), 0, st, a, vector);
+  else hipLaunchKernelGGL((attend_tile_kernel<IO, DP, KT, kTileWaves, MOD>), dim3(grid), dim3(kTileWaves * kWave), 0, st, a, vector);
+  if (h.step) launch_join<IO, 32>(a, h, st);
+  else launch_join<IO, KT>(a, h, st);
 }
 template <typename IO>
 void launch_attend(const AttendArgs& a, const AttendShape& h, bool mod, unsigned grid, hipStream_t st) {
@@ -1598,10 +1946,7 @@ void launch_attend(const AttendArgs& a, const AttendShape& h, bool mod, unsigned
   else if (d <= 128) launch_any<IO, 128>(a, mod, grid, st);
   else if (d <= 256) launch_any<IO, 256>(a, mod, grid, st);
   else launch_any<IO, 512>(a, mod, grid, st);
-  if (h.splits > 1) {
-    const unsigned joins = static_cast<unsigned>((static_cast<int64_t>(a.s.batch.tokens) * a.s.q_heads + 3) / 4);
-    hipLaunchKernelGGL((join_splits_kernel<IO, kAnyKeys>), dim3(joins), dim3(256), 0, st, a, h.rows_per_tile);
-  }
+  launch_join<IO, kAnyKeys>(a, h, st);
 }
 
 template <typename IO, int DP>
@@ -1609,9 +1954,23 @@ void launch_weights_any(const WeightArgs& a, bool mod, unsigned grid, hipStream_
   if (mod) hipLaunchKernelGGL((key_weights_any_kernel<IO, DP, true>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
   else hipLaunchKernelGGL((key_weights_any_kernel<IO, DP, false>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
 }
+template <typename IO, int DP>
+void launch_weights_half(const WeightArgs& a, bool mod, unsigned grid, hipStream_t st) {
+  const int vector = aligned16(a.s.q);
+  if (mod) hipLaunchKernelGGL((key_weights_kernel<IO, DP, true>), dim3(grid), dim3(kWeightWaves * kWave), 0, st, a, vector);
+  else hipLaunchKernelGGL((key_weights_kernel<IO, DP, false>), dim3(grid), dim3(kWeightWaves * kWave), 0, st, a, vector);
+}
 template <typename IO>
 void launch_weights(const WeightArgs& a, bool mod, unsigned grid, hipStream_t st) {
   const int d = a.s.head_dim;
+  if constexpr (sizeof(IO) == 2) {
+    if (a.waves_per_block) {
+      if (d <= 64) launch_weights_half<IO, 64>(a, mod, grid, st);
+      else if (d <= 128) launch_weights_half<IO, 128>(a, mod, grid, st);
+      else launch_weights_half<IO, 256>(a, mod, grid, st);
+      return;
+    }
+  }
   if (d <= 64) launch_weights_any<IO, 64>(a, mod, grid, st);
   else if (d <= 128) launch_weights_any<IO, 128>(a, mod, grid, st);
   else if (d <= 256) launch_weights_any<IO, 256>(a, mod, grid, st);
@@ -1709,7 +2068,7 @@ int cb_paged_attention(const cb_query_batch* batch, int32_t layer, int32_t dtype
                                           round256(static_cast<int64_t>(h.splits) * n * q->heads * head_dim * 4));
   }
   const int64_t grid = static_cast<int64_t>(h.tile_slots) * h.splits * a.s.kv_heads;
-  if (grid > 0x7fffffff) return fail(CB_EINVAL, "too many query tiles");
+  if (grid > 0x7fffffff || static_cast<int64_t>(n) * q->heads > 0x7fffffff) return fail(CB_EINVAL, "too many query tiles");
   const bool mod = a.s.mod;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == CB_DTYPE_BF16) launch_attend<io_bf16>(a, h, mod, static_cast<unsigned>(grid), st);
@@ -1734,7 +2093,13 @@ int cb_add_key_weights(const cb_query_batch* batch, int32_t layer, int32_t dtype
   a.lse = lse;
   a.weights = weights;
   a.weights_stride = weights_stride;
-  a.key_slots = ceil_div(batch->max_length, 16);
+  int keys = 16;
+  if (takes_half(a.s, dtype)) {
+    const int64_t blocks = static_cast<int64_t>(a.s.kv_heads) * ceil_div(static_cast<int64_t>(batch->max_query) * a.s.group, 32);
+    a.waves_per_block = blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
+    keys = 32 * (kWeightWaves / a.waves_per_block);
+  }
+  a.key_slots = ceil_div(batch->max_length, keys);
   const int64_t grid = static_cast<int64_t>(a.key_slots) * batch->num_requests;
   if (grid > 0x7fffffff) return fail(CB_EINVAL, "too many cached tokens");
   const bool mod = a.s.mod;
