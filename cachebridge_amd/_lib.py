@@ -218,7 +218,7 @@ SIGNATURES = {
     "cb_evict_tokens": (
         ctypes.c_int,
         [ctypes.POINTER(CbQueryBatch), ctypes.POINTER(CbQueryBatch), _i32, _i32, _c_void_p, _i64, _i32, _i32,
-         _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
+         _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     ),
 }
 

@@ -1507,7 +1507,7 @@ __global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 2 : 4) void key_w
     const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
     float lse = a.lse[static_cast<int64_t>(r.q0 + i) * s.q_heads + qh];
     // Nothing is added by lanes past the last row and rows that see nothing.
-    lse = (row >= high) | (lse == kNegInf) ? INFINITY : lse;
+    lse = ((row >= high) | (lse == kNegInf)) ? INFINITY : lse;
     float slope = 0;
     if constexpr (MOD) slope = s.slopes ? s.slopes[qh] : 0.0f;
     f32x16 st;
@@ -1573,8 +1573,15 @@ struct EvictArgs {
   int32_t* kept;
   int32_t* kept_lengths;
   float* kept_weights;
-  int2* rows;  // [requests][budget] source and target row of each kept token, -1 for none
 };
+
+// The request's cached tokens, or -1 if it is outside the batch's bounds.
+__device__ inline int evict_length(const EvictArgs& a, int b) {
+  Request r;
+  place_request(a.batch, b, r);
+  const int length = a.batch.lengths[b];
+  return (r.ok & (length >= 0) & (length <= a.batch.max_length)) ? length : -1;
+}
 
 constexpr int kSelectWaves = 16;
 constexpr int kSelectThreads = kSelectWaves * kWave;
@@ -1586,163 +1593,203 @@ __device__ inline uint32_t rank_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__device__ inline void keep_token(const EvictArgs& a, int b, const Request& src, const Request& dst, int at, int j, float w) {
-  const int64_t slot = static_cast<int64_t>(b) * a.budget + at;
-  a.kept[slot] = j;
-  a.kept_weights[slot] = w;
-  const int64_t from = cache_row(a.batch, src, j);
-  const int64_t to = dst.ok ? cache_row(a.target, dst, at) : -1;
-  if (from < 0) flag(a.batch.err, CB_ERROR_CACHE_ROW);
-  if (to < 0) flag(a.batch.err, CB_ERROR_TARGET_ROW);
-  a.rows[slot] = from >= 0 && to >= 0 ? make_int2(static_cast<int>(from), static_cast<int>(to)) : make_int2(-1, -1);
-}
+// Bins of a digit, eight copies each: weights often share a digit (many
+// zeros, one exponent), and lanes that add to one bin take turns, so lane l
+// adds to copy l % 8 (in banks of its own) and a wave of one digit takes 8
+// turns, not 64.
+constexpr int kBins = 2048, kBinCopies = 8, kCopyStride = kBins + 8;
 
-// One workgroup per request. The weights between the first and last tokens
-// are searched for the smallest rank that is still kept, two bits a step from
-// the top: each step counts, by ballots, the ranks at or above three
-// thresholds. No atomics, so no order to depend on.
+// One workgroup per request. The smallest rank that is still kept is found
+// digit by digit from the top (11, 11 and 10 bits): a histogram of the ranks
+// that share the digits so far, then the bin in which the count from the top
+// reaches what is needed. Counts are integers, so the order of the adds does
+// not matter. R ranks a lane stay in registers (R * 1024 tokens between the
+// first and the last), R = 0 reads the weights again on every pass.
+template <int R>
 __global__ __launch_bounds__(kSelectThreads) void select_tokens_kernel(EvictArgs a) {
-  __shared__ int counts[2][3][kSelectWaves];
+  __shared__ __align__(16) int bins[kCopyStride * kBinCopies];
+  __shared__ int totals[2][kSelectWaves];
+  __shared__ int found[2];
   const int b = blockIdx.x;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  Request src, dst;
-  place_request(a.batch, b, src);
-  place_request(a.target, b, dst);
-  const int length = a.batch.lengths[b];
-  src.ok = src.ok && length >= 0 && length <= a.batch.max_length;
-  if (threadIdx.x == 0 && !src.ok) flag(a.batch.err, CB_ERROR_REQUEST);
-  const int64_t slot0 = static_cast<int64_t>(b) * a.budget;
-  if (!src.ok) {  // its outputs stay as they were; nothing is copied
-    for (int j = threadIdx.x; j < a.budget; j += kSelectThreads) a.rows[slot0 + j] = make_int2(-1, -1);
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int length = evict_length(a, b);
+  if (length < 0) {  // its outputs stay as they were; nothing is copied
+    if (threadIdx.x == 0) flag(a.batch.err, CB_ERROR_REQUEST);
     return;
   }
+  const int64_t slot0 = static_cast<int64_t>(b) * a.budget;
   const float* w = a.weights + b * a.weights_stride;
+  int32_t* kept = a.kept + slot0;
+  float* kept_weights = a.kept_weights + slot0;
   const int n = min(length, a.budget);
   if (threadIdx.x == 0) a.kept_lengths[b] = n;
   for (int j = n + threadIdx.x; j < a.budget; j += kSelectThreads) {
-    a.kept[slot0 + j] = -1;
-    a.kept_weights[slot0 + j] = 0.0f;
-    a.rows[slot0 + j] = make_int2(-1, -1);
+    kept[j] = -1;
+    kept_weights[j] = 0.0f;
   }
-  if (length <= a.budget) {
-    for (int j = threadIdx.x; j < length; j += kSelectThreads) keep_token(a, b, src, dst, j, j, w[j]);
-    return;
+  const bool choose = length > a.budget;
+  const int head = choose ? a.first : length, tail = choose ? a.last : 0;
+  for (int j = threadIdx.x; j < head; j += kSelectThreads) {
+    kept[j] = j;
+    kept_weights[j] = w[j];
   }
-  for (int j = threadIdx.x; j < a.first; j += kSelectThreads) keep_token(a, b, src, dst, j, j, w[j]);
-  for (int j = threadIdx.x; j < a.last; j += kSelectThreads)
-    keep_token(a, b, src, dst, n - a.last + j, length - a.last + j, w[length - a.last + j]);
-  const int need = n - a.first - a.last;
-  if (need == 0) return;
-  // Wave v's share of the middle: 64-token groups in order.
-  const int mid = length - a.first - a.last;
-  const int groups = (mid + kWave - 1) / kWave;
-  const int per = (groups + kSelectWaves - 1) / kSelectWaves;
-  const int g0 = wave * per, g1 = min(groups, g0 + per);
-  const float* wm = w + a.first;
-  uint32_t base = 0;  // the largest value found so far with at least `need` ranks at or above it
-  int step = 0;
-  for (int shift = 30; shift >= 0; shift -= 2, ++step) {
-    int c[3] = {0, 0, 0};
-    for (int g = g0; g < g1; ++g) {
-      const int j = g * kWave + lane;
-      const bool in = j < mid;
-      const uint32_t k = in ? rank_of(wm[j]) : 0;
+  for (int j = threadIdx.x; j < tail; j += kSelectThreads) {
+    kept[n - tail + j] = length - tail + j;
+    kept_weights[n - tail + j] = w[length - tail + j];
+  }
+  const int need = choose ? n - head - tail : 0;
+  if (need > 0) {
+    // Wave v's share of the middle: groups of 64 tokens, in order.
+    const int mid = length - head - tail;
+    const int groups = (mid + kWave - 1) / kWave;
+    const int per = (groups + kSelectWaves - 1) / kSelectWaves;
+    const int g0 = wave * per, g1 = min(groups, g0 + per);
+    const float* wm = w + head;
+    // Every rank is above 0, which stands for no token.
+    auto read = [&](int g) { return g < g1 && g * kWave + lane < mid ? rank_of(wm[g * kWave + lane]) : 0u; };
+    uint32_t k[R > 0 ? R : 1];
+    if constexpr (R > 0) {
 #pragma unroll
-      for (int u = 0; u < 3; ++u) c[u] += __popcll(__ballot(in && k >= base + (static_cast<uint32_t>(u + 1) << shift)));
+      for (int i = 0; i < R; ++i) k[i] = read(g0 + i);
     }
-    if (lane == 0)
-      for (int u = 0; u < 3; ++u) counts[step & 1][u][wave] = c[u];
+    auto each = [&](auto&& use) __attribute__((always_inline)) {
+      if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (g0 + i < g1) use(g0 + i, k[i]);
+      } else {
+        for (int g = g0; g < g1; ++g) use(g, read(g));
+      }
+    };
+    uint32_t base = 0, known = 0;
+    int left = need;
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, size = pass == 2 ? 1024 : kBins;
+      for (int x = threadIdx.x; x < kCopyStride * kBinCopies / 4; x += kSelectThreads) reinterpret_cast<int4*>(bins)[x] = make_int4(0, 0, 0, 0);
+      __syncthreads();
+      each([&](int, uint32_t r) {
+        if ((r != 0) & ((r & known) == base)) atomicAdd(bins + (lane & 7) * kCopyStride + ((r >> shift) & (size - 1)), 1);
+      });
+      __syncthreads();
+      // Thread x holds the x-th pair of bins from the top.
+      const int hi = size - 1 - 2 * static_cast<int>(threadIdx.x);
+      int c1 = 0, c0 = 0;
+      if (hi > 0) {
+#pragma unroll
+        for (int x = 0; x < kBinCopies; ++x) {
+          c1 += bins[x * kCopyStride + hi];
+          c0 += bins[x * kCopyStride + hi - 1];
+        }
+      }
+      int sum = c1 + c0;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const int up = __shfl_up(sum, d);
+        sum += lane >= d ? up : 0;
+      }
+      if (lane == kWave - 1) totals[0][wave] = sum;
+      __syncthreads();
+      int before = sum - c1 - c0;
+#pragma unroll
+      for (int v = 0; v < kSelectWaves; ++v) before += v < wave ? totals[0][v] : 0;
+      if ((before < left) & (before + c1 + c0 >= left)) {
+        const bool upper = before + c1 >= left;
+        found[0] = upper ? hi : hi - 1;
+        found[1] = upper ? before : before + c1;
+      }
+      __syncthreads();
+      base |= static_cast<uint32_t>(found[0]) << shift;
+      known |= static_cast<uint32_t>(size - 1) << shift;
+      left -= found[1];
+    }
+    // Ranks above `base` are kept, and of those equal to it the first `left`.
+    int above = 0, equal = 0;
+    each([&](int, uint32_t r) {
+      above += __popcll(__ballot(r > base));
+      equal += __popcll(__ballot(r == base));
+    });
+    if (lane == 0) {
+      totals[0][wave] = above;
+      totals[1][wave] = equal;
+    }
     __syncthreads();
-    uint32_t up = 0;
+    int above_before = 0, equal_before = 0;
 #pragma unroll
-    for (int u = 0; u < 3; ++u) {
-      int total = 0;
-#pragma unroll
-      for (int v = 0; v < kSelectWaves; ++v) total += counts[step & 1][u][v];
-      if (total >= need) up = u + 1;
+    for (int v = 0; v < kSelectWaves; ++v) {
+      above_before += v < wave ? totals[0][v] : 0;
+      equal_before += v < wave ? totals[1][v] : 0;
     }
-    base += up << shift;
-  }
-  // Ranks above `base` are kept, and of those equal to it the first ones.
-  int above = 0, equal = 0;
-  for (int g = g0; g < g1; ++g) {
-    const int j = g * kWave + lane;
-    const bool in = j < mid;
-    const uint32_t k = in ? rank_of(wm[j]) : 0;
-    above += __popcll(__ballot(in && k > base));
-    equal += __popcll(__ballot(in && k == base));
-  }
-  __syncthreads();
-  if (lane == 0) {
-    counts[0][0][wave] = above;
-    counts[0][1][wave] = equal;
-  }
-  __syncthreads();
-  int above_before = 0, equal_before = 0, all_above = 0;
-  for (int v = 0; v < kSelectWaves; ++v) {
-    if (v < wave) {
-      above_before += counts[0][0][v];
-      equal_before += counts[0][1][v];
-    }
-    all_above += counts[0][0][v];
-  }
-  const int ties = need - all_above;
-  const uint64_t below = (uint64_t{1} << lane) - 1;
-  for (int g = g0; g < g1; ++g) {
-    const int j = g * kWave + lane;
-    const bool in = j < mid;
-    const float x = in ? wm[j] : 0.0f;
-    const uint32_t k = rank_of(x);
-    const uint64_t ma = __ballot(in && k > base), me = __ballot(in && k == base);
-    const int ea = equal_before + __popcll(me & below);
-    const bool keep = in && (k > base || (k == base && ea < ties));
-    const int at = a.first + above_before + __popcll(ma & below) + min(ea, ties);
-    if (keep) keep_token(a, b, src, dst, at, a.first + j, x);
-    above_before += __popcll(ma);
-    equal_before += __popcll(me);
+    const uint64_t below = (uint64_t{1} << lane) - 1;
+    each([&](int g, uint32_t r) {
+      const uint64_t ma = __ballot(r > base), me = __ballot(r == base);
+      const int ea = equal_before + __popcll(me & below);
+      const int at = head + above_before + __popcll(ma & below) + min(ea, left);
+      if ((r > base) | ((r == base) & (ea < left))) {
+        const int j = g * kWave + lane;
+        kept[at] = head + j;
+        kept_weights[at] = wm[j];
+      }
+      above_before += __popcll(ma);
+      equal_before += __popcll(me);
+    });
   }
 }
 
 struct MoveArgs {
+  EvictArgs e;
   DevRows src, dst;
-  const int2* rows;
-  int64_t count;
   int32_t chunks_per_row;
   int32_t tokens_per_block;
+  int32_t blocks_per_request;
 };
 
-// Every layer's K and V rows of the kept tokens; a thread keeps four chunks in
-// flight, as copy_rows_kernel.
+// Every layer's K and V rows of the kept tokens. A workgroup moves a run of
+// one request's tokens in one layer; each thread resolves the rows of four
+// chunks, then has the four loads in flight, then stores.
 template <typename V>
 __global__ __launch_bounds__(256) void move_rows_kernel(MoveArgs a) {
   constexpr int U = 4;
+  const EvictArgs& e = a.e;
   const int layer = blockIdx.y >> 1, kind = blockIdx.y & 1;
+  const int b = blockIdx.x / a.blocks_per_request, at0 = (blockIdx.x - b * a.blocks_per_request) * a.tokens_per_block;
+  const int n = min(evict_length(e, b), e.budget);
+  if (at0 >= n) return;
+  Request src, dst;
+  place_request(e.batch, b, src);
+  place_request(e.target, b, dst);
+  const int32_t* kept = e.kept + static_cast<int64_t>(b) * e.budget;
   gcptr sbase = layer_base(a.src, kind, layer);
   gptr dbase = const_cast<gptr>(layer_base(a.dst, kind, layer));
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens_per_block;
-  const int total = static_cast<int>(min(static_cast<int64_t>(a.tokens_per_block), a.count - t0)) * a.chunks_per_row;
+  const int total = min(a.tokens_per_block, n - at0) * a.chunks_per_row;
   for (int base = threadIdx.x; base < total; base += blockDim.x * U) {
-    int64_t so[U], to[U];
+    int64_t from[U], to[U];
+    int at[U], chunk[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int idx = base + u * blockDim.x;
-      so[u] = to[u] = -1;
-      if (idx < total) {
-        const int2 rw = a.rows[t0 + idx / a.chunks_per_row];
-        const int64_t off = (idx % a.chunks_per_row) * static_cast<int>(sizeof(V));
-        if (rw.x >= 0) {
-          so[u] = rw.x * a.src.row_stride_b + off;
-          to[u] = rw.y * a.dst.row_stride_b + off;
-        }
-      }
+      const int idx = min(base + u * static_cast<int>(blockDim.x), total - 1);
+      at[u] = at0 + idx / a.chunks_per_row;
+      chunk[u] = idx % a.chunks_per_row;
+      from[u] = kept[at[u]];
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      from[u] = cache_row(e.batch, src, static_cast<int>(from[u]));
+      to[u] = dst.ok ? cache_row(e.target, dst, at[u]) : -1;
+    }
+    bool ok[U];
     V v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (so[u] >= 0) v[u] = gload<V>(sbase + so[u]);
+    for (int u = 0; u < U; ++u) {
+      const bool in = base + u * static_cast<int>(blockDim.x) < total;
+      if (in & (chunk[u] == 0) & (blockIdx.y == 0) & ((from[u] < 0) | (to[u] < 0)))
+        flag(e.batch.err, (from[u] < 0 ? CB_ERROR_CACHE_ROW : 0) | (to[u] < 0 ? CB_ERROR_TARGET_ROW : 0));
+      ok[u] = in & (from[u] >= 0) & (to[u] >= 0);
+      if (ok[u]) v[u] = gload<V>(sbase + from[u] * a.src.row_stride_b + chunk[u] * static_cast<int>(sizeof(V)));
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (to[u] >= 0) gstore<V>(dbase + to[u], v[u]);
+      if (ok[u]) gstore<V>(dbase + to[u] * a.dst.row_stride_b + chunk[u] * static_cast<int>(sizeof(V)), v[u]);
   }
 }
 
@@ -2113,8 +2160,7 @@ int cb_add_key_weights(const cb_query_batch* batch, int32_t layer, int32_t dtype
 
 int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, int32_t dtype, int32_t head_dim,
                     const float* weights, int64_t weights_stride, int32_t budget, int32_t first, int32_t last,
-                    int32_t* kept, int32_t* kept_lengths, float* kept_weights, void* d_workspace,
-                    int64_t workspace_bytes, int32_t* d_error_flag, void* stream) {
+                    int32_t* kept, int32_t* kept_lengths, float* kept_weights, int32_t* d_error_flag, void* stream) {
   EvictArgs a{};
   MoveArgs m{};
   int rc;
@@ -2130,9 +2176,6 @@ int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, i
   if (weights_stride < batch->max_length) return fail(CB_EINVAL, "weights rows are shorter than max_length");
   if (batch->num_requests == 0) return CB_OK;
   if ((!weights && batch->max_length > 0) || !kept || !kept_lengths || !kept_weights) return fail(CB_EINVAL, "null weights or kept");
-  const int64_t slots = static_cast<int64_t>(batch->num_requests) * budget;
-  if (!d_workspace || workspace_bytes < slots * 8 || reinterpret_cast<uintptr_t>(d_workspace) % 8)
-    return fail(CB_EINVAL, "eviction needs an 8-byte aligned workspace of %lld bytes", static_cast<long long>(slots * 8));
   const int eb = elem_bytes(dtype);
   const int64_t row_bytes = static_cast<int64_t>(batch->cache.heads) * head_dim * eb;
   if (row_bytes > (1 << 24)) return fail(CB_EINVAL, "rows above 16 MB");
@@ -2144,17 +2187,20 @@ int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, i
   a.kept = kept;
   a.kept_lengths = kept_lengths;
   a.kept_weights = kept_weights;
-  a.rows = static_cast<int2*>(d_workspace);
   const bool wide = row_bytes % 16 == 0 && rows_aligned16(m.src, 16) && rows_aligned16(m.dst, 16);
   const int chunk = wide ? 16 : eb;
-  m.rows = a.rows;
-  m.count = slots;
+  m.e = a;
   m.chunks_per_row = static_cast<int32_t>(row_bytes / chunk);
   m.tokens_per_block = std::max(1, 1024 / m.chunks_per_row);
-  const int64_t blocks = (slots + m.tokens_per_block - 1) / m.tokens_per_block;
+  m.blocks_per_request = ceil_div(std::min(budget, std::max(batch->max_length, 1)), m.tokens_per_block);
+  const int64_t blocks = static_cast<int64_t>(m.blocks_per_request) * batch->num_requests;
   if (blocks > 0x7fffffff || batch->cache.num_layers > 32767) return fail(CB_EINVAL, "eviction too large");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(select_tokens_kernel, dim3(static_cast<unsigned>(batch->num_requests)), dim3(kSelectThreads), 0, st, a);
+  const dim3 requests(static_cast<unsigned>(batch->num_requests));
+  const int64_t middle = static_cast<int64_t>(batch->max_length) - first - last;
+  if (middle <= 16 * kSelectThreads) hipLaunchKernelGGL(select_tokens_kernel<16>, requests, dim3(kSelectThreads), 0, st, a);
+  else if (middle <= 64 * kSelectThreads) hipLaunchKernelGGL(select_tokens_kernel<64>, requests, dim3(kSelectThreads), 0, st, a);
+  else hipLaunchKernelGGL(select_tokens_kernel<0>, requests, dim3(kSelectThreads), 0, st, a);
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(2 * batch->cache.num_layers));
   if (wide) hipLaunchKernelGGL(move_rows_kernel<uint4>, grid, dim3(256), 0, st, m);
   else if (eb == 4) hipLaunchKernelGGL(move_rows_kernel<uint32_t>, grid, dim3(256), 0, st, m);

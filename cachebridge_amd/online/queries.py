@@ -337,11 +337,9 @@ def evict_tokens(batch: QueryBatch, weights: torch.Tensor, target: QueryBatch, *
         kept = KeptTokens(torch.empty((b, budget), dtype=torch.int32, device=dev),
                           torch.empty(b, dtype=torch.int32, device=dev),
                           torch.empty((b, budget), dtype=torch.float32, device=dev))
-        work = torch.empty((b, budget), dtype=torch.int64, device=dev)
         _lib.check(_lib.load().cb_evict_tokens(
             batch._tokens(0), target._tokens(0), batch._code, dim, weights.data_ptr(), stride, budget, first, last,
-            kept.tokens.data_ptr(), kept.lengths.data_ptr(), kept.weights.data_ptr(), work.data_ptr(), 8 * b * budget,
-            flag, handle))
+            kept.tokens.data_ptr(), kept.lengths.data_ptr(), kept.weights.data_ptr(), flag, handle))
         batch.rows.hold_for(stream)
         target.rows.hold_for(stream)
     return kept

@@ -402,13 +402,11 @@ int cb_add_key_weights(const cb_query_batch* batch, int32_t layer, int32_t dtype
    kept [requests][budget] gets the cached token of each, then -1;
    kept_lengths [requests] their count; kept_weights [requests][budget] their
    weights, then 0. Of `target` the cache, index, offsets and request_stride
-   are read. d_workspace is 8 * num_requests * budget bytes of device memory.
-   Asynchronous. */
+   are read. Asynchronous. */
 int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, int32_t dtype,
                     int32_t head_dim, const float* weights, int64_t weights_stride, int32_t budget,
                     int32_t first, int32_t last, int32_t* kept, int32_t* kept_lengths,
-                    float* kept_weights, void* d_workspace, int64_t workspace_bytes,
-                    int32_t* d_error_flag, void* stream);
+                    float* kept_weights, int32_t* d_error_flag, void* stream);
 
 #ifdef __cplusplus
 }

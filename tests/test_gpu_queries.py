@@ -401,8 +401,8 @@ def test_evict_row_sizes(dtype, kv_heads, dim):
     _evict_case([120, 77], 50, 4, 4, w, dtype=dtype, kv_heads=kv_heads, dim=dim)
 
 
-def test_evict_long_history():
-    n = 70001
+@pytest.mark.parametrize("n", [17000, 66000, 70001])
+def test_evict_long_history(n):
     w = torch.rand(1, n, generator=torch.Generator().manual_seed(8))
     _evict_case([n], 5000, 4, 64, w, kv_heads=1, dim=8, layers=1)
 

@@ -128,15 +128,14 @@ def test_install_refusals(lib, kw, text):
     refused(lib, install(lib, **kw), text)
 
 
-def evict(lib, b=None, t=None, budget=10, first=1, last=1, stride=100, work=FAKE, n=1 << 20, kept=FAKE):
+def evict(lib, b=None, t=None, budget=10, first=1, last=1, stride=100, kept=FAKE):
     return lib.cb_evict_tokens(ref(batch() if b is None else b), ref(batch() if t is None else t), 0, 128, FAKE, stride,
-                               budget, first, last, kept, FAKE, FAKE, work, n, None, None)
+                               budget, first, last, kept, FAKE, FAKE, None, None)
 
 
 @pytest.mark.parametrize("kw,text", [
     (dict(budget=0), "budget"), (dict(first=6, last=5), "within the budget"), (dict(first=-1), "within the budget"),
-    (dict(stride=99), "max_length"), (dict(work=None), "workspace"), (dict(n=8 * 3 * 10 - 1), "workspace"),
-    (dict(work=FAKE + 4), "workspace"), (dict(kept=None), "null"), (dict(t=batch(num_requests=2)), "requests"),
+    (dict(stride=99), "max_length"), (dict(kept=None), "null"), (dict(t=batch(num_requests=2)), "requests"),
     (dict(t=batch(heads=1, row_stride=256)), "layers or KV heads"), (dict(t=batch(num_layers=1)), "layers or KV heads"),
 ])
 def test_evict_refusals(lib, kw, text):
