@@ -25,6 +25,7 @@ namespace {
 
 typedef __bf16 io_bf16;
 typedef _Float16 io_f16;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -456,6 +457,28 @@ __device__ inline float natural_score(const ScoreArgs& s, float dot, float slope
   return x;
 }
 
+// Raw products of one lane (16 keys of a block that starts at cached token
+// `start`, register e: key 8 (e / 4) + 4 h + e % 4) to scores times `unit`.
+// tanh y = 1 - 2 / (exp(2y) + 1) costs two transcendental operations and holds
+// for either sign; its error, 2^-22 of the cap, is far below the rounding that
+// 16-bit weights get.
+__device__ inline void modify_scores(const ScoreArgs& s, f32x16& x, float unit, float slope, int p, int start, int h) {
+  if (s.cap > 0) {
+    const float in = 2.0f * kLog2e * s.scale / s.cap, out = s.cap * unit;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = __builtin_fmaf(-2.0f * out, __builtin_amdgcn_rcpf(exp2_fast(x[e] * in) + 1.0f), out);
+  } else {
+    const float by = s.scale * unit;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] *= by;
+  }
+  if (s.slopes) {
+    const float by = slope * unit, away = static_cast<float>(p - start - 4 * h);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = __builtin_fmaf(-by, fabsf(away - static_cast<float>(8 * (e >> 2) + (e & 3))), x[e]);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // General attention: any even head_dim up to 512, any type, fp32 products
 // (16x16x4 MFMA: lane l holds A[l % 16][l / 16] and B[l / 16][l % 16], its
@@ -480,10 +503,10 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(Attend
   const int c = lane & 15, g = lane >> 4;
   const int head = blockIdx.x % s.kv_heads;
   const int rest = blockIdx.x / s.kv_heads;
-  const int split = rest % a.splits;
+  const int split = rest / a.tile_slots;
   Request r;
   int b, tile;
-  if (!find_tile(a, rest / a.splits, kAnyRows, r, b, tile)) return;
+  if (!find_tile(a, rest % a.tile_slots, kAnyRows, r, b, tile)) return;
   const int rows = r.n * s.group;
   const int row0 = tile * kAnyRows, row1 = min(rows, row0 + kAnyRows) - 1;
   const KeyRange kr = key_range<KT>(s, r, b, row0, row1);
@@ -698,7 +721,6 @@ __global__ __launch_bounds__(kJoinThreads) void join_splits_kernel(AttendArgs a,
 // one chunk; V: 4 rows of 4 chunks).
 // ---------------------------------------------------------------------------
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -766,70 +788,83 @@ __device__ inline void wait_own() {
   asm volatile("" ::: "memory");
 }
 
-// One lane's part of staging tiles of KT keys: N DMA instructions for K and as
-// many for V, instruction u of this wave covering bytes [(first + u) * 1024,
-// + 1024) of a tile. Index entries are fetched a tile ahead of the rows they
-// name, rows a tile ahead of the products.
+// A tile's pool rows in LDS: one wave resolves them, a key a lane, so that the
+// waves that stage the tile only look them up.
+template <int KT>
+struct TileRows {
+  int row[4][KT];            // pool row of each key of tile t in slot t % 4, 0 where there is none
+  uint32_t valid[4][KT / 32];  // keys that are there
+};
+
+// The index word that names key `lane` of a tile, loaded a tile before it is
+// needed (identity: the row itself; -1 past the end).
+template <int KT>
+__device__ inline int64_t fetch_entry(const QBatch& B, const Request& r, int start, int end) {
+  const int j = start + (threadIdx.x & (kWave - 1));
+  int64_t e = r.first + j;
+  if (B.kind == CB_INDEX_IDENTITY) return j < end ? e : -1;
+  if (B.kind == CB_INDEX_BLOCK_TABLE) {
+    const uint32_t x = r.rem + static_cast<uint32_t>(j);
+    e = r.first + (B.page_shift >= 0 ? x >> B.page_shift : x / static_cast<uint32_t>(B.page_size));
+  }
+  const bool in = (j < end) & (e < B.entries);
+  if (B.entries <= 0) return -1;
+  const int64_t at = in ? e : 0;
+  const int64_t got = B.kind == CB_INDEX_I64 ? reinterpret_cast<const CB_GLOBAL int64_t*>(as_global(B.index))[at]
+                                             : reinterpret_cast<const CB_GLOBAL int32_t*>(as_global(B.index))[at];
+  return in ? got : -1;
+}
+
+template <int KT>
+__device__ inline void place_rows(const QBatch& B, const Request& r, int64_t entry, int start, int end, TileRows<KT>& rows, int slot) {
+  const int lane = threadIdx.x & (kWave - 1), j = start + lane;
+  int64_t row = entry;
+  if (B.kind == CB_INDEX_BLOCK_TABLE) {
+    const uint32_t x = r.rem + static_cast<uint32_t>(j), ps = static_cast<uint32_t>(B.page_size);
+    row = row < 0 ? -1 : row * ps + (B.page_shift >= 0 ? x & (ps - 1) : x % ps);
+  }
+  const bool ok = (row >= 0) & (row < B.rows) & (lane < KT) & (j < end);
+  if (__any(!ok & (j < end) & (lane < KT))) flag(B.err, CB_ERROR_CACHE_ROW);
+  if (lane < KT) rows.row[slot][lane] = ok ? static_cast<int>(row) : 0;
+  const uint64_t valid = __ballot(ok);
+  if (lane < KT / 32) rows.valid[slot][lane] = static_cast<uint32_t>(valid >> (32 * lane));
+}
+
+// One wave's part of a tile's DMA: N instructions for K and as many for V,
+// number u covering bytes [(first + u) * 1024, + 1024) of a tile.
 template <typename IO, int DP, int KT, int N>
 struct Stager {
   static constexpr int C = DP / 8;  // 16-byte chunks a row
-  int64_t entry[N];                 // what the index holds (identity: the row)
-  gcptr kbase, vbase;
-
-  __device__ inline int key(int first, int u) const { return (first + u) * (kWave / C) + (threadIdx.x & (kWave - 1)) / C; }
+  gcptr kbase;                      // K of the head, layer and tile chunk 0
+  int64_t to_v;                     // from K to V
+  uint32_t stride;
 
   __device__ inline void init(const ScoreArgs& s, int head) {
     const int64_t off = static_cast<int64_t>(head) * s.head_dim * 2;
     kbase = layer_base(s.cache, 0, s.layer) + off;
-    vbase = layer_base(s.cache, 1, s.layer) + off;
+    to_v = layer_base(s.cache, 1, s.layer) + off - kbase;
+    stride = static_cast<uint32_t>(s.batch.row_stride_b);
   }
-  __device__ inline void fetch(const QBatch& B, const Request& r, int first, int start, int end) {
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int j = start + key(first, u);
-      int64_t e = r.first + j;
-      if (B.kind == CB_INDEX_IDENTITY) {
-        entry[u] = j < end ? e : -1;
-        continue;
-      }
-      if (B.kind == CB_INDEX_BLOCK_TABLE) {
-        const uint32_t x = r.rem + static_cast<uint32_t>(j);
-        e = r.first + (B.page_shift >= 0 ? x >> B.page_shift : x / static_cast<uint32_t>(B.page_size));
-      }
-      const bool in = (j < end) & (e < B.entries);
-      const int64_t at = in ? e : 0;
-      if (B.entries <= 0) entry[u] = -1;
-      else if (B.kind == CB_INDEX_I64) entry[u] = reinterpret_cast<const CB_GLOBAL int64_t*>(as_global(B.index))[at];
-      else entry[u] = reinterpret_cast<const CB_GLOBAL int32_t*>(as_global(B.index))[at];
-      entry[u] = in ? entry[u] : -1;
-    }
-  }
-  // Issues the DMA of the tile whose entries were fetched. Returns the lanes'
-  // keys below `end` that have no row (a wave's ballots, per instruction).
-  __device__ inline void issue(const ScoreArgs& s, const Request& r, int first, int start, int end, uint32_t lk, uint32_t lv,
-                               uint32_t* bad) {
-    const QBatch& B = s.batch;
+  __device__ __attribute__((always_inline)) inline void issue(const ScoreArgs& s, const TileRows<KT>& rows, int slot, int first,
+                                                              uint32_t lk, uint32_t lv) const {
     const int lane = threadIdx.x & (kWave - 1), pos = lane % C;
+    uint32_t whole = ~0u;
+#pragma unroll
+    for (int k = 0; k < KT / 32; ++k) whole &= rows.valid[slot][k];
+    const bool plain = (__builtin_amdgcn_readfirstlane(whole) == ~0u) & (s.head_dim == DP);
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int k = key(first, u), j = start + k;
-      int64_t row = entry[u];
-      if (B.kind == CB_INDEX_BLOCK_TABLE) {
-        const uint32_t x = r.rem + static_cast<uint32_t>(j), ps = static_cast<uint32_t>(B.page_size);
-        const uint32_t in_page = B.page_shift >= 0 ? x & (ps - 1) : x % ps;
-        row = row < 0 ? -1 : row * ps + in_page;
-      }
-      const bool ok = (row >= 0) & (row < B.rows);
-      if (__any(!ok & (j < end))) {
-        if (!ok & (j < end) & (pos == 0)) {
-          flag(B.err, CB_ERROR_CACHE_ROW);
-          atomicOr(bad + (k >> 5), 1u << (k & 31));
-        }
-      }
+      const int k = (first + u) * (kWave / C) + lane / C;
       const int ck = pos ^ swizzle_k<DP>(k), cv = pos ^ swizzle_v<DP>(k);
-      gcptr zero = as_global(static_cast<const void*>(g_zeros));
-      gcptr ka = (ok & (ck * 8 < s.head_dim)) ? kbase + row * B.row_stride_b + ck * 16 : zero;
-      gcptr va = (ok & (cv * 8 < s.head_dim)) ? vbase + row * B.row_stride_b + cv * 16 : zero;
+      const uint32_t row = static_cast<uint32_t>(rows.row[slot][k]);
+      const gcptr at = kbase + static_cast<uint64_t>(row) * stride;
+      gcptr ka = at + ck * 16, va = at + to_v + cv * 16;
+      if (!plain) {
+        const bool ok = (rows.valid[slot][k >> 5] >> (k & 31)) & 1;
+        gcptr zero = as_global(static_cast<const void*>(g_zeros));
+        ka = (ok & (ck * 8 < s.head_dim)) ? ka : zero;
+        va = (ok & (cv * 8 < s.head_dim)) ? va : zero;
+      }
       dma16(ka, lk + (first + u) * 1024);
       dma16(va, lv + (first + u) * 1024);
     }
@@ -925,28 +960,24 @@ struct RowBlock {
   }
 
   // Their weights, of the tile that starts at cached token `start`. `whole`:
-  // every row sees every key. `bad`: keys without a row, 32 a word.
+  // every row sees every key. `valid`: keys that are there, 32 a word.
   __device__ __attribute__((always_inline)) void weigh(const ScoreArgs& s, const KeyRange& kr, f32x16 (&st)[KB], int start,
-                                                       int end, bool whole, const uint32_t* bad, float scale2,
-                                                       u32x4 (&w)[KB][2]) {
+                                                       bool whole, const uint32_t* valid, float scale2, u32x4 (&w)[KB][2]) {
     const int h = (threadIdx.x & (kWave - 1)) >> 5;
     // Scores times scale2 are in the log2 domain (MOD: scale2 is 1 and they
     // are put there at once).
     if constexpr (MOD) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          st[kb][e] = natural_score<true>(s, st[kb][e], slope, p, start + 32 * kb + 8 * (e >> 2) + 4 * h + (e & 3)) * kLog2e;
+      for (int kb = 0; kb < KB; ++kb) modify_scores(s, st[kb], kLog2e, slope, p, start + 32 * kb, h);
     }
     if (!whole) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        const uint32_t gone = bad[kb];
+        const uint32_t there = valid[kb] >> (4 * h);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int k = 8 * (e >> 2) + 4 * h + (e & 3), j = start + 32 * kb + k;
-          const bool in = (j < end) & sees(s, kr, p, j) & !((gone >> k) & 1);
+          const int k = 8 * (e >> 2) + (e & 3), j = start + 32 * kb + 4 * h + k;
+          const bool in = sees(s, kr, p, j) & ((there >> k) & 1);
           st[kb][e] = in ? st[kb][e] : kNegInf;
         }
       }
@@ -1104,16 +1135,16 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_ker
   constexpr int kTile = KT * DP * 2, N = kTile / 1024 / NW;
   static_assert(N >= 1 && kTile % (1024 * NW) == 0, "a tile is whole DMA instructions of every wave");
   __shared__ __align__(1024) char tiles[4 * kTile];  // K, V of one buffer, K, V of the other
-  __shared__ uint32_t bad[3][KT / 32];
+  __shared__ TileRows<KT> tile_rows;
   __shared__ uint32_t marks[2][NW][32 * (DP / 32)];
   __shared__ uint32_t odd[2];  // this tile holds values that are not finite; some tile did
   const ScoreArgs& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int head = blockIdx.x % s.kv_heads, rest = blockIdx.x / s.kv_heads;
-  const int split = rest % a.splits;
+  const int split = rest / a.tile_slots;
   Request r;
   int b, tile;
-  if (!find_tile(a, rest / a.splits, 32 * NW, r, b, tile)) return;
+  if (!find_tile(a, rest % a.tile_slots, 32 * NW, r, b, tile)) return;
   const int rows = r.n * s.group, row0 = tile * 32 * NW;
   const KeyRange kr = key_range<KT>(s, r, b, row0, min(rows, row0 + 32 * NW) - 1);
   const int t0 = split * a.tiles_per_split, t1 = a.splits > 1 ? min(kr.tiles, t0 + a.tiles_per_split) : kr.tiles;
@@ -1128,33 +1159,38 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_ker
   Stager<IO, DP, KT, N> stage;
   stage.init(s, head);
   const int first = wave * N;
-  if (threadIdx.x < 3 * (KT / 32)) (&bad[0][0])[threadIdx.x] = 0;
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
   for (int w = threadIdx.x; w < 2 * NW * DP; w += NW * kWave) (&marks[0][0][0])[w] = 0;
-  __syncthreads();
-  if (t0 < t1) {
-    stage.fetch(s.batch, r, first, tile_start<KT>(kr, t0), tile_end(kr, t0));
-    stage.issue(s, r, first, tile_start<KT>(kr, t0), tile_end(kr, t0), lds, lds + kTile, bad[0]);
-    if (t0 + 1 < t1) stage.fetch(s.batch, r, first, tile_start<KT>(kr, t0 + 1), tile_end(kr, t0 + 1));
+  auto entry_of = [&](int t) { return t < t1 ? fetch_entry<KT>(s.batch, r, tile_start<KT>(kr, t), tile_end(kr, t)) : -1; };
+  auto place = [&](int64_t entry, int t) {
+    if (t < t1) place_rows<KT>(s.batch, r, entry, tile_start<KT>(kr, t), tile_end(kr, t), tile_rows, t & 3);
+  };
+  int64_t entry = -1;
+  if (wave == 0) {
+    const int64_t e0 = entry_of(t0), e1 = entry_of(t0 + 1);
+    entry = entry_of(t0 + 2);
+    place(e0, t0);
+    place(e1, t0 + 1);
   }
+  __syncthreads();
+  if (t0 < t1) stage.issue(s, tile_rows, t0 & 3, first, lds, lds + kTile);
   uint32_t buf = 0;
-  int slot = 0;
   for (int t = t0; t < t1; ++t) {
     wait_and_meet();
-    const int next = slot == 2 ? 0 : slot + 1;
-    if (threadIdx.x < KT / 32) bad[next == 2 ? 0 : next + 1][threadIdx.x] = 0;
     if (t + 1 < t1) {
-      const int start = tile_start<KT>(kr, t + 1), end = tile_end(kr, t + 1);
       const uint32_t to = lds + (buf ^ (2 * kTile));
-      stage.issue(s, r, first, start, end, to, to + kTile, bad[next]);
-      if (t + 2 < t1) stage.fetch(s.batch, r, first, tile_start<KT>(kr, t + 2), tile_end(kr, t + 2));
+      stage.issue(s, tile_rows, (t + 1) & 3, first, to, to + kTile);
+      if (wave == 0) {
+        place(entry, t + 2);
+        entry = entry_of(t + 3);
+      }
     }
     const int start = tile_start<KT>(kr, t), end = tile_end(kr, t);
-    uint32_t gone[KT / 32], some = 0;
+    uint32_t valid[KT / 32], every = ~0u;
 #pragma unroll
-    for (int k = 0; k < KT / 32; ++k) some |= gone[k] = bad[slot][k];
+    for (int k = 0; k < KT / 32; ++k) every &= valid[k] = tile_rows.valid[t & 3][k];
     const bool all = sees_all(s, kr, start, min(end, start + KT));
-    const bool whole = all && __builtin_amdgcn_readfirstlane(some) == 0 && start + KT <= end;
+    const bool whole = all && __builtin_amdgcn_readfirstlane(every) == ~0u;
     if (!all) {
       const uint32_t lv = lds + buf + kTile + (threadIdx.x & (kWave - 1)) * 16;
       bool strange = false;
@@ -1178,10 +1214,9 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_ker
     f32x16 st[KT / 32];
     u32x4 w[KT / 32][2];
     blk.products(lanes, lds + buf, st);
-    blk.weigh(s, kr, st, start, end, whole, gone, scale2, w);
+    blk.weigh(s, kr, st, start, whole, valid, scale2, w);
     blk.add_values(lanes, lds + buf + kTile, w);
     buf ^= 2 * kTile;
-    slot = next;
   }
   __syncthreads();
   if (odd[1]) blk.add_marks(marks[0][wave], marks[1][wave]);
@@ -1211,10 +1246,10 @@ __global__ __launch_bounds__(NW * kWave, 1) void attend_step_kernel(AttendArgs a
   const QBatch& B = s.batch;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int head = blockIdx.x % s.kv_heads, rest = blockIdx.x / s.kv_heads;
-  const int split = rest % a.splits;
+  const int split = rest / a.tile_slots;
   Request r;
   int b, tile;
-  if (!find_tile(a, rest / a.splits, 32, r, b, tile)) return;
+  if (!find_tile(a, rest % a.tile_slots, 32, r, b, tile)) return;
   const int rows = r.n * s.group, row0 = tile * 32;
   const KeyRange kr = key_range<KT>(s, r, b, row0, min(rows, row0 + 32) - 1);
   const int t0 = split * a.tiles_per_split, t1 = min(kr.tiles, t0 + min(a.tiles_per_split, kStepTiles));
@@ -1265,7 +1300,7 @@ __global__ __launch_bounds__(NW * kWave, 1) void attend_step_kernel(AttendArgs a
   uint32_t buf = 0;
   for (int i = 0; i < n; ++i) {
     const int t = t0 + wave + i * NW, start = tile_start<KT>(kr, t), end = tile_end(kr, t);
-    const uint32_t gone = static_cast<uint32_t>(__ballot(key_rows[(t - t0) * KT + (lane & 31)] < 0));
+    const uint32_t valid = static_cast<uint32_t>(__ballot(key_rows[(t - t0) * KT + (lane & 31)] >= 0));
     if (i + 1 < n) __builtin_amdgcn_s_waitcnt(wait_vm(3 * N));
     else __builtin_amdgcn_s_waitcnt(wait_vm(N));
     asm volatile("" ::: "memory");
@@ -1277,7 +1312,7 @@ __global__ __launch_bounds__(NW * kWave, 1) void attend_step_kernel(AttendArgs a
       request(i + 2, kbase, lds + buf, false);
     }
     const bool all = sees_all(s, kr, start, min(end, start + KT));
-    blk.weigh(s, kr, st, start, end, all & (gone == 0), &gone, scale2, w);
+    blk.weigh(s, kr, st, start, all & (valid == ~0u), &valid, scale2, w);
     if (i + 2 < n) __builtin_amdgcn_s_waitcnt(wait_vm(3 * N));
     else if (i + 1 < n) __builtin_amdgcn_s_waitcnt(wait_vm(2 * N));
     else __builtin_amdgcn_s_waitcnt(wait_vm(0));
@@ -1531,11 +1566,12 @@ __global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 2 : 4) void key_w
     kr.p0 = r.length - r.n + row0 / s.group;
     kr.p1 = r.length - r.n + min(row0 + 31, high - 1) / s.group;
     const bool whole = sees_all(s, kr, start, start + 32);
+    if constexpr (MOD) modify_scores(s, st, 1.0f, slope, p, start, h);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int key = start + 8 * (e >> 2) + 4 * h + (e & 3);
       // The difference first: what is near the row's maximum keeps its bits.
-      const float w = exp2_fast((natural_score<MOD>(s, st[e], slope, p, key) - lse) * kLog2e);
+      const float w = exp2_fast((MOD ? st[e] - lse : __builtin_fmaf(st[e], s.scale, -lse)) * kLog2e);
       sum[e] += (whole | sees(s, kr, p, key)) ? w : 0.0f;
     }
   }
@@ -1910,7 +1946,7 @@ struct AttendShape {
 
 // Whether the 16-bit kernels take the call: whole 16-byte chunks of rows.
 bool takes_half(const ScoreArgs& s, int32_t dtype) {
-  return dtype != CB_DTYPE_F32 && s.head_dim % 8 == 0 && s.head_dim <= kMaxDp && rows_aligned16(s.cache, s.head_dim * 2);
+  return dtype != CB_DTYPE_F32 && s.head_dim % 8 == 0 && s.cache.row_stride_b <= 0xffffffffll && s.head_dim <= kMaxDp && rows_aligned16(s.cache, s.head_dim * 2);
 }
 
 constexpr int kTileWaves = 4;
