@@ -27,6 +27,10 @@ typedef __bf16 io_bf16;
 typedef _Float16 io_f16;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// Helpers that take a request or a key range by reference are always inlined: a
+// call would put the struct, and what the caller keeps, into scratch memory.
+#define CB_INLINE __device__ __attribute__((always_inline)) inline
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -INFINITY;
@@ -64,12 +68,12 @@ struct Request {
   bool ok;
 };
 
-__device__ inline void flag(int32_t* err, int bits) {
+CB_INLINE void flag(int32_t* err, int bits) {
   if (err) atomicOr(err, bits);
 }
 
 // The request's index position alone (eviction: no new tokens involved).
-__device__ inline void place_request(const QBatch& B, int b, Request& r) {
+CB_INLINE void place_request(const QBatch& B, int b, Request& r) {
   const int64_t start = (B.offsets ? B.offsets[b] : b * B.request_stride);
   r.ok = start >= 0 && start <= (int64_t{1} << 61);
   const int64_t u = r.ok ? start + B.index_offset : 0;
@@ -81,7 +85,7 @@ __device__ inline void place_request(const QBatch& B, int b, Request& r) {
   }
 }
 
-__device__ inline Request load_request(const QBatch& B, int b) {
+CB_INLINE Request load_request(const QBatch& B, int b) {
   Request r;
   place_request(B, b, r);
   const int64_t q0 = B.query_start[b], q1 = B.query_start[b + 1];
@@ -97,7 +101,7 @@ __device__ inline Request load_request(const QBatch& B, int b) {
 // Pool row of cached token j, or -1 where its index entry or the row it names
 // is out of range. The arithmetic within a request is 32 bits wide (at most
 // 2^30 tokens); the request's own start is 64.
-__device__ inline int64_t cache_row(const QBatch& B, const Request& r, int j) {
+CB_INLINE int64_t cache_row(const QBatch& B, const Request& r, int j) {
   int64_t row;
   if (B.kind == CB_INDEX_BLOCK_TABLE) {
     const uint32_t x = r.rem + static_cast<uint32_t>(j);
@@ -122,7 +126,7 @@ __device__ inline int64_t cache_row(const QBatch& B, const Request& r, int j) {
 
 // The request that token row t belongs to, or `requests` if none does: a wave
 // counts the requests that end at or before t, 64 at a time.
-__device__ inline int request_of_token(const QBatch& B, int t) {
+CB_INLINE int request_of_token(const QBatch& B, int t) {
   const int lane = threadIdx.x & (kWave - 1);
   int b = 0;
   for (int i = 0; i < B.requests; i += kWave) {
@@ -355,7 +359,7 @@ struct AttendArgs {
 // Tile `i` of the launch: its request, and which of the request's tiles (the
 // last first: under a causal mask it has the most keys). Returns false if
 // there is none.
-__device__ inline bool find_tile(const AttendArgs& a, int i, int rows_per_tile, Request& r, int& b, int& tile) {
+CB_INLINE bool find_tile(const AttendArgs& a, int i, int rows_per_tile, Request& r, int& b, int& tile) {
   const QBatch& B = a.s.batch;
   const int G = a.s.group;
   if (a.request_slots > 0) {
@@ -406,7 +410,7 @@ struct KeyRange {
 };
 
 template <int KT>
-__device__ inline KeyRange key_range(const ScoreArgs& s, const Request& r, int b, int row0, int row1) {
+CB_INLINE KeyRange key_range(const ScoreArgs& s, const Request& r, int b, int row0, int row1) {
   KeyRange k;
   k.np = s.prefix ? max(0, min(s.prefix[b], r.length)) : 0;
   k.p0 = r.length - r.n + row0 / s.group;
@@ -423,38 +427,34 @@ __device__ inline KeyRange key_range(const ScoreArgs& s, const Request& r, int b
 }
 
 template <int KT>
-__device__ inline int tile_start(const KeyRange& k, int t) {
+CB_INLINE int tile_start(const KeyRange& k, int t) {
   return t < k.ta ? t * KT : k.lb + (t - k.ta) * KT;
 }
-__device__ inline int tile_end(const KeyRange& k, int t) { return t < k.ta ? k.na : k.hb; }
+CB_INLINE int tile_end(const KeyRange& k, int t) { return t < k.ta ? k.na : k.hb; }
 
 // Whether every row of the tile sees every key of [start, stop).
-__device__ inline bool sees_all(const ScoreArgs& s, const KeyRange& k, int start, int stop) {
+CB_INLINE bool sees_all(const ScoreArgs& s, const KeyRange& k, int start, int stop) {
   if (stop <= k.np) return true;
   return (!s.causal || stop <= k.p0 + 1) && (s.window == 0 || start > k.p1 - s.window);
 }
 
 // Without branches (bitwise operators): lanes differ in p and j.
-__device__ inline bool sees(const ScoreArgs& s, const KeyRange& k, int p, int j) {
+CB_INLINE bool sees(const ScoreArgs& s, const KeyRange& k, int p, int j) {
   const int above = s.window > 0 ? p - s.window : -1, below = s.causal ? p : 0x7fffffff;
   return (j < k.np) | ((j <= below) & (j > above));
 }
 
 // cap * tanh(x / cap), tanh y = (1 - e) / (1 + e) with e = exp(-2|y|).
-__device__ inline float capped(float x, float cap) {
+CB_INLINE float capped(float x, float cap) {
   const float e = exp2_fast(-2.0f * kLog2e * fabsf(x) / cap);
   return copysignf(cap * (1.0f - e) / (1.0f + e), x);
 }
 
 // A raw product's score, in natural units.
-template <bool MOD>
-__device__ inline float natural_score(const ScoreArgs& s, float dot, float slope, int p, int j) {
+CB_INLINE float natural_score(const ScoreArgs& s, float dot, float slope, int p, int j) {
   float x = dot * s.scale;
-  if constexpr (MOD) {
-    if (s.cap > 0) x = capped(x, s.cap);
-    x -= slope * fabsf(static_cast<float>(p - j));
-  }
-  return x;
+  if (s.cap > 0) x = capped(x, s.cap);
+  return x - slope * fabsf(static_cast<float>(p - j));
 }
 
 // Raw products of one lane (16 keys of a block that starts at cached token
@@ -462,7 +462,7 @@ __device__ inline float natural_score(const ScoreArgs& s, float dot, float slope
 // tanh y = 1 - 2 / (exp(2y) + 1) costs two transcendental operations and holds
 // for either sign; its error, 2^-22 of the cap, is far below the rounding that
 // 16-bit weights get.
-__device__ inline void modify_scores(const ScoreArgs& s, f32x16& x, float unit, float slope, int p, int start, int h) {
+CB_INLINE void modify_scores(const ScoreArgs& s, f32x16& x, float unit, float slope, int p, int start, int h) {
   if (s.cap > 0) {
     const float in = 2.0f * kLog2e * s.scale / s.cap, out = s.cap * unit;
 #pragma unroll
@@ -480,10 +480,59 @@ __device__ inline void modify_scores(const ScoreArgs& s, f32x16& x, float unit, 
 }
 
 // ---------------------------------------------------------------------------
+// Rows of a tile's keys
+// ---------------------------------------------------------------------------
+
+// A tile's pool rows in LDS: one wave resolves them, a key a lane, so that the
+// waves that stage the tile only look them up.
+template <int KT>
+struct TileRows {
+  int row[4][KT];            // pool row of each key of tile t in slot t % 4, 0 where there is none
+  uint32_t valid[4][(KT + 31) / 32];  // keys that are there
+};
+
+// The index word that names key `lane` of a tile, loaded a tile before it is
+// needed (identity: the row itself; -1 past the end).
+template <int KT>
+CB_INLINE int64_t fetch_entry(const QBatch& B, const Request& r, int start, int end) {
+  const int j = start + (threadIdx.x & (kWave - 1));
+  int64_t e = r.first + j;
+  if (B.kind == CB_INDEX_IDENTITY) return j < end ? e : -1;
+  if (B.kind == CB_INDEX_BLOCK_TABLE) {
+    const uint32_t x = r.rem + static_cast<uint32_t>(j);
+    e = r.first + (B.page_shift >= 0 ? x >> B.page_shift : x / static_cast<uint32_t>(B.page_size));
+  }
+  const bool in = (j < end) & (e < B.entries);
+  if (B.entries <= 0) return -1;
+  const int64_t at = in ? e : 0;
+  const int64_t got = B.kind == CB_INDEX_I64 ? reinterpret_cast<const CB_GLOBAL int64_t*>(as_global(B.index))[at]
+                                             : reinterpret_cast<const CB_GLOBAL int32_t*>(as_global(B.index))[at];
+  return in ? got : -1;
+}
+
+template <int KT>
+CB_INLINE void place_rows(const QBatch& B, const Request& r, int64_t entry, int start, int end, TileRows<KT>& rows, int slot) {
+  const int lane = threadIdx.x & (kWave - 1), j = start + lane;
+  int64_t row = entry;
+  if (B.kind == CB_INDEX_BLOCK_TABLE) {
+    const uint32_t x = r.rem + static_cast<uint32_t>(j), ps = static_cast<uint32_t>(B.page_size);
+    row = row < 0 ? -1 : row * ps + (B.page_shift >= 0 ? x & (ps - 1) : x % ps);
+  }
+  const bool ok = (row >= 0) & (row < B.rows) & (lane < KT) & (j < end);
+  if (__any(!ok & (j < end) & (lane < KT))) flag(B.err, CB_ERROR_CACHE_ROW);
+  if (lane < KT) rows.row[slot][lane] = ok ? static_cast<int>(row) : 0;
+  const uint64_t valid = __ballot(ok);
+  if (lane < (KT + 31) / 32) rows.valid[slot][lane] = static_cast<uint32_t>(valid >> (32 * lane));
+}
+
+// ---------------------------------------------------------------------------
 // General attention: any even head_dim up to 512, any type, fp32 products
 // (16x16x4 MFMA: lane l holds A[l % 16][l / 16] and B[l / 16][l % 16], its
 // result rows 4 (l / 16) + e of column l % 16). A workgroup's four waves share
-// tiles of 16 keys in LDS, 16 query rows each.
+// tiles of 16 keys in LDS, 16 query rows each; the next tile's elements are
+// loaded into registers (VE at a time: 16 bytes where rows allow it, else one)
+// while a tile is used. Rows in LDS are DP + 4 floats apart, which puts the 16
+// rows and 4 columns of an operand in distinct banks.
 // ---------------------------------------------------------------------------
 
 constexpr int kAnyWaves = 4;
@@ -494,12 +543,20 @@ __device__ inline f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdg
 
 __device__ inline bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
 
-template <typename IO, int DP, bool MOD>
+template <typename IO, int DP, int VE>
 __global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(AttendArgs a) {
-  constexpr int KT = kAnyKeys, LD = DP + 4, NB = DP / 16;
-  __shared__ float lk[KT * LD], lv[KT * LD];
+  constexpr int KT = kAnyKeys, LD = DP + 4, NB = DP / 16, NT = kAnyWaves * kWave, MW = DP / 32;
+  // A 512-element row's sums and queries fill the registers: no tile waits there.
+  constexpr bool AHEAD = DP <= 256;
+  constexpr int NC = AHEAD ? (KT * DP / VE + NT - 1) / NT : 1;
+  typedef IO vec __attribute__((ext_vector_type(VE)));
+  __shared__ __align__(16) float lk[KT * LD];
+  __shared__ __align__(16) float lv[KT * LD];
+  __shared__ TileRows<KT> tile_rows;
+  __shared__ uint32_t marks[2][kAnyRows * MW];
+  __shared__ uint32_t odd[2];
   const ScoreArgs& s = a.s;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = lane & 15, g = lane >> 4;
   const int head = blockIdx.x % s.kv_heads;
   const int rest = blockIdx.x / s.kv_heads;
@@ -510,13 +567,29 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(Attend
   const int rows = r.n * s.group;
   const int row0 = tile * kAnyRows, row1 = min(rows, row0 + kAnyRows) - 1;
   const KeyRange kr = key_range<KT>(s, r, b, row0, row1);
-  const int t0 = split * a.tiles_per_split, t1 = min(kr.tiles, t0 + a.tiles_per_split);
+  const int t0 = split * a.tiles_per_split, t1 = a.splits > 1 ? min(kr.tiles, t0 + a.tiles_per_split) : kr.tiles;
   if (a.splits > 1 && t0 >= t1) return;
+
+  auto entry_of = [&](int t) { return t < t1 ? fetch_entry<KT>(s.batch, r, tile_start<KT>(kr, t), tile_end(kr, t)) : -1; };
+  auto place = [&](int64_t entry, int t) {
+    if (t < t1) place_rows<KT>(s.batch, r, entry, tile_start<KT>(kr, t), tile_end(kr, t), tile_rows, t & 3);
+  };
+  int64_t entry = -1;
+  if (wave == 0) {
+    const int64_t e0 = entry_of(t0), e1 = entry_of(t0 + 1);
+    entry = entry_of(t0 + 2);
+    place(e0, t0);
+    place(e1, t0 + 1);
+  }
+  // Elements past head_dim are zeros for good: no tile writes them.
+  for (int x = threadIdx.x; x < KT * LD; x += NT) lk[x] = lv[x] = 0.0f;
+  for (int x = threadIdx.x; x < 2 * kAnyRows * MW; x += NT) (&marks[0][0])[x] = 0;
+  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
 
   const int row = row0 + 16 * wave + c;  // this lane's query row
   const bool live = row < rows;
   const int i = min(row, rows - 1) / s.group;
-  const int qh = head * s.group + min(row, rows - 1) % s.group;
+  const int qh = head * s.group + min(row, rows - 1) - i * s.group;
   const int p = r.length - r.n + i;
   const int D = s.head_dim;
   const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
@@ -524,47 +597,119 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(Attend
 #pragma unroll
   for (int e = 0; e < DP / 4; ++e)
     q[e] = 4 * e + g < D ? to_f32(load_elem<IO>(qp + (4 * e + g) * static_cast<int>(sizeof(IO)))) : 0.0f;
-  float slope = 0;
-  if constexpr (MOD) slope = s.slopes ? s.slopes[qh] : 0.0f;
+  const float slope = s.slopes ? s.slopes[qh] : 0.0f;
 
-  const char* kbase = (const char*)layer_base(s.cache, 0, s.layer) + static_cast<int64_t>(head) * D * sizeof(IO);
-  const char* vbase = (const char*)layer_base(s.cache, 1, s.layer) + static_cast<int64_t>(head) * D * sizeof(IO);
+  gcptr kbase = layer_base(s.cache, 0, s.layer) + static_cast<int64_t>(head) * D * sizeof(IO);
+  gcptr vbase = layer_base(s.cache, 1, s.layer) + static_cast<int64_t>(head) * D * sizeof(IO);
+  const int per_row = D / VE;
+  int key_of[NC], elem_of[NC];  // this thread's chunks of a tile
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int x = n * NT + threadIdx.x;
+    key_of[n] = x / per_row;
+    elem_of[n] = (x - key_of[n] * per_row) * VE;
+  }
+  vec rk[NC], rv[NC];
+  auto load = [&](int t) __attribute__((always_inline)) {
+    if constexpr (!AHEAD) return;
+    const uint32_t valid = tile_rows.valid[t & 3][0];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const bool in = (key_of[n] < KT) && ((valid >> key_of[n]) & 1);
+      rk[n] = rv[n] = vec(static_cast<IO>(0.0f));
+      if (in) {
+        const int64_t off = static_cast<int64_t>(tile_rows.row[t & 3][key_of[n]]) * s.batch.row_stride_b + elem_of[n] * static_cast<int>(sizeof(IO));
+        rk[n] = gload<vec>(kbase + off);
+        rv[n] = gload<vec>(vbase + off);
+      }
+    }
+  };
+  auto store = [&](int t) __attribute__((always_inline)) {
+    if constexpr (!AHEAD) {
+      const uint32_t valid = tile_rows.valid[t & 3][0];
+#pragma unroll 1
+      for (int k = wave; k < KT; k += kAnyWaves) {
+        const bool in = (valid >> k) & 1;
+        const int64_t off = static_cast<int64_t>(tile_rows.row[t & 3][k]) * s.batch.row_stride_b;
+#pragma unroll 2
+        for (int d = lane; d < D; d += kWave) {
+          lk[k * LD + d] = in ? static_cast<float>(gload<IO>(kbase + off + d * static_cast<int>(sizeof(IO)))) : 0.0f;
+          lv[k * LD + d] = in ? static_cast<float>(gload<IO>(vbase + off + d * static_cast<int>(sizeof(IO)))) : 0.0f;
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+      if (key_of[n] < KT) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          lk[key_of[n] * LD + elem_of[n] + e] = static_cast<float>(rk[n][e]);
+          lv[key_of[n] * LD + elem_of[n] + e] = static_cast<float>(rv[n][e]);
+        }
+      }
+  };
   f32x4 o[NB];
 #pragma unroll
   for (int d = 0; d < NB; ++d) o[d] = f32x4{0, 0, 0, 0};
   float m = kNegInf, l = 0;
+  __syncthreads();
+  if (t0 < t1) load(t0);
   for (int t = t0; t < t1; ++t) {
     const int start = tile_start<KT>(kr, t), end = tile_end(kr, t);
     __syncthreads();
-    bool missing = false;
-#pragma unroll
-    for (int u = 0; u < KT / kAnyWaves; ++u) {
-      const int key = wave * (KT / kAnyWaves) + u, j = start + key;
-      const int64_t kvrow = j < end ? cache_row(s.batch, r, j) : -1;
-      if (j < end && kvrow < 0) {
-        missing = true;
-        if (lane == 0) flag(s.batch.err, CB_ERROR_CACHE_ROW);
+    store(t);
+    if (t + 1 < t1) {
+      load(t + 1);
+      if (wave == 0) {
+        place(entry, t + 2);
+        entry = entry_of(t + 3);
       }
-      for (int d = lane; d < DP; d += kWave) {
-        const bool in = kvrow >= 0 && d < D;
-        const int64_t off = kvrow * s.cache.row_stride_b + d * static_cast<int>(sizeof(IO));
-        lk[key * LD + d] = in ? to_f32(load_elem<IO>(kbase + off)) : 0.0f;
-        lv[key * LD + d] = in ? to_f32(load_elem<IO>(vbase + off)) : 0.0f;
-      }
-      if (lane == 0) lk[key * LD + DP] = kvrow >= 0 ? 1.0f : 0.0f;  // whether the key has a row
     }
-    const bool any_missing = __syncthreads_or(missing);
-    f32x4 st = {0, 0, 0, 0};
+    const uint32_t valid = tile_rows.valid[t & 3][0];
+    const bool all = sees_all(s, kr, start, min(end, start + KT)), whole = all && valid == 0xffffu;
+    __syncthreads();
+    if (!all) {
+      // Values that are not finite leave the tile, noted for the rows that see
+      // them (as in the 16-bit kernels).
+      bool strange = false;
+      for (int x = threadIdx.x; x < KT * LD; x += NT) strange |= not_finite(lv[x]);
+      if (strange) odd[0] = odd[1] = 1;
+      __syncthreads();
+      if (odd[0]) {
+        for (int x = lane; x < 16 * D; x += kWave) {
+          const int y = x / D, d = x - y * D, at = row0 + 16 * wave + y;
+          if (at >= rows) break;
+          const int mine = r.length - r.n + at / s.group;
+          bool up = false, down = false;
+          for (int k = 0; k < KT; ++k) {
+            const float v = lv[k * LD + d];
+            const bool seen = sees(s, kr, mine, start + k) & ((valid >> k) & 1);
+            up |= seen & ((v != v) | (v == INFINITY));
+            down |= seen & ((v != v) | (v == kNegInf));
+          }
+          if (up) atomicOr(&marks[0][(16 * wave + y) * MW + (d >> 5)], 1u << (d & 31));
+          if (down) atomicOr(&marks[1][(16 * wave + y) * MW + (d >> 5)], 1u << (d & 31));
+        }
+        __syncthreads();
+        for (int x = threadIdx.x; x < KT * LD; x += NT) lv[x] = not_finite(lv[x]) ? 0.0f : lv[x];
+        if (threadIdx.x == 0) odd[0] = 0;
+        __syncthreads();
+      }
+    }
+    f32x4 st = {0, 0, 0, 0}, st2 = {0, 0, 0, 0};
 #pragma unroll
-    for (int e = 0; e < DP / 4; ++e) st = mfma4(lk[c * LD + 4 * e + g], q[e], st);
-    const bool whole = !any_missing && start + KT <= end && sees_all(s, kr, start, start + KT);
+    for (int e = 0; e < DP / 4; e += 2) {
+      st = mfma4(lk[c * LD + 4 * e + g], q[e], st);
+      st2 = mfma4(lk[c * LD + 4 * e + 4 + g], q[e + 1], st2);
+    }
     float x[4], top = kNegInf;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int j = start + 4 * g + e;
-      x[e] = natural_score<MOD>(s, st[e], slope, p, j) * kLog2e;
-      const bool in = whole | ((j < end) & sees(s, kr, p, j) & (lk[(4 * g + e) * LD + DP] != 0.0f));
-      x[e] = in ? x[e] : kNegInf;
+      const int k = 4 * g + e;
+      const float y = natural_score(s, st[e] + st2[e], slope, p, start + k) * kLog2e;
+      const bool in = whole | (sees(s, kr, p, start + k) & ((valid >> k) & 1));
+      x[e] = in ? y : kNegInf;
       top = fmaxf(top, x[e]);
     }
     top = fmaxf(top, __shfl_xor(top, 16));
@@ -584,24 +729,19 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(Attend
     for (int d = 0; d < NB; ++d) {
       o[d] *= alpha;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float v = lv[(4 * g + e) * LD + 16 * d + c];
-        if (!whole && __any(not_finite(v))) {
-          // Zero weights times infinities would be NaN in rows that do not
-          // see them: such values go in by what they do to a sum instead.
-          const float vis = pr[e] != 0.0f ? 1.0f : 0.0f;
-          const bool nan = v != v;
-          const f32x4 z = {0, 0, 0, 0};
-          const f32x4 up = mfma4(nan || v == INFINITY ? 1.0f : 0.0f, vis, z);
-          const f32x4 dn = mfma4(nan || v == kNegInf ? 1.0f : 0.0f, vis, z);
+      for (int e = 0; e < 4; ++e) o[d] = mfma4(lv[(4 * g + e) * LD + 16 * d + c], pr[e], o[d]);
+    }
+  }
+  __syncthreads();
+  if (odd[1]) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            if (up[w] > 0) o[d][w] += INFINITY;
-            if (dn[w] > 0) o[d][w] += kNegInf;
-          }
-          v = not_finite(v) ? 0.0f : v;
-        }
-        o[d] = mfma4(v, pr[e], o[d]);
+    for (int d = 0; d < NB; ++d) {
+      const int at = (16 * wave + c) * MW + (d >> 1);
+      const uint32_t up = marks[0][at] >> (16 * (d & 1) + 4 * g), down = marks[1][at] >> (16 * (d & 1) + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[d][e] += (up >> e) & 1 ? INFINITY : 0.0f;
+        o[d][e] += (down >> e) & 1 ? kNegInf : 0.0f;
       }
     }
   }
@@ -788,48 +928,6 @@ __device__ inline void wait_own() {
   asm volatile("" ::: "memory");
 }
 
-// A tile's pool rows in LDS: one wave resolves them, a key a lane, so that the
-// waves that stage the tile only look them up.
-template <int KT>
-struct TileRows {
-  int row[4][KT];            // pool row of each key of tile t in slot t % 4, 0 where there is none
-  uint32_t valid[4][KT / 32];  // keys that are there
-};
-
-// The index word that names key `lane` of a tile, loaded a tile before it is
-// needed (identity: the row itself; -1 past the end).
-template <int KT>
-__device__ inline int64_t fetch_entry(const QBatch& B, const Request& r, int start, int end) {
-  const int j = start + (threadIdx.x & (kWave - 1));
-  int64_t e = r.first + j;
-  if (B.kind == CB_INDEX_IDENTITY) return j < end ? e : -1;
-  if (B.kind == CB_INDEX_BLOCK_TABLE) {
-    const uint32_t x = r.rem + static_cast<uint32_t>(j);
-    e = r.first + (B.page_shift >= 0 ? x >> B.page_shift : x / static_cast<uint32_t>(B.page_size));
-  }
-  const bool in = (j < end) & (e < B.entries);
-  if (B.entries <= 0) return -1;
-  const int64_t at = in ? e : 0;
-  const int64_t got = B.kind == CB_INDEX_I64 ? reinterpret_cast<const CB_GLOBAL int64_t*>(as_global(B.index))[at]
-                                             : reinterpret_cast<const CB_GLOBAL int32_t*>(as_global(B.index))[at];
-  return in ? got : -1;
-}
-
-template <int KT>
-__device__ inline void place_rows(const QBatch& B, const Request& r, int64_t entry, int start, int end, TileRows<KT>& rows, int slot) {
-  const int lane = threadIdx.x & (kWave - 1), j = start + lane;
-  int64_t row = entry;
-  if (B.kind == CB_INDEX_BLOCK_TABLE) {
-    const uint32_t x = r.rem + static_cast<uint32_t>(j), ps = static_cast<uint32_t>(B.page_size);
-    row = row < 0 ? -1 : row * ps + (B.page_shift >= 0 ? x & (ps - 1) : x % ps);
-  }
-  const bool ok = (row >= 0) & (row < B.rows) & (lane < KT) & (j < end);
-  if (__any(!ok & (j < end) & (lane < KT))) flag(B.err, CB_ERROR_CACHE_ROW);
-  if (lane < KT) rows.row[slot][lane] = ok ? static_cast<int>(row) : 0;
-  const uint64_t valid = __ballot(ok);
-  if (lane < KT / 32) rows.valid[slot][lane] = static_cast<uint32_t>(valid >> (32 * lane));
-}
-
 // One wave's part of a tile's DMA: N instructions for K and as many for V,
 // number u covering bytes [(first + u) * 1024, + 1024) of a tile.
 template <typename IO, int DP, int KT, int N>
@@ -845,7 +943,7 @@ struct Stager {
     to_v = layer_base(s.cache, 1, s.layer) + off - kbase;
     stride = static_cast<uint32_t>(s.batch.row_stride_b);
   }
-  __device__ __attribute__((always_inline)) inline void issue(const ScoreArgs& s, const TileRows<KT>& rows, int slot, int first,
+  CB_INLINE void issue(const ScoreArgs& s, const TileRows<KT>& rows, int slot, int first,
                                                               uint32_t lk, uint32_t lv) const {
     const int lane = threadIdx.x & (kWave - 1), pos = lane % C;
     uint32_t whole = ~0u;
@@ -947,7 +1045,7 @@ struct RowBlock {
   }
 
   // Raw products of the rows with a tile of KT keys.
-  __device__ __attribute__((always_inline)) void products(const Lanes& a, uint32_t lk, f32x16 (&st)[KB]) {
+  CB_INLINE void products(const Lanes& a, uint32_t lk, f32x16 (&st)[KB]) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       f32x16 z;
@@ -961,7 +1059,7 @@ struct RowBlock {
 
   // Their weights, of the tile that starts at cached token `start`. `whole`:
   // every row sees every key. `valid`: keys that are there, 32 a word.
-  __device__ __attribute__((always_inline)) void weigh(const ScoreArgs& s, const KeyRange& kr, f32x16 (&st)[KB], int start,
+  CB_INLINE void weigh(const ScoreArgs& s, const KeyRange& kr, f32x16 (&st)[KB], int start,
                                                        bool whole, const uint32_t* valid, float scale2, u32x4 (&w)[KB][2]) {
     const int h = (threadIdx.x & (kWave - 1)) >> 5;
     // Scores times scale2 are in the log2 domain (MOD: scale2 is 1 and they
@@ -1011,7 +1109,7 @@ struct RowBlock {
       }
   }
 
-  __device__ __attribute__((always_inline)) void add_values(const Lanes& a, uint32_t lv, const u32x4 (&w)[KB][2]) {
+  CB_INLINE void add_values(const Lanes& a, uint32_t lv, const u32x4 (&w)[KB][2]) {
 #pragma unroll
     for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
@@ -1092,7 +1190,7 @@ __device__ inline bool has_not_finite(u32x4 x) {
 // One wave notes, for its 32 rows (marks [32][DP / 32], lane l < 32 owns row
 // l's words), every such value of the V tile at lv.
 template <typename IO, int DP, int KT>
-__device__ __attribute__((always_inline)) inline void mark_not_finite(uint32_t lv, int np, int below, int above, int start, int end,
+CB_INLINE void mark_not_finite(uint32_t lv, int np, int below, int above, int start, int end,
                                                           CB_LDS_SPACE uint32_t* up, CB_LDS_SPACE uint32_t* down) {
   constexpr int C = DP / 8;
   const int lane = threadIdx.x & (kWave - 1);
@@ -1413,7 +1511,7 @@ struct WeightArgs {
 
 // The new tokens of a request that may see any of the cached tokens
 // [start, start + keys): all below a prefix, else those between.
-__device__ inline void query_range(const ScoreArgs& s, const Request& r, int np, int start, int keys, int* i0, int* i1) {
+CB_INLINE void query_range(const ScoreArgs& s, const Request& r, int np, int start, int keys, int* i0, int* i1) {
   *i0 = 0;
   *i1 = r.n;
   if (start < np) return;
@@ -1425,7 +1523,7 @@ __device__ inline void query_range(const ScoreArgs& s, const Request& r, int np,
 // General form: a workgroup owns 16 keys of a request, its waves take every
 // fourth block of 16 query rows of each KV head; partial sums meet in LDS in
 // wave order.
-template <typename IO, int DP, bool MOD>
+template <typename IO, int DP>
 __global__ __launch_bounds__(kAnyWaves * kWave, 1) void key_weights_any_kernel(WeightArgs a) {
   __shared__ float sums[kAnyWaves][16];
   const ScoreArgs& s = a.s;
@@ -1460,14 +1558,13 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void key_weights_any_kernel(W
       for (int e = 0; e < DP / 4; ++e)
         st = mfma4(k[e], 4 * e + g < D ? to_f32(load_elem<IO>(qp + (4 * e + g) * static_cast<int>(sizeof(IO)))) : 0.0f, st);
       const float lse = a.lse[static_cast<int64_t>(r.q0 + i) * s.q_heads + qh];
-      float slope = 0;
-      if constexpr (MOD) slope = s.slopes ? s.slopes[qh] : 0.0f;
+      const float slope = s.slopes ? s.slopes[qh] : 0.0f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int j = start + 4 * g + e;
         const bool in = (row0 + c < i1 * s.group) & (lse != kNegInf) & sees(s, kr, p, j);
         // The difference first: what is near the row's maximum keeps its bits.
-        const float w = exp2_fast((natural_score<MOD>(s, st[e], slope, p, j) - lse) * kLog2e);
+        const float w = exp2_fast((natural_score(s, st[e], slope, p, j) - lse) * kLog2e);
         sum[e] += in ? w : 0.0f;
       }
     }
@@ -1612,7 +1709,7 @@ struct EvictArgs {
 };
 
 // The request's cached tokens, or -1 if it is outside the batch's bounds.
-__device__ inline int evict_length(const EvictArgs& a, int b) {
+CB_INLINE int evict_length(const EvictArgs& a, int b) {
   Request r;
   place_request(a.batch, b, r);
   const int length = a.batch.lengths[b];
@@ -1971,7 +2068,7 @@ AttendShape attend_shape(const ScoreArgs& s, int32_t dtype) {
   const int key_tiles = std::max(1, ceil_div(keys, h.keys_per_tile) + (s.prefix ? 1 : 0));
   const int64_t groups = static_cast<int64_t>(h.tile_slots) * s.kv_heads;
   const int64_t target = h.step ? kStepGroups : kTargetGroups;
-  int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(1, groups), key_tiles / 8)));
+  int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(1, groups), key_tiles / (h.half ? 8 : 2))));
   if (h.step) splits = std::max(splits, ceil_div(key_tiles, kStepTiles));
   h.tiles_per_split = ceil_div(key_tiles, splits);
   h.splits = ceil_div(key_tiles, h.tiles_per_split);
@@ -1996,9 +2093,13 @@ void launch_join(const AttendArgs& a, const AttendShape& h, hipStream_t st) {
 }
 
 template <typename IO, int DP>
-void launch_any(const AttendArgs& a, bool mod, unsigned grid, hipStream_t st) {
-  if (mod) hipLaunchKernelGGL((attend_any_kernel<IO, DP, true>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
-  else hipLaunchKernelGGL((attend_any_kernel<IO, DP, false>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
+void launch_any(const AttendArgs& a, unsigned grid, hipStream_t st) {
+  constexpr int VE = 16 / sizeof(IO);
+  if constexpr (DP == 512) hipLaunchKernelGGL((attend_any_kernel<IO, DP, 1>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
+  else if (a.s.head_dim % VE == 0 && rows_aligned16(a.s.cache, a.s.head_dim * static_cast<int>(sizeof(IO))))
+    hipLaunchKernelGGL((attend_any_kernel<IO, DP, VE>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
+  else
+    hipLaunchKernelGGL((attend_any_kernel<IO, DP, 1>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
 }
 template <typename IO, int DP, int KT, bool MOD>
 void launch_half(const AttendArgs& a, const AttendShape& h, unsigned grid, hipStream_t st) {
@@ -2025,17 +2126,16 @@ void launch_attend(const AttendArgs& a, const AttendShape& h, bool mod, unsigned
       return;
     }
   }
-  if (d <= 64) launch_any<IO, 64>(a, mod, grid, st);
-  else if (d <= 128) launch_any<IO, 128>(a, mod, grid, st);
-  else if (d <= 256) launch_any<IO, 256>(a, mod, grid, st);
-  else launch_any<IO, 512>(a, mod, grid, st);
+  if (d <= 64) launch_any<IO, 64>(a, grid, st);
+  else if (d <= 128) launch_any<IO, 128>(a, grid, st);
+  else if (d <= 256) launch_any<IO, 256>(a, grid, st);
+  else launch_any<IO, 512>(a, grid, st);
   launch_join<IO, kAnyKeys>(a, h, st);
 }
 
 template <typename IO, int DP>
-void launch_weights_any(const WeightArgs& a, bool mod, unsigned grid, hipStream_t st) {
-  if (mod) hipLaunchKernelGGL((key_weights_any_kernel<IO, DP, true>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
-  else hipLaunchKernelGGL((key_weights_any_kernel<IO, DP, false>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
+void launch_weights_any(const WeightArgs& a, unsigned grid, hipStream_t st) {
+  hipLaunchKernelGGL((key_weights_any_kernel<IO, DP>), dim3(grid), dim3(kAnyWaves * kWave), 0, st, a);
 }
 template <typename IO, int DP>
 void launch_weights_half(const WeightArgs& a, bool mod, unsigned grid, hipStream_t st) {
@@ -2054,10 +2154,10 @@ void launch_weights(const WeightArgs& a, bool mod, unsigned grid, hipStream_t st
       return;
     }
   }
-  if (d <= 64) launch_weights_any<IO, 64>(a, mod, grid, st);
-  else if (d <= 128) launch_weights_any<IO, 128>(a, mod, grid, st);
-  else if (d <= 256) launch_weights_any<IO, 256>(a, mod, grid, st);
-  else launch_weights_any<IO, 512>(a, mod, grid, st);
+  if (d <= 64) launch_weights_any<IO, 64>(a, grid, st);
+  else if (d <= 128) launch_weights_any<IO, 128>(a, grid, st);
+  else if (d <= 256) launch_weights_any<IO, 256>(a, grid, st);
+  else launch_weights_any<IO, 512>(a, grid, st);
 }
 
 template <typename IO>
@@ -2105,7 +2205,7 @@ int cb_install_tokens(const cb_query_batch* batch, int32_t layer, int32_t dtype,
   const bool wide = (rotary_dim / 2) % vec == 0 && head_dim % vec == 0 && aligned16(a.q) && aligned16(a.q_out) &&
                     aligned16(a.k) && aligned16(a.v) && rows_aligned16(a.cache, head_dim * eb);
   const int items = (q->heads + kv) * (head_dim - rotary_dim / 2) / (wide ? vec : 1) + kv * head_dim / (wide ? vec : 1);
-  a.slices = std::max(1, std::min(64, items / (4 * kWave)));
+  a.slices = std::max(1, std::min(64, ceil_div(items, kWave)));  // an item a lane: one round of memory latency
   const int64_t grid = (static_cast<int64_t>(n) * a.slices + kInstallWaves - 1) / kInstallWaves;
   if (grid > 0x7fffffff) return fail(CB_EINVAL, "too many tokens");
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -39,32 +39,43 @@ from .. import _lib
 from ..plan import Rows, io_dtype_code
 from ..rope import rope_frequencies
 
+_raw_stream = _lib._raw_stream
+
 ERROR_CACHE_ROW = _lib.CB_ERROR_CACHE_ROW
 ERROR_TARGET_ROW = _lib.CB_ERROR_TARGET_ROW
 ERROR_REQUEST = _lib.CB_ERROR_REQUEST
 
 
 class _On:
-    """The launch's device and stream: allocations and launches inside use them."""
+    """A launch's device and stream, entered: allocations and launches inside use them.
 
-    def __init__(self, device: torch.device, stream: torch.cuda.Stream | None):
-        index = device.index if device.index is not None else torch.cuda.current_device()
-        if stream is not None and stream.device.index != index:
-            raise ValueError("stream belongs to another device than the batch")
-        self._contexts = []
+    Yields the stream's handle. With the batch's device current and no stream
+    named, which every layer of a model's step is, nothing is entered: a
+    context object would cost as much host time as the launch itself.
+    """
+
+    __slots__ = ("handle", "_context")
+
+    def __init__(self, batch: "QueryBatch", stream: torch.cuda.Stream | None):
+        index = batch.device.index
         if stream is not None:
-            self._contexts.append(torch.cuda.stream(stream))
-        elif index != torch.cuda.current_device():
-            self._contexts.append(torch.cuda.device(index))
+            if stream.device.index != index:
+                raise ValueError("stream belongs to another device than the batch")
+            self._context = torch.cuda.stream(stream)
+            self.handle = _lib.stream_handle(stream)
+            return
+        current = index == torch.cuda.current_device()
+        self._context = None if current else torch.cuda.device(index)
+        self.handle = int(torch.cuda.current_stream(index).cuda_stream) if _raw_stream is None else _raw_stream(index)
 
     def __enter__(self) -> int:
-        for c in self._contexts:
-            c.__enter__()
-        return _lib.stream_handle()
+        if self._context is not None:
+            self._context.__enter__()
+        return self.handle
 
     def __exit__(self, *exc):
-        for c in reversed(self._contexts):
-            c.__exit__(*exc)
+        if self._context is not None:
+            self._context.__exit__(*exc)
 
 
 def _device_vector(t: torch.Tensor, name: str, dtypes, device, entries: int | None) -> int:
@@ -94,10 +105,11 @@ class QueryBatch:
                  max_query: int | None = None, offsets: torch.Tensor | None = None, request_stride: int = 0):
         if rows.device.type != "cuda":
             raise ValueError("the query batch lives on a GPU device")
+        for t in rows.keep:
+            if t.ndim == 1 and not t.is_contiguous():
+                raise ValueError("pool indices must be contiguous")
         if rows.c.k_layers and any(t.data_ptr() % 16 for t in rows.keep if t.ndim == 3):
             raise ValueError("pool layers must be 16-byte aligned")
-        if any(t.ndim == 1 and not t.is_contiguous() for t in rows.keep):
-            raise ValueError("pool indices must be contiguous")
         requests = lengths.numel()
         c = _lib.CbQueryBatch()
         c.cache = rows.c
@@ -131,10 +143,11 @@ class QueryBatch:
         c.max_query = n if self.max_query is None else min(self.max_query, n)
         return ctypes.byref(c)
 
-    def _heads(self, t: torch.Tensor, name: str, tokens: int | None = None, heads: int | None = None):
-        if t.ndim != 3 or t.dtype != self.dtype or t.device != self.device:
+    def _heads(self, t: torch.Tensor, name: str, tokens: int | None = None, heads: int | None = None) -> _lib.CbHeads:
+        shape = t.shape
+        if len(shape) != 3 or t.dtype != self.dtype or t.device != self.device:
             raise ValueError(f"{name} must be [tokens, heads, head_dim] of {self.dtype} on {self.device}")
-        n, h, d = t.shape
+        n, h, d = shape
         if d != self.head_dim:
             raise ValueError(f"{name} must have the pool's head_dim {self.head_dim}")
         if (tokens is not None and n != tokens) or (heads is not None and h != heads):
@@ -194,9 +207,9 @@ def install_tokens(batch: QueryBatch, layer: int, q: torch.Tensor, k: torch.Tens
         pos = _device_vector(positions, "positions", (torch.int32, torch.int64), batch.device, n)
         kind = _lib.CB_INDEX_I64 if positions.dtype == torch.int64 else _lib.CB_INDEX_I32
     flag = _flag_pointer(batch, error_flag)
-    with _On(batch.device, stream) as handle:
+    with _On(batch, stream) as handle:
         if out is None:
-            out = torch.empty((n, heads, dim), dtype=q.dtype, device=q.device)
+            out = q.new_empty((n, heads, dim))
         co = batch._heads(out, "out", n, heads)
         _lib.check(_lib.load().cb_install_tokens(
             batch._tokens(n), layer, batch._code, dim, ctypes.byref(cq), ctypes.byref(co), ctypes.byref(ck),
@@ -244,16 +257,16 @@ def paged_attention(batch: QueryBatch, layer: int, q: torch.Tensor, *, scale: fl
     scores = _scores(batch, heads, dim, scale, causal, window, cap, slopes, prefix_lengths)
     flag = _flag_pointer(batch, error_flag)
     lib = _lib.load()
-    with _On(batch.device, stream) as handle:
+    with _On(batch, stream) as handle:
         if out is None:
-            out = torch.empty((n, heads, dim), dtype=q.dtype, device=q.device)
+            out = q.new_empty((n, heads, dim))
         co = batch._heads(out, "out", n, heads)
-        lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if return_lse else None
+        lse = q.new_empty((n, heads), dtype=torch.float32) if return_lse else None
         c = batch._tokens(n)
         need = ctypes.c_int64(0)
         _lib.check(lib.cb_attention_workspace_bytes(c, batch._code, dim, ctypes.byref(scores), heads,
                                                     ctypes.byref(need)))
-        work = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+        work = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
         _lib.check(lib.cb_paged_attention(
             c, layer, batch._code, dim, ctypes.byref(scores), ctypes.byref(cq), ctypes.byref(co),
             None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), need.value, flag,
@@ -280,7 +293,7 @@ def add_key_weights(batch: QueryBatch, layer: int, q: torch.Tensor, lse: torch.T
     stride = _weights_stride(batch, weights)
     scores = _scores(batch, heads, dim, scale, causal, window, cap, slopes, prefix_lengths)
     flag = _flag_pointer(batch, error_flag)
-    with _On(batch.device, stream) as handle:
+    with _On(batch, stream) as handle:
         _lib.check(_lib.load().cb_add_key_weights(
             batch._tokens(n), layer, batch._code, dim, ctypes.byref(scores), ctypes.byref(cq), lse.data_ptr(),
             weights.data_ptr(), stride, flag, handle))
@@ -333,7 +346,7 @@ def evict_tokens(batch: QueryBatch, weights: torch.Tensor, target: QueryBatch, *
         raise ValueError("budget must be positive and hold the first and last tokens")
     flag = _flag_pointer(batch, error_flag)
     b, dev = batch.requests, batch.device
-    with _On(dev, stream) as handle:
+    with _On(batch, stream) as handle:
         kept = KeptTokens(torch.empty((b, budget), dtype=torch.int32, device=dev),
                           torch.empty(b, dtype=torch.int32, device=dev),
                           torch.empty((b, budget), dtype=torch.float32, device=dev))
