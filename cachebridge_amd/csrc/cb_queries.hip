@@ -772,9 +772,80 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(Attend
   if (a.lse && g == 0) a.lse[at] = lse2 * kLn2;
 }
 
-// Joins the splits of one (token, head) a workgroup: out = sum 2^(lse_z - lse)
-// out_z. Threads of one group of LANES hold four elements each of a
-// split's row, the groups take splits in turn and meet in LDS in group order.
+// Splits of a (token, head): its first row of partial results and how many of
+// the launch's splits its tile has; 0 rows of no request.
+CB_INLINE int splits_of(const AttendArgs& a, const KeyRange& kr) {
+  return min(a.splits, (kr.tiles + a.tiles_per_split - 1) / a.tiles_per_split);
+}
+template <int KT>
+CB_INLINE int row_splits(const AttendArgs& a, int t, int qh, int rows_per_tile) {
+  const ScoreArgs& s = a.s;
+  const int b = request_of_token(s.batch, t);
+  if (b >= s.batch.requests) return -1;
+  const Request r = load_request(s.batch, b);
+  if (!r.ok || t < r.q0 || t >= r.q0 + r.n) return -1;
+  const int row = (t - r.q0) * s.group + qh % s.group;
+  const int row0 = row / rows_per_tile * rows_per_tile;
+  return splits_of(a, key_range<KT>(s, r, b, row0, min(r.n * s.group, row0 + rows_per_tile) - 1));
+}
+
+// Joins few splits: out = sum 2^(lse_z - lse) out_z, a wave a row. Lane z holds
+// split z's statistics, then every lane E elements of the row.
+constexpr int kJoinFew = 16;
+
+template <typename IO, int KT, int E>
+__global__ __launch_bounds__(256) void join_few_kernel(AttendArgs a, int rows_per_tile) {
+  typedef float vec __attribute__((ext_vector_type(E)));
+  const ScoreArgs& s = a.s;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t step = static_cast<int64_t>(s.batch.tokens) * s.q_heads;
+  if (at >= step) return;
+  const int t = static_cast<int>(at / s.q_heads), qh = static_cast<int>(at % s.q_heads);
+  const float got = a.part_lse[min(lane, a.splits - 1) * step + at];  // before what it waits for is known
+  const int n = __builtin_amdgcn_readfirstlane(row_splits<KT>(a, t, qh, rows_per_tile));
+  if (n < 0) return;
+  const float lse = lane < n ? got : kNegInf;
+  float top = lse;
+#pragma unroll
+  for (int d = 1; d < kJoinFew; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  top = __shfl(top, 0);
+  const float mu = top == kNegInf ? 0.0f : top;
+  const float w = exp2_fast(lse - mu);
+  float total = w;
+#pragma unroll
+  for (int d = 1; d < kJoinFew; d <<= 1) total += __shfl_xor(total, d);
+  total = __shfl(total, 0);
+  const int D = s.head_dim, d0 = lane * E;
+  float o[E] = {};
+  if (d0 < D) {
+    for (int z = 0; z < n; ++z) {
+      // Read from lanes that may hold no element and are off here.
+      const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), z));
+      const float* from = a.part_out + (z * step + at) * D + d0;
+      if (f == 0.0f) continue;
+      if (D % E == 0) {
+        const vec x = *reinterpret_cast<const vec*>(from);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += f * x[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (d0 + e < D) o[e] += f * from[e];
+      }
+    }
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  char* op = a.out.data + static_cast<int64_t>(t) * a.out.token_b + qh * a.out.head_b;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (d0 + e < D) store_elem<IO>(op + (d0 + e) * static_cast<int>(sizeof(IO)), from_f32<IO>(o[e] * inv));
+  if (a.lse && lane == 0) a.lse[at] = total == 0.0f ? kNegInf : (top + log2_fast(total)) * kLn2;
+}
+
+// Joins many splits, a workgroup a row: threads of one group of LANES hold four
+// elements each of a split's row, the groups take splits in turn and meet in
+// LDS in group order.
 constexpr int kJoinThreads = 256;
 
 template <typename IO, int KT, int LANES>
@@ -786,14 +857,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_splits_kernel(AttendArgs a,
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int64_t at = blockIdx.x;
   const int t = static_cast<int>(at / s.q_heads), qh = static_cast<int>(at % s.q_heads);
-  const int b = request_of_token(s.batch, t);
-  if (b >= s.batch.requests) return;
-  const Request r = load_request(s.batch, b);
-  if (!r.ok || t < r.q0 || t >= r.q0 + r.n) return;
-  const int row = (t - r.q0) * s.group + qh % s.group;
-  const int row0 = row / rows_per_tile * rows_per_tile;
-  const KeyRange kr = key_range<KT>(s, r, b, row0, min(r.n * s.group, row0 + rows_per_tile) - 1);
-  const int n = min(a.splits, (kr.tiles + a.tiles_per_split - 1) / a.tiles_per_split);
+  const int n = row_splits<KT>(a, t, qh, rows_per_tile);
+  if (n < 0) return;
   const int64_t step = static_cast<int64_t>(s.batch.tokens) * s.q_heads;
   const float* lse = a.part_lse + at;
   float top = kNegInf;
@@ -2048,7 +2113,7 @@ bool takes_half(const ScoreArgs& s, int32_t dtype) {
 
 constexpr int kTileWaves = 4;
 constexpr int kStepRows = 32;  // query rows per KV head up to which attend_step_kernel is taken
-constexpr int kStepGroups = 1024;
+constexpr int kStepGroups = 512, kStepGroupsRagged = 1024;
 constexpr int kStepWaves = 2;
 
 AttendShape attend_shape(const ScoreArgs& s, int32_t dtype) {
@@ -2067,7 +2132,7 @@ AttendShape attend_shape(const ScoreArgs& s, int32_t dtype) {
   if (s.window > 0 && s.causal && !s.prefix) keys = std::min<int64_t>(keys, static_cast<int64_t>(s.window) + std::min<int64_t>(B.max_query, h.rows_per_tile / s.group + 2));
   const int key_tiles = std::max(1, ceil_div(keys, h.keys_per_tile) + (s.prefix ? 1 : 0));
   const int64_t groups = static_cast<int64_t>(h.tile_slots) * s.kv_heads;
-  const int64_t target = h.step ? kStepGroups : kTargetGroups;
+  const int64_t target = !h.step ? kTargetGroups : B.requests > 1 ? kStepGroupsRagged : kStepGroups;
   int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(1, groups), key_tiles / (h.half ? 8 : 2))));
   if (h.step) splits = std::max(splits, ceil_div(key_tiles, kStepTiles));
   h.tiles_per_split = ceil_div(key_tiles, splits);
@@ -2087,7 +2152,14 @@ int64_t attend_workspace(const ScoreArgs& s, const AttendShape& h) {
 template <typename IO, int KT>
 void launch_join(const AttendArgs& a, const AttendShape& h, hipStream_t st) {
   if (h.splits <= 1) return;
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.s.batch.tokens) * a.s.q_heads));
+  const int64_t rows = static_cast<int64_t>(a.s.batch.tokens) * a.s.q_heads;
+  if (h.splits <= kJoinFew) {
+    const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
+    if (a.s.head_dim <= 128) hipLaunchKernelGGL((join_few_kernel<IO, KT, 2>), grid, dim3(256), 0, st, a, h.rows_per_tile);
+    else hipLaunchKernelGGL((join_few_kernel<IO, KT, 8>), grid, dim3(256), 0, st, a, h.rows_per_tile);
+    return;
+  }
+  const dim3 grid(static_cast<unsigned>(rows));
   if (a.s.head_dim <= 128) hipLaunchKernelGGL((join_splits_kernel<IO, KT, 32>), grid, dim3(kJoinThreads), 0, st, a, h.rows_per_tile);
   else hipLaunchKernelGGL((join_splits_kernel<IO, KT, 128>), grid, dim3(kJoinThreads), 0, st, a, h.rows_per_tile);
 }
