@@ -1134,6 +1134,7 @@ struct RowBlock {
       for (int kb = 0; kb < KB; ++kb) modify_scores(s, st[kb], kLog2e, slope, p, start + 32 * kb, h);
     }
     if (!whole) {
+      asm volatile("");  // a branch: as selects, every tile would pay for the mask (250 instructions)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         const uint32_t there = valid[kb] >> (4 * h);
@@ -1729,12 +1730,18 @@ __global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 2 : 4) void key_w
     kr.p1 = r.length - r.n + min(row0 + 31, high - 1) / s.group;
     const bool whole = sees_all(s, kr, start, start + 32);
     if constexpr (MOD) modify_scores(s, st, 1.0f, slope, p, start, h);
+    // The difference first: what is near the row's maximum keeps its bits.
+    auto weight = [&](int e) { return exp2_fast((MOD ? st[e] - lse : __builtin_fmaf(st[e], s.scale, -lse)) * kLog2e); };
+    if (whole) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int key = start + 8 * (e >> 2) + 4 * h + (e & 3);
-      // The difference first: what is near the row's maximum keeps its bits.
-      const float w = exp2_fast((MOD ? st[e] - lse : __builtin_fmaf(st[e], s.scale, -lse)) * kLog2e);
-      sum[e] += (whole | sees(s, kr, p, key)) ? w : 0.0f;
+      for (int e = 0; e < 16; ++e) sum[e] += weight(e);
+    } else {
+      asm volatile("");  // a branch, as in RowBlock::weigh
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float w = weight(e);
+        sum[e] += sees(s, kr, p, start + 8 * (e >> 2) + 4 * h + (e & 3)) ? w : 0.0f;
+      }
     }
   }
   // Sums over the 32 lanes of a half: each exchange halves what a lane holds.
