@@ -485,10 +485,10 @@ CB_INLINE void modify_scores(const ScoreArgs& s, f32x16& x, float unit, float sl
 
 // A tile's pool rows in LDS: one wave resolves them, a key a lane, so that the
 // waves that stage the tile only look them up.
-template <int KT>
+template <int KT, int SLOTS = 4>
 struct TileRows {
-  int row[4][KT];            // pool row of each key of tile t in slot t % 4, 0 where there is none
-  uint32_t valid[4][(KT + 31) / 32];  // keys that are there
+  int row[SLOTS][KT];  // pool row of each key of tile t in slot t % SLOTS, 0 where there is none
+  uint32_t valid[SLOTS][(KT + 31) / 32];  // keys that are there
 };
 
 // The index word that names key `lane` of a tile, loaded a tile before it is
@@ -510,8 +510,8 @@ CB_INLINE int64_t fetch_entry(const QBatch& B, const Request& r, int start, int 
   return in ? got : -1;
 }
 
-template <int KT>
-CB_INLINE void place_rows(const QBatch& B, const Request& r, int64_t entry, int start, int end, TileRows<KT>& rows, int slot) {
+template <int KT, int SLOTS>
+CB_INLINE void place_rows(const QBatch& B, const Request& r, int64_t entry, int start, int end, TileRows<KT, SLOTS>& rows, int slot) {
   const int lane = threadIdx.x & (kWave - 1), j = start + lane;
   int64_t row = entry;
   if (B.kind == CB_INDEX_BLOCK_TABLE) {
@@ -572,7 +572,7 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(Attend
 
   auto entry_of = [&](int t) { return t < t1 ? fetch_entry<KT>(s.batch, r, tile_start<KT>(kr, t), tile_end(kr, t)) : -1; };
   auto place = [&](int64_t entry, int t) {
-    if (t < t1) place_rows<KT>(s.batch, r, entry, tile_start<KT>(kr, t), tile_end(kr, t), tile_rows, t & 3);
+    if (t < t1) place_rows(s.batch, r, entry, tile_start<KT>(kr, t), tile_end(kr, t), tile_rows, t & 3);
   };
   int64_t entry = -1;
   if (wave == 0) {
@@ -966,6 +966,7 @@ struct Half<io_f16> {
 __device__ const uint4 g_zeros[1] = {};
 
 constexpr int kMaxDp = 256;
+constexpr float kLag = 1024;  // a lane's sum of weights of a tile up to which its maximum may stand
 
 template <int DP>
 __device__ inline int swizzle_k(int key) {
@@ -983,6 +984,7 @@ __device__ inline void dma16(gcptr src, uint32_t lds) {
 }
 
 // s_waitcnt operands (gfx9 layout): everything, or the LDS DMA alone.
+constexpr int wait_vm(int n) { return (n & 15) | 0x70 | 0xf00 | ((n >> 4) << 14); }
 constexpr int kWaitAll = 0x0070;     // vmcnt 0, expcnt 7, lgkmcnt 0
 __device__ inline void wait_and_meet() {
   __builtin_amdgcn_s_waitcnt(kWaitAll);
@@ -995,21 +997,21 @@ __device__ inline void wait_own() {
 
 // One wave's part of a tile's DMA: N instructions for K and as many for V,
 // number u covering bytes [(first + u) * 1024, + 1024) of a tile.
-template <typename IO, int DP, int KT, int N>
+template <typename IO, int DP, int KT, int N, int SLOTS>
 struct Stager {
   static constexpr int C = DP / 8;  // 16-byte chunks a row
-  gcptr kbase;                      // K of the head, layer and tile chunk 0
-  int64_t to_v;                     // from K to V
+  gcptr kbase, vbase;               // the head's rows in the layer
   uint32_t stride;
 
   __device__ inline void init(const ScoreArgs& s, int head) {
     const int64_t off = static_cast<int64_t>(head) * s.head_dim * 2;
     kbase = layer_base(s.cache, 0, s.layer) + off;
-    to_v = layer_base(s.cache, 1, s.layer) + off - kbase;
+    vbase = layer_base(s.cache, 1, s.layer) + off;
     stride = static_cast<uint32_t>(s.batch.row_stride_b);
   }
-  CB_INLINE void issue(const ScoreArgs& s, const TileRows<KT>& rows, int slot, int first,
-                                                              uint32_t lk, uint32_t lv) const {
+  // VALUE: the tile's V rows, else its K rows, to LDS at `to`.
+  template <bool VALUE>
+  CB_INLINE void issue(const ScoreArgs& s, const TileRows<KT, SLOTS>& rows, int slot, int first, uint32_t to) const {
     const int lane = threadIdx.x & (kWave - 1), pos = lane % C;
     uint32_t whole = ~0u;
 #pragma unroll
@@ -1018,21 +1020,37 @@ struct Stager {
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       const int k = (first + u) * (kWave / C) + lane / C;
-      const int ck = pos ^ swizzle_k<DP>(k), cv = pos ^ swizzle_v<DP>(k);
+      const int c = pos ^ (VALUE ? swizzle_v<DP>(k) : swizzle_k<DP>(k));
       const uint32_t row = static_cast<uint32_t>(rows.row[slot][k]);
-      const gcptr at = kbase + static_cast<uint64_t>(row) * stride;
-      gcptr ka = at + ck * 16, va = at + to_v + cv * 16;
+      gcptr at = (VALUE ? vbase : kbase) + static_cast<uint64_t>(row) * stride + c * 16;
       if (!plain) {
         const bool ok = (rows.valid[slot][k >> 5] >> (k & 31)) & 1;
-        gcptr zero = as_global(static_cast<const void*>(g_zeros));
-        ka = (ok & (ck * 8 < s.head_dim)) ? ka : zero;
-        va = (ok & (cv * 8 < s.head_dim)) ? va : zero;
+        at = (ok & (c * 8 < s.head_dim)) ? at : as_global(static_cast<const void*>(g_zeros));
       }
-      dma16(ka, lk + (first + u) * 1024);
-      dma16(va, lv + (first + u) * 1024);
+      dma16(at, to + (first + u) * 1024);
     }
   }
 };
+
+// Whether a 16-byte chunk holds an infinity or NaN.
+template <typename IO>
+__device__ inline bool has_not_finite(u32x4 x) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) any |= ((x[u] & Half<IO>::kExponent) + Half<IO>::kCarry) & 0x80008000u;
+  return any != 0;
+}
+
+// Zeros in place of the values of a chunk that are not finite.
+template <typename IO>
+__device__ inline u32x4 finite_part(u32x4 x) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const uint32_t c = ((x[u] & Half<IO>::kExponent) + Half<IO>::kCarry) & 0x80008000u;
+    x[u] &= ~((c & 0x8000u ? 0xffffu : 0u) | (c & 0x80000000u ? 0xffff0000u : 0u));
+  }
+  return x;
+}
 
 // 32 query rows of one wave: their operands, statistics and sums.
 template <typename IO, int DP, int KT, bool MOD>
@@ -1098,34 +1116,43 @@ struct RowBlock {
     return a;
   }
 
-  static __device__ inline u32x4 k_frag(const Lanes& a, uint32_t base, int kb, int ks) {
-    return *lds_at<const u32x4>(a.k[ks & 7] + base + kb * 32 * DP * 2 + (ks >> 3) * 256);
+  static __device__ inline u32x4 k_frag(const Lanes& a, int kb, int ks) {
+    return *lds_at<const u32x4>(a.k[ks & 7] + kb * 32 * DP * 2 + (ks >> 3) * 256);
   }
-  static __device__ inline u32x4 v_frag(const Lanes& a, uint32_t base, int step, int db) {
-    const uint32_t at = a.v[db & 3] + base + step * 16 * DP * 2 + (db >> 2) * 256;
+  static __device__ inline u32x4 v_frag(const Lanes& a, int step, int db) {
+    const uint32_t at = a.v[db & 3] + step * 16 * DP * 2 + (db >> 2) * 256;
     const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(at));
     const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(at + 8 * DP * 2));
     const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
     return u32x4{x.x, x.y, y.x, y.y};
   }
 
-  // Raw products of the rows with a tile of KT keys.
-  CB_INLINE void products(const Lanes& a, uint32_t lk, f32x16 (&st)[KB]) {
+  // Raw products of the rows with a tile of KT keys. Operands are read from
+  // LDS a few steps ahead of their use; the scheduling barriers keep the
+  // compiler from moving the reads back to it, where each would be waited for.
+  CB_INLINE void products(const Lanes& a, f32x16 (&st)[KB]) {
+    constexpr int STEPS = KB * KS, AHEAD = 4;
+    u32x4 f[AHEAD];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      f32x16 z;
+    for (int n = 0; n < AHEAD; ++n) f[n] = k_frag(a, n % KB, n / KB);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) z[e] = 0;
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) z = H::mul(k_frag(a, lk, kb, ks), q[ks], z);
-      st[kb] = z;
+      for (int e = 0; e < 16; ++e) st[kb][e] = 0;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < STEPS; ++n) {
+      st[n % KB] = H::mul(f[n % AHEAD], q[n / KB], st[n % KB]);
+      if (n + AHEAD < STEPS) f[n % AHEAD] = k_frag(a, (n + AHEAD) % KB, (n + AHEAD) / KB);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
-  // Their weights, of the tile that starts at cached token `start`. `whole`:
-  // every row sees every key. `valid`: keys that are there, 32 a word.
-  CB_INLINE void weigh(const ScoreArgs& s, const KeyRange& kr, f32x16 (&st)[KB], int start,
-                                                       bool whole, const uint32_t* valid, float scale2, u32x4 (&w)[KB][2]) {
+  // Raw products of the tile that starts at cached token `start` made ready
+  // for their weights: modified and masked. `whole`: every row sees every key.
+  // `valid`: keys that are there, 32 a word.
+  CB_INLINE void ready(const ScoreArgs& s, const KeyRange& kr, f32x16 (&st)[KB], int start, bool whole,
+                       const uint32_t* valid) {
     const int h = (threadIdx.x & (kWave - 1)) >> 5;
     // Scores times scale2 are in the log2 domain (MOD: scale2 is 1 and they
     // are put there at once).
@@ -1146,40 +1173,88 @@ struct RowBlock {
         }
       }
     }
-    float top = kNegInf;
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, st[kb][e]);
-    top *= scale2;
-    // The maximum may lag by 2^8: weights up to 256 lose no digits in fp32
-    // sums or in 16 bits, and the sums are scaled again only when a row's
-    // maximum has really grown.
-    if (__any(top > m + 8.0f)) {
-      const float both = fmaxf(top, __shfl_xor(top, 32));
-      const float m1 = fmaxf(m, both);
-      const float alpha = m1 == kNegInf ? 1.0f : exp2_fast(m - m1);
-      m = m1;
-      l *= alpha;
-#pragma unroll
-      for (int d = 0; d < DB; ++d) o[d] *= alpha;
-    }
+  }
+
+  // Weights by the maximum that stands, packed as the next product's operands,
+  // and their sum.
+  CB_INLINE float try_weights(const f32x16 (&st)[KB], float scale2, u32x4 (&w)[KB][2]) const {
     const float mu = m == kNegInf ? 0.0f : m;
+    float sum = 0;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
         const float x = exp2_fast(__builtin_fmaf(st[kb][e], scale2, -mu)), y = exp2_fast(__builtin_fmaf(st[kb][e + 1], scale2, -mu));
-        l += x + y;
+        sum += x + y;
         w[kb][e >> 3][(e & 7) >> 1] = H::pack(x, y);
       }
+    return sum;
+  }
+  // A row's maximum is looked for only if a lane's weights show that it has
+  // grown by much (their sum tells) or is not known yet: up to kLag, weights
+  // lose no digits in fp32 sums or 16 bits. Vector instructions that are not
+  // exponentials cost the matrix unit their time here (16 ns a product alone or
+  // beside 2 exponentials a wave, 26 ns with 6 multiply-adds more), so the
+  // maxima of every tile would.
+  CB_INLINE void weights(const f32x16 (&st)[KB], float scale2, u32x4 (&w)[KB][2]) {
+    float sum = try_weights(st, scale2, w);
+    if (__any(!(sum < kLag) | (m == kNegInf))) {
+      float top = kNegInf;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, st[kb][e]);
+      top *= scale2;
+      const float m1 = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+      const float alpha = m1 == kNegInf ? 1.0f : exp2_fast(m - m1);
+      m = m1;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= alpha;
+      sum = try_weights(st, scale2, w);
+    }
+    l += sum;
   }
 
-  CB_INLINE void add_values(const Lanes& a, uint32_t lv, const u32x4 (&w)[KB][2]) {
+  // The first operands of a tile's values, read before its weights are made.
+  static constexpr int kValuesAhead = 4;
+  struct Values {
+    u32x4 f[kValuesAhead];
+  };
+  // Lane addresses within the tiles at lk and lv: the rest of an address then
+  // fits the instruction.
+  static CB_INLINE Lanes place(const Lanes& a, uint32_t lk, uint32_t lv) {
+    Lanes at = a;
 #pragma unroll
-    for (int t = 0; t < 2 * KB; ++t)
+    for (int x = 0; x < (DP == 64 ? 4 : 8); ++x) {
+      at.k[x] += lk;
+      asm("" : "+v"(at.k[x]));
+    }
 #pragma unroll
-      for (int d = 0; d < DB; ++d) o[d] = H::mul(v_frag(a, lv, t, d), w[t >> 1][t & 1], o[d]);
+    for (int x = 0; x < (DP == 64 ? 2 : 4); ++x) {
+      at.v[x] += lv;
+      asm("" : "+v"(at.v[x]));
+    }
+    return at;
+  }
+
+  static CB_INLINE Values first_values(const Lanes& a) {
+    Values v;
+#pragma unroll
+    for (int n = 0; n < kValuesAhead; ++n) v.f[n] = v_frag(a, n / DB, n % DB);
+    __builtin_amdgcn_sched_barrier(0);
+    return v;
+  }
+  CB_INLINE void add_values(const Lanes& a, const u32x4 (&w)[KB][2], Values& v) {
+    constexpr int STEPS = 2 * KB * DB;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < STEPS; ++n) {
+      const int t = n / DB, d = n % DB;
+      o[d] = H::mul(v.f[n % kValuesAhead], w[t >> 1][t & 1], o[d]);
+      if (n + kValuesAhead < STEPS) v.f[n % kValuesAhead] = v_frag(a, (n + kValuesAhead) / DB, (n + kValuesAhead) % DB);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 
   // Adds the infinities that were taken out of V tiles (see mark_not_finite).
@@ -1244,15 +1319,6 @@ struct RowBlock {
 // taken out of the tile and noted, a bit per (row, element), for the rows that
 // see their key; the sums get them at the end (+inf, -inf, both for NaN).
 
-// Whether a 16-byte chunk holds an infinity or NaN.
-template <typename IO>
-__device__ inline bool has_not_finite(u32x4 x) {
-  uint32_t any = 0;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) any |= ((x[u] & Half<IO>::kExponent) + Half<IO>::kCarry) & 0x80008000u;
-  return any != 0;
-}
-
 // One wave notes, for its 32 rows (marks [32][DP / 32], lane l < 32 owns row
 // l's words), every such value of the V tile at lv.
 template <typename IO, int DP, int KT>
@@ -1279,17 +1345,6 @@ CB_INLINE void mark_not_finite(uint32_t lv, int np, int below, int above, int st
       }
     }
   }
-}
-
-// Zeros in place of the values of this thread's chunk that are not finite.
-template <typename IO>
-__device__ inline u32x4 finite_part(u32x4 x) {
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const uint32_t c = ((x[u] & Half<IO>::kExponent) + Half<IO>::kCarry) & 0x80008000u;
-    x[u] &= ~((c & 0x8000u ? 0xffffu : 0u) | (c & 0x80000000u ? 0xffff0000u : 0u));
-  }
-  return x;
 }
 
 // Many query rows: a workgroup's NW waves hold 32 rows each and share K and V
@@ -1320,14 +1375,14 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_ker
   const typename Block::Lanes lanes = Block::lanes();
   const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((CB_LDS_SPACE char*)tiles));
   const float scale2 = MOD ? 1.0f : s.scale * kLog2e;
-  Stager<IO, DP, KT, N> stage;
+  Stager<IO, DP, KT, N, 4> stage;
   stage.init(s, head);
   const int first = wave * N;
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
   for (int w = threadIdx.x; w < 2 * NW * DP; w += NW * kWave) (&marks[0][0][0])[w] = 0;
   auto entry_of = [&](int t) { return t < t1 ? fetch_entry<KT>(s.batch, r, tile_start<KT>(kr, t), tile_end(kr, t)) : -1; };
   auto place = [&](int64_t entry, int t) {
-    if (t < t1) place_rows<KT>(s.batch, r, entry, tile_start<KT>(kr, t), tile_end(kr, t), tile_rows, t & 3);
+    if (t < t1) place_rows(s.batch, r, entry, tile_start<KT>(kr, t), tile_end(kr, t), tile_rows, t & 3);
   };
   int64_t entry = -1;
   if (wave == 0) {
@@ -1337,18 +1392,20 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_ker
     place(e1, t0 + 1);
   }
   __syncthreads();
-  if (t0 < t1) stage.issue(s, tile_rows, t0 & 3, first, lds, lds + kTile);
+  if (t0 < t1) {
+    stage.template issue<false>(s, tile_rows, t0 & 3, first, lds);
+    stage.template issue<true>(s, tile_rows, t0 & 3, first, lds + kTile);
+  }
   uint32_t buf = 0;
   for (int t = t0; t < t1; ++t) {
     wait_and_meet();
+    if (wave == 0) place(entry, t + 2);
     if (t + 1 < t1) {
       const uint32_t to = lds + (buf ^ (2 * kTile));
-      stage.issue(s, tile_rows, (t + 1) & 3, first, to, to + kTile);
-      if (wave == 0) {
-        place(entry, t + 2);
-        entry = entry_of(t + 3);
-      }
+      stage.template issue<false>(s, tile_rows, (t + 1) & 3, first, to);
+      stage.template issue<true>(s, tile_rows, (t + 1) & 3, first, to + kTile);
     }
+    if (wave == 0) entry = entry_of(t + 3);
     const int start = tile_start<KT>(kr, t), end = tile_end(kr, t);
     uint32_t valid[KT / 32], every = ~0u;
 #pragma unroll
@@ -1377,9 +1434,12 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_ker
     }
     f32x16 st[KT / 32];
     u32x4 w[KT / 32][2];
-    blk.products(lanes, lds + buf, st);
-    blk.weigh(s, kr, st, start, whole, valid, scale2, w);
-    blk.add_values(lanes, lds + buf + kTile, w);
+    const typename Block::Lanes at = Block::place(lanes, lds + buf, lds + buf + kTile);
+    blk.products(at, st);
+    blk.ready(s, kr, st, start, whole, valid);
+    typename Block::Values v = Block::first_values(at);
+    blk.weights(st, scale2, w);
+    blk.add_values(at, w, v);
     buf ^= 2 * kTile;
   }
   __syncthreads();
@@ -1395,8 +1455,6 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_ker
 // names are resolved into LDS first, so that the loop's only vector memory
 // operations are the DMA, whose count tells what has arrived.
 constexpr int kStepTiles = 64;  // tiles a split holds at most
-
-constexpr int wait_vm(int n) { return (n & 15) | 0x70 | 0xf00 | ((n >> 4) << 14); }
 
 template <typename IO, int DP, int NW, bool MOD>
 __global__ __launch_bounds__(NW * kWave, 1) void attend_step_kernel(AttendArgs a, int vector) {
@@ -1470,18 +1528,20 @@ __global__ __launch_bounds__(NW * kWave, 1) void attend_step_kernel(AttendArgs a
     asm volatile("" ::: "memory");
     f32x16 st[1];
     u32x4 w[1][2];
-    blk.products(lanes, lds + buf, st);
+    const uint32_t lv = lds + 2 * kTile + buf;
+    const typename Block::Lanes at = Block::place(lanes, lds + buf, lv);
+    blk.products(at, st);
     if (i + 2 < n) {
       __builtin_amdgcn_s_waitcnt(0xc07f);  // the products' LDS reads
       request(i + 2, kbase, lds + buf, false);
     }
     const bool all = sees_all(s, kr, start, min(end, start + KT));
-    blk.weigh(s, kr, st, start, all & (valid == ~0u), &valid, scale2, w);
+    blk.ready(s, kr, st, start, all & (valid == ~0u), &valid);
+    blk.weights(st, scale2, w);
     if (i + 2 < n) __builtin_amdgcn_s_waitcnt(wait_vm(3 * N));
     else if (i + 1 < n) __builtin_amdgcn_s_waitcnt(wait_vm(2 * N));
     else __builtin_amdgcn_s_waitcnt(wait_vm(0));
     asm volatile("" ::: "memory");
-    const uint32_t lv = lds + 2 * kTile + buf;
     if (!all) {
       bool strange = false;
 #pragma unroll
@@ -1497,7 +1557,8 @@ __global__ __launch_bounds__(NW * kWave, 1) void attend_step_kernel(AttendArgs a
         }
       }
     }
-    blk.add_values(lanes, lv, w);
+    typename Block::Values v = Block::first_values(at);
+    blk.add_values(at, w, v);
     if (i + 2 < n) {
       __builtin_amdgcn_s_waitcnt(0xc07f);
       request(i + 2, vbase, lv, true);
@@ -1736,7 +1797,7 @@ __global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 2 : 4) void key_w
 #pragma unroll
       for (int e = 0; e < 16; ++e) sum[e] += weight(e);
     } else {
-      asm volatile("");  // a branch, as in RowBlock::weigh
+      asm volatile("");  // a branch, as in RowBlock::ready
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const float w = weight(e);

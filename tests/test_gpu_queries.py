@@ -36,6 +36,9 @@ SHAPES = {
     "no-new": ([50, 60], [0, 2], (4, 4)),
     "long": ([2100], [3], (4, 1)),
     "chunk-long": ([1500], [150], (4, 2)),
+    "wide": ([420, 1, 300], [300, 1, 130], (4, 2)),
+    "wide-long": ([1300], [260], (6, 2)),
+    "wide-odd": ([333], [333], (5, 1)),
 }
 
 
@@ -64,7 +67,7 @@ MASKS = {
 
 @pytest.mark.parametrize("dtype,dim", [(BF16, 64), (BF16, 128), (BF16, 256), (FP16, 128), (FP32, 64)])
 @pytest.mark.parametrize("mask", list(MASKS))
-@pytest.mark.parametrize("new", [[1, 1, 1], [90, 7, 33]])
+@pytest.mark.parametrize("new", [[1, 1, 1], [90, 7, 33], [180, 290, 33]])
 def test_attention_and_weights_masks(new, mask, dtype, dim):
     case = make([190, 301, 33], new, heads=8, kv_heads=2, dim=dim, dtype=dtype, seed=3)
     how = dict(MASKS[mask])
@@ -125,10 +128,11 @@ def test_many_ragged_requests(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
-@pytest.mark.parametrize("new", [1, 20, 150])
-def test_what_is_not_seen_never_counts(new, dtype):
+@pytest.mark.parametrize("new,dim", [(1, 64), (20, 64), (150, 64), (20, 128), (150, 128), (20, 256), (150, 256)])
+@pytest.mark.parametrize("heads", [4, 8])
+def test_what_is_not_seen_never_counts(new, dim, heads, dtype):
     """Infinities and NaN behind the mask, past the length and in pages of nobody leave every row as it was."""
-    case = make([170, 170], [new, new], dim=64, dtype=dtype, seed=6)
+    case = make([170, 170], [new, new], heads=heads, dim=dim, dtype=dtype, seed=6)
     want, want_lse = attend(case, window=9)
     k, v = case.pool
     inside = torch.zeros(k.shape[1], dtype=torch.bool)
@@ -153,12 +157,14 @@ def test_what_is_not_seen_never_counts(new, dtype):
         assert torch.isposinf(got[new - 1]).all()
         assert torch.equal(got[new:2 * new - 2], want[new:2 * new - 2])
         assert torch.isnan(got[2 * new - 2:, :, 3]).all()
-        keep = [d for d in range(64) if d != 3]
+        keep = [d for d in range(dim) if d != 3]
         assert torch.equal(got[2 * new - 2:, :, keep], want[2 * new - 2:, :, keep])
 
 
-def test_infinite_values_of_both_signs_meet_as_nan():
-    case = make([60], [30], dim=64, seed=2)
+@pytest.mark.parametrize("new", [30, 300])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_infinite_values_of_both_signs_meet_as_nan(dim, new):
+    case = make([30 + new], [new], dim=dim, seed=2)
     _, v = case.pool
     want, _ = attend(case)
     v[0, case.slots[0][40], 0, 5] = math.inf
@@ -167,6 +173,8 @@ def test_infinite_values_of_both_signs_meet_as_nan():
     assert torch.equal(got[:10], want[:10])
     assert torch.isposinf(got[10:20, :2, 5]).all() and torch.isnan(got[20:, :2, 5]).all()
     assert torch.equal(got[:, 2:], want[:, 2:])
+    keep = [d for d in range(dim) if d != 5]
+    assert torch.equal(got[..., keep], want[..., keep])
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
