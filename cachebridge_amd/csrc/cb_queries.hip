@@ -2163,13 +2163,14 @@ int check_scores(const cb_query_batch* batch, int32_t layer, int32_t dtype, int3
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
-constexpr int kTargetGroups = 512;  // workgroups that fill the 256 CUs twice
+constexpr int kTargetGroups = 512;  // workgroups of four waves that fill the 256 CUs twice
 
 // How the launch is cut: query tiles, and key splits where the tiles alone
 // would leave CUs idle.
 struct AttendShape {
   bool half;  // the 16-bit kernels
   bool step;  // of these, the one for few rows
+  int waves;
   int rows_per_tile, keys_per_tile;
   int tile_slots, request_slots, splits, tiles_per_split;
 };
@@ -2179,7 +2180,14 @@ bool takes_half(const ScoreArgs& s, int32_t dtype) {
   return dtype != CB_DTYPE_F32 && s.head_dim % 8 == 0 && s.cache.row_stride_b <= 0xffffffffll && s.head_dim <= kMaxDp && rows_aligned16(s.cache, s.head_dim * 2);
 }
 
-constexpr int kTileWaves = 4;
+// Waves of attend_tile_kernel: eight share a tile's staging among twice the
+// rows, if there are that many and a head's registers leave two waves a SIMD.
+// That pays once a launch has work for all CUs (16 query heads, 2 KV heads,
+// kernel and join, eight waves against four): 256 new tokens over 4096 cached
+// 41.1 / 37.1 us, 64 over 32768 46.1 / 49.2, 1024 over 4096 63 / 70, 256 over
+// 32768 106 / 120; 1000 of 1000 with 8 heads 39.4 / 34.1.
+constexpr int kWideRows = 512;               // query rows per KV head, and
+constexpr int64_t kWideScores = 24ll << 20;  // scores of the launch, from which eight are taken
 constexpr int kStepRows = 32;  // query rows per KV head up to which attend_step_kernel is taken
 constexpr int kStepGroups = 512, kStepGroupsRagged = 1024;
 constexpr int kStepWaves = 2;
@@ -2189,7 +2197,11 @@ AttendShape attend_shape(const ScoreArgs& s, int32_t dtype) {
   h.half = takes_half(s, dtype);
   const QBatch& B = s.batch;
   h.step = h.half && static_cast<int64_t>(B.max_query) * s.group <= kStepRows;
-  h.rows_per_tile = h.step ? 32 : h.half ? 32 * kTileWaves : kAnyRows;
+  const int64_t seen = s.window > 0 && s.causal && !s.prefix ? std::min<int64_t>(B.max_length, s.window) : B.max_length;
+  h.waves = h.half && s.head_dim <= 128 && static_cast<int64_t>(B.max_query) * s.group >= kWideRows &&
+                    static_cast<int64_t>(B.tokens) * s.q_heads * seen >= kWideScores
+                ? 8 : 4;
+  h.rows_per_tile = h.step ? 32 : h.half ? 32 * h.waves : kAnyRows;
   h.keys_per_tile = !h.half ? kAnyKeys : !h.step && s.head_dim <= (s.mod ? 64 : 128) ? 64 : 32;
   const int per_request = std::max(1, ceil_div(static_cast<int64_t>(B.max_query) * s.group, h.rows_per_tile));
   const int64_t by_request = static_cast<int64_t>(per_request) * B.requests;
@@ -2200,7 +2212,7 @@ AttendShape attend_shape(const ScoreArgs& s, int32_t dtype) {
   if (s.window > 0 && s.causal && !s.prefix) keys = std::min<int64_t>(keys, static_cast<int64_t>(s.window) + std::min<int64_t>(B.max_query, h.rows_per_tile / s.group + 2));
   const int key_tiles = std::max(1, ceil_div(keys, h.keys_per_tile) + (s.prefix ? 1 : 0));
   const int64_t groups = static_cast<int64_t>(h.tile_slots) * s.kv_heads;
-  const int64_t target = !h.step ? kTargetGroups : B.requests > 1 ? kStepGroupsRagged : kStepGroups;
+  const int64_t target = !h.step ? kTargetGroups * 4 / h.waves : B.requests > 1 ? kStepGroupsRagged : kStepGroups;
   int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(1, groups), key_tiles / (h.half ? 8 : 2))));
   if (h.step) splits = std::max(splits, ceil_div(key_tiles, kStepTiles));
   h.tiles_per_split = ceil_div(key_tiles, splits);
@@ -2245,7 +2257,8 @@ template <typename IO, int DP, int KT, bool MOD>
 void launch_half(const AttendArgs& a, const AttendShape& h, unsigned grid, hipStream_t st) {
   const int vector = aligned16(a.s.q) && aligned16(a.out);
   if (h.step) hipLaunchKernelGGL((attend_step_kernel<IO, DP, kStepWaves, MOD>), dim3(grid), dim3(kStepWaves * kWave), 0, st, a, vector);
-  else hipLaunchKernelGGL((attend_tile_kernel<IO, DP, KT, kTileWaves, MOD>), dim3(grid), dim3(kTileWaves * kWave), 0, st, a, vector);
+  else if (DP <= 128 && h.waves == 8) hipLaunchKernelGGL((attend_tile_kernel<IO, DP, KT, DP <= 128 ? 8 : 4, MOD>), dim3(grid), dim3(8 * kWave), 0, st, a, vector);
+  else hipLaunchKernelGGL((attend_tile_kernel<IO, DP, KT, 4, MOD>), dim3(grid), dim3(4 * kWave), 0, st, a, vector);
   if (h.step) launch_join<IO, 32>(a, h, st);
   else launch_join<IO, KT>(a, h, st);
 }

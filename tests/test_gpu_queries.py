@@ -177,6 +177,49 @@ def test_infinite_values_of_both_signs_meet_as_nan(dim, new):
     assert torch.equal(got[..., keep], want[..., keep])
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, BF16), (128, FP16), (96, FP16)])
+@pytest.mark.parametrize("how", [{}, dict(window=300, prefix=[37, 8]), dict(cap=4.0, causal=False)])
+def test_large_launches(how, dim, dtype):
+    """Enough scores for eight waves a workgroup; a sample of the rows against the oracle, values that are not finite
+    and bad rows among them."""
+    new, heads, lengths = [700, 40], 16, [2400, 500]
+    case = make(lengths, new, heads=heads, kv_heads=2, dim=dim, dtype=dtype, seed=21, index="i32")
+    how = dict(how)
+    prefix = how.pop("prefix", None)
+    more = {} if prefix is None else dict(prefix_lengths=torch.tensor(prefix, dtype=torch.int32).cuda())
+    assert sum(new) * heads * (lengths[0] if prefix else min(lengths[0], how.get("window", 1 << 30))) >= 24 << 20
+    out, lse = attend(case, **how, **more)
+    u = torch.finfo(dtype).eps / 2
+    def check(out, lse):
+        for b, at, m in ((0, 0, 700), (1, 700, 40)):
+            rows = sorted({0, 1, 31, 63, 64, 127, 128, 255, 256, 300, 511, 640, 699} & set(range(m)))
+            for h in (0, 7, 8, 15):
+                k, v = (x[0, case.slots[b], h // 8].double() for x in (case.k, case.v))
+                seen = oracle.visible(lengths[b], m, **{x: y for x, y in how.items() if x != "cap"}, prefix=prefix[b] if prefix else 0)[rows]
+                q = case.q[at:at + m, h].double()
+                x = oracle.scores(q, k, scale=dim ** -0.5, cap=how.get("cap", 0.0))[rows].masked_fill(~seen, -math.inf)
+                w = torch.softmax(x, 1)
+                want, mag = w @ v, w @ v.abs()
+                # The bounds of query_cases.check_attention.
+                d = oracle.score_error(q, k, scale=dim ** -0.5) + 2.0 ** -21 * how.get("cap", 0.0)
+                tol = u * want.abs() + u * mag + mag * (4 * d + (lengths[b] + 16) * 2.0 ** -23) + 2.0 ** -25 * lengths[b] * v.abs().max()
+                got = out[at:at + m, h].double().cpu()[rows]
+                assert ((got - want).abs() - tol).max() <= 0, (b, h)
+                z = torch.logsumexp(x, 1)
+                assert ((lse[at:at + m, h].double().cpu()[rows] - z).abs() - (d + (lengths[b] + 16) * 2.0 ** -23 + 2.0 ** -22 * z.abs())).max() <= 0
+    check(out, lse)
+    if how.get("causal", True) and prefix is None:
+        _, v = case.pool
+        v[0, case.slots[0][2100], 0, 5] = math.inf   # new token 400 and later ones see it
+        v[0, case.slots[0][2200], 1, 6] = math.nan
+        got, _ = attend(case, **how, **more)
+        assert torch.equal(got[:400], out[:400]) and torch.equal(got[700:], out[700:])
+        assert torch.isposinf(got[400:700, :8, 5]).all() and torch.isnan(got[500:700, 8:, 6]).all()
+        assert torch.equal(got[400:500, 8:], out[400:500, 8:])
+        keep = [d for d in range(dim) if d not in (5, 6)]
+        assert torch.equal(got[..., keep], out[..., keep])
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_large_scores(dtype):
     """Rows whose maximum grows from tile to tile, by little and by much, and scores far from zero."""
