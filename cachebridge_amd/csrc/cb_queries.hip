@@ -342,6 +342,7 @@ struct ScoreArgs {
   const float* slopes;
   const int32_t* prefix;
   int32_t mod;  // scores are more than a product times a positive scale
+  int32_t group_shift;  // log2(group), or -1
 };
 
 struct AttendArgs {
@@ -431,6 +432,10 @@ CB_INLINE int tile_start(const KeyRange& k, int t) {
   return t < k.ta ? t * KT : k.lb + (t - k.ta) * KT;
 }
 CB_INLINE int tile_end(const KeyRange& k, int t) { return t < k.ta ? k.na : k.hb; }
+
+// New token of a query row: a shift for the usual groups of a power of two,
+// where a division costs some 25 instructions.
+CB_INLINE int token_of_row(const ScoreArgs& s, int row) { return s.group_shift >= 0 ? row >> s.group_shift : row / s.group; }
 
 // Whether every row of the tile sees every key of [start, stop).
 CB_INLINE bool sees_all(const ScoreArgs& s, const KeyRange& k, int start, int stop) {
@@ -541,6 +546,16 @@ constexpr int kAnyKeys = 16;
 
 __device__ inline f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
+// Elements 4 e + g of a row of `dim`, zeros past it; loaded at clamped places
+// and selected after, so that no load waits for another.
+template <typename IO, int N>
+CB_INLINE void load_spread(const char* row, int dim, int g, float (&x)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) x[e] = to_f32(load_elem<IO>(row + min(4 * e + g, dim - 1) * static_cast<int>(sizeof(IO))));
+#pragma unroll
+  for (int e = 0; e < N; ++e) x[e] = 4 * e + g < dim ? x[e] : 0.0f;
+}
+
 __device__ inline bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
 
 template <typename IO, int DP, int VE>
@@ -594,9 +609,7 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(Attend
   const int D = s.head_dim;
   const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
   float q[DP / 4];
-#pragma unroll
-  for (int e = 0; e < DP / 4; ++e)
-    q[e] = 4 * e + g < D ? to_f32(load_elem<IO>(qp + (4 * e + g) * static_cast<int>(sizeof(IO)))) : 0.0f;
+  load_spread<IO>(qp, D, g, q);
   const float slope = s.slopes ? s.slopes[qh] : 0.0f;
 
   gcptr kbase = layer_base(s.cache, 0, s.layer) + static_cast<int64_t>(head) * D * sizeof(IO);
@@ -1052,6 +1065,26 @@ __device__ inline u32x4 finite_part(u32x4 x) {
   return x;
 }
 
+// The operands of one row of `dim` elements: chunks 2 k + h of 16 bytes, zeros
+// past dim. Loads are at clamped places and selected after: as branches each
+// would wait for the one before.
+template <int KS>
+CB_INLINE void load_operands(const char* row, int dim, int h, bool vector, u32x4 (&x)[KS]) {
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    const char* at = row + 2 * min(16 * k + 8 * h, dim - 8);
+    if (vector) {
+      x[k] = gload<u32x4>(as_global(static_cast<const void*>(at)));
+    } else {
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        x[k][w] = load_elem<uint16_t>(at + 4 * w) | static_cast<uint32_t>(load_elem<uint16_t>(at + 4 * w + 2)) << 16;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < KS; ++k) x[k] = 16 * k + 8 * h < dim ? x[k] : u32x4{0, 0, 0, 0};
+}
+
 // 32 query rows of one wave: their operands, statistics and sums.
 template <typename IO, int DP, int KT, bool MOD>
 struct RowBlock {
@@ -1074,21 +1107,7 @@ struct RowBlock {
     qh = head * s.group + at - i * s.group;
     p = r.length - r.n + i;
     const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const int d = 16 * k + 8 * h;
-      u32x4 x = {0, 0, 0, 0};
-      if (d < s.head_dim) {
-        if (vector) {
-          x = gload<u32x4>(as_global(static_cast<const void*>(qp + 2 * d)));
-        } else {
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            x[w] = load_elem<uint16_t>(qp + 2 * d + 4 * w) | static_cast<uint32_t>(load_elem<uint16_t>(qp + 2 * d + 4 * w + 2)) << 16;
-        }
-      }
-      q[k] = x;
-    }
+    load_operands<KS>(qp, s.head_dim, h, vector, q);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -1671,19 +1690,20 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void key_weights_any_kernel(W
   const uint64_t rows_ok = __ballot(mine >= 0);
   float sum[4] = {0, 0, 0, 0};
   for (int head = 0; head < s.kv_heads; ++head) {
-    const char* kp = (const char*)layer_base(s.cache, 0, s.layer) + static_cast<int64_t>(head) * D * sizeof(IO) + mine * s.cache.row_stride_b;
+    const char* kp = (const char*)layer_base(s.cache, 0, s.layer) + static_cast<int64_t>(head) * D * sizeof(IO) + (mine >= 0 ? mine : 0) * s.cache.row_stride_b;
     float k[DP / 4];
+    load_spread<IO>(kp, D, g, k);
 #pragma unroll
-    for (int e = 0; e < DP / 4; ++e)
-      k[e] = mine >= 0 && 4 * e + g < D ? to_f32(load_elem<IO>(kp + (4 * e + g) * static_cast<int>(sizeof(IO)))) : 0.0f;
+    for (int e = 0; e < DP / 4; ++e) k[e] = mine >= 0 ? k[e] : 0.0f;
     for (int row0 = i0 * s.group + 16 * wave; row0 < i1 * s.group; row0 += kAnyRows) {
       const int row = min(row0 + c, i1 * s.group - 1);
       const int i = row / s.group, qh = head * s.group + row % s.group, p = r.length - r.n + i;
       const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
       f32x4 st = {0, 0, 0, 0};
+      float q[DP / 4];
+      load_spread<IO>(qp, D, g, q);
 #pragma unroll
-      for (int e = 0; e < DP / 4; ++e)
-        st = mfma4(k[e], 4 * e + g < D ? to_f32(load_elem<IO>(qp + (4 * e + g) * static_cast<int>(sizeof(IO)))) : 0.0f, st);
+      for (int e = 0; e < DP / 4; ++e) st = mfma4(k[e], q[e], st);
       const float lse = a.lse[static_cast<int64_t>(r.q0 + i) * s.q_heads + qh];
       const float slope = s.slopes ? s.slopes[qh] : 0.0f;
 #pragma unroll
@@ -1712,17 +1732,22 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void key_weights_any_kernel(W
 }
 
 // 16-bit form: a wave holds 32 keys of one KV head as MFMA operands in
-// registers and walks blocks of 32 query rows, whose operands come straight
-// from memory (the few rows of a batch stay in cache); S^T keeps a row a lane
-// pair, so a key's sum over rows is a sum over lanes, made once at the end.
-// The waves that share a block of keys (4 if there are 4 or more blocks of
-// rows to walk, else fewer, so that none idles) meet in LDS in wave order.
+// registers and walks blocks of 32 query rows; S^T keeps a row a lane pair, so a
+// key's sum over rows is a sum over lanes, made once at the end. The waves that
+// share a block of keys (4 if there are 4 or more blocks of rows to walk, else
+// fewer, so that none idles) meet in LDS in wave order.
+//
+// Keys and query rows come through LDS of the wave's own: loaded straight into
+// operands, four lanes in a row touch four rows, and the address unit takes a
+// cycle for each lane of such a load (1 us for four blocks of rows a CU).
 constexpr int kWeightWaves = 4;
 
 template <typename IO, int DP, bool MOD>
-__global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 2 : 4) void key_weights_kernel(WeightArgs a, int vector) {
+__global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 1 : 2) void key_weights_kernel(WeightArgs a, int vector) {
   typedef Half<IO> H;
-  constexpr int KS = DP / 16;
+  typedef RowBlock<IO, DP, 32, MOD> Block;
+  constexpr int KS = DP / 16, kTile = 32 * DP * 2, N = kTile / 1024, C = DP / 8;
+  __shared__ __align__(1024) char tiles[kWeightWaves * 2 * kTile];  // a wave's keys, then its rows
   __shared__ float sums[kWeightWaves][32];
   const ScoreArgs& s = a.s;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -1743,56 +1768,96 @@ __global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 2 : 4) void key_w
   if ((j < r.length) & (mine < 0) & (sub == 0) & (h == 0)) flag(s.batch.err, CB_ERROR_CACHE_ROW);
   const uint32_t there = static_cast<uint32_t>(__ballot(mine >= 0));
   const int D = s.head_dim;
-  const int low = i0 * s.group, high = i1 * s.group, blocks = (high - low + 31) / 32;
+  const int low = i0 * s.group, high = i1 * s.group, blocks = (high - low + 31) / 32, items = s.kv_heads * blocks;
+  const uint32_t lk = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((CB_LDS_SPACE char*)tiles)) + wave * 2 * kTile, lq = lk + kTile;
+  const typename Block::Lanes lanes = Block::lanes();
+  auto operand = [&](uint32_t base, int x) __attribute__((always_inline)) { return *lds_at<const u32x4>(lanes.k[x & 7] + base + (x >> 3) * 256); };
+
+  // 32 rows to LDS at `to`; lane y < 32 holds the y-th one's address.
+  auto stage = [&](uint64_t row, uint32_t there, uint32_t to, bool direct) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int y = u * (kWave / C) + lane / C, chunk = (lane % C) ^ swizzle_k<DP>(y);
+      const uint64_t at = static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(row), y))) |
+                          static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(row >> 32), y))) << 32;
+      const bool in = ((there >> y) & 1) & (chunk * 8 < D);
+      if (direct) {
+        dma16(in ? reinterpret_cast<gcptr>(at) + chunk * 16 : as_global(static_cast<const void*>(g_zeros)), to + u * 1024);
+      } else {
+        u32x4 x = {0, 0, 0, 0};
+        if (in) {
+          const char* from = reinterpret_cast<const char*>(at) + chunk * 16;
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            x[w] = load_elem<uint16_t>(from + 4 * w) | static_cast<uint32_t>(load_elem<uint16_t>(from + 4 * w + 2)) << 16;
+        }
+        *lds_at<u32x4>(to + u * 1024 + lane * 16) = x;
+      }
+    }
+  };
+  struct Rows {
+    float lse, slope;
+    int row0, p;
+  };
+  auto ask = [&](int head, int item) __attribute__((always_inline)) {
+    Rows x;
+    x.row0 = low + (item - head * blocks) * 32;
+    const int row = x.row0 + c, at = min(row, high - 1), i = token_of_row(s, at), qh = head * s.group + at - i * s.group;
+    x.p = r.length - r.n + i;
+    const float lse = a.lse[static_cast<int64_t>(r.q0 + i) * s.q_heads + qh];
+    // Nothing is added by lanes past the last row and rows that see nothing.
+    x.lse = ((row >= high) | (lse == kNegInf)) ? INFINITY : lse;
+    x.slope = 0;
+    if constexpr (MOD) x.slope = s.slopes ? s.slopes[qh] : 0.0f;
+    stage(reinterpret_cast<uint64_t>(s.q.data) + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b, ~0u, lq, vector != 0);
+    return x;
+  };
+  auto ask_keys = [&](int head) __attribute__((always_inline)) {
+    const uint64_t base = reinterpret_cast<uint64_t>(layer_base(s.cache, 0, s.layer)) + static_cast<int64_t>(head) * D * 2;
+    stage(base + (mine >= 0 ? mine : 0) * s.batch.row_stride_b, there, lk, true);
+  };
+
   float sum[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) sum[e] = 0;
-  int held = -1;
   u32x4 k[KS];
-  for (int item = sub; item < s.kv_heads * blocks; item += share) {
-    const int head = item / blocks, row0 = low + (item - head * blocks) * 32;
+  Rows now{};
+  int head = 0, held = -1;
+  if (sub < items) {
+    while (sub >= (head + 1) * blocks) ++head;
+    ask_keys(head);
+    now = ask(head, sub);
+  }
+  for (int item = sub; item < items; item += share) {
+    wait_own();
     if (head != held) {
       held = head;
-      gcptr kp = layer_base(s.cache, 0, s.layer) + static_cast<int64_t>(head) * D * 2 + mine * s.batch.row_stride_b;
 #pragma unroll
-      for (int x = 0; x < KS; ++x) {
-        const int d = 16 * x + 8 * h;
-        k[x] = u32x4{0, 0, 0, 0};
-        if ((mine >= 0) & (d < D)) k[x] = gload<u32x4>(kp + 2 * d);
-      }
+      for (int x = 0; x < KS; ++x) k[x] = operand(lk, x);
     }
-    const int row = row0 + c, at = min(row, high - 1), i = at / s.group, qh = head * s.group + at - i * s.group;
-    const int p = r.length - r.n + i;
-    const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
-    float lse = a.lse[static_cast<int64_t>(r.q0 + i) * s.q_heads + qh];
-    // Nothing is added by lanes past the last row and rows that see nothing.
-    lse = ((row >= high) | (lse == kNegInf)) ? INFINITY : lse;
-    float slope = 0;
-    if constexpr (MOD) slope = s.slopes ? s.slopes[qh] : 0.0f;
+    u32x4 q[KS];
+#pragma unroll
+    for (int x = 0; x < KS; ++x) q[x] = operand(lq, x);
+    const Rows at = now;
+    if (item + share < items) {
+      // Both are in registers: their places in LDS are free.
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      asm volatile("" ::: "memory");
+      while (item + share >= (head + 1) * blocks) ++head;
+      if (head != held) ask_keys(head);
+      now = ask(head, item + share);
+    }
     f32x16 st;
 #pragma unroll
     for (int e = 0; e < 16; ++e) st[e] = 0;
 #pragma unroll
-    for (int x = 0; x < KS; ++x) {
-      const int d = 16 * x + 8 * h;
-      u32x4 q = {0, 0, 0, 0};
-      if (d < D) {
-        if (vector) {
-          q = gload<u32x4>(as_global(static_cast<const void*>(qp + 2 * d)));
-        } else {
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            q[w] = load_elem<uint16_t>(qp + 2 * d + 4 * w) | static_cast<uint32_t>(load_elem<uint16_t>(qp + 2 * d + 4 * w + 2)) << 16;
-        }
-      }
-      st = H::mul(k[x], q, st);
-    }
-    kr.p0 = r.length - r.n + row0 / s.group;
-    kr.p1 = r.length - r.n + min(row0 + 31, high - 1) / s.group;
+    for (int x = 0; x < KS; ++x) st = H::mul(k[x], q[x], st);
+    kr.p0 = r.length - r.n + token_of_row(s, at.row0);
+    kr.p1 = r.length - r.n + token_of_row(s, min(at.row0 + 31, high - 1));
     const bool whole = sees_all(s, kr, start, start + 32);
-    if constexpr (MOD) modify_scores(s, st, 1.0f, slope, p, start, h);
+    if constexpr (MOD) modify_scores(s, st, 1.0f, at.slope, at.p, start, h);
     // The difference first: what is near the row's maximum keeps its bits.
-    auto weight = [&](int e) { return exp2_fast((MOD ? st[e] - lse : __builtin_fmaf(st[e], s.scale, -lse)) * kLog2e); };
+    auto weight = [&](int e) { return exp2_fast((MOD ? st[e] - at.lse : __builtin_fmaf(st[e], s.scale, -at.lse)) * kLog2e); };
     if (whole) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) sum[e] += weight(e);
@@ -1801,7 +1866,7 @@ __global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 2 : 4) void key_w
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const float w = weight(e);
-        sum[e] += sees(s, kr, p, start + 8 * (e >> 2) + 4 * h + (e & 3)) ? w : 0.0f;
+        sum[e] += sees(s, kr, at.p, start + 8 * (e >> 2) + 4 * h + (e & 3)) ? w : 0.0f;
       }
     }
   }
@@ -2150,6 +2215,7 @@ int check_scores(const cb_query_batch* batch, int32_t layer, int32_t dtype, int3
   s->q_heads = q_heads;
   s->kv_heads = kv;
   s->group = q_heads / kv;
+  s->group_shift = (s->group & (s->group - 1)) ? -1 : __builtin_ctz(static_cast<unsigned>(s->group));
   s->scale = sc->scale;
   s->cap = sc->cap;
   s->window = sc->window;
