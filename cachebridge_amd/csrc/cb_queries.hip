@@ -1732,22 +1732,17 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void key_weights_any_kernel(W
 }
 
 // 16-bit form: a wave holds 32 keys of one KV head as MFMA operands in
-// registers and walks blocks of 32 query rows; S^T keeps a row a lane pair, so a
-// key's sum over rows is a sum over lanes, made once at the end. The waves that
-// share a block of keys (4 if there are 4 or more blocks of rows to walk, else
-// fewer, so that none idles) meet in LDS in wave order.
-//
-// Keys and query rows come through LDS of the wave's own: loaded straight into
-// operands, four lanes in a row touch four rows, and the address unit takes a
-// cycle for each lane of such a load (1 us for four blocks of rows a CU).
+// registers and walks blocks of 32 query rows, whose operands come straight
+// from memory (the few rows of a batch stay in cache); S^T keeps a row a lane
+// pair, so a key's sum over rows is a sum over lanes, made once at the end.
+// The waves that share a block of keys (4 if there are 4 or more blocks of
+// rows to walk, else fewer, so that none idles) meet in LDS in wave order.
 constexpr int kWeightWaves = 4;
 
 template <typename IO, int DP, bool MOD>
-__global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 1 : 2) void key_weights_kernel(WeightArgs a, int vector) {
+__global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 2 : 4) void key_weights_kernel(WeightArgs a, int vector) {
   typedef Half<IO> H;
-  typedef RowBlock<IO, DP, 32, MOD> Block;
-  constexpr int KS = DP / 16, kTile = 32 * DP * 2, N = kTile / 1024, C = DP / 8;
-  __shared__ __align__(1024) char tiles[kWeightWaves * 2 * kTile];  // a wave's keys, then its rows
+  constexpr int KS = DP / 16;
   __shared__ float sums[kWeightWaves][32];
   const ScoreArgs& s = a.s;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -1768,96 +1763,56 @@ __global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 1 : 2) void key_w
   if ((j < r.length) & (mine < 0) & (sub == 0) & (h == 0)) flag(s.batch.err, CB_ERROR_CACHE_ROW);
   const uint32_t there = static_cast<uint32_t>(__ballot(mine >= 0));
   const int D = s.head_dim;
-  const int low = i0 * s.group, high = i1 * s.group, blocks = (high - low + 31) / 32, items = s.kv_heads * blocks;
-  const uint32_t lk = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((CB_LDS_SPACE char*)tiles)) + wave * 2 * kTile, lq = lk + kTile;
-  const typename Block::Lanes lanes = Block::lanes();
-  auto operand = [&](uint32_t base, int x) __attribute__((always_inline)) { return *lds_at<const u32x4>(lanes.k[x & 7] + base + (x >> 3) * 256); };
-
-  // 32 rows to LDS at `to`; lane y < 32 holds the y-th one's address.
-  auto stage = [&](uint64_t row, uint32_t there, uint32_t to, bool direct) __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int y = u * (kWave / C) + lane / C, chunk = (lane % C) ^ swizzle_k<DP>(y);
-      const uint64_t at = static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(row), y))) |
-                          static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(row >> 32), y))) << 32;
-      const bool in = ((there >> y) & 1) & (chunk * 8 < D);
-      if (direct) {
-        dma16(in ? reinterpret_cast<gcptr>(at) + chunk * 16 : as_global(static_cast<const void*>(g_zeros)), to + u * 1024);
-      } else {
-        u32x4 x = {0, 0, 0, 0};
-        if (in) {
-          const char* from = reinterpret_cast<const char*>(at) + chunk * 16;
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            x[w] = load_elem<uint16_t>(from + 4 * w) | static_cast<uint32_t>(load_elem<uint16_t>(from + 4 * w + 2)) << 16;
-        }
-        *lds_at<u32x4>(to + u * 1024 + lane * 16) = x;
-      }
-    }
-  };
-  struct Rows {
-    float lse, slope;
-    int row0, p;
-  };
-  auto ask = [&](int head, int item) __attribute__((always_inline)) {
-    Rows x;
-    x.row0 = low + (item - head * blocks) * 32;
-    const int row = x.row0 + c, at = min(row, high - 1), i = token_of_row(s, at), qh = head * s.group + at - i * s.group;
-    x.p = r.length - r.n + i;
-    const float lse = a.lse[static_cast<int64_t>(r.q0 + i) * s.q_heads + qh];
-    // Nothing is added by lanes past the last row and rows that see nothing.
-    x.lse = ((row >= high) | (lse == kNegInf)) ? INFINITY : lse;
-    x.slope = 0;
-    if constexpr (MOD) x.slope = s.slopes ? s.slopes[qh] : 0.0f;
-    stage(reinterpret_cast<uint64_t>(s.q.data) + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b, ~0u, lq, vector != 0);
-    return x;
-  };
-  auto ask_keys = [&](int head) __attribute__((always_inline)) {
-    const uint64_t base = reinterpret_cast<uint64_t>(layer_base(s.cache, 0, s.layer)) + static_cast<int64_t>(head) * D * 2;
-    stage(base + (mine >= 0 ? mine : 0) * s.batch.row_stride_b, there, lk, true);
-  };
-
+  const int low = i0 * s.group, high = i1 * s.group, blocks = (high - low + 31) / 32;
   float sum[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) sum[e] = 0;
+  int held = -1;
   u32x4 k[KS];
-  Rows now{};
-  int head = 0, held = -1;
-  if (sub < items) {
-    while (sub >= (head + 1) * blocks) ++head;
-    ask_keys(head);
-    now = ask(head, sub);
-  }
-  for (int item = sub; item < items; item += share) {
-    wait_own();
+  for (int item = sub; item < s.kv_heads * blocks; item += share) {
+    const int head = item / blocks, row0 = low + (item - head * blocks) * 32;
     if (head != held) {
       held = head;
+      gcptr kp = layer_base(s.cache, 0, s.layer) + static_cast<int64_t>(head) * D * 2 + mine * s.batch.row_stride_b;
 #pragma unroll
-      for (int x = 0; x < KS; ++x) k[x] = operand(lk, x);
+      for (int x = 0; x < KS; ++x) {
+        const int d = 16 * x + 8 * h;
+        k[x] = u32x4{0, 0, 0, 0};
+        if ((mine >= 0) & (d < D)) k[x] = gload<u32x4>(kp + 2 * d);
+      }
     }
-    u32x4 q[KS];
-#pragma unroll
-    for (int x = 0; x < KS; ++x) q[x] = operand(lq, x);
-    const Rows at = now;
-    if (item + share < items) {
-      // Both are in registers: their places in LDS are free.
-      __builtin_amdgcn_s_waitcnt(0xc07f);
-      asm volatile("" ::: "memory");
-      while (item + share >= (head + 1) * blocks) ++head;
-      if (head != held) ask_keys(head);
-      now = ask(head, item + share);
-    }
+    const int row = row0 + c, at = min(row, high - 1), i = at / s.group, qh = head * s.group + at - i * s.group;
+    const int p = r.length - r.n + i;
+    const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
+    float lse = a.lse[static_cast<int64_t>(r.q0 + i) * s.q_heads + qh];
+    // Nothing is added by lanes past the last row and rows that see nothing.
+    lse = ((row >= high) | (lse == kNegInf)) ? INFINITY : lse;
+    float slope = 0;
+    if constexpr (MOD) slope = s.slopes ? s.slopes[qh] : 0.0f;
     f32x16 st;
 #pragma unroll
     for (int e = 0; e < 16; ++e) st[e] = 0;
 #pragma unroll
-    for (int x = 0; x < KS; ++x) st = H::mul(k[x], q[x], st);
-    kr.p0 = r.length - r.n + token_of_row(s, at.row0);
-    kr.p1 = r.length - r.n + token_of_row(s, min(at.row0 + 31, high - 1));
+    for (int x = 0; x < KS; ++x) {
+      const int d = 16 * x + 8 * h;
+      u32x4 q = {0, 0, 0, 0};
+      if (d < D) {
+        if (vector) {
+          q = gload<u32x4>(as_global(static_cast<const void*>(qp + 2 * d)));
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            q[w] = load_elem<uint16_t>(qp + 2 * d + 4 * w) | static_cast<uint32_t>(load_elem<uint16_t>(qp + 2 * d + 4 * w + 2)) << 16;
+        }
+      }
+      st = H::mul(k[x], q, st);
+    }
+    kr.p0 = r.length - r.n + row0 / s.group;
+    kr.p1 = r.length - r.n + min(row0 + 31, high - 1) / s.group;
     const bool whole = sees_all(s, kr, start, start + 32);
-    if constexpr (MOD) modify_scores(s, st, 1.0f, at.slope, at.p, start, h);
+    if constexpr (MOD) modify_scores(s, st, 1.0f, slope, p, start, h);
     // The difference first: what is near the row's maximum keeps its bits.
-    auto weight = [&](int e) { return exp2_fast((MOD ? st[e] - at.lse : __builtin_fmaf(st[e], s.scale, -at.lse)) * kLog2e); };
+    auto weight = [&](int e) { return exp2_fast((MOD ? st[e] - lse : __builtin_fmaf(st[e], s.scale, -lse)) * kLog2e); };
     if (whole) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) sum[e] += weight(e);
@@ -1866,7 +1821,7 @@ __global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 1 : 2) void key_w
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const float w = weight(e);
-        sum[e] += sees(s, kr, at.p, start + 8 * (e >> 2) + 4 * h + (e & 3)) ? w : 0.0f;
+        sum[e] += sees(s, kr, p, start + 8 * (e >> 2) + 4 * h + (e & 3)) ? w : 0.0f;
       }
     }
   }
