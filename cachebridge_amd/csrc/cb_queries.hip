@@ -956,6 +956,7 @@ template <>
 struct Half<io_bf16> {
   typedef io_bf16 x8 __attribute__((ext_vector_type(8)));
   static constexpr uint32_t kExponent = 0x7f807f80u, kCarry = 0x00800080u, kInf = 0x7f80u;
+  static constexpr float kRoom = 0, kLag = 1024;
   static __device__ inline f32x16 mul(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
   }
@@ -966,6 +967,9 @@ struct Half<io_f16> {
   typedef io_f16 x8 __attribute__((ext_vector_type(8)));
   typedef io_f16 x2 __attribute__((ext_vector_type(2)));
   static constexpr uint32_t kExponent = 0x7c007c00u, kCarry = 0x04000400u, kInf = 0x7c00u;
+  // Weights count from 2^8, not 1: the many small ones of a long request keep
+  // eight more bits above the type's least step of 2^-24.
+  static constexpr float kRoom = 8, kLag = 32768;
   static __device__ inline f32x16 mul(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
   }
@@ -979,7 +983,6 @@ struct Half<io_f16> {
 __device__ const uint4 g_zeros[1] = {};
 
 constexpr int kMaxDp = 256;
-constexpr float kLag = 1024;  // a lane's sum of weights of a tile up to which its maximum may stand
 
 template <int DP>
 __device__ inline int swizzle_k(int key) {
@@ -1211,19 +1214,19 @@ struct RowBlock {
   }
   // A row's maximum is looked for only if a lane's weights show that it has
   // grown by much (their sum tells) or is not known yet: up to kLag, weights
-  // lose no digits in fp32 sums or 16 bits. Vector instructions that are not
+  // lose no digits in fp32 sums or 16 bits (m is the maximum less kRoom). Vector instructions that are not
   // exponentials cost the matrix unit their time here (16 ns a product alone or
   // beside 2 exponentials a wave, 26 ns with 6 multiply-adds more), so the
   // maxima of every tile would.
   CB_INLINE void weights(const f32x16 (&st)[KB], float scale2, u32x4 (&w)[KB][2]) {
     float sum = try_weights(st, scale2, w);
-    if (__any(!(sum < kLag) | (m == kNegInf))) {
+    if (__any(!(sum < H::kLag) | (m == kNegInf))) {
       float top = kNegInf;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, st[kb][e]);
-      top *= scale2;
+      top = __builtin_fmaf(top, scale2, -H::kRoom);
       const float m1 = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
       const float alpha = m1 == kNegInf ? 1.0f : exp2_fast(m - m1);
       m = m1;
@@ -1899,22 +1902,19 @@ __global__ __launch_bounds__(kSelectThreads) void select_tokens_kernel(EvictArgs
   const int b = blockIdx.x;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int length = evict_length(a, b);
-  if (length < 0) {  // its outputs stay as they were; nothing is copied
-    if (threadIdx.x == 0) flag(a.batch.err, CB_ERROR_REQUEST);
-    return;
-  }
+  if (length < 0 && threadIdx.x == 0) flag(a.batch.err, CB_ERROR_REQUEST);  // nothing of it is kept
   const int64_t slot0 = static_cast<int64_t>(b) * a.budget;
   const float* w = a.weights + b * a.weights_stride;
   int32_t* kept = a.kept + slot0;
   float* kept_weights = a.kept_weights + slot0;
-  const int n = min(length, a.budget);
+  const int n = max(0, min(length, a.budget));
   if (threadIdx.x == 0) a.kept_lengths[b] = n;
   for (int j = n + threadIdx.x; j < a.budget; j += kSelectThreads) {
     kept[j] = -1;
     kept_weights[j] = 0.0f;
   }
   const bool choose = length > a.budget;
-  const int head = choose ? a.first : length, tail = choose ? a.last : 0;
+  const int head = choose ? a.first : n, tail = choose ? a.last : 0;
   for (int j = threadIdx.x; j < head; j += kSelectThreads) {
     kept[j] = j;
     kept_weights[j] = w[j];

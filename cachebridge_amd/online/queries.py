@@ -111,6 +111,13 @@ class QueryBatch:
         if rows.c.k_layers and any(t.data_ptr() % 16 for t in rows.keep if t.ndim == 3):
             raise ValueError("pool layers must be 16-byte aligned")
         requests = lengths.numel()
+        # The C fields are 32 bits wide, and ctypes drops what does not fit.
+        if not 0 <= max_length <= 1 << 30:
+            raise ValueError("max_length must be 0 to 2^30")
+        if max_query is not None and max_query < 0:
+            raise ValueError("max_query must not be negative")
+        if not 0 <= request_stride <= 1 << 31:
+            raise ValueError("request_stride must be 0 to 2^31")
         c = _lib.CbQueryBatch()
         c.cache = rows.c
         c.index_entries = rows.index_entries
@@ -135,6 +142,11 @@ class QueryBatch:
     @property
     def kv_heads(self) -> int:
         return self.c.cache.heads
+
+    def _layer(self, layer: int) -> int:
+        if not 0 <= layer < self.rows.num_layers:
+            raise ValueError(f"layer {layer} outside the cache")
+        return layer
 
     def _tokens(self, n: int):
         """The C description for token tensors of ``n`` rows (a copy: calls may run side by side)."""
@@ -212,7 +224,7 @@ def install_tokens(batch: QueryBatch, layer: int, q: torch.Tensor, k: torch.Tens
             out = q.new_empty((n, heads, dim))
         co = batch._heads(out, "out", n, heads)
         _lib.check(_lib.load().cb_install_tokens(
-            batch._tokens(n), layer, batch._code, dim, ctypes.byref(cq), ctypes.byref(co), ctypes.byref(ck),
+            batch._tokens(n), batch._layer(layer), batch._code, dim, ctypes.byref(cq), ctypes.byref(co), ctypes.byref(ck),
             ctypes.byref(cv), inv.data_ptr(), 2 * inv.numel(), int(rotary.interleaved), rotary.magnitude, pos, kind,
             flag, handle))
         batch.rows.hold_for(stream)
@@ -220,6 +232,8 @@ def install_tokens(batch: QueryBatch, layer: int, q: torch.Tensor, k: torch.Tens
 
 
 def _scores(batch: QueryBatch, heads: int, dim: int, scale, causal, window, cap, slopes, prefix_lengths):
+    if not 0 <= window <= 0x7FFFFFFF:
+        raise ValueError("window must be 0 to 2^31 - 1")
     c = _lib.CbScores(dim ** -0.5 if scale is None else scale, cap, window, int(causal))
     if not math.isfinite(c.scale):
         raise ValueError("scale must be finite")
@@ -268,7 +282,7 @@ def paged_attention(batch: QueryBatch, layer: int, q: torch.Tensor, *, scale: fl
                                                     ctypes.byref(need)))
         work = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
         _lib.check(lib.cb_paged_attention(
-            c, layer, batch._code, dim, ctypes.byref(scores), ctypes.byref(cq), ctypes.byref(co),
+            c, batch._layer(layer), batch._code, dim, ctypes.byref(scores), ctypes.byref(cq), ctypes.byref(co),
             None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), need.value, flag,
             handle))
         batch.rows.hold_for(stream)
@@ -295,7 +309,7 @@ def add_key_weights(batch: QueryBatch, layer: int, q: torch.Tensor, lse: torch.T
     flag = _flag_pointer(batch, error_flag)
     with _On(batch, stream) as handle:
         _lib.check(_lib.load().cb_add_key_weights(
-            batch._tokens(n), layer, batch._code, dim, ctypes.byref(scores), ctypes.byref(cq), lse.data_ptr(),
+            batch._tokens(n), batch._layer(layer), batch._code, dim, ctypes.byref(scores), ctypes.byref(cq), lse.data_ptr(),
             weights.data_ptr(), stride, flag, handle))
         batch.rows.hold_for(stream)
 
@@ -313,8 +327,9 @@ def _weights_stride(batch: QueryBatch, weights: torch.Tensor) -> int:
 @dataclass
 class KeptTokens:
     """What an eviction kept: ``tokens`` and ``weights`` ``[requests, budget]``
-    (then -1 and 0), ``lengths`` ``[requests]``. ``tokens`` holds the places
-    the kept tokens had, which stay their positions."""
+    (then -1 and 0), ``lengths`` ``[requests]`` (0 for a request outside the
+    batch's bounds). ``tokens`` holds the places the kept tokens had, which
+    stay their positions."""
 
     tokens: torch.Tensor
     lengths: torch.Tensor
@@ -342,8 +357,8 @@ def evict_tokens(batch: QueryBatch, weights: torch.Tensor, target: QueryBatch, *
     dim = batch.head_dim
     if target.kv_heads != batch.kv_heads or target.head_dim != dim or target.rows.num_layers != batch.rows.num_layers:
         raise ValueError("batch and target must share layers, KV heads and head_dim")
-    if budget < 1 or first < 0 or last < 0 or first + last > budget:
-        raise ValueError("budget must be positive and hold the first and last tokens")
+    if not 1 <= budget <= 1 << 30 or first < 0 or last < 0 or first + last > budget:
+        raise ValueError("budget must be 1 to 2^30 and hold the first and last tokens")
     flag = _flag_pointer(batch, error_flag)
     b, dev = batch.requests, batch.device
     with _On(batch, stream) as handle:

@@ -401,7 +401,8 @@ int cb_add_key_weights(const cb_query_batch* batch, int32_t layer, int32_t dtype
    (another pool, or pages of this one that no kept token is read from).
    kept [requests][budget] gets the cached token of each, then -1;
    kept_lengths [requests] their count; kept_weights [requests][budget] their
-   weights, then 0. Of `target` the cache, index, offsets and request_stride
+   weights, then 0. A request outside the batch's bounds is flagged and keeps
+   none. Of `target` the cache, index, offsets and request_stride
    are read. Asynchronous. */
 int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, int32_t dtype,
                     int32_t head_dim, const float* weights, int64_t weights_stride, int32_t budget,

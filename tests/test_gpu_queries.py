@@ -233,6 +233,26 @@ def test_large_scores(dtype):
     check_attention(case, *attend(case, scale=0.0), scale=0.0)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("new", [1, 40, 600])
+def test_many_small_weights_keep_their_sum(new, dtype):
+    """One token takes nearly all the weight; 65535 others have 1.02 * 2^-25 of its."""
+    n, dim, w = 65536, 64, 1.02 * 2.0 ** -25
+    k, v = torch.zeros(1, n, 1, dim, dtype=dtype).cuda(), torch.ones(1, n, 1, dim, dtype=dtype).cuda()
+    k[0, 0], v[0, 0] = 1, 0
+    start, lengths = torch.tensor([0, new]).int().cuda(), torch.tensor([n]).int().cuda()
+    batch = QueryBatch(rows_from_stacked(k, v), start, lengths, max_length=n)
+    out = paged_attention(batch, 0, torch.ones(new, 1, dim, dtype=dtype).cuda(), scale=-math.log(w) / dim, causal=False)
+    want = (n - 1) * w / (1 + (n - 1) * w)
+    # Scores of 17.3 in fp32: two roundings of 2^-24 of them, times as much again for the exponential. A weight's
+    # rounding: half a step of the type; fp16 weights of 1.02 * 2^-17 (they count from 2^8) have a step of 2^-24.
+    half = torch.finfo(dtype).eps / 2
+    weight = {BF16: half, FP16: 2.0 ** -25 / (1.02 * 2.0 ** -17), FP32: half}[dtype]
+    # fp32 sums of 65536 terms in chains of at most 65536 / 16, each step off by 2^-24.
+    tolerance = weight + half + 4 * 17.4 * 2.0 ** -24 + 4096 * 2.0 ** -24
+    assert ((out.double() / want - 1).abs() <= tolerance).all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_rows_of_no_request_and_strides(dtype):
     case = make([40, 90], [6, 11], heads=6, kv_heads=2, dim=128, dtype=dtype, seed=11, padding=5)
@@ -477,6 +497,25 @@ def test_evict_bad_rows_are_flagged():
     assert (k[0, 32:] == 0).all()
 
 
+def test_evict_keeps_nothing_of_a_request_outside_the_bounds():
+    case = make([50, 50, 50], [1, 1, 1], heads=2, kv_heads=2, dim=64, index="i32", seed=2)
+    qs, ln, off = case.batch._keep
+    ln = ln.clone()
+    ln[0], ln[2] = -1, 51
+    batch = QueryBatch(rows_from_stacked(*case.pool, index=case.batch.rows.keep[-1]), qs, ln, offsets=off, max_length=50)
+    k, v = torch.zeros(1, 96, 2, 64, dtype=BF16).cuda(), torch.zeros(1, 96, 2, 64, dtype=BF16).cuda()
+    target = QueryBatch(rows_from_stacked(k, v), qs, ln, request_stride=32, max_length=50)
+    for budget in (20, 60):  # fewer than a request has, and more
+        torch.full((64, 1 << 10), -7, dtype=torch.int32).cuda()  # what new tensors may be made of
+        flag = torch.zeros(1, dtype=torch.int32).cuda()
+        kept = evict_tokens(batch, torch.ones(3, 50).cuda(), target, budget=budget, error_flag=flag)
+        assert int(flag) & ERROR_REQUEST and kept.lengths.tolist() == [0, min(budget, 50), 0]
+        for b in (0, 2):
+            assert (kept.tokens[b] == -1).all() and (kept.weights[b] == 0).all()
+        # Request 1 has rows 32 to 32 + 49 at most; all others stay.
+        assert (k[0, :32] == 0).all() and (k[0, 82:] == 0).all() and (k[0, 32:52] != 0).any()
+
+
 def _serve(case, spin, fused, weights, stream=None):
     """One pass of all operators: store the new tokens, attend, add weights."""
     h, kv = case.heads, case.kv_heads
@@ -624,3 +663,19 @@ def test_refusals_on_the_gpu():
     with pytest.raises(ValueError, match="positions"):
         install_tokens(case.batch, 0, q, q[:, :2], q[:, :2], Rotary.build(64, 1e4), positions=torch.zeros(2).long().cuda())
     assert paged_attention(case.batch, 0, q[:0]).shape == (0, 4, 64)
+
+
+def test_integers_past_32_bits_are_refused():
+    case = make([40], [2], heads=2, kv_heads=1, dim=64)
+    qs, ln, off = case.batch._keep
+    big = 1 << 32
+    q = case.q.cuda()
+    with pytest.raises(ValueError, match="layer"):
+        paged_attention(case.batch, big, q)
+    with pytest.raises(ValueError, match="window"):
+        paged_attention(case.batch, 0, q, window=big + 5)
+    for kw in (dict(max_length=big + 40), dict(max_length=40, max_query=-big), dict(max_length=40, request_stride=1 << 64)):
+        with pytest.raises(ValueError, match=list(kw)[-1]):
+            QueryBatch(case.batch.rows, qs, ln, **kw)
+    with pytest.raises(ValueError, match="budget"):
+        evict_tokens(case.batch, torch.zeros(1, 40).cuda(), case.batch, budget=big + 1)

@@ -226,7 +226,8 @@ def test_no_query_kernel_uses_scratch(built_library, tmp_path):
                 if "private_segment_fixed_size" in fields:
                     kernels[block.split()[0]] = {k: int(v) for k, v in fields.items()}
     names = " ".join(kernels)
-    for expected in ("map_install_stream_kernel", "install_tokens_kernel", "attend_any_kernel", "join_splits_kernel",
-                     "key_weights_any_kernel", "select_tokens_kernel", "move_rows_kernel"):
+    for expected in ("map_install_stream_kernel", "install_tokens_kernel", "attend_any_kernel", "attend_tile_kernel",
+                     "attend_step_kernel", "join_few_kernel", "join_splits_kernel", "key_weights_any_kernel",
+                     "key_weights_kernel", "select_tokens_kernel", "move_rows_kernel"):
         assert expected in names, expected
     assert not {n: m for n, m in kernels.items() if any(m.values())}
