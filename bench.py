@@ -351,7 +351,7 @@ def sampled_parity(h, sh, label: str) -> dict:
     return out
 
 
-KERNEL_SOURCES = [ROOT / "cachebridge_amd" / "csrc" / name for name in ("cb_handoff.hip", "cb_items.h")]
+KERNEL_SOURCES = [ROOT / "cachebridge_amd" / "csrc" / name for name in ("cb_handoff.hip", "cb_items.h", "cb_common.h")]
 
 
 def kernel_source_sha16() -> str:
