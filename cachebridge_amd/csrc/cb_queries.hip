@@ -232,10 +232,14 @@ __device__ inline void store_vec(char* p, const float* in) {
   }
 }
 
-// One wave per (token, slice of its heads' elements). Lanes compute the
-// token's angles once into LDS, then each item is V pairs of a head (two
-// vectors) or V elements that are copied. Bound by memory: every element is
-// read once and written once.
+// y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin for the pairs (a, b) of the
+// rotated part, angles position * inv_freq. One wave per (token, slice of its
+// heads' elements): lanes compute the token's angles once into LDS, then each
+// item is V pairs of a head (two vectors) or V elements that are copied; slices
+// are cut to an item a lane, so that a wave waits for memory once. Every element
+// is read once and written once: 2048 tokens of 16 query and 2 KV heads of 128
+// in bf16 (21 MB) take 8.7 us, 2.4 TB/s with the launch; 64 tokens of 64 and 8
+// heads 4.7 us, the latency of a launch and of three dependent loads.
 template <typename IO, int V>
 __global__ __launch_bounds__(kInstallWaves * kWave) void install_tokens_kernel(InstallArgs a) {
   __shared__ float2 turn[kInstallWaves][kMaxPairs];
@@ -537,7 +541,10 @@ CB_INLINE void place_rows(const QBatch& B, const Request& r, int64_t entry, int 
 // tiles of 16 keys in LDS, 16 query rows each; the next tile's elements are
 // loaded into registers (VE at a time: 16 bytes where rows allow it, else one)
 // while a tile is used. Rows in LDS are DP + 4 floats apart, which puts the 16
-// rows and 4 columns of an operand in distinct banks.
+// rows and 4 columns of an operand in distinct banks. A prompt of 250 fp32
+// tokens with 4 heads of 64 takes 15.8 us and its join 5.0 us: at this size the
+// two barriers and the row lookup of each tile bound it, not its 37 MFLOP; with
+// a tile's loads waited for in place it was 41 us.
 // ---------------------------------------------------------------------------
 
 constexpr int kAnyWaves = 4;
@@ -803,8 +810,13 @@ CB_INLINE int row_splits(const AttendArgs& a, int t, int qh, int rows_per_tile) 
 }
 
 // Joins few splits: out = sum 2^(lse_z - lse) out_z, a wave a row. Lane z holds
-// split z's statistics, then every lane E elements of the row.
-constexpr int kJoinFew = 16;
+// split z's statistics, then every lane E elements of the row. Taken where
+// there are rows enough for all CUs: with 128 new tokens (2048 rows of 128) over
+// 4096 it takes 6.6 us where a workgroup a row takes 7.9, with 64 times 16
+// tokens 13.4 against 37.2, with 1000 rows of 64 5.0 against 5.8; with 37 tokens
+// (592 rows) 5.9 against 5.1, with 4 9.0 against 5.0.
+constexpr int kJoinFew = 16;    // splits up to which, and
+constexpr int kJoinRows = 768;  // rows from which it is taken
 
 template <typename IO, int KT, int E>
 __global__ __launch_bounds__(256) void join_few_kernel(AttendArgs a, int rows_per_tile) {
@@ -1370,7 +1382,15 @@ CB_INLINE void mark_not_finite(uint32_t lv, int np, int below, int above, int st
 }
 
 // Many query rows: a workgroup's NW waves hold 32 rows each and share K and V
-// tiles, double buffered: while a tile is used the next one arrives.
+// tiles, double buffered: while a tile is used the next one arrives. 2048 new
+// tokens over 32768 (16 heads of 128, 2 KV heads, bf16, 533 GFLOP) take 534 us,
+// 1.00 PFLOP/s, where a library product of 8192^3 reaches 1.21. What bounds it:
+// matrix steps and vector instructions that are not exponentials do not overlap
+// (see RowBlock::weights), so a tile costs its products plus its multiply-adds,
+// packs and sums. 32 rows a wave: 64 have twice the products a K or V operand
+// read, but took twice the time (1080 us; one wave a SIMD is left, and nothing
+// runs while it waits). 64 keys a tile where they fit two workgroups' LDS:
+// 32 took 847 us where 64 took 640.
 template <typename IO, int DP, int KT, int NW, bool MOD>
 __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_kernel(AttendArgs a, int vector) {
   constexpr int kTile = KT * DP * 2, N = kTile / 1024 / NW;
@@ -1475,7 +1495,11 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_ker
 // of K and V are in flight, the next K is asked for as soon as the products
 // have read its place, the next V after its sums. The rows that the index
 // names are resolved into LDS first, so that the loop's only vector memory
-// operations are the DMA, whose count tells what has arrived.
+// operations are the DMA, whose count tells what has arrived. One request of
+// 32768 tokens (64 heads of 128, 8 KV heads, bf16, 134 MB) takes 32 us, 4.2 TB/s,
+// as fast as this card reads; 64 ragged requests of 2550 on average (16 heads,
+// 2 KV heads, 167 MB) 47.5 us, 3.5 TB/s: ragged lengths leave
+// CUs without work at the end.
 constexpr int kStepTiles = 64;  // tiles a split holds at most
 
 template <typename IO, int DP, int NW, bool MOD>
@@ -1669,6 +1693,9 @@ CB_INLINE void query_range(const ScoreArgs& s, const Request& r, int np, int sta
   if (s.window > 0) *i1 = max(*i0, static_cast<int>(min(static_cast<int64_t>(r.n), static_cast<int64_t>(start) + keys - 1 + s.window - first)));
 }
 
+// w_j = sum over rows of exp(score - lse): one workgroup owns a key, so its sum
+// needs no atomics and has one order.
+//
 // General form: a workgroup owns 16 keys of a request, its waves take every
 // fourth block of 16 query rows of each KV head; partial sums meet in LDS in
 // wave order.
@@ -1740,6 +1767,12 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void key_weights_any_kernel(W
 // pair, so a key's sum over rows is a sum over lanes, made once at the end.
 // The waves that share a block of keys (4 if there are 4 or more blocks of
 // rows to walk, else fewer, so that none idles) meet in LDS in wave order.
+// 32 tokens over 32768 (16 heads of 128, 2 KV heads, bf16, 17 MB, 4.3 GFLOP)
+// take 28.3 us, 64 ragged steps over 2550 on average (85 MB) 29.8 us. Bound by
+// vector instructions and the address unit: a block of 32 rows and 32 keys has 8
+// products and some 260 other instructions, and four lanes of an operand's load
+// touch as many rows. Keys and rows through LDS of the wave's own took 26.1 and
+// 39.9 us: fewer waves then have loads in flight.
 constexpr int kWeightWaves = 4;
 
 template <typename IO, int DP, bool MOD>
@@ -1893,7 +1926,10 @@ constexpr int kBins = 2048, kBinCopies = 8, kCopyStride = kBins + 8;
 // that share the digits so far, then the bin in which the count from the top
 // reaches what is needed. Counts are integers, so the order of the adds does
 // not matter. R ranks a lane stay in registers (R * 1024 tokens between the
-// first and the last), R = 0 reads the weights again on every pass.
+// first and the last), R = 0 reads the weights again on every pass. 4096 of
+// 16384 tokens take 23 us, 700 of some 2000 in 16 requests 15 us: three rounds
+// of clearing, adding and scanning bins with a barrier between each, on one CU a
+// request. Adds of equal digits gathered by ballots first took 37 us.
 template <int R>
 __global__ __launch_bounds__(kSelectThreads) void select_tokens_kernel(EvictArgs a) {
   __shared__ __align__(16) int bins[kCopyStride * kBinCopies];
@@ -2032,7 +2068,10 @@ struct MoveArgs {
 
 // Every layer's K and V rows of the kept tokens. A workgroup moves a run of
 // one request's tokens in one layer; each thread resolves the rows of four
-// chunks, then has the four loads in flight, then stores.
+// chunks, then has the four loads in flight, then stores. Bound by memory: 4096
+// tokens of 64 layers of 2 heads of 128 in bf16 (537 MB read and written) take
+// 113 us, 4.8 TB/s; 16 requests' 700 of 62 layers 284 us, 5.0 TB/s, a plain
+// copy's rate.
 template <typename V>
 __global__ __launch_bounds__(256) void move_rows_kernel(MoveArgs a) {
   constexpr int U = 4;
@@ -2184,7 +2223,10 @@ int check_scores(const cb_query_batch* batch, int32_t layer, int32_t dtype, int3
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
-constexpr int kTargetGroups = 512;  // workgroups of four waves that fill the 256 CUs twice
+// Workgroups of four waves that a launch is split into at least: two a CU. 512 new
+// tokens over 32768 take 262, 173 and 185 us with 256, 512 and 1024, 64 requests of
+// 8 new tokens over 2048 47, 38.5 and 39 us.
+constexpr int kTargetGroups = 512;
 
 // How the launch is cut: query tiles, and key splits where the tiles alone
 // would leave CUs idle.
@@ -2209,7 +2251,16 @@ bool takes_half(const ScoreArgs& s, int32_t dtype) {
 // 32768 106 / 120; 1000 of 1000 with 8 heads 39.4 / 34.1.
 constexpr int kWideRows = 512;               // query rows per KV head, and
 constexpr int64_t kWideScores = 24ll << 20;  // scores of the launch, from which eight are taken
-constexpr int kStepRows = 32;  // query rows per KV head up to which attend_step_kernel is taken
+// Query rows per KV head up to which attend_step_kernel is taken: one block of
+// rows, so that K and V are read once (8 query heads a KV head, this kernel against
+// the tile kernel: 64 ragged requests of 2550 on average, one new token 47 / 94
+// us, four 51 / 88; one request of 32768, 31 / 35 and 38 / 37; two blocks, 64
+// requests of 8 new tokens, 68 / 38. Where all lengths are alike the tile kernel
+// is as good: 64 of 2048 39 / 35).
+constexpr int kStepRows = 32;
+// Its workgroups: one request has all its splits at work, of several requests many
+// are shorter than the bound that splits are cut by. 512, 1024, 2048: one request
+// of 32768 tokens 34, 40, 40 us; 64 ragged ones 73, 47, 60 us (64 alike 31, 39, 39).
 constexpr int kStepGroups = 512, kStepGroupsRagged = 1024;
 constexpr int kStepWaves = 2;
 
@@ -2254,7 +2305,7 @@ template <typename IO, int KT>
 void launch_join(const AttendArgs& a, const AttendShape& h, hipStream_t st) {
   if (h.splits <= 1) return;
   const int64_t rows = static_cast<int64_t>(a.s.batch.tokens) * a.s.q_heads;
-  if (h.splits <= kJoinFew) {
+  if (h.splits <= kJoinFew && rows >= kJoinRows) {
     const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
     if (a.s.head_dim <= 128) hipLaunchKernelGGL((join_few_kernel<IO, KT, 2>), grid, dim3(256), 0, st, a, h.rows_per_tile);
     else hipLaunchKernelGGL((join_few_kernel<IO, KT, 8>), grid, dim3(256), 0, st, a, h.rows_per_tile);
