@@ -357,8 +357,9 @@ struct AttendArgs {
   float* part_lse;   // [splits][tokens * q_heads], log2
   int32_t tile_slots;     // query tiles launched per KV head
   int32_t request_slots;  // tiles per request if tiles are laid out by request, else 0
-  int32_t splits;
-  int32_t tiles_per_split;
+  int32_t splits;       // workgroups that may share a tile's keys
+  int32_t least_tiles;  // key tiles that each has at least
+  uint32_t by_splits;   // ceil(2^32 / splits), or 0: all have least_tiles
 };
 
 // Tile `i` of the launch: its request, and which of the request's tiles (the
@@ -436,6 +437,15 @@ CB_INLINE int tile_start(const KeyRange& k, int t) {
   return t < k.ta ? t * KT : k.lb + (t - k.ta) * KT;
 }
 CB_INLINE int tile_end(const KeyRange& k, int t) { return t < k.ta ? k.na : k.hb; }
+
+// Key tiles of each split of a tile that has `tiles`: its own keys in equal
+// parts, whatever the bound that the launch was made for (64 new tokens over 4096
+// in 8 requests, with parts cut by a bound of 32768: 131 us; by their own keys 35).
+// The product is the quotient, or more by its 32 bits' error.
+CB_INLINE int split_tiles(const AttendArgs& a, int tiles) {
+  if (a.splits == 1) return tiles;
+  return max(a.least_tiles, static_cast<int>(__umulhi(static_cast<uint32_t>(tiles + a.splits - 1), a.by_splits)));
+}
 
 // New token of a query row: a shift for the usual groups of a power of two,
 // where a division costs some 25 instructions.
@@ -589,7 +599,7 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(Attend
   const int rows = r.n * s.group;
   const int row0 = tile * kAnyRows, row1 = min(rows, row0 + kAnyRows) - 1;
   const KeyRange kr = key_range<KT>(s, r, b, row0, row1);
-  const int t0 = split * a.tiles_per_split, t1 = a.splits > 1 ? min(kr.tiles, t0 + a.tiles_per_split) : kr.tiles;
+  const int per = split_tiles(a, kr.tiles), t0 = split * per, t1 = min(kr.tiles, t0 + per);
   if (a.splits > 1 && t0 >= t1) return;
 
   auto entry_of = [&](int t) { return t < t1 ? fetch_entry<KT>(s.batch, r, tile_start<KT>(kr, t), tile_end(kr, t)) : -1; };
@@ -792,11 +802,7 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(Attend
   if (a.lse && g == 0) a.lse[at] = lse2 * kLn2;
 }
 
-// Splits of a (token, head): its first row of partial results and how many of
-// the launch's splits its tile has; 0 rows of no request.
-CB_INLINE int splits_of(const AttendArgs& a, const KeyRange& kr) {
-  return min(a.splits, (kr.tiles + a.tiles_per_split - 1) / a.tiles_per_split);
-}
+// How many splits the tile of a (token, head) has; -1 for rows of no request.
 template <int KT>
 CB_INLINE int row_splits(const AttendArgs& a, int t, int qh, int rows_per_tile) {
   const ScoreArgs& s = a.s;
@@ -806,7 +812,9 @@ CB_INLINE int row_splits(const AttendArgs& a, int t, int qh, int rows_per_tile) 
   if (!r.ok || t < r.q0 || t >= r.q0 + r.n) return -1;
   const int row = (t - r.q0) * s.group + qh % s.group;
   const int row0 = row / rows_per_tile * rows_per_tile;
-  return splits_of(a, key_range<KT>(s, r, b, row0, min(r.n * s.group, row0 + rows_per_tile) - 1));
+  const KeyRange kr = key_range<KT>(s, r, b, row0, min(r.n * s.group, row0 + rows_per_tile) - 1);
+  const int per = split_tiles(a, kr.tiles);
+  return per > 0 ? (kr.tiles + per - 1) / per : 0;
 }
 
 // Joins few splits: out = sum 2^(lse_z - lse) out_z, a wave a row. Lane z holds
@@ -1408,7 +1416,7 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_ker
   if (!find_tile(a, rest % a.tile_slots, 32 * NW, r, b, tile)) return;
   const int rows = r.n * s.group, row0 = tile * 32 * NW;
   const KeyRange kr = key_range<KT>(s, r, b, row0, min(rows, row0 + 32 * NW) - 1);
-  const int t0 = split * a.tiles_per_split, t1 = a.splits > 1 ? min(kr.tiles, t0 + a.tiles_per_split) : kr.tiles;
+  const int per = split_tiles(a, kr.tiles), t0 = split * per, t1 = min(kr.tiles, t0 + per);
   if (a.splits > 1 && t0 >= t1) return;
 
   typedef RowBlock<IO, DP, KT, MOD> Block;
@@ -1520,7 +1528,7 @@ __global__ __launch_bounds__(NW * kWave, 1) void attend_step_kernel(AttendArgs a
   if (!find_tile(a, rest % a.tile_slots, 32, r, b, tile)) return;
   const int rows = r.n * s.group, row0 = tile * 32;
   const KeyRange kr = key_range<KT>(s, r, b, row0, min(rows, row0 + 32) - 1);
-  const int t0 = split * a.tiles_per_split, t1 = min(kr.tiles, t0 + min(a.tiles_per_split, kStepTiles));
+  const int per = min(split_tiles(a, kr.tiles), kStepTiles), t0 = split * per, t1 = min(kr.tiles, t0 + per);
   if (a.splits > 1 && t0 >= t1) return;
 
   for (int k = threadIdx.x; k < (t1 - t0) * KT; k += NW * kWave) {
@@ -2235,7 +2243,7 @@ struct AttendShape {
   bool step;  // of these, the one for few rows
   int waves;
   int rows_per_tile, keys_per_tile;
-  int tile_slots, request_slots, splits, tiles_per_split;
+  int tile_slots, request_slots, splits, least_tiles;
 };
 
 // Whether the 16-bit kernels take the call: whole 16-byte chunks of rows.
@@ -2285,11 +2293,15 @@ AttendShape attend_shape(const ScoreArgs& s, int32_t dtype) {
   const int key_tiles = std::max(1, ceil_div(keys, h.keys_per_tile) + (s.prefix ? 1 : 0));
   const int64_t groups = static_cast<int64_t>(h.tile_slots) * s.kv_heads;
   const int64_t target = !h.step ? kTargetGroups * 4 / h.waves : B.requests > 1 ? kStepGroupsRagged : kStepGroups;
-  int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(1, groups), key_tiles / (h.half ? 8 : 2))));
-  if (h.step) splits = std::max(splits, ceil_div(key_tiles, kStepTiles));
-  h.tiles_per_split = ceil_div(key_tiles, splits);
-  h.splits = ceil_div(key_tiles, h.tiles_per_split);
-  if (h.splits == 1 && !h.step) h.tiles_per_split = 0x7fffffff;  // one split takes whatever there is
+  h.least_tiles = h.half ? 8 : 2;
+  h.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(1, groups), key_tiles / h.least_tiles)));
+  if (h.step) {
+    // Parts of one size for all requests, cut by the bound: their workgroups end
+    // together (64 ragged requests 47 us, with parts by each one's own keys 68).
+    h.splits = std::max(h.splits, ceil_div(key_tiles, kStepTiles));
+    h.least_tiles = ceil_div(key_tiles, h.splits);
+    h.splits = ceil_div(key_tiles, h.least_tiles);
+  }
   return h;
 }
 
@@ -2469,7 +2481,8 @@ int cb_paged_attention(const cb_query_batch* batch, int32_t layer, int32_t dtype
   a.tile_slots = h.tile_slots;
   a.request_slots = h.request_slots;
   a.splits = h.splits;
-  a.tiles_per_split = h.tiles_per_split;
+  a.least_tiles = h.least_tiles;
+  a.by_splits = h.splits > 1 && !h.step ? static_cast<uint32_t>(((int64_t{1} << 32) + h.splits - 1) / h.splits) : 0;
   if (need > 0) {
     a.part_out = static_cast<float*>(d_workspace);
     a.part_lse = reinterpret_cast<float*>(static_cast<char*>(d_workspace) +

@@ -679,3 +679,15 @@ def test_integers_past_32_bits_are_refused():
             QueryBatch(case.batch.rows, qs, ln, **kw)
     with pytest.raises(ValueError, match="budget"):
         evict_tokens(case.batch, torch.zeros(1, 40).cuda(), case.batch, budget=big + 1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("new", [1, 30, 200])
+def test_bounds_far_above_the_lengths(new, dtype):
+    case = make([1500, 300, 210], [new, new, min(new, 7)], heads=4, kv_heads=2, dim=64, dtype=dtype, seed=new)
+    qs, ln, off = case.batch._keep
+    for bound in (1500, 40000, 1 << 20):
+        batch = QueryBatch(case.batch.rows, qs, ln, offsets=off, max_length=bound, max_query=new,
+                           request_stride=case.batch.c.request_stride)
+        out, lse = paged_attention(batch, 0, case.q.cuda(), return_lse=True)
+        check_attention(case, out, lse)
