@@ -8,6 +8,10 @@ Public API (mirrors the reference's mapper / online primitives):
   ``install_unpublished``, ``SourceLease`` (``cachebridge_amd.online.blocks``)
 - ``PipelinedSourceLease``, ``StagedHandoff`` (``cachebridge_amd.online.pipeline``)
 
+Beside the reference's: ``QueryBatch``, ``install_tokens``,
+``paged_attention``, ``add_key_weights`` and ``evict_tokens``
+(``cachebridge_amd.online.queries``), which answer on an installed prefix.
+
 All compute runs in ``libcachebridge_hip.so`` (HIP, gfx950); importing the
 package does not load it, the first plan or copy does, and raises if it is
 not built.

@@ -552,7 +552,7 @@ CB_INLINE void place_rows(const QBatch& B, const Request& r, int64_t entry, int 
 // loaded into registers (VE at a time: 16 bytes where rows allow it, else one)
 // while a tile is used. Rows in LDS are DP + 4 floats apart, which puts the 16
 // rows and 4 columns of an operand in distinct banks. A prompt of 250 fp32
-// tokens with 4 heads of 64 takes 15.8 us and its join 5.0 us: at this size the
+// tokens with 4 heads of 64 takes 14.4 us and its join 5.5 us: at this size the
 // two barriers and the row lookup of each tile bound it, not its 37 MFLOP; with
 // a tile's loads waited for in place it was 41 us.
 // ---------------------------------------------------------------------------
@@ -1391,8 +1391,8 @@ CB_INLINE void mark_not_finite(uint32_t lv, int np, int below, int above, int st
 
 // Many query rows: a workgroup's NW waves hold 32 rows each and share K and V
 // tiles, double buffered: while a tile is used the next one arrives. 2048 new
-// tokens over 32768 (16 heads of 128, 2 KV heads, bf16, 533 GFLOP) take 534 us,
-// 1.00 PFLOP/s, where a library product of 8192^3 reaches 1.21. What bounds it:
+// tokens over 32768 (16 heads of 128, 2 KV heads, bf16, 533 GFLOP) take 521
+// to 559 us by box, 1.0 PFLOP/s, where a library product of 8192^3 reaches 1.21. What bounds it:
 // matrix steps and vector instructions that are not exponentials do not overlap
 // (see RowBlock::weights), so a tile costs its products plus its multiply-adds,
 // packs and sums. 32 rows a wave: 64 have twice the products a K or V operand

@@ -1,1 +1,1 @@
-"""Online handoff primitives: block packing, fused install, leases, pipeline."""
+"""Online handoff primitives: block packing, fused install, leases, pipeline, queries."""

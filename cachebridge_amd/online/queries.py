@@ -98,7 +98,8 @@ class QueryBatch:
     a ``[requests, width]`` block table given flat, ``width * page_size``.
     ``max_query`` and ``max_length`` bound the new and cached tokens of any
     request (default bounds read nothing from the device: ``max_query`` is
-    every token row, so give it where it is known).
+    every token row, so give it where it is known; a decoding step divides its
+    keys by ``max_length``, so a bound far above the lengths costs time).
     """
 
     def __init__(self, rows: Rows, query_start: torch.Tensor, lengths: torch.Tensor, *, max_length: int,
