@@ -1392,7 +1392,8 @@ CB_INLINE void mark_not_finite(uint32_t lv, int np, int below, int above, int st
 // Many query rows: a workgroup's NW waves hold 32 rows each and share K and V
 // tiles, double buffered: while a tile is used the next one arrives. 2048 new
 // tokens over 32768 (16 heads of 128, 2 KV heads, bf16, 533 GFLOP) take 521
-// to 559 us by box, 1.0 PFLOP/s, where a library product of 8192^3 reaches 1.21. What bounds it:
+// to 559 us on several cards, 1.0 PFLOP/s, where a library product of 8192^3
+// reaches 1.21. What bounds it:
 // matrix steps and vector instructions that are not exponentials do not overlap
 // (see RowBlock::weights), so a tile costs its products plus its multiply-adds,
 // packs and sums. 32 rows a wave: 64 have twice the products a K or V operand
