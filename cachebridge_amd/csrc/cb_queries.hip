@@ -1901,6 +1901,7 @@ struct EvictArgs {
   const float* weights;
   int64_t weights_stride;
   int32_t budget, first, last;
+  int64_t target_span;  // index entries of the target that are a request's own
   int32_t* kept;
   int32_t* kept_lengths;
   float* kept_weights;
@@ -2109,7 +2110,7 @@ __global__ __launch_bounds__(256) void move_rows_kernel(MoveArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       from[u] = cache_row(e.batch, src, static_cast<int>(from[u]));
-      to[u] = dst.ok ? cache_row(e.target, dst, at[u]) : -1;
+      to[u] = (dst.ok & (at[u] < e.target_span)) ? cache_row(e.target, dst, at[u]) : -1;
     }
     bool ok[U];
     V v[U];
@@ -2134,6 +2135,16 @@ __global__ __launch_bounds__(256) void move_rows_kernel(MoveArgs a) {
 int elem_bytes(int32_t dtype) {
   return dtype == CB_DTYPE_F32 ? 4 : dtype == CB_DTYPE_BF16 || dtype == CB_DTYPE_F16 ? 2 : 0;
 }
+
+// Index entries that are a request's own: with starts request_stride apart, its
+// stride, and what lies behind belongs to the next request. Offsets are the
+// caller's, one request has the index to itself, and a stride of zero shares
+// one history among all (which calls that store rows refuse).
+int64_t request_span(const cb_query_batch& b) {
+  return b.offsets || b.num_requests < 2 || b.request_stride == 0 ? int64_t{1} << 30 : b.request_stride;
+}
+
+bool shares_rows(const cb_query_batch& b) { return !b.offsets && b.num_requests > 1 && b.request_stride == 0; }
 
 int check_batch(const cb_query_batch* batch, int32_t dtype, int32_t head_dim, int32_t* err, bool queries, QBatch* B,
                 DevRows* rows) {
@@ -2174,7 +2185,7 @@ int check_batch(const cb_query_batch* batch, int32_t dtype, int32_t head_dim, in
   B->requests = batch->num_requests;
   B->tokens = batch->num_tokens;
   B->max_query = batch->max_query;
-  B->max_length = batch->max_length;
+  B->max_length = static_cast<int32_t>(std::min<int64_t>(batch->max_length, request_span(*batch)));
   B->err = err;
   return CB_OK;
 }
@@ -2428,6 +2439,7 @@ int cb_install_tokens(const cb_query_batch* batch, int32_t layer, int32_t dtype,
   if (!std::isfinite(magnitude)) return fail(CB_EINVAL, "magnitude must be finite");
   if (positions && positions_kind != CB_INDEX_I32 && positions_kind != CB_INDEX_I64)
     return fail(CB_EINVAL, "positions must be int32 or int64");
+  if (shares_rows(*batch)) return fail(CB_EINVAL, "several requests need offsets or a request_stride");
   if (n == 0 || batch->num_requests == 0) return CB_OK;
   a.layer = layer;
   a.head_dim = head_dim;
@@ -2551,6 +2563,7 @@ int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, i
   if (weights_stride < batch->max_length) return fail(CB_EINVAL, "weights rows are shorter than max_length");
   if (batch->num_requests == 0) return CB_OK;
   if ((!weights && batch->max_length > 0) || !kept || !kept_lengths || !kept_weights) return fail(CB_EINVAL, "null weights or kept");
+  if (shares_rows(*target)) return fail(CB_EINVAL, "several requests of target need offsets or a request_stride");
   const int eb = elem_bytes(dtype);
   const int64_t row_bytes = static_cast<int64_t>(batch->cache.heads) * head_dim * eb;
   if (row_bytes > (1 << 24)) return fail(CB_EINVAL, "rows above 16 MB");
@@ -2559,6 +2572,7 @@ int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, i
   a.budget = budget;
   a.first = first;
   a.last = last;
+  a.target_span = request_span(*target);
   a.kept = kept;
   a.kept_lengths = kept_lengths;
   a.kept_weights = kept_weights;

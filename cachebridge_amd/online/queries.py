@@ -95,7 +95,10 @@ class QueryBatch:
     the token tensors; they are the last of its ``lengths[b]`` (int32) cached
     tokens. Its cached token ``j`` is index token ``offsets[b] + j`` (int64,
     the target offset of a ``RequestSpan``), or ``b * request_stride + j``: for
-    a ``[requests, width]`` block table given flat, ``width * page_size``.
+    a ``[requests, width]`` block table given flat, ``width * page_size``. A
+    request longer than ``request_stride`` would reach into the next one's
+    tokens: it is outside the batch's bounds. What ``offsets`` leave each
+    request is the caller's to keep to.
     ``max_query`` and ``max_length`` bound the new and cached tokens of any
     request (default bounds read nothing from the device: ``max_query`` is
     every token row, so give it where it is known; a decoding step divides its
@@ -119,6 +122,8 @@ class QueryBatch:
             raise ValueError("max_query must not be negative")
         if not 0 <= request_stride <= 1 << 31:
             raise ValueError("request_stride must be 0 to 2^31")
+        if requests > 1 and offsets is None and request_stride == 0:
+            raise ValueError("several requests need offsets or a request_stride")
         c = _lib.CbQueryBatch()
         c.cache = rows.c
         c.index_entries = rows.index_entries
@@ -346,7 +351,9 @@ def evict_tokens(batch: QueryBatch, weights: torch.Tensor, target: QueryBatch, *
     those of the largest ``weights`` (fp32 ``[requests, >= max_length]``; equal
     ones: the lower place first; NaN counts above every number). They go, in
     order, to tokens 0, 1, ... of the same request of ``target``, a batch over
-    unpublished pages of the same or another pool (its lengths are not read).
+    unpublished pages of the same or another pool (its lengths are not read; a
+    token past its ``request_stride`` is not copied and sets
+    ``ERROR_TARGET_ROW``).
     Its rows must not be rows that kept tokens are read from. A request of at
     most ``budget`` tokens is copied whole.
     """

@@ -299,14 +299,16 @@ int cb_plan_read_errors(cb_plan* plan, int32_t* flags, void* stream);
  * lengths[b] cached tokens (their K/V rows are part of the cache, see
  * cb_install_tokens). Its cached token j is at index entry u = start + j of
  * the cache's index (the cb_rows rules, index_offset included), with
- * start = offsets[b], or b * request_stride without offsets. The arrays are
+ * start = offsets[b], or b * request_stride without offsets; several requests
+ * have at most request_stride cached tokens each then, unless it is 0 and all
+ * share one history (not for calls that store rows). The arrays are
  * device memory and are read by the kernels, so a captured graph follows
  * their values; max_query and max_length are the host's upper bounds of new
  * and cached tokens per request.
  *
  * A request that breaks these bounds (query_start falling or past
  * num_tokens, more new tokens than max_query or than cached ones, a length
- * above max_length, a negative start) is left out whole: its rows of every
+ * above max_length or request_stride, a negative start) is left out whole: its rows of every
  * output stay as they were. A cached token whose index entry lies outside
  * the index or names a row outside the pool is left out by itself. Both are
  * flagged in *d_error_flag (bits CB_ERROR_*) where it is not NULL; it is
@@ -403,7 +405,9 @@ int cb_add_key_weights(const cb_query_batch* batch, int32_t layer, int32_t dtype
    kept_lengths [requests] their count; kept_weights [requests][budget] their
    weights, then 0. A request outside the batch's bounds is flagged and keeps
    none. Of `target` the cache, index, offsets and request_stride
-   are read. Asynchronous. */
+   are read: without offsets a token past a request's request_stride has no
+   row (CB_ERROR_TARGET_ROW), since the next request's begin there.
+   Asynchronous. */
 int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, int32_t dtype,
                     int32_t head_dim, const float* weights, int64_t weights_stride, int32_t budget,
                     int32_t first, int32_t last, int32_t* kept, int32_t* kept_lengths,

@@ -1,0 +1,122 @@
+"""GPU: which requests, index tokens and rows of a query batch belong to whom."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cachebridge_amd.online.queries import (ERROR_REQUEST, ERROR_TARGET_ROW, QueryBatch, Rotary, add_key_weights,
+                                            evict_tokens, install_tokens, paged_attention)
+from cachebridge_amd.plan import rows_from_stacked
+from oracle import queries as oracle
+
+from .query_cases import check_attention, make
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def int32(*x):
+    return torch.tensor(x, dtype=torch.int32).cuda()
+
+
+def new_flag():
+    return torch.zeros(1, dtype=torch.int32).cuda()
+
+
+def close(got, q, k, v, **how):
+    """One head's rows against the oracle: roundings of the result and of the weights, and fp32 sums of 100 terms."""
+    want, _, mag = oracle.attention(q, k, v, scale=q.shape[1] ** -0.5, **how)
+    u = torch.finfo(q.dtype).eps / 2
+    return ((got.double().cpu() - want).abs() - (u * want.abs() + (u + 2.0 ** -14) * mag)).max() <= 0
+
+
+def slots_of_32(index, g):
+    """(rows arguments, pool row of each of 3 * 32 index tokens)."""
+    if index == "identity":
+        return {}, torch.arange(96)
+    pages = torch.randperm(6, generator=g)
+    t = torch.arange(96)
+    return dict(block_table=pages.int().cuda(), page_size=16), pages[t // 16] * 16 + t % 16
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("index", ["identity", "table"])
+def test_a_request_longer_than_its_stride_is_left_out(index, dtype):
+    """Request 0 has 40 cached tokens where 32 are its own: the next ones are request 1's."""
+    g = torch.Generator().manual_seed(1)
+    dim, lengths = 64, [40, 30, 32]
+    k, v = (torch.randn(1, 96, 2, dim, generator=g).to(dtype) for _ in range(2))
+    fused = torch.randn(6, 8, dim, generator=g).to(dtype)
+    more, slot = slots_of_32(index, g)
+    kd, vd = k.cuda(), v.cuda()
+    batch = QueryBatch(rows_from_stacked(kd, vd, **more), int32(0, 2, 4, 6), int32(*lengths), max_length=50, max_query=2,
+                       request_stride=32)
+    fd = fused.cuda()
+    out = torch.full_like(fd[:, :4], 5.0)
+    flag = new_flag()
+    q = install_tokens(batch, 0, fd[:, :4], fd[:, 4:6], fd[:, 6:], Rotary.build(dim, 1e4), out=out, error_flag=flag)
+    assert int(flag) == ERROR_REQUEST and (q[:2] == 5.0).all()
+    stored = torch.cat([slot[32 * b + n - 2:32 * b + n] for b, n in ((1, 30), (2, 32))])
+    assert torch.equal(vd[0, stored].cpu(), fused[2:, 6:])
+    rest = torch.ones(96, dtype=torch.bool)
+    rest[stored] = False
+    for x, y in ((kd, k), (vd, v)):
+        assert torch.equal(x[0].cpu()[rest], y[0][rest])
+
+    out = torch.full_like(q, 7.0)
+    flag = new_flag()
+    _, lse = paged_attention(batch, 0, q, out=out, return_lse=True, error_flag=flag)
+    assert int(flag) == ERROR_REQUEST and (out[:2] == 7.0).all()
+    for b in (1, 2):
+        at = slot[32 * b:32 * b + lengths[b]]
+        for h in range(4):
+            assert close(out[2 * b:2 * b + 2, h], q[2 * b:2 * b + 2, h].cpu(), kd[0, at, h // 2].cpu(), vd[0, at, h // 2].cpu())
+
+    weights = torch.full((3, 50), 3.0).cuda()
+    flag = new_flag()
+    lse[:2] = 0.0
+    add_key_weights(batch, 0, q, lse, weights, error_flag=flag)
+    assert int(flag) == ERROR_REQUEST and (weights[0] == 3.0).all()
+    assert (weights[1, :30] > 3.0).all() and (weights[1, 30:] == 3.0).all() and (weights[2, :32] > 3.0).all()
+
+    tk, tv = torch.zeros_like(kd), torch.zeros_like(vd)
+    target = QueryBatch(rows_from_stacked(tk, tv), int32(0, 2, 4, 6), int32(*lengths), max_length=50, request_stride=32)
+    flag = new_flag()
+    kept = evict_tokens(batch, weights, target, budget=20, error_flag=flag)
+    assert int(flag) == ERROR_REQUEST and kept.lengths.tolist() == [0, 20, 20]
+    assert (tk[0, :32] == 0).all() and torch.equal(tk[0, 32], kd[0, slot[32 + int(kept.tokens[1, 0])]])
+
+
+def test_evicted_tokens_stay_within_their_request_s_stride():
+    """A budget above the target's stride: what is past it is not copied over the next request's rows."""
+    case = make([50, 20, 45], [1, 1, 1], heads=2, kv_heads=2, dim=64, seed=2)
+    k, v = torch.zeros(1, 96, 2, 64, dtype=BF16).cuda(), torch.zeros(1, 96, 2, 64, dtype=BF16).cuda()
+    target = QueryBatch(rows_from_stacked(k, v), *case.batch._keep[:2], request_stride=32, max_length=50)
+    flag = new_flag()
+    kept = evict_tokens(case.batch, torch.ones(3, 50).cuda(), target, budget=60, error_flag=flag)
+    assert int(flag) == ERROR_TARGET_ROW and kept.lengths.tolist() == [50, 20, 45]
+    for b, n in ((0, 32), (1, 20), (2, 32)):
+        for got, src in ((k, case.k), (v, case.v)):
+            assert torch.equal(got[0, 32 * b:32 * b + n].cpu(), src[0, case.slots[b][:n]])
+    assert (k[0, 52:64] == 0).all()
+
+
+def test_several_requests_need_places_of_their_own():
+    case = make([30, 20], [1, 1], dim=64, index="i32")
+    qs, ln, _ = case.batch._keep
+    with pytest.raises(ValueError, match="offsets or a request_stride"):
+        QueryBatch(case.batch.rows, qs, ln, max_length=30)
+    QueryBatch(case.batch.rows, qs, ln, max_length=30, offsets=torch.zeros(2, dtype=torch.int64).cuda())  # one history
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("new", [1, 30, 200])
+def test_bounds_far_above_the_lengths_without_a_stride(new, dtype):
+    case = make([1500, 300, 210], [new, new, min(new, 7)], heads=4, kv_heads=2, dim=64, dtype=dtype, seed=new, index="offsets")
+    qs, ln, off = case.batch._keep
+    for bound in (1500, 40000, 1 << 20):
+        batch = QueryBatch(case.batch.rows, qs, ln, offsets=off, max_length=bound, max_query=new)
+        out, lse = paged_attention(batch, 0, case.q.cuda(), return_lse=True)
+        check_attention(case, out, lse)
