@@ -2117,8 +2117,11 @@ __global__ __launch_bounds__(256) void move_rows_kernel(MoveArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool in = base + u * static_cast<int>(blockDim.x) < total;
-      if (in & (chunk[u] == 0) & (blockIdx.y == 0) & ((from[u] < 0) | (to[u] < 0)))
+      if (in & (chunk[u] == 0) & (blockIdx.y == 0) & ((from[u] < 0) | (to[u] < 0))) {
         flag(e.batch.err, (from[u] < 0 ? CB_ERROR_CACHE_ROW : 0) | (to[u] < 0 ? CB_ERROR_TARGET_ROW : 0));
+        // Its target row, if there is one, keeps what it held: the request's length says that it may not be used.
+        if (from[u] < 0) e.kept_lengths[b] = 0;
+      }
       ok[u] = in & (from[u] >= 0) & (to[u] >= 0);
       if (ok[u]) v[u] = gload<V>(sbase + from[u] * a.src.row_stride_b + chunk[u] * static_cast<int>(sizeof(V)));
     }

@@ -333,9 +333,12 @@ def _weights_stride(batch: QueryBatch, weights: torch.Tensor) -> int:
 @dataclass
 class KeptTokens:
     """What an eviction kept: ``tokens`` and ``weights`` ``[requests, budget]``
-    (then -1 and 0), ``lengths`` ``[requests]`` (0 for a request outside the
-    batch's bounds). ``tokens`` holds the places the kept tokens had, which
-    stay their positions."""
+    (then -1 and 0), ``lengths`` ``[requests]``. ``tokens`` holds the places the
+    kept tokens had, which stay their positions. A length is 0 for a request
+    outside the batch's bounds, and for one whose kept tokens are not all in
+    the target because a cached row is missing: its target rows then hold in
+    part what they held before, and ``tokens`` and ``weights`` only tell what
+    was chosen."""
 
     tokens: torch.Tensor
     lengths: torch.Tensor

@@ -404,7 +404,11 @@ int cb_add_key_weights(const cb_query_batch* batch, int32_t layer, int32_t dtype
    kept [requests][budget] gets the cached token of each, then -1;
    kept_lengths [requests] their count; kept_weights [requests][budget] their
    weights, then 0. A request outside the batch's bounds is flagged and keeps
-   none. Of `target` the cache, index, offsets and request_stride
+   none. A request of which some kept token has no row to be copied from is
+   flagged (CB_ERROR_CACHE_ROW) and its kept_lengths entry is 0: the target rows
+   of such tokens hold what they held before, which must not be attended to
+   (kept and kept_weights still name what was chosen). A token without a row in
+   the target counts, since the target's index leaves it out by itself. Of `target` the cache, index, offsets and request_stride
    are read: without offsets a token past a request's request_stride has no
    row (CB_ERROR_TARGET_ROW), since the next request's begin there.
    Asynchronous. */
