@@ -376,6 +376,9 @@ CB_INLINE bool find_tile(const AttendArgs& a, int i, int rows_per_tile, Request&
     if (!r.ok && threadIdx.x == 0 && i == b * a.request_slots) flag(B.err, CB_ERROR_REQUEST);
     return tile >= 0;
   }
+  // The last place looks at every request: where one is left out, the others'
+  // tiles end before it (their rows' whole tiles and one more each).
+  const bool watch = i == a.tile_slots - 1;
   const int lane = threadIdx.x & (kWave - 1);
   int64_t before = 0;
   for (int b0 = 0; b0 < B.requests; b0 += kWave) {
@@ -383,7 +386,7 @@ CB_INLINE bool find_tile(const AttendArgs& a, int i, int rows_per_tile, Request&
     if (b0 + lane < B.requests) {
       const Request m = load_request(B, b0 + lane);
       c = (static_cast<int64_t>(m.n) * G + rows_per_tile - 1) / rows_per_tile;
-      if (!m.ok && i == 0 && threadIdx.x < kWave) flag(B.err, CB_ERROR_REQUEST);
+      if (!m.ok && watch && threadIdx.x < kWave) flag(B.err, CB_ERROR_REQUEST);
     }
     int64_t sum = c;
 #pragma unroll

@@ -120,3 +120,24 @@ def test_bounds_far_above_the_lengths_without_a_stride(new, dtype):
         batch = QueryBatch(case.batch.rows, qs, ln, offsets=off, max_length=bound, max_query=new)
         out, lse = paged_attention(batch, 0, case.q.cuda(), return_lse=True)
         check_attention(case, out, lse)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("bad", [0, 63, 70, 149])
+def test_a_bad_request_among_many_is_flagged(bad, dtype):
+    """Query tiles found by a search: whichever of the searched requests is outside the bounds."""
+    lengths, new = [20 + b % 9 for b in range(150)], [1 + b % 3 for b in range(150)]
+    new[5] = 20  # by-request places would be twenty times the tiles
+    case = make(lengths, new, heads=64, kv_heads=2, dim=64, dtype=dtype, seed=5)
+    qs, ln, _ = case.batch._keep
+    ln = ln.clone()
+    ln[bad] = 60
+    batch = QueryBatch(case.batch.rows, qs, ln, max_length=50, max_query=20, request_stride=case.batch.c.request_stride)
+    out = torch.full_like(case.q, 9.0).cuda()
+    flag = new_flag()
+    paged_attention(batch, 0, case.q.cuda(), out=out, error_flag=flag)
+    assert int(flag) == ERROR_REQUEST
+    mine = torch.zeros(case.tokens, dtype=torch.bool)
+    mine[sum(new[:bad]):sum(new[:bad + 1])] = True
+    want = paged_attention(case.batch, 0, case.q.cuda())
+    assert (out[mine.cuda()] == 9.0).all() and torch.equal(out[~mine.cuda()], want[~mine.cuda()])
