@@ -1904,7 +1904,7 @@ struct EvictArgs {
   const float* weights;
   int64_t weights_stride;
   int32_t budget, first, last;
-  int64_t target_span;  // index entries of the target that are a request's own
+  int32_t target_span;  // index entries of the target that are a request's own
   int32_t* kept;
   int32_t* kept_lengths;
   float* kept_weights;
@@ -2099,7 +2099,8 @@ __global__ __launch_bounds__(256) void move_rows_kernel(MoveArgs a) {
   const int32_t* kept = e.kept + static_cast<int64_t>(b) * e.budget;
   gcptr sbase = layer_base(a.src, kind, layer);
   gptr dbase = const_cast<gptr>(layer_base(a.dst, kind, layer));
-  const int total = min(a.tokens_per_block, n - at0) * a.chunks_per_row;
+  const int stop = min(n, at0 + a.tokens_per_block);
+  const int total = max(0, min(stop, e.target_span) - at0) * a.chunks_per_row;  // past the span: the next request's
   for (int base = threadIdx.x; base < total; base += blockDim.x * U) {
     int64_t from[U], to[U];
     int at[U], chunk[U];
@@ -2113,7 +2114,7 @@ __global__ __launch_bounds__(256) void move_rows_kernel(MoveArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       from[u] = cache_row(e.batch, src, static_cast<int>(from[u]));
-      to[u] = (dst.ok & (at[u] < e.target_span)) ? cache_row(e.target, dst, at[u]) : -1;
+      to[u] = dst.ok ? cache_row(e.target, dst, at[u]) : -1;
     }
     bool ok[U];
     V v[U];
@@ -2132,6 +2133,7 @@ __global__ __launch_bounds__(256) void move_rows_kernel(MoveArgs a) {
     for (int u = 0; u < U; ++u)
       if (ok[u]) gstore<V>(dbase + to[u] * a.dst.row_stride_b + chunk[u] * static_cast<int>(sizeof(V)), v[u]);
   }
+  if (stop > e.target_span && blockIdx.y == 0 && threadIdx.x == 0) flag(e.batch.err, CB_ERROR_TARGET_ROW);
 }
 
 // ---------------------------------------------------------------------------
@@ -2578,7 +2580,7 @@ int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, i
   a.budget = budget;
   a.first = first;
   a.last = last;
-  a.target_span = request_span(*target);
+  a.target_span = static_cast<int32_t>(std::min<int64_t>(request_span(*target), 1 << 30));
   a.kept = kept;
   a.kept_lengths = kept_lengths;
   a.kept_weights = kept_weights;
