@@ -306,13 +306,14 @@ int cb_plan_read_errors(cb_plan* plan, int32_t* flags, void* stream);
  * their values; max_query and max_length are the host's upper bounds of new
  * and cached tokens per request.
  *
- * A request that breaks these bounds (query_start falling or past
- * num_tokens, more new tokens than max_query or than cached ones, a length
- * above max_length or request_stride, a negative start) is left out whole: its rows of every
- * output stay as they were. A cached token whose index entry lies outside
- * the index or names a row outside the pool is left out by itself. Both are
- * flagged in *d_error_flag (bits CB_ERROR_*) where it is not NULL; it is
- * never cleared. Rows of no request stay as they were.
+ * A request that breaks these bounds (query_start negative, past num_tokens,
+ * falling, or below an earlier request's; more new tokens than max_query or
+ * than cached ones; a length above max_length or request_stride; a negative
+ * start) is left out whole: its rows of every output stay as they were. A
+ * cached token whose index entry lies outside the index or names a row outside
+ * the pool is left out by itself. Both are flagged in *d_error_flag (bits
+ * CB_ERROR_*) where it is not NULL; it is never cleared. Rows of no request
+ * stay as they were.
  * No counterpart in the reference, whose target engine answers the queries.
  */
 #define CB_ERROR_CACHE_ROW 1 /* a cached token without a valid row */

@@ -141,3 +141,72 @@ def test_a_bad_request_among_many_is_flagged(bad, dtype):
     mine[sum(new[:bad]):sum(new[:bad + 1])] = True
     want = paged_attention(case.batch, 0, case.q.cuda())
     assert (out[mine.cuda()] == 9.0).all() and torch.equal(out[~mine.cuda()], want[~mine.cuda()])
+
+
+# Query starts, and the requests whose rows are their own; max_query is 8.
+STARTS = {
+    "falls": ([0, 8, 4, 12], [0]),               # request 1 falls, request 2 starts behind row 8
+    "past the end": ([0, 100, 3, 6], []),         # requests 1 and 2 start before the 100th row
+    "last past the end": ([0, 3, 100], [0]),
+    "late": ([2, 1, 0, 8], []),                  # every later start is below the first
+    "twice": ([0, 3, 1, 3, 3, 9, 8, 12], [0, 3, 4]),
+    "negative": ([-2, 3, 7], [1]),
+}
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("length,dtype", [(30, BF16), (30, FP32), (3000, BF16), (3000, FP32)])
+@pytest.mark.parametrize("starts", list(STARTS))
+def test_rows_of_falling_starts_have_one_owner(starts, length, dtype, many):
+    """Install, attention (keys split or not) and key weights answer the same requests and leave all other rows.
+
+    ``many``: 70 empty requests stand before them, and tiles are found by a search."""
+    start, good = STARTS[starts]
+    front = 70 if many else 0
+    n, heads, dim = len(start) - 1, 4, 64
+    case = make([length] * (n + front), [0] * (n + front), heads=heads, kv_heads=2, dim=dim, dtype=dtype, seed=7, page=16)
+    qs = int32(*[start[0]] * front, *start)
+    tokens = 12
+    batch = QueryBatch(case.batch.rows, qs, case.batch._keep[1], max_length=length, max_query=8,
+                       request_stride=case.batch.c.request_stride)
+    g = torch.Generator().manual_seed(2)
+    fused = torch.randn(tokens, 8, dim, generator=g).to(dtype).cuda()
+    owner = {t: front + b for b in good for t in range(start[b], start[b + 1])}
+    mine = torch.tensor([t in owner for t in range(tokens)])
+    before = [x.clone() for x in case.pool]
+    out = torch.full((tokens, heads, dim), 5.0, dtype=dtype).cuda()
+    flag = new_flag()
+    q = install_tokens(batch, 0, fused[:, :4], fused[:, 4:6], fused[:, 6:], Rotary.build(dim, 1e4), out=out, error_flag=flag)
+    assert int(flag) == ERROR_REQUEST
+    assert torch.equal((q == 5.0).all(-1).all(-1).cpu(), ~mine)
+    stored = torch.zeros(before[0].shape[1], dtype=torch.bool)
+    for b in good:
+        m = start[b + 1] - start[b]
+        at = case.slots[front + b][length - m:] if m else case.slots[front + b][:0]
+        stored[at] = True
+        assert torch.equal(case.pool[1][0, at].cpu(), fused[start[b]:start[b + 1], 6:].cpu())
+    for x, y in zip(case.pool, before):
+        assert torch.equal(x[0][~stored.cuda()], y[0][~stored.cuda()])
+
+    out = torch.full_like(q, 7.0)
+    flag = new_flag()
+    _, lse = paged_attention(batch, 0, q, out=out, return_lse=True, error_flag=flag)
+    assert int(flag) == ERROR_REQUEST
+    assert torch.equal((out == 7.0).all(-1).all(-1).cpu(), ~mine)
+    kc, vc = (x.cpu() for x in case.pool)
+    for b in good:
+        at = case.slots[front + b]
+        for h in (0, 3):
+            rows = slice(start[b], start[b + 1])
+            assert start[b] == start[b + 1] or close(out[rows, h], q[rows, h].cpu(), kc[0, at, h // 2], vc[0, at, h // 2])
+
+    lse[~mine.cuda()] = 0.0
+    weights = torch.zeros(n + front, length).cuda()
+    flag = new_flag()
+    add_key_weights(batch, 0, q, lse, weights, error_flag=flag)
+    assert int(flag) == ERROR_REQUEST
+    want = torch.zeros(n + front)
+    for b in owner.values():
+        want[b] += heads
+    # Each row's weights sum to one: fp32 sums of up to 3000 terms, and scores of at most 16.
+    assert ((weights.sum(1).cpu() - want).abs() <= want * (3000 * 2.0 ** -23 + 2.0 ** -16)).all()
