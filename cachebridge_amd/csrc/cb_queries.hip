@@ -2305,6 +2305,27 @@ int check_heads(const char* name, const cb_heads* h, int32_t heads, int eb, int3
   return CB_OK;
 }
 
+// Whether two rows of a token tensor lie on one another: rows of an output that
+// do would be stored by several workgroups at once.
+bool rows_overlap(const cb_heads& h, int64_t tokens, int64_t dim) {
+  const int64_t ts = h.token_stride, hs = h.head_stride;
+  if (tokens < 2 && h.heads < 2) return false;
+  if ((hs >= dim || h.heads < 2) && (ts >= (h.heads - 1) * hs + dim || tokens < 2)) return false;  // heads within tokens
+  if ((ts >= dim || tokens < 2) && (hs >= (tokens - 1) * ts + dim || h.heads < 2)) return false;   // tokens within heads
+  if (tokens > 1 && ts < dim) return true;
+  for (int64_t i = 1; i < h.heads; ++i) {  // head i of token 0 against the tokens of head 0 beside it
+    const int64_t at = i * hs, t = ts > 0 ? std::min(at / ts, tokens - 1) : 0;
+    if (at - t * ts < dim || (t + 1 < tokens && (t + 1) * ts - at < dim)) return true;
+  }
+  return false;
+}
+
+int check_output(const char* name, const cb_heads* h, int32_t heads, int eb, int32_t tokens, int32_t dim, Strided* out) {
+  if (int rc = check_heads(name, h, heads, eb, tokens, out)) return rc;
+  if (rows_overlap(*h, tokens, dim)) return fail(CB_EINVAL, "%s has rows that share memory", name);
+  return CB_OK;
+}
+
 bool aligned16(const Strided& s) {
   return (reinterpret_cast<uintptr_t>(s.data) | static_cast<uintptr_t>(s.token_b) | static_cast<uintptr_t>(s.head_b)) % 16 == 0;
 }
@@ -2538,7 +2559,7 @@ int cb_install_tokens(const cb_query_batch* batch, int32_t layer, int32_t dtype,
   if (!q) return fail(CB_EINVAL, "null q");
   const int eb = elem_bytes(dtype), kv = batch->cache.heads, n = batch->num_tokens;
   if (q->heads < 1 || q->heads > (1 << 16)) return fail(CB_EINVAL, "q needs 1 to 65536 heads");
-  if ((rc = check_heads("q", q, q->heads, eb, n, &a.q)) || (rc = check_heads("q_out", q_out, q->heads, eb, n, &a.q_out)) ||
+  if ((rc = check_heads("q", q, q->heads, eb, n, &a.q)) || (rc = check_output("q_out", q_out, q->heads, eb, n, head_dim, &a.q_out)) ||
       (rc = check_heads("k", k, kv, eb, n, &a.k)) || (rc = check_heads("v", v, kv, eb, n, &a.v)))
     return rc;
   if (rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2)
@@ -2592,7 +2613,7 @@ int cb_paged_attention(const cb_query_batch* batch, int32_t layer, int32_t dtype
   int rc;
   if ((rc = check_scores(batch, layer, dtype, head_dim, scores, q->heads, d_error_flag, &a.s))) return rc;
   const int eb = elem_bytes(dtype), n = batch->num_tokens;
-  if ((rc = check_heads("q", q, q->heads, eb, n, &a.s.q)) || (rc = check_heads("out", out, q->heads, eb, n, &a.out))) return rc;
+  if ((rc = check_heads("q", q, q->heads, eb, n, &a.s.q)) || (rc = check_output("out", out, q->heads, eb, n, head_dim, &a.out))) return rc;
   if (n == 0 || batch->num_requests == 0) return CB_OK;
   const AttendShape h = attend_shape(a.s, dtype);
   const int64_t need = attend_workspace(a.s, h);

@@ -335,7 +335,7 @@ typedef struct cb_query_batch {
 } cb_query_batch;
 
 /* A token tensor [num_tokens][heads][head_dim], head_dim contiguous; strides
-   in elements. */
+   in elements. Rows of an output must not share memory. */
 typedef struct cb_heads {
   void* data;
   int64_t token_stride;

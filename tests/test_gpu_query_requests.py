@@ -210,3 +210,16 @@ def test_rows_of_falling_starts_have_one_owner(starts, length, dtype, many):
         want[b] += heads
     # Each row's weights sum to one: fp32 sums of up to 3000 terms, and scores of at most 16.
     assert ((weights.sum(1).cpu() - want).abs() <= want * (3000 * 2.0 ** -23 + 2.0 ** -16)).all()
+
+
+def test_outputs_whose_rows_share_memory_are_refused():
+    case = make([30], [3], dim=64)
+    q = case.q.cuda()
+    for out in (q[:1].expand(3, 4, 64), q[:, :1].expand(3, 4, 64)):
+        with pytest.raises(ValueError, match="share memory"):
+            paged_attention(case.batch, 0, q, out=out)
+        with pytest.raises(ValueError, match="share memory"):
+            install_tokens(case.batch, 0, q, q[:, :2], q[:, 2:], Rotary.build(64, 1e4), out=out)
+    # Inputs may: one row of queries for every token.
+    got = paged_attention(case.batch, 0, q[:1].expand(3, 4, 64))
+    assert torch.equal(got[0], paged_attention(case.batch, 0, q)[0])
