@@ -43,7 +43,7 @@ def _at_offset(rows: Rows, index_offset: int) -> Rows:
     """The same description with another index offset (no new device tables)."""
     c = _lib.CbRows.from_buffer_copy(rows.c)
     c.index_offset = index_offset
-    return Rows(c, rows.dtype, rows.device, rows.keep)
+    return Rows(c, rows.dtype, rows.device, rows.keep, index_entries=rows.index_entries)
 
 
 def coalesced_runs(rows: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

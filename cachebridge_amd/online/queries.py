@@ -114,6 +114,8 @@ class QueryBatch:
                 raise ValueError("pool indices must be contiguous")
         if rows.c.k_layers and any(t.data_ptr() % 16 for t in rows.keep if t.ndim == 3):
             raise ValueError("pool layers must be 16-byte aligned")
+        if rows.c.index_kind != _lib.CB_INDEX_IDENTITY and rows.index_entries < 1:
+            raise ValueError("rows do not say how many entries their index has")
         requests = lengths.numel()
         # The C fields are 32 bits wide, and ctypes drops what does not fit.
         if not 0 <= max_length <= 1 << 30:

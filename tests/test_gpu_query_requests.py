@@ -7,7 +7,8 @@ import torch
 
 from cachebridge_amd.online.queries import (ERROR_REQUEST, ERROR_TARGET_ROW, QueryBatch, Rotary, add_key_weights,
                                             evict_tokens, install_tokens, paged_attention)
-from cachebridge_amd.plan import rows_from_stacked
+from cachebridge_amd.online.delivery import _at_offset
+from cachebridge_amd.plan import Rows, rows_from_stacked
 from oracle import queries as oracle
 
 from .query_cases import check_attention, make
@@ -223,3 +224,20 @@ def test_outputs_whose_rows_share_memory_are_refused():
     # Inputs may: one row of queries for every token.
     got = paged_attention(case.batch, 0, q[:1].expand(3, 4, 64))
     assert torch.equal(got[0], paged_attention(case.batch, 0, q)[0])
+
+
+def test_rows_have_to_say_how_long_their_index_is():
+    """Without it every cached token would count as missing."""
+    case = make([30], [3], dim=64, index="i32")
+    rows = case.batch.rows
+    qs, ln, _ = case.batch._keep
+    with pytest.raises(ValueError, match="entries"):
+        QueryBatch(Rows(rows.c, rows.dtype, rows.device, rows.keep), qs, ln, max_length=30)
+    # Another offset into the same index.
+    moved = _at_offset(rows, 10)
+    flag = new_flag()
+    out = paged_attention(QueryBatch(moved, int32(0, 3), int32(20), max_length=20), 0, case.q.cuda(), error_flag=flag)
+    assert int(flag) == 0
+    at = case.slots[0][10:]
+    for h in range(4):
+        assert close(out[:, h], case.q[:, h], case.k[0, at, h // 2], case.v[0, at, h // 2])
