@@ -2370,6 +2370,9 @@ int check_scores(const cb_query_batch* batch, int32_t layer, int32_t dtype, int3
   return CB_OK;
 }
 
+// HIP counts a launch's threads in 32 bits.
+bool launch_fits(int64_t workgroups, int threads) { return workgroups <= 0xffffffffll / threads; }
+
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
 // Workgroups of four waves that a launch is split into at least: two a CU. 512 new
@@ -2384,7 +2387,8 @@ struct AttendShape {
   bool step;  // of these, the one for few rows
   int waves;
   int rows_per_tile, keys_per_tile;
-  int tile_slots, request_slots, splits, least_tiles;
+  int64_t tile_slots;
+  int request_slots, splits, least_tiles;
 };
 
 // Whether the 16-bit kernels take the call: whole 16-byte chunks of rows.
@@ -2428,11 +2432,11 @@ AttendShape attend_shape(const ScoreArgs& s, int32_t dtype) {
   const int64_t by_request = static_cast<int64_t>(per_request) * B.requests;
   const int64_t packed = ceil_div(static_cast<int64_t>(B.tokens) * s.group, h.rows_per_tile) + static_cast<int64_t>(B.requests);
   h.request_slots = by_request <= packed ? per_request : 0;
-  h.tile_slots = static_cast<int>(std::min(by_request, packed));
+  h.tile_slots = std::min(by_request, packed);
   int64_t keys = B.max_length;
   if (s.window > 0 && s.causal && !s.prefix) keys = std::min<int64_t>(keys, static_cast<int64_t>(s.window) + std::min<int64_t>(B.max_query, h.rows_per_tile / s.group + 2));
   const int key_tiles = std::max(1, ceil_div(keys, h.keys_per_tile) + (s.prefix ? 1 : 0));
-  const int64_t groups = static_cast<int64_t>(h.tile_slots) * s.kv_heads;
+  const int64_t groups = h.tile_slots * s.kv_heads;
   const int64_t target = !h.step ? kTargetGroups * 4 / h.waves : B.requests > 1 ? kStepGroupsRagged : kStepGroups;
   h.least_tiles = h.half ? 8 : 2;
   h.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(1, groups), key_tiles / h.least_tiles)));
@@ -2454,11 +2458,13 @@ int64_t attend_workspace(const ScoreArgs& s, const AttendShape& h) {
   return round256(rows * s.head_dim * 4) + round256(rows * 4);
 }
 
+bool joins_by_wave(int splits, int64_t rows) { return splits <= kJoinFew && rows >= kJoinRows; }
+
 template <typename IO, int KT>
 void launch_join(const AttendArgs& a, const AttendShape& h, hipStream_t st) {
   if (h.splits <= 1) return;
   const int64_t rows = static_cast<int64_t>(a.s.batch.tokens) * a.s.q_heads;
-  if (h.splits <= kJoinFew && rows >= kJoinRows) {
+  if (joins_by_wave(h.splits, rows)) {
     const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
     if (a.s.head_dim <= 128) hipLaunchKernelGGL((join_few_kernel<IO, KT, 2>), grid, dim3(256), 0, st, a, h.rows_per_tile);
     else hipLaunchKernelGGL((join_few_kernel<IO, KT, 8>), grid, dim3(256), 0, st, a, h.rows_per_tile);
@@ -2586,7 +2592,7 @@ int cb_install_tokens(const cb_query_batch* batch, int32_t layer, int32_t dtype,
   const int items = (q->heads + kv) * (head_dim - rotary_dim / 2) / (wide ? vec : 1) + kv * head_dim / (wide ? vec : 1);
   a.slices = std::max(1, std::min(64, ceil_div(items, kWave)));  // an item a lane: one round of memory latency
   const int64_t grid = (static_cast<int64_t>(n) * a.slices + kInstallWaves - 1) / kInstallWaves + (d_error_flag ? 1 : 0);
-  if (grid > 0x7fffffff) return fail(CB_EINVAL, "too many tokens");
+  if (!launch_fits(grid, kInstallWaves * kWave)) return fail(CB_EINVAL, "too many tokens");
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == CB_DTYPE_BF16) launch_install<io_bf16>(a, wide, static_cast<unsigned>(grid), st);
   else if (dtype == CB_DTYPE_F16) launch_install<io_f16>(a, wide, static_cast<unsigned>(grid), st);
@@ -2620,7 +2626,6 @@ int cb_paged_attention(const cb_query_batch* batch, int32_t layer, int32_t dtype
   if (need > 0 && (!d_workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(d_workspace) % 256))
     return fail(CB_EINVAL, "attention needs a 256-byte aligned workspace of %lld bytes", static_cast<long long>(need));
   a.lse = lse;
-  a.tile_slots = h.tile_slots;
   a.request_slots = h.request_slots;
   a.splits = h.splits;
   a.least_tiles = h.least_tiles;
@@ -2630,8 +2635,12 @@ int cb_paged_attention(const cb_query_batch* batch, int32_t layer, int32_t dtype
     a.part_lse = reinterpret_cast<float*>(static_cast<char*>(d_workspace) +
                                           round256(static_cast<int64_t>(h.splits) * n * q->heads * head_dim * 4));
   }
-  const int64_t grid = static_cast<int64_t>(h.tile_slots) * h.splits * a.s.kv_heads;
-  if (grid > 0x7fffffff || static_cast<int64_t>(n) * q->heads > 0x7fffffff) return fail(CB_EINVAL, "too many query tiles");
+  const int64_t grid = h.tile_slots * h.splits * a.s.kv_heads;
+  const int64_t rows = static_cast<int64_t>(n) * q->heads;
+  if (!launch_fits(grid, (h.step ? kStepWaves : h.waves) * kWave) || rows > 0x7fffffff ||
+      (h.splits > 1 && !joins_by_wave(h.splits, rows) && !launch_fits(rows, kJoinThreads)))
+    return fail(CB_EINVAL, "too many query tiles");
+  a.tile_slots = static_cast<int32_t>(h.tile_slots);
   const bool mod = a.s.mod;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == CB_DTYPE_BF16) launch_attend<io_bf16>(a, h, mod, static_cast<unsigned>(grid), st);
@@ -2664,7 +2673,7 @@ int cb_add_key_weights(const cb_query_batch* batch, int32_t layer, int32_t dtype
   }
   a.key_slots = ceil_div(batch->max_length, keys);
   const int64_t grid = static_cast<int64_t>(a.key_slots) * batch->num_requests;
-  if (grid > 0x7fffffff) return fail(CB_EINVAL, "too many cached tokens");
+  if (!launch_fits(grid, kWeightWaves * kWave)) return fail(CB_EINVAL, "too many cached tokens");
   const bool mod = a.s.mod;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == CB_DTYPE_BF16) launch_weights<io_bf16>(a, mod, static_cast<unsigned>(grid), st);
@@ -2712,7 +2721,8 @@ int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, i
   m.tokens_per_block = std::max(1, 1024 / m.chunks_per_row);
   m.blocks_per_request = ceil_div(std::min(budget, std::max(batch->max_length, 1)), m.tokens_per_block);
   const int64_t blocks = static_cast<int64_t>(m.blocks_per_request) * batch->num_requests;
-  if (blocks > 0x7fffffff || batch->cache.num_layers > 32767) return fail(CB_EINVAL, "eviction too large");
+  if (!launch_fits(blocks, 256) || !launch_fits(batch->num_requests, kSelectThreads) || batch->cache.num_layers > 32767)
+    return fail(CB_EINVAL, "eviction too large");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 requests(static_cast<unsigned>(batch->num_requests));
   const int64_t middle = static_cast<int64_t>(batch->max_length) - first - last;

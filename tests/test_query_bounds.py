@@ -2,11 +2,13 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 
 from cachebridge_amd import _lib
 
-from .test_queries import FAKE, attend, batch, evict, heads, lib, ref, refused  # noqa: F401
+from .test_queries import FAKE, attend, batch, evict, heads, lib, ref, refused, scores  # noqa: F401
 
 
 def test_requests_that_store_rows_need_places_of_their_own(lib):  # noqa: F811
@@ -39,3 +41,19 @@ def test_outputs_with_rows_apart_are_taken(lib, strides):  # noqa: F811
     assert all(b - a >= dim for a, b in zip(places, places[1:])), "the case itself"
     b = batch(max_length=100000, rows=200000, row_stride=256)
     refused(lib, attend(lib, b, dim=dim, q=heads(dim=dim), out=heads(token_stride=strides[0], head_stride=strides[1])), "workspace")
+
+
+def test_launches_past_32_bits_of_threads_are_refused(lib):  # noqa: F811
+    """Bounds that the arguments allow, but no grid: 2^32 threads or more."""
+    s, q, kv, far = scores(), heads(), heads(2), 1 << 30
+    b = batch(max_length=far, request_stride=far, rows=far)
+    rc = lib.cb_add_key_weights(ref(b), 0, 0, 128, ref(s), ref(q), FAKE, FAKE, far, None, None)
+    refused(lib, rc, "too many cached tokens")
+    refused(lib, evict(lib, b=b, t=b, budget=far, stride=far), "too large")
+    b = batch(num_tokens=1 << 27, request_stride=far)
+    rc = lib.cb_install_tokens(ref(b), 0, 0, 128, ref(q), ref(q), ref(kv), ref(kv), FAKE, 128, 0, 1.0, None, 0, None, None)
+    refused(lib, rc, "too many tokens")
+    b = batch(max_length=far, request_stride=far, rows=far, num_requests=32, num_tokens=32, max_query=1)
+    need = ctypes.c_int64(0)
+    assert lib.cb_attention_workspace_bytes(ref(b), 0, 128, ref(s), 4, ctypes.byref(need)) == 0
+    refused(lib, attend(lib, b, work=FAKE, work_bytes=need.value), "too many query tiles")
