@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/cachebridge_hip.h"
 #include "cb_common.h"
@@ -251,16 +252,23 @@ constexpr int kMaxPairs = 256;  // head_dim <= 512
 // sin and cos of `turns` revolutions. The angle is reduced to an eighth of a
 // turn either side of a quarter's multiple in 64 bits (positions times a
 // frequency reach thousands of radians, where 32 bits leave no digits of the
-// phase), then both are Taylor polynomials in fp32: |x| <= pi/4, first
-// terms left out x^11/11! and x^12/12! below 2^-29.
-__device__ inline void sincos_turns(double turns, float* sn, float* cs) {
+// phase), then both are Taylor polynomials, |x| <= pi/4: in fp32 for 16-bit
+// rows, first terms left out x^11/11! and x^12/12! below 2^-29; in fp64 for fp32
+// rows, x^15/15! and x^16/16! below 2^-45.
+template <typename T>
+__device__ inline void sincos_turns(double turns, T* sn, T* cs) {
   const double q = __builtin_rint(turns * 4.0);
-  const float x = static_cast<float>((turns - q * 0.25) * 6.283185307179586476925);
+  const T x = static_cast<T>((turns - q * 0.25) * 6.283185307179586476925);
   const int quadrant = static_cast<int>(static_cast<int64_t>(q) & 3);
-  const float y = x * x;
-  const float s = x + x * y * (-1.0f / 6 + y * (1.0f / 120 + y * (-1.0f / 5040 + y * (1.0f / 362880))));
-  const float c = 1.0f + y * (-0.5f + y * (1.0f / 24 + y * (-1.0f / 720 + y * (1.0f / 40320 + y * (-1.0f / 3628800)))));
-  const float a = (quadrant & 1) ? c : s, b = (quadrant & 1) ? s : c;
+  const T y = x * x, one = 1;
+  T s = 0, c = 0;
+  if constexpr (sizeof(T) == 8) {
+    s = y * y * (one / -39916800 + y * (one / 6227020800));
+    c = y * y * (one / 479001600 + y * (one / -87178291200));
+  }
+  s = x + x * y * (-one / 6 + y * (one / 120 + y * (-one / 5040 + y * (one / 362880) + s)));
+  c = one + y * (-one / 2 + y * (one / 24 + y * (-one / 720 + y * (one / 40320 + y * (-one / 3628800) + c))));
+  const T a = (quadrant & 1) ? c : s, b = (quadrant & 1) ? s : c;
   *sn = (quadrant & 2) ? -a : a;
   *cs = (quadrant == 1 || quadrant == 2) ? -b : b;
 }
@@ -302,7 +310,12 @@ __device__ inline void store_vec(char* p, const float* in) {
 // heads 4.7 us, the latency of a launch and of three dependent loads.
 template <typename IO, int V>
 __global__ __launch_bounds__(kInstallWaves * kWave) void install_tokens_kernel(InstallArgs a) {
-  __shared__ float2 turn[kInstallWaves][kMaxPairs];
+  // fp32 rows are rotated in fp64 and rounded once: in fp32 the cosine, sine and two
+  // products would each round to the digits that are stored (2048 tokens of 16 and 2
+  // heads of 128 13.9 us for 13.6).
+  typedef std::conditional_t<sizeof(IO) == 4, double, float> T;
+  typedef T pair __attribute__((ext_vector_type(2)));
+  __shared__ pair turn[kInstallWaves][kMaxPairs];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * kInstallWaves + wave;
   if (a.batch.err && blockIdx.x == gridDim.x - 1) {  // a workgroup more than there are tokens for
@@ -324,9 +337,9 @@ __global__ __launch_bounds__(kInstallWaves * kWave) void install_tokens_kernel(I
                                            : static_cast<const int32_t*>(a.positions)[t];
   const int pairs = a.rotary_dim / 2;
   for (int i = lane; i < pairs; i += kWave) {
-    float s, c;
+    T s, c;
     sincos_turns(static_cast<double>(pos) * a.inv_freq[i] * 0.15915494309189533577, &s, &c);
-    turn[wave][i] = make_float2(c * a.magnitude, s * a.magnitude);
+    turn[wave][i] = pair{c * a.magnitude, s * a.magnitude};
   }
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -377,13 +390,13 @@ __global__ __launch_bounds__(kInstallWaves * kWave) void install_tokens_kernel(I
     load_vec<IO, V>(src + ob * E, x + V);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float2 cs = turn[wave][first + i];
+      const pair cs = turn[wave][first + i];
       if (a.interleaved) {
-        y[2 * i] = x[2 * i] * cs.x - x[2 * i + 1] * cs.y;
-        y[2 * i + 1] = x[2 * i + 1] * cs.x + x[2 * i] * cs.y;
+        y[2 * i] = static_cast<float>(x[2 * i] * cs.x - x[2 * i + 1] * cs.y);
+        y[2 * i + 1] = static_cast<float>(x[2 * i + 1] * cs.x + x[2 * i] * cs.y);
       } else {
-        y[i] = x[i] * cs.x - x[i + V] * cs.y;
-        y[i + V] = x[i + V] * cs.x + x[i] * cs.y;
+        y[i] = static_cast<float>(x[i] * cs.x - x[i + V] * cs.y);
+        y[i + V] = static_cast<float>(x[i + V] * cs.x + x[i] * cs.y);
       }
     }
     store_vec<IO, V>(dst + oa * E, y);

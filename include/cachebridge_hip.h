@@ -365,7 +365,7 @@ typedef struct cb_scores {
    rotary_dim / 2 of them; the angle is reduced in 64 bits) and is scaled by
    magnitude. positions (CB_INDEX_I32 or CB_INDEX_I64 entries, one per token
    row) replaces p where it is not NULL. q_out may be q itself. Rotated values
-   are computed in fp32 and rounded once. Asynchronous. */
+   are computed in fp32, of fp32 rows in fp64, and rounded once. Asynchronous. */
 int cb_install_tokens(const cb_query_batch* batch, int32_t layer, int32_t dtype, int32_t head_dim,
                       const cb_heads* q, const cb_heads* q_out, const cb_heads* k,
                       const cb_heads* v, const double* inv_freq, int32_t rotary_dim,
