@@ -161,6 +161,8 @@ class CbScores(ctypes.Structure):
         ("causal", _i32),
         ("slopes", _c_void_p),
         ("prefix_lengths", _c_void_p),
+        ("fp32_weights", _i32),
+        ("reserved", _i32),
     ]
 
 

@@ -1326,7 +1326,13 @@ struct RowBlock {
   }
 
   // Weights by the maximum that stands, packed as the next product's operands,
-  // and their sum.
+  // and their sum (of the weights as they were). The rounding to 16 bits is
+  // the price of 16-bit products with V: over random keys it adds as much as the
+  // result's own rounding does (bf16 errors of 2.4e-3 of the result where fp32 weights
+  // leave 1.7e-3, fp16 2.7e-4 and 2.1e-4); a second product for the part rounded
+  // off would be half as many matrix steps again. Calls that ask for fp32 weights
+  // take attend_any_kernel: a step of 64 requests of 2048 151 us for 42, a prompt
+  // of 4096 (16 heads of 128) 1126 for 135.
   CB_INLINE float try_weights(const f32x16 (&st)[KB], float scale2, u32x4 (&w)[KB][2]) const {
     const float mu = m == kNegInf ? 0.0f : m;
     float sum = 0;
@@ -2430,9 +2436,9 @@ constexpr int kStepRows = 32;
 constexpr int kStepGroups = 512, kStepGroupsRagged = 1024;
 constexpr int kStepWaves = 2;
 
-AttendShape attend_shape(const ScoreArgs& s, int32_t dtype) {
+AttendShape attend_shape(const ScoreArgs& s, int32_t dtype, bool fp32_weights) {
   AttendShape h{};
-  h.half = takes_half(s, dtype);
+  h.half = !fp32_weights && takes_half(s, dtype);
   const QBatch& B = s.batch;
   h.step = h.half && static_cast<int64_t>(B.max_query) * s.group <= kStepRows;
   const int64_t seen = s.window > 0 && s.causal && !s.prefix ? std::min<int64_t>(B.max_length, s.window) : B.max_length;
@@ -2620,7 +2626,7 @@ int cb_attention_workspace_bytes(const cb_query_batch* batch, int32_t dtype, int
   ScoreArgs s{};
   int rc;
   if ((rc = check_scores(batch, 0, dtype, head_dim, scores, query_heads, nullptr, &s))) return rc;
-  *bytes = s.batch.tokens && s.batch.requests ? attend_workspace(s, attend_shape(s, dtype)) : 0;
+  *bytes = s.batch.tokens && s.batch.requests ? attend_workspace(s, attend_shape(s, dtype, scores->fp32_weights != 0)) : 0;
   return CB_OK;
 }
 
@@ -2634,7 +2640,7 @@ int cb_paged_attention(const cb_query_batch* batch, int32_t layer, int32_t dtype
   const int eb = elem_bytes(dtype), n = batch->num_tokens;
   if ((rc = check_heads("q", q, q->heads, eb, n, &a.s.q)) || (rc = check_output("out", out, q->heads, eb, n, head_dim, &a.out))) return rc;
   if (n == 0 || batch->num_requests == 0) return CB_OK;
-  const AttendShape h = attend_shape(a.s, dtype);
+  const AttendShape h = attend_shape(a.s, dtype, scores->fp32_weights != 0);
   const int64_t need = attend_workspace(a.s, h);
   if (need > 0 && (!d_workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(d_workspace) % 256))
     return fail(CB_EINVAL, "attention needs a 256-byte aligned workspace of %lld bytes", static_cast<long long>(need));

@@ -255,8 +255,8 @@ def _scores(batch: QueryBatch, heads: int, dim: int, scale, causal, window, cap,
 
 def paged_attention(batch: QueryBatch, layer: int, q: torch.Tensor, *, scale: float | None = None, causal: bool = True,
                     window: int = 0, cap: float = 0.0, slopes: torch.Tensor | None = None,
-                    prefix_lengths: torch.Tensor | None = None, out: torch.Tensor | None = None,
-                    return_lse: bool = False, error_flag: torch.Tensor | None = None,
+                    prefix_lengths: torch.Tensor | None = None, fp32_weights: bool = False,
+                    out: torch.Tensor | None = None, return_lse: bool = False, error_flag: torch.Tensor | None = None,
                     stream: torch.cuda.Stream | None = None):
     """Attention of the new tokens over the cached ones of their requests.
 
@@ -272,11 +272,15 @@ def paged_attention(batch: QueryBatch, layer: int, q: torch.Tensor, *, scale: fl
     exponentials. A token that sees nothing gets zeros and ``-inf``; rows of no
     request are not written. What a token does not see never reaches its row,
     NaN and infinities in the cache included. Scores, statistics and sums are
-    fp32; the weights are rounded to the pool's type for their product with V.
+    fp32; the weights of a 16-bit pool are rounded to its type for their product
+    with V, which adds about as much error as the result's own rounding, unless
+    ``fp32_weights``, which takes fp32 products (8 to 13 times as long for
+    prompts, 2 to 4 times for steps and short questions).
     """
     n, heads, dim = q.shape if q.ndim == 3 else (0, 0, 0)
     cq = batch._heads(q, "q")
     scores = _scores(batch, heads, dim, scale, causal, window, cap, slopes, prefix_lengths)
+    scores.fp32_weights = bool(fp32_weights)
     flag = _flag_pointer(batch, error_flag)
     lib = _lib.load()
     with _On(batch, stream) as handle:

@@ -356,6 +356,9 @@ typedef struct cb_scores {
   int32_t causal;
   const float* slopes;           /* device, one per query head, or NULL */
   const int32_t* prefix_lengths; /* device, one per request, or NULL */
+  int32_t fp32_weights; /* cb_paged_attention: softmax weights keep fp32 for their product with V;
+                           0: they are rounded to the type of a 16-bit cache */
+  int32_t reserved;
 } cb_scores;
 
 /* Rotate the new tokens' queries and keys to their positions and store their
