@@ -421,7 +421,6 @@ struct ScoreArgs {
   float inner;   // scale / cap, finite
   float gentle;  // raw products below it have |inner x| < kSmallAngle
   int32_t mod;  // scores are more than a product times a positive scale
-  int32_t group_shift;  // log2(group), or -1
 };
 
 struct AttendArgs {
@@ -520,10 +519,6 @@ CB_INLINE int split_tiles(const AttendArgs& a, int tiles) {
   if (a.splits == 1) return tiles;
   return max(a.least_tiles, static_cast<int>(__umulhi(static_cast<uint32_t>(tiles + a.splits - 1), a.by_splits)));
 }
-
-// New token of a query row: a shift for the usual groups of a power of two,
-// where a division costs some 25 instructions.
-CB_INLINE int token_of_row(const ScoreArgs& s, int row) { return s.group_shift >= 0 ? row >> s.group_shift : row / s.group; }
 
 // Whether every row of the tile sees every key of [start, stop).
 CB_INLINE bool sees_all(const ScoreArgs& s, const KeyRange& k, int start, int stop) {
@@ -1133,10 +1128,6 @@ constexpr int kWaitAll = 0x0070;     // vmcnt 0, expcnt 7, lgkmcnt 0
 __device__ inline void wait_and_meet() {
   __builtin_amdgcn_s_waitcnt(kWaitAll);
   asm volatile("s_barrier" ::: "memory");
-}
-__device__ inline void wait_own() {
-  __builtin_amdgcn_s_waitcnt(kWaitAll);
-  asm volatile("" ::: "memory");
 }
 
 // One wave's part of a tile's DMA: N instructions for K and as many for V,
@@ -2374,7 +2365,6 @@ int check_scores(const cb_query_batch* batch, int32_t layer, int32_t dtype, int3
   s->q_heads = q_heads;
   s->kv_heads = kv;
   s->group = q_heads / kv;
-  s->group_shift = (s->group & (s->group - 1)) ? -1 : __builtin_ctz(static_cast<unsigned>(s->group));
   s->scale = sc->scale;
   s->cap = sc->cap;
   // Bounded so that a product of zero stays zero however small the cap is.
