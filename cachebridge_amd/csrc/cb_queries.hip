@@ -134,9 +134,13 @@ CB_INLINE int64_t cache_row(const QBatch& B, const Request& r, int j) {
 CB_INLINE int starts_to(const QBatch& B, int b) {
   const int lane = threadIdx.x & (kWave - 1);
   const CB_GLOBAL int32_t* start = reinterpret_cast<const CB_GLOBAL int32_t*>(as_global(B.query_start));
+  typedef int32_t four __attribute__((ext_vector_type(4), aligned(4)));
   int top = start[min(lane, b)];
 #pragma unroll 2
-  for (int i = kWave; i < b; i += kWave) top = max(top, start[min(i + lane, b)]);
+  for (int i = kWave; i < b; i += 4 * kWave) {
+    const four x = *reinterpret_cast<const CB_GLOBAL four*>(start + min(i + 4 * lane, b - 3));
+    top = max(max(top, max(x[0], x[1])), max(x[2], x[3]));
+  }
   return top;
 }
 
@@ -679,7 +683,7 @@ CB_INLINE void load_spread(const char* row, int dim, int g, float (&x)[N]) {
 __device__ inline bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
 
 template <typename IO, int DP, int VE>
-__global__ __launch_bounds__(kAnyWaves * kWave, 1) void attend_any_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kAnyWaves * kWave, DP == 64 ? 3 : DP == 128 ? 2 : 1) void attend_any_kernel(AttendArgs a) {
   constexpr int KT = kAnyKeys, LD = DP + 4, NB = DP / 16, NT = kAnyWaves * kWave, MW = DP / 32;
   // A 512-element row's sums and queries fill the registers: no tile waits there.
   constexpr bool AHEAD = DP <= 256;
@@ -1891,7 +1895,7 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void key_weights_any_kernel(W
 constexpr int kWeightWaves = 4;
 
 template <typename IO, int DP, bool MOD>
-__global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 2 : 4) void key_weights_kernel(WeightArgs a, int vector) {
+__global__ __launch_bounds__(kWeightWaves * kWave, DP < 256 ? 4 : MOD ? 2 : 3) void key_weights_kernel(WeightArgs a, int vector) {
   typedef Half<IO> H;
   constexpr int KS = DP / 16;
   __shared__ float sums[kWeightWaves][32];
@@ -1906,7 +1910,9 @@ __global__ __launch_bounds__(kWeightWaves * kWave, DP == 256 ? 2 : 4) void key_w
   if (first_key >= r.length && first_key > 0) return;
   // Asked for by the waves that store, and looked at where they do: waited for
   // here by all it took the step 34.0 us a call, not 31.7.
-  const int top = sub == 0 ? starts_to(s.batch, b) : 0;
+  // At head 256 there is no register left for it (158 us of a step for 164).
+  int top = sub == 0 ? starts_to(s.batch, b) : 0;
+  if constexpr (DP == 256) top = __any(top > r.q0) ? 0x7fffffff : -1;
   KeyRange kr{};
   kr.np = s.prefix ? max(0, min(s.prefix[b], r.length)) : 0;
   int i0 = 0, i1 = 0;

@@ -241,3 +241,32 @@ def test_rows_have_to_say_how_long_their_index_is():
     at = case.slots[0][10:]
     for h in range(4):
         assert close(out[:, h], case.q[:, h], case.k[0, at, h // 2], case.v[0, at, h // 2])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("at,to", [(3, 50), (3, 640), (300, 690), (699, 0)])
+def test_a_start_out_of_order_among_many(at, to, dtype):
+    """Steps of 700 requests, one start misplaced: those that start below an earlier one are left out, the others are not."""
+    n = 700
+    case = make([9] * n, [1] * n, heads=4, kv_heads=2, dim=64, dtype=dtype, seed=4)
+    start = list(range(n + 1))
+    start[at] = to
+    bad = [b for b in range(n) if not 0 <= start[b + 1] - start[b] <= 1 or start[b] < max(start[:b + 1])]
+    batch = QueryBatch(case.batch.rows, int32(*start), case.batch._keep[1], max_length=9, max_query=1,
+                       request_stride=case.batch.c.request_stride)
+    q = case.q.cuda()
+    want, want_lse = paged_attention(case.batch, 0, q, return_lse=True)
+    flag, out = new_flag(), torch.full_like(q, 7.0)
+    paged_attention(batch, 0, q, out=out, error_flag=flag)
+    assert int(flag) == ERROR_REQUEST
+    rows = [start[b] for b in range(n) if b not in bad and start[b + 1] > start[b]]
+    mine = torch.zeros(n, dtype=torch.bool)
+    mine[rows] = True
+    assert torch.equal(out[mine.cuda()], want[mine.cuda()]) and (out[~mine.cuda()] == 7.0).all()
+    weights = torch.zeros(2, n, 9).cuda()
+    flag = new_flag()
+    add_key_weights(case.batch, 0, q, want_lse, weights[0])
+    add_key_weights(batch, 0, q, want_lse, weights[1], error_flag=flag)
+    assert int(flag) == ERROR_REQUEST
+    good = torch.tensor([b not in bad and start[b + 1] > start[b] for b in range(n)]).cuda()
+    assert torch.equal(weights[1][good], weights[0][good]) and (weights[1][~good] == 0).all()
