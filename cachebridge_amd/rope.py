@@ -58,7 +58,9 @@ def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None)
     ``scaling`` is None or a dictionary with ``rope_type`` ``"linear"`` (every
     frequency divided by ``factor``), ``"yarn"`` (the blend of
     ``_inverse_frequency``) or ``"llama3"`` (slow turns divided by ``factor``,
-    fast ones kept, blended between the two wavelengths).
+    fast ones kept, blended between the two wavelengths). Fields of YaRN that
+    change its magnitude or bounds otherwise than ``attn_factor``,
+    ``extrapolation_factor`` and the betas do are refused.
     """
     if type(rotary_dim) is not int or rotary_dim < 2 or rotary_dim % 2:
         raise ValueError("RoPE head dimension must be even")
@@ -83,6 +85,11 @@ def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None)
         turns = original * inv / (2 * math.pi)
         keep = ((turns - low) / (high - low)).clamp(0, 1)
         return inv / factor * (1 - keep) + inv * keep, 1.0
+    for name in ("attention_factor", "mscale", "mscale_all_dim"):
+        if scaling.get(name) is not None:
+            raise ValueError(f"unsupported YaRN field: {name!r}")
+    if scaling.get("truncate", True) is not True:
+        raise ValueError("unsupported YaRN field: 'truncate'")
     bounds = [rotary_dim * math.log(original / (float(scaling.get(name, default)) * 2 * math.pi))
               / (2 * math.log(theta)) for name, default in (("beta_fast", 32), ("beta_slow", 1))]
     first, stop = max(math.floor(bounds[0]), 0), min(math.ceil(bounds[1]), rotary_dim - 1)
