@@ -130,24 +130,33 @@ CB_INLINE int64_t cache_row(const QBatch& B, const Request& r, int j) {
 // Whether request b starts before an earlier one, b the same in all lanes:
 // this lane's largest start of those up to b's is above b's in some lane. Where
 // query starts fall, such a request is outside the bounds, which leaves requests
-// that own rows apart from each other whatever the starts are.
+// that own rows apart from each other whatever the starts are. MANY: past the
+// first 64, four starts a lane and load, for kernels of short workgroups (steps of
+// 2048 requests of 300: 152 us for 163; 148 without a look at the earlier starts).
+template <bool MANY>
 CB_INLINE int starts_to(const QBatch& B, int b) {
   const int lane = threadIdx.x & (kWave - 1);
   const CB_GLOBAL int32_t* start = reinterpret_cast<const CB_GLOBAL int32_t*>(as_global(B.query_start));
-  typedef int32_t four __attribute__((ext_vector_type(4), aligned(4)));
   int top = start[min(lane, b)];
+  if constexpr (MANY) {
+    typedef int32_t four __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll 2
-  for (int i = kWave; i < b; i += 4 * kWave) {
-    const four x = *reinterpret_cast<const CB_GLOBAL four*>(start + min(i + 4 * lane, b - 3));
-    top = max(max(top, max(x[0], x[1])), max(x[2], x[3]));
+    for (int i = kWave; i < b; i += 4 * kWave) {
+      const four x = *reinterpret_cast<const CB_GLOBAL four*>(start + min(i + 4 * lane, b - 3));
+      top = max(max(top, max(x[0], x[1])), max(x[2], x[3]));
+    }
+  } else {
+#pragma unroll 2
+    for (int i = kWave; i < b; i += kWave) top = max(top, start[min(i + lane, b)]);
   }
   return top;
 }
 
 // Request b, the same in all lanes, with its place among the others (asked for
 // ahead of its own fields, so that both wait together).
+template <bool MANY = false>
 CB_INLINE Request own_request(const QBatch& B, int b) {
-  const int top = starts_to(B, b);
+  const int top = starts_to<MANY>(B, b);
   Request r = load_request(B, b);
   if (__any(top > r.q0)) {
     r.ok = false;
@@ -443,12 +452,13 @@ struct AttendArgs {
 // Tile `i` of the launch: its request, and which of the request's tiles (the
 // last first: under a causal mask it has the most keys). Returns false if
 // there is none.
+template <bool MANY = false>
 CB_INLINE bool find_tile(const AttendArgs& a, int i, int rows_per_tile, Request& r, int& b, int& tile) {
   const QBatch& B = a.s.batch;
   const int G = a.s.group;
   if (a.request_slots > 0) {
     b = i / a.request_slots;
-    r = own_request(B, b);
+    r = own_request<MANY>(B, b);
     const int tiles = static_cast<int>((static_cast<int64_t>(r.n) * G + rows_per_tile - 1) / rows_per_tile);
     tile = tiles - 1 - (i - b * a.request_slots);
     if (!r.ok && threadIdx.x == 0 && i == b * a.request_slots) flag(B.err, CB_ERROR_REQUEST);
@@ -1635,7 +1645,7 @@ __global__ __launch_bounds__(NW * kWave, 1) void attend_step_kernel(AttendArgs a
   const int split = rest / a.tile_slots;
   Request r;
   int b, tile;
-  if (!find_tile(a, rest % a.tile_slots, 32, r, b, tile)) return;
+  if (!find_tile<true>(a, rest % a.tile_slots, 32, r, b, tile)) return;
   const int rows = r.n * s.group, row0 = tile * 32;
   const KeyRange kr = key_range<KT>(s, r, b, row0, min(rows, row0 + 32) - 1);
   const int per = min(split_tiles(a, kr.tiles), kStepTiles), t0 = split * per, t1 = min(kr.tiles, t0 + per);
@@ -1910,8 +1920,8 @@ __global__ __launch_bounds__(kWeightWaves * kWave, DP < 256 ? 4 : MOD ? 2 : 3) v
   if (first_key >= r.length && first_key > 0) return;
   // Asked for by the waves that store, and looked at where they do: waited for
   // here by all it took the step 34.0 us a call, not 31.7.
-  // At head 256 there is no register left for it (158 us of a step for 164).
-  int top = sub == 0 ? starts_to(s.batch, b) : 0;
+  // At head 256 there is no register left for it (a step of 64 requests of 2048 161 us for 164).
+  int top = sub == 0 ? starts_to<true>(s.batch, b) : 0;
   if constexpr (DP == 256) top = __any(top > r.q0) ? 0x7fffffff : -1;
   KeyRange kr{};
   kr.np = s.prefix ? max(0, min(s.prefix[b], r.length)) : 0;
