@@ -318,9 +318,9 @@ __device__ inline void store_vec(char* p, const float* in) {
 // heads' elements): lanes compute the token's angles once into LDS, then each
 // item is V pairs of a head (two vectors) or V elements that are copied; slices
 // are cut to an item a lane, so that a wave waits for memory once. Every element
-// is read once and written once: 2048 tokens of 16 query and 2 KV heads of 128
-// in bf16 (21 MB) take 8.7 us, 2.4 TB/s with the launch; 64 tokens of 64 and 8
-// heads 4.7 us, the latency of a launch and of three dependent loads.
+// is read once and written once. 64 tokens of 64 query and 8 KV heads of 128 in bf16
+// take 4.8 us, the latency of a launch and of three dependent loads; 2048 of 16
+// and 2 (21 MB) 9.3 us, that latency and the bytes' time at a copy's rate.
 template <typename IO, int V>
 __global__ __launch_bounds__(kInstallWaves * kWave) void install_tokens_kernel(InstallArgs a) {
   // fp32 rows are rotated in fp64 and rounded once: in fp32 the cosine, sine and two
@@ -669,7 +669,7 @@ CB_INLINE void place_rows(const QBatch& B, const Request& r, int64_t entry, int 
 // loaded into registers (VE at a time: 16 bytes where rows allow it, else one)
 // while a tile is used. Rows in LDS are DP + 4 floats apart, which puts the 16
 // rows and 4 columns of an operand in distinct banks. A prompt of 250 fp32
-// tokens with 4 heads of 64 takes 14.4 us and its join 5.5 us: at this size the
+// tokens with 4 heads of 64 takes 14.0 us and its join 5.8 us: at this size the
 // two barriers and the row lookup of each tile bound it, not its 37 MFLOP; with
 // a tile's loads waited for in place it was 41 us.
 // ---------------------------------------------------------------------------
@@ -1510,9 +1510,10 @@ CB_INLINE void mark_not_finite(uint32_t lv, int np, int below, int above, int st
 
 // Many query rows: a workgroup's NW waves hold 32 rows each and share K and V
 // tiles, double buffered: while a tile is used the next one arrives. 2048 new
-// tokens over 32768 (16 heads of 128, 2 KV heads, bf16, 533 GFLOP) take 521
-// to 559 us on several cards, 1.0 PFLOP/s, where a library product of 8192^3
-// reaches 1.21. What bounds it:
+// tokens over 32768 (16 heads of 128, 2 KV heads, bf16, 533 GFLOP) take 529 us
+// once the clocks have settled (up to 696 in the first 40 passes after a pause;
+// calls of 531 to 571 with the join on several cards), 1.0 PFLOP/s, where a library
+// product of 8192^3 reaches 1.21. What bounds it:
 // matrix steps and vector instructions that are not exponentials do not overlap
 // (see RowBlock::weights), so a tile costs its products plus its multiply-adds,
 // packs and sums. 32 rows a wave: 64 have twice the products a K or V operand
@@ -1624,10 +1625,10 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_ker
 // have read its place, the next V after its sums. The rows that the index
 // names are resolved into LDS first, so that the loop's only vector memory
 // operations are the DMA, whose count tells what has arrived. One request of
-// 32768 tokens (64 heads of 128, 8 KV heads, bf16, 134 MB) takes 32 us, 4.2 TB/s,
-// as fast as this card reads; 64 ragged requests of 2550 on average (16 heads,
-// 2 KV heads, 167 MB) 47.5 us, 3.5 TB/s: ragged lengths leave
-// CUs without work at the end.
+// 32768 tokens (64 heads of 128, 8 KV heads, bf16, 134 MB) takes 31.7 us, 4.2 TB/s; four
+// times the bytes (64 requests of 8192, 16 heads and 2 KV heads) 107 us, 5.0
+// TB/s, a large copy's rate. 64 ragged requests of 2550 on average (167 MB) take
+// 46 us, 3.6 TB/s: ragged lengths leave CUs without work at the end.
 constexpr int kStepTiles = 64;  // tiles a split holds at most
 
 template <typename IO, int DP, int NW, bool MOD>
@@ -1897,11 +1898,11 @@ __global__ __launch_bounds__(kAnyWaves * kWave, 1) void key_weights_any_kernel(W
 // The waves that share a block of keys (4 if there are 4 or more blocks of
 // rows to walk, else fewer, so that none idles) meet in LDS in wave order.
 // 32 tokens over 32768 (16 heads of 128, 2 KV heads, bf16, 17 MB, 4.3 GFLOP)
-// take 28.3 us, 64 ragged steps over 2550 on average (85 MB) 29.8 us. Bound by
+// take 28.3 us, 64 ragged steps over 2550 on average (85 MB) 31.0 us. Bound by
 // vector instructions and the address unit: a block of 32 rows and 32 keys has 8
 // products and some 260 other instructions, and four lanes of an operand's load
-// touch as many rows. Keys and rows through LDS of the wave's own took 26.1 and
-// 39.9 us: fewer waves then have loads in flight.
+// touch as many rows. Keys and rows through LDS of the wave's own took 26.0 and
+// 42.6 us a call for 28.5 and 32.5: fewer waves then have loads in flight.
 constexpr int kWeightWaves = 4;
 
 template <typename IO, int DP, bool MOD>
@@ -2430,15 +2431,15 @@ bool takes_half(const ScoreArgs& s, int32_t dtype) {
 constexpr int kWideRows = 512;               // query rows per KV head, and
 constexpr int64_t kWideScores = 24ll << 20;  // scores of the launch, from which eight are taken
 // Query rows per KV head up to which attend_step_kernel is taken: one block of
-// rows, so that K and V are read once (8 query heads a KV head, this kernel against
-// the tile kernel: 64 ragged requests of 2550 on average, one new token 47 / 94
-// us, four 51 / 88; one request of 32768, 31 / 35 and 38 / 37; two blocks, 64
-// requests of 8 new tokens, 68 / 38. Where all lengths are alike the tile kernel
-// is as good: 64 of 2048 39 / 35).
+// rows, so that K and V are read once. This kernel against the tile kernel, each
+// with its join, 8 query heads a KV head: 64 ragged requests of 2550 on average 52 /
+// 100 us; one request of 32768 38 / 38. Where all lengths are alike the tile
+// kernel is ahead: 64 of 2048 42 / 35, with four new tokens 57 / 40.
 constexpr int kStepRows = 32;
 // Its workgroups: one request has all its splits at work, of several requests many
-// are shorter than the bound that splits are cut by. 512, 1024, 2048: one request
-// of 32768 tokens 34, 40, 40 us; 64 ragged ones 73, 47, 60 us (64 alike 31, 39, 39).
+// are shorter than the bound that splits are cut by. With the join, 512, 1024
+// and 2048: 64 ragged requests 73, 52, 67 us; 64 of 2048 33, 42, 42; one request of
+// 32768 38 with 512 and 47 with 1024.
 constexpr int kStepGroups = 512, kStepGroupsRagged = 1024;
 constexpr int kStepWaves = 2;
 

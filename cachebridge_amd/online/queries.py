@@ -102,7 +102,10 @@ class QueryBatch:
     ``max_query`` and ``max_length`` bound the new and cached tokens of any
     request (default bounds read nothing from the device: ``max_query`` is
     every token row, so give it where it is known; a decoding step divides its
-    keys by ``max_length``, so a bound far above the lengths costs time).
+    keys by ``max_length``, so a bound far above the lengths costs time, and
+    memory: its calls allocate ``max_length / 2048 * tokens * heads *
+    head_dim`` floats, 1 GB for 64 tokens with 64 heads of 128 and a bound of
+    2^20).
     """
 
     def __init__(self, rows: Rows, query_start: torch.Tensor, lengths: torch.Tensor, *, max_length: int,
@@ -365,6 +368,11 @@ def evict_tokens(batch: QueryBatch, weights: torch.Tensor, target: QueryBatch, *
     ``ERROR_TARGET_ROW``).
     Its rows must not be rows that kept tokens are read from. A request of at
     most ``budget`` tokens is copied whole.
+
+    The other calls take a cached token's place for its position where they
+    use a window or ``slopes``, and ``install_tokens`` alone takes
+    ``positions``: on an evicted cache, windows and slopes measure the places
+    that are left. Models with either should not go on from one.
     """
     stride = _weights_stride(batch, weights)
     if target.device != batch.device or target.dtype != batch.dtype:

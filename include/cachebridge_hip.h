@@ -375,7 +375,9 @@ int cb_install_tokens(const cb_query_batch* batch, int32_t layer, int32_t dtype,
                       int32_t interleaved, float magnitude, const void* positions,
                       int32_t positions_kind, int32_t* d_error_flag, void* stream);
 
-/* Device workspace bytes of cb_paged_attention for this batch (0: none). */
+/* Device workspace bytes of cb_paged_attention for this batch (0: none). With
+   few query rows per KV head it grows with the bound, max_length / 2048 *
+   num_tokens * query_heads * head_dim floats or more. */
 int cb_attention_workspace_bytes(const cb_query_batch* batch, int32_t dtype, int32_t head_dim,
                                  const cb_scores* scores, int32_t query_heads, int64_t* bytes);
 
@@ -412,7 +414,9 @@ int cb_add_key_weights(const cb_query_batch* batch, int32_t layer, int32_t dtype
    flagged (CB_ERROR_CACHE_ROW) and its kept_lengths entry is 0: the target rows
    of such tokens hold what they held before, which must not be attended to
    (kept and kept_weights still name what was chosen). A token without a row in
-   the target counts, since the target's index leaves it out by itself. Of `target` the cache, index, offsets and request_stride
+   the target counts, since the target's index leaves it out by itself. Windows
+   and slopes of later calls on the target measure places that are left, not
+   the tokens' positions. Of `target` the cache, index, offsets and request_stride
    are read: without offsets a token past a request's request_stride has no
    row (CB_ERROR_TARGET_ROW), since the next request's begin there.
    Asynchronous. */
