@@ -270,3 +270,51 @@ def test_a_start_out_of_order_among_many(at, to, dtype):
     assert int(flag) == ERROR_REQUEST
     good = torch.tensor([b not in bad and start[b + 1] > start[b] for b in range(n)]).cuda()
     assert torch.equal(weights[1][good], weights[0][good]) and (weights[1][~good] == 0).all()
+
+
+@pytest.mark.parametrize("fp32_weights", [False, True])
+def test_a_captured_step_stops_at_the_stride(fp32_weights):
+    """Two graphs of one step, replayed in turn while lengths grow: request 0 reaches its stride of 32 and is left out
+    from then on, request 1 goes on as before."""
+    g = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(1, 96, 2, 64, generator=g).to(BF16).cuda() for _ in range(2))
+    fused = torch.randn(2, 8, 64, generator=g).to(BF16).cuda()
+    lengths, start, flag = int32(29, 9), int32(0, 1, 2), new_flag()
+    batch = QueryBatch(rows_from_stacked(k, v), start, lengths, max_length=50, max_query=1, request_stride=32)
+    alone = QueryBatch(rows_from_stacked(k, v), start, lengths, max_length=50, max_query=1, offsets=torch.tensor([64, 32]).cuda())
+    spin, weights = Rotary.build(64, 1e4), torch.zeros(2, 50).cuda()
+    out = torch.zeros(2, 4, 64, dtype=BF16).cuda()
+
+    def step(batch):
+        q = install_tokens(batch, 0, fused[:, :4], fused[:, 4:6], fused[:, 6:], spin, error_flag=flag)
+        _, lse = paged_attention(batch, 0, q, out=out, return_lse=True, cap=20.0, fp32_weights=fp32_weights, error_flag=flag)
+        add_key_weights(batch, 0, q, torch.nan_to_num(lse, neginf=-1e30), weights, cap=20.0, error_flag=flag)
+
+    step(batch)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step(batch)
+        graphs.append(graph)
+    for turn in range(6):
+        lengths += 1
+        flag.zero_()
+        out.fill_(7.0)
+        weights.zero_()
+        before = k.clone(), v.clone()
+        torch.cuda.synchronize()
+        graphs[turn % 2].replay()
+        torch.cuda.synchronize()
+        past = 30 + turn > 32
+        assert int(flag) == (ERROR_REQUEST if past else 0), turn
+        assert bool((out[0] == 7.0).all()) == past and bool((weights[0] == 0).all()) == past
+        changed = (v != before[1])[0].flatten(1).any(1).nonzero().flatten().tolist()
+        assert set(changed) <= ({32 + 9 + turn} if past else {29 + turn, 32 + 9 + turn}), turn
+        got, w = out[1].clone(), weights[1].clone()
+        weights.zero_()
+        step(alone)  # request 0 elsewhere: request 1 has the same bits
+        assert torch.equal(out[1], got) and torch.equal(weights[1], w)
+        k.copy_(before[0])
+        v.copy_(before[1])
