@@ -166,6 +166,33 @@ class CbScores(ctypes.Structure):
     ]
 
 
+class CbRotation(ctypes.Structure):
+    _fields_ = [
+        ("inv_freq", _c_void_p),
+        ("positions", _c_void_p),
+        ("pair_axis", ctypes.c_char_p),
+        ("axis_stride", _i64),
+        ("rotary_dim", _i32),
+        ("interleaved", _i32),
+        ("positions_kind", _i32),
+        ("axes", _i32),
+        ("magnitude", ctypes.c_float),
+        ("reserved", _i32),
+    ]
+
+
+class CbPageScales(ctypes.Structure):
+    _fields_ = [
+        ("k", _c_void_p),
+        ("v", _c_void_p),
+        ("layer_stride", _i64),
+        ("page_stride", _i64),
+        ("pages", _i64),
+        ("page_size", _i32),
+        ("reserved", _i32),
+    ]
+
+
 # Every symbol the header declares, with (restype, argtypes).
 SIGNATURES = {
     "cb_last_error": (ctypes.c_char_p, []),
@@ -202,6 +229,32 @@ SIGNATURES = {
         [ctypes.POINTER(CbQueryBatch), _i32, _i32, _i32, ctypes.POINTER(CbHeads), ctypes.POINTER(CbHeads),
          ctypes.POINTER(CbHeads), ctypes.POINTER(CbHeads), _c_void_p, _i32, _i32, ctypes.c_float, _c_void_p,
          _i32, _c_void_p, _c_void_p],
+    ),
+    "cb_install_rotated": (
+        ctypes.c_int,
+        [ctypes.POINTER(CbQueryBatch), _i32, _i32, _i32, ctypes.POINTER(CbHeads), ctypes.POINTER(CbHeads),
+         ctypes.POINTER(CbHeads), ctypes.POINTER(CbHeads), ctypes.POINTER(CbRotation), _c_void_p, _c_void_p],
+    ),
+    "cb_install_quantized": (
+        ctypes.c_int,
+        [ctypes.POINTER(CbQueryBatch), ctypes.POINTER(CbPageScales), _i32, _i32, _i32, ctypes.POINTER(CbHeads),
+         ctypes.POINTER(CbHeads), ctypes.POINTER(CbHeads), ctypes.POINTER(CbHeads), ctypes.POINTER(CbRotation),
+         _c_void_p, _c_void_p],
+    ),
+    "cb_quantize_tokens": (
+        ctypes.c_int,
+        [ctypes.POINTER(CbQueryBatch), ctypes.POINTER(CbQueryBatch), ctypes.POINTER(CbPageScales), _i32, _i32,
+         _c_void_p, _c_void_p, _c_void_p],
+    ),
+    "cb_quantized_attention_workspace_bytes": (
+        ctypes.c_int,
+        [ctypes.POINTER(CbQueryBatch), ctypes.POINTER(CbPageScales), _i32, _i32, ctypes.POINTER(CbScores), _i32,
+         ctypes.POINTER(_i64)],
+    ),
+    "cb_quantized_attention": (
+        ctypes.c_int,
+        [ctypes.POINTER(CbQueryBatch), ctypes.POINTER(CbPageScales), _i32, _i32, _i32, ctypes.POINTER(CbScores),
+         ctypes.POINTER(CbHeads), ctypes.POINTER(CbHeads), _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
     ),
     "cb_attention_workspace_bytes": (
         ctypes.c_int,

@@ -13,7 +13,8 @@ import tempfile
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
-SOURCES = [PACKAGE / "csrc" / "cb_handoff.hip", PACKAGE / "csrc" / "cb_queries.hip"]
+SOURCES = [PACKAGE / "csrc" / "cb_handoff.hip", PACKAGE / "csrc" / "cb_queries.hip",
+           PACKAGE / "csrc" / "cb_quantized.hip"]
 OUTPUT = PACKAGE / "libcachebridge_hip.so"
 ARCH = os.environ.get("CACHEBRIDGE_OFFLOAD_ARCH", "gfx950")
 

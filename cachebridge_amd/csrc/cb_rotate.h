@@ -1,0 +1,255 @@
+// Rotation of new tokens and the store of their rows, for the kernels that do it.
+#pragma once
+
+#include "cb_query_common.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// New tokens: rotation and store
+// ---------------------------------------------------------------------------
+
+constexpr int kInstallWaves = 4;
+constexpr int kMaxPairs = 256;  // head_dim <= 512
+constexpr int kMaxAxes = 8;
+
+struct InstallArgs {
+  QBatch batch;
+  DevRows cache;
+  int32_t layer;
+  int32_t head_dim, rotary_dim, interleaved;
+  int32_t q_heads, kv_heads;
+  int32_t slices;  // waves per token
+  Strided q, q_out, k, v;
+  const double* inv_freq;
+  const void* positions;
+  int32_t positions_kind;
+  float magnitude;
+  int32_t axes;         // rows of positions, axis_stride entries apart
+  int64_t axis_stride;
+  uint8_t pair_axis[kMaxPairs];  // the axis of each pair
+};
+
+
+// sin and cos of `turns` revolutions. The angle is reduced to an eighth of a
+// turn either side of a quarter's multiple in 64 bits (positions times a
+// frequency reach thousands of radians, where 32 bits leave no digits of the
+// phase), then both are Taylor polynomials, |x| <= pi/4: in fp32 for 16-bit
+// rows, first terms left out x^11/11! and x^12/12! below 2^-29; in fp64 for fp32
+// rows, x^15/15! and x^16/16! below 2^-45.
+template <typename T>
+__device__ inline void sincos_turns(double turns, T* sn, T* cs) {
+  const double q = __builtin_rint(turns * 4.0);
+  const T x = static_cast<T>((turns - q * 0.25) * 6.283185307179586476925);
+  const int quadrant = static_cast<int>(static_cast<int64_t>(q) & 3);
+  const T y = x * x, one = 1;
+  T s = 0, c = 0;
+  if constexpr (sizeof(T) == 8) {
+    s = y * y * (one / -39916800 + y * (one / 6227020800));
+    c = y * y * (one / 479001600 + y * (one / -87178291200));
+  }
+  s = x + x * y * (-one / 6 + y * (one / 120 + y * (-one / 5040 + y * (one / 362880) + s)));
+  c = one + y * (-one / 2 + y * (one / 24 + y * (-one / 720 + y * (one / 40320 + y * (-one / 3628800) + c))));
+  const T a = (quadrant & 1) ? c : s, b = (quadrant & 1) ? s : c;
+  *sn = (quadrant & 2) ? -a : a;
+  *cs = (quadrant == 1 || quadrant == 2) ? -b : b;
+}
+
+// V elements as one access where V * sizeof(IO) is 16, else element by element.
+template <typename IO, int V>
+__device__ inline void load_vec(const char* p, float* out) {
+  if constexpr (V * sizeof(IO) == 16) {
+    typedef IO vec __attribute__((ext_vector_type(V)));
+    const vec x = gload<vec>(as_global(static_cast<const void*>(p)));
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = static_cast<float>(x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = to_f32(load_elem<IO>(p + i * sizeof(IO)));
+  }
+}
+template <typename IO, int V>
+__device__ inline void store_vec(char* p, const float* in) {
+  if constexpr (V * sizeof(IO) == 16) {
+    typedef IO vec __attribute__((ext_vector_type(V)));
+    vec x;
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = from_f32<IO>(in[i]);
+    gstore<vec>(as_global(static_cast<void*>(p)), x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) store_elem<IO>(p + i * sizeof(IO), from_f32<IO>(in[i]));
+  }
+}
+
+// What the rotation of IO rows is computed in: fp32 rows are rotated in fp64 and
+// rounded once, since in fp32 the cosine, sine and two products would each round
+// to the digits that are stored (2048 tokens of 16 and 2 heads of 128 13.9 us for
+// 13.6).
+template <typename IO>
+using turn_t = std::conditional_t<sizeof(IO) == 4, double, float>;
+
+template <typename IO>
+using turn_pair = turn_t<IO> __attribute__((ext_vector_type(2)));
+
+// The cosine and sine, times the magnitude, by which pair `i` of token row t at
+// place p turns.
+template <typename PAIR, typename T>
+CB_INLINE PAIR turn_of(const InstallArgs& a, int t, int p, int i) {
+  int64_t pos = p;
+  if (a.positions) {
+    const int64_t at = a.axes > 1 ? a.pair_axis[i] * a.axis_stride + t : t;
+    pos = a.positions_kind == CB_INDEX_I64 ? static_cast<const int64_t*>(a.positions)[at]
+                                           : static_cast<const int32_t*>(a.positions)[at];
+  }
+  T s, c;
+  sincos_turns(static_cast<double>(pos) * a.inv_freq[i] * 0.15915494309189533577, &s, &c);
+  return PAIR{c * a.magnitude, s * a.magnitude};
+}
+
+// V pairs x (2 V elements: both vectors of the pairs, or neighbours) turned.
+template <int V, typename PAIR>
+CB_INLINE void turn_pairs(const float (&x)[2 * V], const PAIR* turn, bool interleaved, float (&y)[2 * V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const PAIR cs = turn[i];
+    if (interleaved) {
+      y[2 * i] = static_cast<float>(x[2 * i] * cs.x - x[2 * i + 1] * cs.y);
+      y[2 * i + 1] = static_cast<float>(x[2 * i + 1] * cs.x + x[2 * i] * cs.y);
+    } else {
+      y[i] = static_cast<float>(x[i] * cs.x - x[i + V] * cs.y);
+      y[i + V] = static_cast<float>(x[i + V] * cs.x + x[i] * cs.y);
+    }
+  }
+}
+
+// y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin for the pairs (a, b) of the
+// rotated part, angles position * inv_freq. One wave per (token, slice of its
+// heads' elements): lanes compute the token's angles once into LDS, then each
+// item is V pairs of a head (two vectors) or V elements that are copied; slices
+// are cut to an item a lane, so that a wave waits for memory once. Every element
+// is read once and written once. 64 tokens of 64 query and 8 KV heads of 128 in bf16
+// take 4.8 us, the latency of a launch and of three dependent loads; 2048 of 16
+// and 2 (21 MB) 9.3 us, that latency and the bytes' time at a copy's rate.
+// KV: K and V rows go into the cache as they are, else queries alone are written.
+// WHOLE: requests that do not start at a page's first slot are outside the bounds.
+template <typename IO, int V, bool KV, bool WHOLE>
+CB_INLINE void install_rows(const InstallArgs& a, int64_t unit, turn_pair<IO>* turn) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int t = static_cast<int>(unit / a.slices), slice = static_cast<int>(unit % a.slices);
+  if (t >= a.batch.tokens) return;
+  const int b = request_of_token(a.batch, t);
+  if (b >= a.batch.requests) return;
+  const Request r = load_request(a.batch, b);
+  if (!r.ok | (WHOLE & (r.rem != 0))) return;
+  const int p = r.length - r.n + (t - r.q0);
+  int64_t row = -1;
+  if constexpr (KV) {
+    row = cache_row(a.batch, r, p);
+    if (row < 0 && lane == 0) flag(a.batch.err, CB_ERROR_TARGET_ROW);
+  }
+  const int pairs = a.rotary_dim / 2, kv_heads = KV ? a.kv_heads : 0;
+  for (int i = lane; i < pairs; i += kWave) turn[i] = turn_of<turn_pair<IO>, turn_t<IO>>(a, t, p, i);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const int rot_items = pairs / V, pass_items = (a.head_dim - a.rotary_dim) / V, head_items = rot_items + pass_items;
+  const int v_items = a.head_dim / V;
+  const int turned = (a.q_heads + kv_heads) * head_items;
+  const int total = turned + kv_heads * v_items;
+  const int per = (total + a.slices - 1) / a.slices;
+  const int stop = min(total, (slice + 1) * per);
+  char* krow = const_cast<char*>((const char*)layer_base(a.cache, 0, a.layer)) + row * a.cache.row_stride_b;
+  char* vrow = const_cast<char*>((const char*)layer_base(a.cache, 1, a.layer)) + row * a.cache.row_stride_b;
+  constexpr int E = sizeof(IO);
+  for (int idx = slice * per + lane; idx < stop; idx += kWave) {
+    const char* src;
+    char* dst;
+    int item;
+    if (idx < turned) {
+      const int head = idx / head_items;
+      item = idx - head * head_items;
+      if (head < a.q_heads) {
+        src = a.q.data + t * a.q.token_b + head * a.q.head_b;
+        dst = a.q_out.data + t * a.q_out.token_b + head * a.q_out.head_b;
+      } else {
+        src = a.k.data + t * a.k.token_b + (head - a.q_heads) * a.k.head_b;
+        dst = krow + static_cast<int64_t>(head - a.q_heads) * a.head_dim * E;
+        if (row < 0) continue;
+      }
+    } else {
+      if (row < 0) continue;
+      const int head = (idx - turned) / v_items;
+      const int off = (idx - turned - head * v_items) * V;
+      float x[V];
+      load_vec<IO, V>(a.v.data + t * a.v.token_b + head * a.v.head_b + off * E, x);
+      store_vec<IO, V>(vrow + (static_cast<int64_t>(head) * a.head_dim + off) * E, x);
+      continue;
+    }
+    if (item >= rot_items) {
+      const int off = a.rotary_dim + (item - rot_items) * V;
+      float x[V];
+      load_vec<IO, V>(src + off * E, x);
+      store_vec<IO, V>(dst + off * E, x);
+      continue;
+    }
+    const int first = item * V;
+    const int oa = a.interleaved ? 2 * first : first, ob = a.interleaved ? oa + V : first + pairs;
+    float x[2 * V], y[2 * V];
+    load_vec<IO, V>(src + oa * E, x);
+    load_vec<IO, V>(src + ob * E, x + V);
+    turn_pairs<V>(x, turn + first, a.interleaved, y);
+    store_vec<IO, V>(dst + oa * E, y);
+    store_vec<IO, V>(dst + ob * E, y + V);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+// The token tensors and the rotation of an install, checked; the batch and the
+// cache are the caller's.
+int check_install(const cb_query_batch* batch, int32_t layer, int32_t dtype, int32_t head_dim, const cb_heads* q,
+                  const cb_heads* q_out, const cb_heads* k, const cb_heads* v, const cb_rotation* rotation, InstallArgs* a) {
+  int rc;
+  if (layer < 0 || layer >= batch->cache.num_layers) return fail(CB_EINVAL, "layer %d outside the cache", layer);
+  if (!q) return fail(CB_EINVAL, "null q");
+  const int eb = elem_bytes(dtype), kv = batch->cache.heads, n = batch->num_tokens;
+  if (q->heads < 1 || q->heads > (1 << 16)) return fail(CB_EINVAL, "q needs 1 to 65536 heads");
+  if ((rc = check_heads("q", q, q->heads, eb, n, &a->q)) || (rc = check_output("q_out", q_out, q->heads, eb, n, head_dim, &a->q_out)) ||
+      (rc = check_heads("k", k, kv, eb, n, &a->k)) || (rc = check_heads("v", v, kv, eb, n, &a->v)))
+    return rc;
+  if (!rotation) return fail(CB_EINVAL, "null rotation");
+  const cb_rotation& o = *rotation;
+  if (o.rotary_dim < 2 || o.rotary_dim > head_dim || o.rotary_dim % 2)
+    return fail(CB_EINVAL, "rotary_dim must be even, 2 to head_dim");
+  if (!o.inv_freq) return fail(CB_EINVAL, "null inv_freq");
+  if (!std::isfinite(o.magnitude)) return fail(CB_EINVAL, "magnitude must be finite");
+  if (o.positions && o.positions_kind != CB_INDEX_I32 && o.positions_kind != CB_INDEX_I64)
+    return fail(CB_EINVAL, "positions must be int32 or int64");
+  a->axes = 1;
+  if (o.pair_axis) {
+    if (o.axes < 1 || o.axes > kMaxAxes) return fail(CB_EINVAL, "a rotation has 1 to %d axes", kMaxAxes);
+    if (o.positions && o.axis_stride < n) return fail(CB_EINVAL, "axes of positions are shorter than num_tokens");
+    for (int i = 0; i < o.rotary_dim / 2; ++i) {
+      if (o.pair_axis[i] >= o.axes) return fail(CB_EINVAL, "pair %d turns by axis %d of %d", i, o.pair_axis[i], o.axes);
+      a->pair_axis[i] = o.pair_axis[i];
+    }
+    a->axes = o.axes;
+    a->axis_stride = o.axis_stride;
+  }
+  if (shares_rows(*batch)) return fail(CB_EINVAL, "several requests need offsets or a request_stride");
+  a->layer = layer;
+  a->head_dim = head_dim;
+  a->rotary_dim = o.rotary_dim;
+  a->interleaved = o.interleaved != 0;
+  a->q_heads = q->heads;
+  a->kv_heads = kv;
+  a->inv_freq = o.inv_freq;
+  a->positions = o.positions;
+  a->positions_kind = o.positions_kind;
+  a->magnitude = o.magnitude;
+  return CB_OK;
+}
+
+}  // namespace

@@ -10,7 +10,10 @@ model answers on it, layer by layer:
   whole, capped scores, biases by distance, grouped heads);
 - ``add_key_weights``: add to each cached token the attention it got;
 - ``evict_tokens``: keep the first, the last and the heaviest tokens of long
-  histories, copied in order to other pages.
+  histories, copied in order to other pages;
+- ``quantize_tokens``: move histories into the pages of a ``QuantizedKVPool``
+  (e4m3 codes, a scale for each page and head), on which ``install_tokens`` and
+  ``paged_attention`` go on at half the bytes of a 16-bit pool.
 
 ``QueryBatch`` describes the batch once for all layers. Its lengths and
 offsets are device tensors that the kernels read, so a captured graph follows
@@ -99,6 +102,8 @@ class QueryBatch:
     request longer than ``request_stride`` would reach into the next one's
     tokens: it is outside the batch's bounds. What ``offsets`` leave each
     request is the caller's to keep to.
+    Over 8-bit rows (``rows`` with scales) token tensors are of the scales'
+    ``dtype``.
     ``max_query`` and ``max_length`` bound the new and cached tokens of any
     request (default bounds read nothing from the device: ``max_query`` is
     every token row, so give it where it is known; a decoding step divides its
@@ -146,8 +151,10 @@ class QueryBatch:
         self.max_query = None if max_query is None else int(max_query)
         self.max_length = int(max_length)
         self.device = rows.device
-        self.dtype = rows.dtype
-        self._code = io_dtype_code(rows.dtype)
+        self.scales = rows.c_scales
+        self._scales = None if self.scales is None else ctypes.byref(self.scales)
+        self.dtype = rows.dtype if rows.scales is None else rows.scales.dtype
+        self._code = io_dtype_code(self.dtype)
         self._keep = (query_start, lengths, offsets)
 
     @property
@@ -185,18 +192,46 @@ class Rotary(NamedTuple):
     """Rotation of new tokens: radians per position of each pair (float64, on
     the batch's device), the magnitude of scaled contexts, and whether pairs
     are neighbours instead of halves of the rotated part. The rotated part is
-    the head's first ``2 * len(inv_freq)`` elements."""
+    the head's first ``2 * len(inv_freq)`` elements.
+
+    ``axes`` (bytes, one per pair) makes positions of several axes, such as time,
+    height and width of image patches: pair ``i`` turns by the position along
+    axis ``axes[i]``."""
 
     inv_freq: torch.Tensor
     magnitude: float = 1.0
     interleaved: bool = False
+    axes: bytes | None = None
+
+    @staticmethod
+    def axis_of_pairs(sections, *, cyclic: bool = False) -> bytes:
+        """The axis of each pair, ``sections[a]`` pairs of axis ``a``.
+
+        In blocks, axis after axis, or ``cyclic``: the axes in turn from pair to
+        pair, axis 0 in place of one whose pairs are used up (which needs the
+        first section to be the largest).
+        """
+        sections = [int(n) for n in sections]
+        if not 1 <= len(sections) <= 8 or min(sections) < 0 or sum(sections) < 1:
+            raise ValueError("a rotation has 1 to 8 axes of some pairs")
+        if not cyclic:
+            return bytes(a for a, n in enumerate(sections) for _ in range(n))
+        axes = [i % len(sections) if i // len(sections) < sections[i % len(sections)] else 0
+                for i in range(sum(sections))]
+        if any(axes.count(a) != n for a, n in enumerate(sections)):
+            raise ValueError("cyclic axes need the first section to be the largest")
+        return bytes(axes)
 
     @classmethod
     def build(cls, rotary_dim: int, theta: float, scaling: dict | None = None, *, interleaved: bool = False,
-              device="cuda") -> "Rotary":
-        """Frequencies of ``rope_frequencies`` (plain, linear, YaRN or Llama 3 scaling)."""
+              sections=None, cyclic: bool = False, device="cuda") -> "Rotary":
+        """Frequencies of ``rope_frequencies`` (plain, linear, YaRN or Llama 3 scaling), with ``sections`` the axes of
+        ``axis_of_pairs`` over ``rotary_dim / 2`` pairs."""
         inv, magnitude = rope_frequencies(rotary_dim, theta, scaling)
-        return cls(inv.to(device), magnitude, interleaved)
+        axes = None if sections is None else cls.axis_of_pairs(sections, cyclic=cyclic)
+        if axes is not None and len(axes) != inv.numel():
+            raise ValueError(f"the sections must have rotary_dim / 2 = {inv.numel()} pairs")
+        return cls(inv.to(device), magnitude, interleaved, axes)
 
 
 def _flag_pointer(batch: QueryBatch, error_flag: torch.Tensor | None):
@@ -216,30 +251,56 @@ def install_tokens(batch: QueryBatch, layer: int, q: torch.Tensor, k: torch.Tens
     kv_heads, head_dim]``, of any token and head strides (views of a fused
     projection). Returns the rotated ``q``: ``out``, which may be ``q``, or a
     new tensor. ``positions`` (int32 or int64, one per token row) replaces the
-    tokens' places in the cache where these differ, as after an eviction. Rows
-    of no request are neither stored nor written.
+    tokens' places in the cache where these differ, as after an eviction; with
+    ``rotary.axes`` it is ``[axes, tokens]``, contiguous. Rows of no request are
+    neither stored nor written.
+
+    Into an 8-bit pool, K/V rows are rounded to e4m3 under their page's and
+    head's scale: the least power of two that keeps every finite element within
+    448 times it. A page that holds cached tokens keeps its scale unless the new
+    rows need a larger one, to which the cached ones are then rounded. Infinities
+    and NaN are stored as NaN. Such a batch needs a block table of the pool's
+    page size, and requests that start at a page's first slot.
     """
     n, heads, dim = q.shape if q.ndim == 3 else (0, 0, 0)
     cq = batch._heads(q, "q")
     ck = batch._heads(k, "k", n, batch.kv_heads)
     cv = batch._heads(v, "v", n, batch.kv_heads)
-    inv = rotary.inv_freq
-    _device_vector(inv, "inv_freq", (torch.float64,), batch.device, None)
-    kind, pos = 0, None
-    if positions is not None:
-        pos = _device_vector(positions, "positions", (torch.int32, torch.int64), batch.device, n)
-        kind = _lib.CB_INDEX_I64 if positions.dtype == torch.int64 else _lib.CB_INDEX_I32
+    turn = _rotation(batch, rotary, positions, n)
     flag = _flag_pointer(batch, error_flag)
     with _On(batch, stream) as handle:
         if out is None:
             out = q.new_empty((n, heads, dim))
         co = batch._heads(out, "out", n, heads)
-        _lib.check(_lib.load().cb_install_tokens(
-            batch._tokens(n), batch._layer(layer), batch._code, dim, ctypes.byref(cq), ctypes.byref(co), ctypes.byref(ck),
-            ctypes.byref(cv), inv.data_ptr(), 2 * inv.numel(), int(rotary.interleaved), rotary.magnitude, pos, kind,
-            flag, handle))
+        how = (batch._layer(layer), batch._code, dim, ctypes.byref(cq), ctypes.byref(co), ctypes.byref(ck),
+               ctypes.byref(cv), ctypes.byref(turn), flag, handle)
+        lib = _lib.load()
+        if batch.scales is None:
+            _lib.check(lib.cb_install_rotated(batch._tokens(n), *how))
+        else:
+            _lib.check(lib.cb_install_quantized(batch._tokens(n), batch._scales, *how))
         batch.rows.hold_for(stream)
     return out
+
+
+def _rotation(batch: QueryBatch, rotary: Rotary, positions: torch.Tensor | None, n: int) -> _lib.CbRotation:
+    inv, axes = rotary.inv_freq, rotary.axes
+    c = _lib.CbRotation(_device_vector(inv, "inv_freq", (torch.float64,), batch.device, None), None, None, n,
+                        2 * inv.numel(), int(rotary.interleaved), 0, 1, rotary.magnitude)
+    if axes is not None:
+        if not isinstance(axes, bytes) or len(axes) != inv.numel() or max(axes) > 7:
+            raise ValueError("axes must be bytes, 0 to 7, one for each pair of inv_freq")
+        c.pair_axis, c.axes = axes, max(axes) + 1
+    if positions is not None:
+        if axes is not None:
+            if positions.ndim != 2 or positions.shape[0] < c.axes or positions.shape[1] != n:
+                raise ValueError("positions must be [axes, tokens] with one row for each of the rotation's axes")
+            # One row a axis is all that is read: the flat vector holds them one after another.
+            positions = positions.view(-1) if positions.is_contiguous() else positions
+        c.positions = _device_vector(positions, "positions", (torch.int32, torch.int64), batch.device,
+                                     n if axes is None else None)
+        c.positions_kind = _lib.CB_INDEX_I64 if positions.dtype == torch.int64 else _lib.CB_INDEX_I32
+    return c
 
 
 def _scores(batch: QueryBatch, heads: int, dim: int, scale, causal, window, cap, slopes, prefix_lengths):
@@ -278,7 +339,9 @@ def paged_attention(batch: QueryBatch, layer: int, q: torch.Tensor, *, scale: fl
     fp32; the weights of a 16-bit pool are rounded to its type for their product
     with V, which adds about as much error as the result's own rounding, unless
     ``fp32_weights``, which takes fp32 products (8 to 13 times as long for
-    prompts, 2 to 4 times for steps and short questions).
+    prompts, 2 to 4 times for steps and short questions). Over an 8-bit pool the
+    cached values are codes times scales, and ``q`` and the result are of the
+    scales' ``dtype``.
     """
     n, heads, dim = q.shape if q.ndim == 3 else (0, 0, 0)
     cq = batch._heads(q, "q")
@@ -293,11 +356,12 @@ def paged_attention(batch: QueryBatch, layer: int, q: torch.Tensor, *, scale: fl
         lse = q.new_empty((n, heads), dtype=torch.float32) if return_lse else None
         c = batch._tokens(n)
         need = ctypes.c_int64(0)
-        _lib.check(lib.cb_attention_workspace_bytes(c, batch._code, dim, ctypes.byref(scores), heads,
-                                                    ctypes.byref(need)))
+        ask, attend, more = ((lib.cb_attention_workspace_bytes, lib.cb_paged_attention, ()) if batch.scales is None else
+                             (lib.cb_quantized_attention_workspace_bytes, lib.cb_quantized_attention, (batch._scales,)))
+        _lib.check(ask(c, *more, batch._code, dim, ctypes.byref(scores), heads, ctypes.byref(need)))
         work = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
-        _lib.check(lib.cb_paged_attention(
-            c, batch._layer(layer), batch._code, dim, ctypes.byref(scores), ctypes.byref(cq), ctypes.byref(co),
+        _lib.check(attend(
+            c, *more, batch._layer(layer), batch._code, dim, ctypes.byref(scores), ctypes.byref(cq), ctypes.byref(co),
             None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), need.value, flag,
             handle))
         batch.rows.hold_for(stream)
@@ -315,6 +379,7 @@ def add_key_weights(batch: QueryBatch, layer: int, q: torch.Tensor, lse: torch.T
     ``[requests, >= max_length]`` and keeps what no new token sees. The order
     of every sum is fixed: the same call gives the same bits.
     """
+    _plain_pool(batch)
     n, heads, dim = q.shape if q.ndim == 3 else (0, 0, 0)
     cq = batch._heads(q, "q")
     if lse.shape != (n, heads) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != batch.device:
@@ -327,6 +392,11 @@ def add_key_weights(batch: QueryBatch, layer: int, q: torch.Tensor, lse: torch.T
             batch._tokens(n), batch._layer(layer), batch._code, dim, ctypes.byref(scores), ctypes.byref(cq), lse.data_ptr(),
             weights.data_ptr(), stride, flag, handle))
         batch.rows.hold_for(stream)
+
+
+def _plain_pool(batch: QueryBatch) -> None:
+    if batch.scales is not None:
+        raise ValueError("8-bit pools are read by paged_attention alone; weigh and evict before quantize_tokens")
 
 
 def _weights_stride(batch: QueryBatch, weights: torch.Tensor) -> int:
@@ -374,6 +444,8 @@ def evict_tokens(batch: QueryBatch, weights: torch.Tensor, target: QueryBatch, *
     ``positions``: on an evicted cache, windows and slopes measure the places
     that are left. Models with either should not go on from one.
     """
+    _plain_pool(batch)
+    _plain_pool(target)
     stride = _weights_stride(batch, weights)
     if target.device != batch.device or target.dtype != batch.dtype:
         raise ValueError("batch and target must share device and dtype")
@@ -396,3 +468,40 @@ def evict_tokens(batch: QueryBatch, weights: torch.Tensor, target: QueryBatch, *
         batch.rows.hold_for(stream)
         target.rows.hold_for(stream)
     return kept
+
+
+def quantize_tokens(batch: QueryBatch, target: QueryBatch, *, out: torch.Tensor | None = None,
+                    error_flag: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Move the cached tokens of each request, all layers, to tokens 0, 1, ... of the same request of ``target``.
+
+    ``target`` is a batch over unpublished pages of an 8-bit pool whose
+    ``dtype`` is ``batch``'s, with a block table of the pool's page size and
+    requests that start at a page's first slot (its lengths are not read; a token
+    past its ``request_stride`` is not copied and sets ``ERROR_TARGET_ROW``).
+    Every page and head gets the least scale that keeps its finite elements
+    within 448 times it; slots behind a request's last token keep their codes.
+
+    Returns int32 ``[requests]`` lengths (``out`` or a new tensor): a request's
+    own, or 0 where it is outside the batch's bounds or some cached token has no
+    row (``ERROR_REQUEST``, ``ERROR_CACHE_ROW``): its pages then hold in part
+    what they held before.
+    """
+    _plain_pool(batch)
+    if target.scales is None:
+        raise ValueError("target must be a batch over an 8-bit pool")
+    if target.device != batch.device or target.dtype != batch.dtype:
+        raise ValueError("batch and target must share device and dtype")
+    if target.requests != batch.requests:
+        raise ValueError("batch and target must have the same requests")
+    dim = batch.head_dim
+    if target.kv_heads != batch.kv_heads or target.head_dim != dim or target.rows.num_layers != batch.rows.num_layers:
+        raise ValueError("batch and target must share layers, KV heads and head_dim")
+    flag = _flag_pointer(batch, error_flag)
+    with _On(batch, stream) as handle:
+        if out is None:
+            out = torch.empty(batch.requests, dtype=torch.int32, device=batch.device)
+        _lib.check(_lib.load().cb_quantize_tokens(
+            batch._tokens(0), target._tokens(0), target._scales, batch._code, dim,
+            _device_vector(out, "out", (torch.int32,), batch.device, batch.requests), flag, handle))
+        batch.rows.hold_for(stream)
+    return out

@@ -30,6 +30,38 @@ def io_dtype_code(dtype: torch.dtype) -> int:
         raise ValueError(f"unsupported KV dtype {dtype}; expected bfloat16, float16 or float32") from None
 
 
+@dataclass(frozen=True)
+class BlockScales:
+    """Scales of an 8-bit pool: one power of two per layer, page and KV head, for K and for V.
+
+    ``k`` and ``v`` are contiguous ``[layers, pages, kv_heads]`` tensors of
+    ``float8_e8m0fnu`` (the exponent alone); row ``r`` of the pool is in page
+    ``r // page_size``. An element's value is its e4m3 code's times its page's
+    and head's scale. ``dtype`` is the type of the rows that are stored and of
+    the queries and outputs: bfloat16, float16 or float32.
+    """
+
+    k: torch.Tensor
+    v: torch.Tensor
+    page_size: int
+    dtype: torch.dtype = torch.bfloat16
+
+    def c(self, codes: torch.dtype, layers: int, rows: int, heads: int, device) -> _lib.CbPageScales:
+        """The C description, for pools of ``codes`` with these sizes."""
+        if codes != torch.float8_e4m3fn:
+            raise ValueError("a pool with scales must be of float8_e4m3fn")
+        io_dtype_code(self.dtype)
+        if type(self.page_size) is not int or not 1 <= self.page_size <= 1 << 20:
+            raise ValueError("the scales' page_size must be 1 to 2^20")
+        pages = -(-rows // self.page_size)
+        for t in (self.k, self.v):
+            if t.dtype != torch.float8_e8m0fnu or t.device != device or not t.is_contiguous():
+                raise ValueError(f"scales must be contiguous float8_e8m0fnu tensors on {device}")
+            if t.shape != (layers, pages, heads):
+                raise ValueError(f"scales must be [layers, pages, kv_heads], here {[layers, pages, heads]}")
+        return _lib.CbPageScales(self.k.data_ptr(), self.v.data_ptr(), pages * heads, heads, pages, self.page_size)
+
+
 @dataclass
 class Rows:
     """One side of a launch: K/V layer buffers, row geometry and token -> row index.
@@ -49,6 +81,8 @@ class Rows:
     keep: list = field(default_factory=list)
     owned: list = field(default_factory=list)
     index_entries: int = 0
+    scales: BlockScales | None = None
+    c_scales: _lib.CbPageScales | None = None
 
     @property
     def num_layers(self) -> int:
@@ -149,8 +183,8 @@ def rows_from_layers(k_layers: Sequence[torch.Tensor], v_layers: Sequence[torch.
 
 def rows_from_stacked(k: torch.Tensor, v: torch.Tensor, *, index=None, block_table=None,
                       page_size=None, index_offset: int = 0, head_offset: int = 0,
-                      tokens=None) -> Rows:
-    """Stacked ``[layers, rows, heads, head_dim]`` K and V tensors."""
+                      tokens=None, scales: BlockScales | None = None) -> Rows:
+    """Stacked ``[layers, rows, heads, head_dim]`` K and V tensors, with ``scales`` of e4m3 codes."""
     if k.ndim != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
         raise ValueError("stacked K/V must be matching [layers, rows, kv_heads, head_dim]")
     if not (k.is_contiguous() and v.is_contiguous()):
@@ -159,7 +193,11 @@ def rows_from_stacked(k: torch.Tensor, v: torch.Tensor, *, index=None, block_tab
     kind, idx_ptr, keep = _index_fields(index, block_table, page_size, index_offset, tokens)
     c = _lib.CbRows(None, None, k.data_ptr(), v.data_ptr(), rows * heads * dim, heads * dim, rows, layers, head_offset,
                     heads, kind, idx_ptr, index_offset, page_size or 0)
-    return Rows(c, k.dtype, k.device, [k, v, *keep], index_entries=keep[0].numel() if keep else 0)
+    r = Rows(c, k.dtype, k.device, [k, v, *keep], index_entries=keep[0].numel() if keep else 0)
+    if scales is not None:
+        r.scales, r.c_scales = scales, scales.c(k.dtype, layers, rows, heads, k.device)
+        r.keep += [scales.k, scales.v]
+    return r
 
 
 @dataclass(frozen=True)

@@ -17,7 +17,7 @@ import weakref
 
 import torch
 
-from .plan import Rows, copy_rows, rows_from_layers, rows_from_page, rows_from_stacked
+from .plan import BlockScales, Rows, copy_rows, io_dtype_code, rows_from_layers, rows_from_page, rows_from_stacked
 
 
 class PagedKVPool:
@@ -86,6 +86,54 @@ class PagedKVPool:
                   row_elements=self.head_num * self.head_dim)
 
 
+class QuantizedKVPool:
+    """Paged KV pool of 8-bit rows: e4m3 codes and a power of two as scale for each page and head.
+
+    ``k_data`` and ``v_data`` are ``[layers, rows, heads, head_dim]`` of
+    ``float8_e4m3fn``, ``k_scale`` and ``v_scale`` ``[layers, pages, heads]`` of
+    ``float8_e8m0fnu``. ``dtype`` is the type of the rows that it is given and
+    of the queries that are answered on it. Pages are filled by
+    ``quantize_tokens`` (an installed prefix) and ``install_tokens`` (new
+    tokens), read by ``paged_attention`` (all of
+    ``cachebridge_amd.online.queries``); the other operators refuse such a pool.
+    """
+
+    def __init__(self, *, layer_num: int, pages: int, head_num: int, head_dim: int, page_size: int = 16,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda", start_layer: int = 0, fill: str | None = None):
+        if not 1 <= page_size <= 1 << 20 or pages < 1:
+            raise ValueError("pages must be positive and page_size 1 to 2^20")
+        io_dtype_code(dtype)
+        self.layer_num = int(layer_num)
+        self.start_layer = int(start_layer)
+        self.page_size = int(page_size)
+        self.pages = int(pages)
+        self.size = self.pages * self.page_size
+        self.head_num = int(head_num)
+        self.head_dim = int(head_dim)
+        self.dtype = dtype
+        self.device = torch.device(device)
+        shape = (self.layer_num, self.size, self.head_num, self.head_dim)
+        self.k_data = torch.empty(shape, dtype=torch.float8_e4m3fn, device=self.device)
+        self.v_data = torch.empty(shape, dtype=torch.float8_e4m3fn, device=self.device)
+        if fill == "zeros":
+            self.k_data.view(torch.uint8).zero_()
+            self.v_data.view(torch.uint8).zero_()
+        # The least scale: a page grows from it with what is stored.
+        scales = torch.ones((2, self.layer_num, self.pages, self.head_num), dtype=torch.uint8, device=self.device)
+        self.k_scale, self.v_scale = scales.view(torch.float8_e8m0fnu).unbind(0)
+
+    def rows(self, *, index=None, block_table=None, page_size=None, index_offset: int = 0, head_offset: int = 0,
+             tokens=None, layers: slice | None = None) -> Rows:
+        """Describe this pool (optionally a layer sub-range) with a token -> row index."""
+        part = slice(None) if layers is None else layers
+        if block_table is not None and page_size is None:
+            page_size = self.page_size
+        scales = BlockScales(self.k_scale[part], self.v_scale[part], self.page_size, self.dtype)
+        return rows_from_stacked(self.k_data[part], self.v_data[part], index=index, block_table=block_table,
+                                 page_size=page_size, index_offset=index_offset, head_offset=head_offset,
+                                 tokens=tokens, scales=scales)
+
+
 # Per-pool device tables of per-layer K/V pointers, for pools that are not a
 # PagedKVPool (one buffer per layer, e.g. SGLang's MHATokenToKVPool): built
 # once per pool and rebuilt only when the pool's buffers move.
@@ -107,7 +155,7 @@ def pool_rows(pool, *, index=None, block_table=None, page_size=None, index_offse
     layer pointers. Without ``pointer_cache`` the table is kept per pool, so
     it is uploaded once, not per call; launches record it on their stream.
     """
-    if isinstance(pool, PagedKVPool):
+    if isinstance(pool, (PagedKVPool, QuantizedKVPool)):
         return pool.rows(index=index, block_table=block_table, page_size=page_size,
                          index_offset=index_offset, head_offset=head_offset, tokens=tokens)
     if pointer_cache is None:

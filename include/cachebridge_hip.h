@@ -375,6 +375,29 @@ int cb_install_tokens(const cb_query_batch* batch, int32_t layer, int32_t dtype,
                       int32_t interleaved, float magnitude, const void* positions,
                       int32_t positions_kind, int32_t* d_error_flag, void* stream);
 
+/* A rotation whose pairs turn by positions of several axes (time, height, width
+   of image patches): pair i turns by positions[pair_axis[i] * axis_stride + t]
+   * inv_freq[i]. The other fields are cb_install_tokens's arguments. */
+typedef struct cb_rotation {
+  const double* inv_freq;   /* device, rotary_dim / 2 entries */
+  const void* positions;    /* device, [axes] rows of num_tokens entries, axis_stride apart, or NULL:
+                               a token's place along every axis */
+  const uint8_t* pair_axis; /* HOST array of rotary_dim / 2 axes, read during the call, or NULL: one axis */
+  int64_t axis_stride;      /* read with pair_axis and positions: at least num_tokens */
+  int32_t rotary_dim;
+  int32_t interleaved;
+  int32_t positions_kind;
+  int32_t axes;             /* 1 to 8, read with pair_axis */
+  float magnitude;
+  int32_t reserved;
+} cb_rotation;
+
+/* cb_install_tokens with positions of several axes. Asynchronous. */
+int cb_install_rotated(const cb_query_batch* batch, int32_t layer, int32_t dtype, int32_t head_dim,
+                       const cb_heads* q, const cb_heads* q_out, const cb_heads* k,
+                       const cb_heads* v, const cb_rotation* rotation, int32_t* d_error_flag,
+                       void* stream);
+
 /* Device workspace bytes of cb_paged_attention for this batch (0: none). With
    few query rows per KV head it grows with the bound, max_length / 2048 *
    num_tokens * query_heads * head_dim floats or more. */
@@ -424,6 +447,63 @@ int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, i
                     int32_t head_dim, const float* weights, int64_t weights_stride, int32_t budget,
                     int32_t first, int32_t last, int32_t* kept, int32_t* kept_lengths,
                     float* kept_weights, int32_t* d_error_flag, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Queries on an 8-bit cache. K and V rows hold e4m3 codes (the OCP format: no
+ * infinities, 0x7f and 0xff are NaN), a byte an element; an element's value is
+ * its code's times 2^(byte - 127), byte the scale of its layer, page and KV head
+ * (1 to 254). Pages are page_size rows: row r is in page r / page_size. Such a
+ * cache is described by the same cb_query_batch (strides of its cb_rows count
+ * bytes) and the scales beside it; the token tensors are of `dtype`.
+ *
+ * Rows that are stored choose the scale: the least that holds every finite
+ * element of the page's stored rows up to 448 times it (2^-126 where all are
+ * zero). Codes are rounded to nearest even; infinities and NaN become NaN.
+ * With dtype CB_DTYPE_F16 a scale is at most 2^7, which keeps values within that
+ * type (larger elements are stored as 448 times the scale).
+ * No counterpart in the reference, whose caches are 16 bits wide.
+ */
+typedef struct cb_page_scales {
+  uint8_t* k;            /* device: [layer * layer_stride + page * page_stride + head] */
+  uint8_t* v;
+  int64_t layer_stride;
+  int64_t page_stride;   /* at least the KV heads */
+  int64_t pages;         /* pages * page_size must cover the cache's rows */
+  int32_t page_size;
+  int32_t reserved;
+} cb_page_scales;
+
+/* cb_install_rotated into an 8-bit cache. Its index must be a block table of
+   the scales' page_size and a request must start at a page's first slot (else
+   it is outside the bounds): a page then belongs to one request, and one wave
+   stores it. A page whose first slots hold cached tokens keeps its scale unless
+   the new rows need a larger one: those tokens' codes are then rounded to it.
+   Slots behind the new tokens keep their codes. Asynchronous. */
+int cb_install_quantized(const cb_query_batch* batch, const cb_page_scales* scales, int32_t layer,
+                         int32_t dtype, int32_t head_dim, const cb_heads* q, const cb_heads* q_out,
+                         const cb_heads* k, const cb_heads* v, const cb_rotation* rotation,
+                         int32_t* d_error_flag, void* stream);
+
+/* The cached tokens of every request of `batch` (a cache of dtype), all
+   layers, to tokens 0, 1, ... of the same request of the 8-bit cache `target`
+   (its cache, index, offsets and request_stride are read; block table and starts
+   as for cb_install_quantized). query_start is not read. lengths_out [requests]
+   gets the length of each, or 0 for a request outside the bounds or with a
+   cached token without a row (the target's slots of such tokens keep their
+   codes). A token without a row in the target, or past its request_stride, is
+   flagged CB_ERROR_TARGET_ROW and counts. Asynchronous. */
+int cb_quantize_tokens(const cb_query_batch* batch, const cb_query_batch* target,
+                       const cb_page_scales* scales, int32_t dtype, int32_t head_dim,
+                       int32_t* lengths_out, int32_t* d_error_flag, void* stream);
+
+/* cb_paged_attention over an 8-bit cache (any index), and its workspace. */
+int cb_quantized_attention_workspace_bytes(const cb_query_batch* batch, const cb_page_scales* scales,
+                                           int32_t dtype, int32_t head_dim, const cb_scores* scores,
+                                           int32_t query_heads, int64_t* bytes);
+int cb_quantized_attention(const cb_query_batch* batch, const cb_page_scales* scales, int32_t layer,
+                           int32_t dtype, int32_t head_dim, const cb_scores* scores,
+                           const cb_heads* q, const cb_heads* out, float* lse, void* d_workspace,
+                           int64_t workspace_bytes, int32_t* d_error_flag, void* stream);
 
 #ifdef __cplusplus
 }
