@@ -173,7 +173,8 @@ CB_INLINE float natural_score(const ScoreArgs& s, float dot, float slope, int p,
 }
 
 // Raw products of one lane (16 keys of a block that starts at cached token
-// `start`, register e: key 8 (e / 4) + 4 h + e % 4) to scores times `unit`.
+// `start`, register e: key 8 (e / 4) + 4 h + e % 4; or N keys, STEP (e / 4) + 4 h
+// + e % 4) to scores times `unit`.
 // Capped: where no lane's angle reaches kSmallAngle, which is the rule, the
 // polynomial (READY: by factors made ahead, four registers, seven instructions,
 // else nine). A block of 32 rows and keys with larger ones takes tanh y = 1 - 2 /
@@ -182,17 +183,17 @@ CB_INLINE float natural_score(const ScoreArgs& s, float dot, float slope, int p,
 // where the products' own sums are off by more. 8192 tokens with 16 heads of 128 take
 // 419 us with blocks of the first kind and 428 with all of the second; with a
 // selection by element the latter took 599, with the second form alone both 414.
-template <bool READY>
-CB_INLINE void modify_scores(const ScoreArgs& s, f32x16& x, float unit, float slope, int p, int start, int h) {
+template <bool READY, int N = 16, int STEP = 8, typename VEC = f32x16>
+CB_INLINE void modify_scores(const ScoreArgs& s, VEC& x, float unit, float slope, int p, int start, int h) {
   const float by = s.scale * unit;
   if (s.cap > 0) {
     float far = 0;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) far = fmaxf(far, fabsf(x[e]));
+    for (int e = 0; e < N; ++e) far = fmaxf(far, fabsf(x[e]));
     if (__all(far < s.gentle)) {
       const float k3 = kTanh3 * by, k5 = kTanh5 * by, k7 = kTanh7 * by, k9 = kTanh9 * by;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
+      for (int e = 0; e < N; ++e) {
         const float y = x[e] * s.inner, t = y * y, w = x[e] * by;
         if constexpr (READY)
           x[e] *= __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, k9, k7), k5), k3), by);
@@ -203,16 +204,16 @@ CB_INLINE void modify_scores(const ScoreArgs& s, f32x16& x, float unit, float sl
     } else {
       const float in = 2.0f * kLog2e * s.inner, out = s.cap * unit;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = __builtin_fmaf(-2.0f * out, __builtin_amdgcn_rcpf(exp2_fast(x[e] * in) + 1.0f), out);
+      for (int e = 0; e < N; ++e) x[e] = __builtin_fmaf(-2.0f * out, __builtin_amdgcn_rcpf(exp2_fast(x[e] * in) + 1.0f), out);
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] *= by;
+    for (int e = 0; e < N; ++e) x[e] *= by;
   }
   if (s.slopes) {
     const float by = slope * unit, away = static_cast<float>(p - start - 4 * h);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = __builtin_fmaf(-by, fabsf(away - static_cast<float>(8 * (e >> 2) + (e & 3))), x[e]);
+    for (int e = 0; e < N; ++e) x[e] = __builtin_fmaf(-by, fabsf(away - static_cast<float>(STEP * (e >> 2) + (e & 3))), x[e]);
   }
 }
 
@@ -830,12 +831,14 @@ __device__ inline u32x4 finite_part(u32x4 x) {
 
 // The operands of one row of `dim` elements: chunks 2 k + h of 16 bytes, zeros
 // past dim. Loads are at clamped places and selected after: as branches each
-// would wait for the one before.
-template <int KS>
+// would wait for the one before. WIDE: a lane's chunks 2 k and 2 k + 1 are
+// neighbours, as 16 codes of an 8-bit row are (dim a multiple of 16).
+template <int KS, bool WIDE = false>
 CB_INLINE void load_operands(const char* row, int dim, int h, bool vector, u32x4 (&x)[KS]) {
 #pragma unroll
   for (int k = 0; k < KS; ++k) {
-    const char* at = row + 2 * min(16 * k + 8 * h, dim - 8);
+    const int first = WIDE ? 32 * (k >> 1) + 16 * h + 8 * (k & 1) : 16 * k + 8 * h;
+    const char* at = row + 2 * min(first, dim - 8);
     if (vector) {
       x[k] = gload<u32x4>(as_global(static_cast<const void*>(at)));
     } else {
@@ -845,7 +848,7 @@ CB_INLINE void load_operands(const char* row, int dim, int h, bool vector, u32x4
     }
   }
 #pragma unroll
-  for (int k = 0; k < KS; ++k) x[k] = 16 * k + 8 * h < dim ? x[k] : u32x4{0, 0, 0, 0};
+  for (int k = 0; k < KS; ++k) x[k] = (WIDE ? 32 * (k >> 1) + 16 * h : 16 * k + 8 * h) < dim ? x[k] : u32x4{0, 0, 0, 0};
 }
 
 // 32 query rows of one wave: their operands, statistics and sums.
@@ -860,6 +863,7 @@ struct RowBlock {
   int row, i, qh, p;  // this lane's query row
   bool live;
 
+  template <bool WIDE = false>
   __device__ inline void init(const ScoreArgs& s, const Request& r, int head, int row0, bool vector) {
     const int lane = threadIdx.x & (kWave - 1), h = lane >> 5;
     const int rows = r.n * s.group;
@@ -870,7 +874,7 @@ struct RowBlock {
     qh = head * s.group + at - i * s.group;
     p = r.length - r.n + i;
     const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
-    load_operands<KS>(qp, s.head_dim, h, vector, q);
+    load_operands<KS, WIDE>(qp, s.head_dim, h, vector, q);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -1135,6 +1139,79 @@ CB_INLINE void mark_not_finite(uint32_t lv, int np, int below, int above, int st
   }
 }
 
+// Sums of NW waves that lie in LDS, each wave's of its own keys (ROWS rows of DP + 4
+// floats, `stride` bytes a wave, with their maxima and totals in stats), become the
+// rows of the result or of a part.
+template <int DP, int NW, int ROWS, typename H>
+CB_INLINE void join_sums(const AttendArgs& a, const Request& r, int head, int row0, int rows, int split, int vector, const char* sums,
+                         int stride, const float (&stats)[2][NW][ROWS]) {
+  constexpr int LD = DP + 4;
+  const ScoreArgs& s = a.s;
+  const int D = s.head_dim, live = min(ROWS, rows - row0), pairs = D / 2;
+  for (int x = threadIdx.x; x < live * pairs; x += NW * kWave) {
+    const int y = x / pairs, d = 2 * (x - y * pairs);
+    float m = kNegInf;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, stats[0][w][y]);
+    const float mu = m == kNegInf ? 0.0f : m;
+    float l = 0, o0 = 0, o1 = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = exp2_fast(stats[0][w][y] - mu);
+      const float* from = reinterpret_cast<const float*>(sums + w * stride) + y * LD + d;
+      l += f * stats[1][w][y];
+      // A wave that saw nothing of this row has nothing to add.
+      o0 += f != 0.0f ? f * from[0] : 0.0f;
+      o1 += f != 0.0f ? f * from[1] : 0.0f;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float lse2 = l == 0.0f ? kNegInf : m + log2_fast(l);
+    const int row = row0 + y, i = row / s.group, qh = head * s.group + row - i * s.group;
+    const int64_t at = static_cast<int64_t>(r.q0 + i) * s.q_heads + qh;
+    if (a.splits > 1) {
+      const int64_t slot = static_cast<int64_t>(split) * s.batch.tokens * s.q_heads + at;
+      *reinterpret_cast<float2*>(a.part_out + slot * D + d) = make_float2(o0 * inv, o1 * inv);
+      if (d == 0) a.part_lse[slot] = lse2;
+    } else {
+      char* op = a.out.data + static_cast<int64_t>(r.q0 + i) * a.out.token_b + qh * a.out.head_b + d * 2;
+      const uint32_t packed = H::pack(o0 * inv, o1 * inv);
+      if (vector) {
+        gstore<uint32_t>(as_global(static_cast<void*>(op)), packed);
+      } else {
+        store_elem<uint16_t>(op, static_cast<uint16_t>(packed));
+        store_elem<uint16_t>(op + 2, static_cast<uint16_t>(packed >> 16));
+      }
+      if (a.lse && d == 0) a.lse[at] = lse2 * kLn2;
+    }
+  }
+}
+
+// The sums of a workgroup's NW waves, each of its own keys, meet in LDS (each
+// wave's in `stride` bytes of its own).
+template <int DP, int NW, typename BLOCK>
+CB_INLINE void join_waves(BLOCK& blk, const AttendArgs& a, const Request& r, int head, int row0, int rows, int split, int vector,
+                          char* sums, int stride, float (&stats)[2][NW][32]) {
+  constexpr int LD = DP + 4;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  blk.l += __shfl_xor(blk.l, 32);
+  const int c = lane & 31, h = lane >> 5;
+  float* mine = reinterpret_cast<float*>(sums + wave * stride) + c * LD;
+  if (blk.live) {
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(mine + 32 * d + 8 * g + 4 * h) =
+            f32x4{blk.o[d][4 * g], blk.o[d][4 * g + 1], blk.o[d][4 * g + 2], blk.o[d][4 * g + 3]};
+  }
+  if (h == 0) {
+    stats[0][wave][c] = blk.m;
+    stats[1][wave][c] = blk.l;
+  }
+  __syncthreads();
+  join_sums<DP, NW, 32, typename BLOCK::H>(a, r, head, row0, rows, split, vector, sums, stride, stats);
+}
+
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
@@ -1180,6 +1257,68 @@ struct AttendShape {
   int64_t tile_slots;
   int request_slots, splits, least_tiles;
 };
+
+constexpr int kStepTiles = 64;  // tiles a split holds at most
+
+// Workgroups of four waves that a launch is split into at least: two a CU. 512 new
+// tokens over 32768 take 262, 173 and 185 us with 256, 512 and 1024, 64 requests of
+// 8 new tokens over 2048 47, 38.5 and 39 us.
+constexpr int kTargetGroups = 512;
+
+// Waves of attend_tile_kernel: eight share a tile's staging among twice the
+// rows, if there are that many and a head's registers leave two waves a SIMD.
+// That pays once a launch has work for all CUs (16 query heads, 2 KV heads,
+// kernel and join, eight waves against four): 256 new tokens over 4096 cached
+// 41.1 / 37.1 us, 64 over 32768 46.1 / 49.2, 1024 over 4096 63 / 70, 256 over
+// 32768 106 / 120; 1000 of 1000 with 8 heads 39.4 / 34.1.
+constexpr int kWideRows = 512;               // query rows per KV head, and
+constexpr int64_t kWideScores = 24ll << 20;  // scores of the launch, from which eight are taken
+// Query rows per KV head up to which attend_step_kernel is taken: one block of
+// rows, so that K and V are read once. This kernel against the tile kernel, each
+// with its join, 8 query heads a KV head: 64 ragged requests of 2550 on average 52 /
+// 100 us; one request of 32768 38 / 38. Where all lengths are alike the tile
+// kernel is ahead: 64 of 2048 42 / 35, with four new tokens 57 / 40.
+constexpr int kStepRows = 32;
+// Its workgroups: one request has all its splits at work, of several requests many
+// are shorter than the bound that splits are cut by. With the join, 512, 1024
+// and 2048: 64 ragged requests 73, 52, 67 us; 64 of 2048 33, 42, 42; one request of
+// 32768 38 with 512 and 47 with 1024.
+constexpr int kStepGroups = 512, kStepGroupsRagged = 1024;
+constexpr int kStepWaves = 2;
+
+// half: the kernels of 16-bit products take the call.
+AttendShape attend_shape(const ScoreArgs& s, bool half, int step_tiles = kStepTiles) {
+  AttendShape h{};
+  h.half = half;
+  const QBatch& B = s.batch;
+  h.step = h.half && static_cast<int64_t>(B.max_query) * s.group <= kStepRows;
+  const int64_t seen = s.window > 0 && s.causal && !s.prefix ? std::min<int64_t>(B.max_length, s.window) : B.max_length;
+  h.waves = h.half && s.head_dim <= 128 && static_cast<int64_t>(B.max_query) * s.group >= kWideRows &&
+                    static_cast<int64_t>(B.tokens) * s.q_heads * seen >= kWideScores
+                ? 8 : 4;
+  h.rows_per_tile = h.step ? 32 : h.half ? 32 * h.waves : kAnyRows;
+  h.keys_per_tile = !h.half ? kAnyKeys : !h.step && s.head_dim <= (s.mod ? 64 : 128) ? 64 : 32;
+  const int per_request = std::max(1, ceil_div(static_cast<int64_t>(B.max_query) * s.group, h.rows_per_tile));
+  const int64_t by_request = static_cast<int64_t>(per_request) * B.requests;
+  const int64_t packed = ceil_div(static_cast<int64_t>(B.tokens) * s.group, h.rows_per_tile) + static_cast<int64_t>(B.requests);
+  h.request_slots = by_request <= packed ? per_request : 0;
+  h.tile_slots = std::min(by_request, packed);
+  int64_t keys = B.max_length;
+  if (s.window > 0 && s.causal && !s.prefix) keys = std::min<int64_t>(keys, static_cast<int64_t>(s.window) + std::min<int64_t>(B.max_query, h.rows_per_tile / s.group + 2));
+  const int key_tiles = std::max(1, ceil_div(keys, h.keys_per_tile) + (s.prefix ? 1 : 0));
+  const int64_t groups = h.tile_slots * s.kv_heads;
+  const int64_t target = !h.step ? kTargetGroups * 4 / h.waves : B.requests > 1 ? kStepGroupsRagged : kStepGroups;
+  h.least_tiles = h.half ? 8 : 2;
+  h.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(1, groups), key_tiles / h.least_tiles)));
+  if (h.step) {
+    // Parts of one size for all requests, cut by the bound: their workgroups end
+    // together (64 ragged requests 47 us, with parts by each one's own keys 68).
+    h.splits = std::max(h.splits, ceil_div(key_tiles, step_tiles));
+    h.least_tiles = ceil_div(key_tiles, h.splits);
+    h.splits = ceil_div(key_tiles, h.least_tiles);
+  }
+  return h;
+}
 
 int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 

@@ -33,7 +33,29 @@ struct PageScales {
   }
 };
 
-__device__ inline float scale_value(uint32_t byte) { return __uint_as_float(byte << 23); }
+// Bytes above the largest that is ever stored read as it: 448 times that is
+// finite, and a value that no row sees must not become an infinity.
+constexpr float kMaxCode = 448.0f;
+constexpr int kLeastExponent = -126, kMostExponent = 119, kMostExponentF16 = 7;
+
+__device__ inline float scale_value(uint32_t byte, int most = kMostExponent) {
+  return __uint_as_float(min(byte, static_cast<uint32_t>(most + 127)) << 23);
+}
+
+// The scales of one layer and head.
+struct HeadScales {
+  const CB_GLOBAL uint8_t* k;
+  const CB_GLOBAL uint8_t* v;
+  uint32_t page_stride, page_size;
+  int32_t page_shift;
+
+  CB_INLINE HeadScales(const PageScales& s, int layer, int head)
+      : k(s.at(0, layer, 0, head)), v(s.at(1, layer, 0, head)), page_stride(s.page_stride), page_size(s.page_size), page_shift(s.page_shift) {}
+  // Where the scale of pool row `row` is: its page's, pages times page_stride being below 2^32.
+  CB_INLINE uint32_t at(int row) const {
+    return (page_shift >= 0 ? static_cast<uint32_t>(row) >> page_shift : static_cast<uint32_t>(row) / page_size) * page_stride;
+  }
+};
 
 struct ScaledCache {
   typedef uint8_t elem;
@@ -44,9 +66,6 @@ struct ScaledCache {
   }
   static __device__ inline float value(uint8_t x) { return __builtin_amdgcn_cvt_f32_fp8(x, 0); }
 };
-
-constexpr float kMaxCode = 448.0f;
-constexpr int kLeastExponent = -126, kMostExponent = 127, kMostExponentF16 = 7;
 
 __device__ inline float finite_size(float x) {
   const float a = fabsf(x);
@@ -60,8 +79,8 @@ __device__ inline int needed_exponent(float top, int most) {
   return u == 0 ? kLeastExponent : max(kLeastExponent, min(most, e));
 }
 
-// 2^-e for e in [-126, 127], exact but for the last, whose reciprocal is subnormal.
-__device__ inline float inverse_scale(int e) { return __uint_as_float(e < 127 ? static_cast<uint32_t>(127 - e) << 23 : 1u << 22); }
+// 2^-e for e in [-126, 126].
+__device__ inline float inverse_scale(int e) { return __uint_as_float(static_cast<uint32_t>(127 - e) << 23); }
 
 // An element over the scale, ready to be rounded: what the scale's bound leaves
 // out stays at 448, what is not finite becomes NaN.
@@ -253,7 +272,7 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t
     return;
   }
   CB_GLOBAL uint8_t* scale = q.scales.at(kind, a.layer, to_page, head);
-  const int had = slot > 0 ? static_cast<int>(*scale) - 127 : kLeastExponent;
+  const int had = slot > 0 ? max(kLeastExponent, min(q.most, static_cast<int>(*scale) - 127)) : kLeastExponent;
   const int D = a.head_dim, pairs = a.rotary_dim / 2;
   gptr to = const_cast<gptr>(layer_base(a.cache, kind, a.layer)) + to_page * ps * a.cache.row_stride_b + static_cast<int64_t>(head) * D;
   const Strided& from = kind ? a.v : a.k;
@@ -333,7 +352,7 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t
         if (m.on & m.two) store_codes<V>(at + m.second, y[u] + V, inv);
       }
   if (e > had && slot > 0) {  // cached tokens of a page whose scale grows
-    const float by = inverse_scale(min(e - had, 127));
+    const float by = inverse_scale(min(e - had, 126));  // codes times 2^-126 are zeros
     const int words = D / 2;
     for (int x = lane; x < slot * words; x += kWave) {
       gptr at = to + x / words * a.cache.row_stride_b + x % words * 2;
@@ -379,6 +398,636 @@ __global__ __launch_bounds__(kInstallWaves * kWave) void install_quantized_kerne
 }
 
 // ---------------------------------------------------------------------------
+// Attention in 16-bit types over codes, head_dim a multiple of 16 up to 256
+// (padded with zeros to DP = 64, 128 or 256). Codes become elements of the matrix
+// products in registers, K times its scale: e4m3 times a power of two is exact
+// in bf16, and in fp16 down to half its least step.
+// ---------------------------------------------------------------------------
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+// 16 codes as 16 elements times `scale` (a power of two).
+template <typename IO>
+CB_INLINE void widen(u32x4 codes, float scale, u32x4& lo, u32x4& hi) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int c = static_cast<int>(codes[w]);
+    uint32_t x, y;
+    if constexpr (std::is_same_v<IO, io_bf16>) {
+      x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, false));
+      y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, true));
+    } else {
+      x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, scale, false));
+      y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, scale, true));
+    }
+    if (w < 2) {
+      lo[2 * w] = x;
+      lo[2 * w + 1] = y;
+    } else {
+      hi[2 * w - 4] = x;
+      hi[2 * w - 3] = y;
+    }
+  }
+}
+
+template <typename IO>
+constexpr int kMostRead = std::is_same_v<IO, io_f16> ? kMostExponentF16 : kMostExponent;
+
+// Bits 7 of the bytes that are NaN codes.
+__device__ inline uint32_t nan_codes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// A workgroup's request, the same in all lanes, in scalar registers: what follows
+// from it (the tiles, their bounds and waits) is then scalar too.
+CB_INLINE int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+CB_INLINE int64_t uniform(int64_t x) {
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(x >> 32)))) << 32 | static_cast<uint32_t>(uniform(static_cast<int>(x))));
+}
+CB_INLINE Request uniform(const Request& r) {
+  Request u = r;
+  u.q0 = uniform(r.q0);
+  u.n = uniform(r.n);
+  u.length = uniform(r.length);
+  u.first = uniform(r.first);
+  u.rem = static_cast<uint32_t>(uniform(static_cast<int>(r.rem)));
+  return u;
+}
+
+// The launch's arguments (the kernel's first), read when this is called: held from the
+// start, those that the end alone needs cost the main loop its scalar registers.
+CB_INLINE AttendArgs late_args() {
+  auto* from = reinterpret_cast<const CB_CONST uint32_t*>((const CB_CONST void*)__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(from));
+  struct Raw {
+    uint32_t w[sizeof(AttendArgs) / 4];
+  } raw;
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(AttendArgs) / 4; ++i) raw.w[i] = from[i];
+  return __builtin_bit_cast(AttendArgs, raw);
+}
+
+// Many query rows: attend_tile_kernel's scheme on tiles that are widened once for
+// all of a workgroup's waves. A tile's codes come to LDS by DMA, each wave reads
+// the ones it asked for (16 a lane), and writes them as elements to where the
+// 16-bit kernel's DMA would have put them; the tile after that is on its way
+// while one is used.
+template <typename IO, int DP, int KT, int NW, bool MOD>
+__global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_codes_kernel(AttendArgs a, ScaledCache cache, int vector) {
+  constexpr int C = DP / 16, kTile = KT * DP * 2, kCodes = KT * DP, kHalf = kCodes / 1024, M = 2 * kHalf / NW, N = kTile / 1024 / NW;
+  static_assert(M >= 1 && 2 * kHalf % NW == 0 && N >= 1 && kTile % (1024 * NW) == 0, "a tile is whole DMA instructions of every wave");
+  __shared__ __align__(1024) char tiles[4 * kTile];  // K, V of one buffer, K, V of the other
+  __shared__ __align__(1024) char codes[2 * kCodes];
+  __shared__ TileRows<KT> tile_rows;
+  __shared__ uint32_t marks[2][NW][32 * (DP / 32)];
+  __shared__ uint32_t odd[2];  // this tile holds values that are not finite; some tile did
+  const ScoreArgs& s = a.s;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int head = blockIdx.x % s.kv_heads, rest = blockIdx.x / s.kv_heads;
+  const int split = rest / a.tile_slots;
+  Request r;
+  int b, tile;
+  if (!find_tile(a, rest % a.tile_slots, 32 * NW, r, b, tile)) return;
+  r = uniform(r), b = uniform(b), tile = uniform(tile);
+  const int rows = r.n * s.group, row0 = tile * 32 * NW;
+  const KeyRange kr = key_range<KT>(s, r, b, row0, min(rows, row0 + 32 * NW) - 1);
+  const int per = split_tiles(a, kr.tiles), t0 = split * per, t1 = min(kr.tiles, t0 + per);
+  if (a.splits > 1 && t0 >= t1) return;
+
+  typedef RowBlock<IO, DP, KT, MOD> Block;
+  Block blk;
+  blk.init(s, r, head, row0 + 32 * wave, vector);
+  const typename Block::Lanes lanes = Block::lanes();
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((CB_LDS_SPACE char*)tiles));
+  const uint32_t lds_codes = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((CB_LDS_SPACE char*)codes)) + wave * M * 1024;
+  const float scale2 = MOD ? 1.0f : s.scale * kLog2e;
+  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+  for (int w = threadIdx.x; w < 2 * NW * DP; w += NW * kWave) (&marks[0][0][0])[w] = 0;
+  auto entry_of = [&](int t) { return t < t1 ? fetch_entry<KT>(s.batch, r, tile_start<KT>(kr, t), tile_end(kr, t)) : -1; };
+  auto place = [&](int64_t entry, int t) {
+    if (t < t1) place_rows(s.batch, r, entry, tile_start<KT>(kr, t), tile_end(kr, t), tile_rows, t & 3);
+  };
+  int64_t entry = -1;
+  if (wave == 0) {
+    const int64_t e0 = entry_of(t0), e1 = entry_of(t0 + 1), e2 = entry_of(t0 + 2);
+    entry = entry_of(t0 + 3);
+    place(e0, t0);
+    place(e1, t0 + 1);
+    place(e2, t0 + 2);
+  }
+  const int64_t off = static_cast<int64_t>(head) * s.head_dim;
+  gcptr kbase = layer_base(s.cache, 0, s.layer) + off, vbase = layer_base(s.cache, 1, s.layer) + off;
+  gcptr zero = as_global(static_cast<const void*>(g_zeros));
+  const uint32_t stride = static_cast<uint32_t>(s.batch.row_stride_b);
+  // Instruction u of a tile: chunk lane % C of key (u % kHalf) * (64 / C) + lane / C, V from kHalf on.
+  const HeadScales hs(cache.scales, s.layer, head);
+  uint32_t scale[M];
+  auto ask = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const int u = wave * M + m, value = u >= kHalf, k = (u - value * kHalf) * (kWave / C) + lane / C, c = lane % C;
+      const uint32_t row = static_cast<uint32_t>(tile_rows.row[t & 3][k]);
+      const bool ok = ((tile_rows.valid[t & 3][k >> 5] >> (k & 31)) & 1) & (c * 16 < s.head_dim);
+      gcptr at = (value ? vbase : kbase) + static_cast<uint64_t>(row) * stride + c * 16;
+      scale[m] = (value ? hs.v : hs.k)[hs.at(row)];
+      dma16(ok ? at : zero, lds_codes + m * 1024);
+    }
+  };
+  // This wave's codes of a tile, widened to the buffer at `to`.
+  auto put = [&](uint32_t to, int next) __attribute__((always_inline)) {
+    u32x4 x[M];
+    float by[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      x[m] = *lds_at<const u32x4>(lds_codes + m * 1024 + lane * 16);
+      by[m] = scale_value(scale[m], kMostRead<IO>);
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // the codes are read: others may come
+    asm volatile("" ::: "memory");
+    if (next < t1) ask(next);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const int u = wave * M + m, value = u >= kHalf, k = (u - value * kHalf) * (kWave / C) + lane / C, c = 2 * (lane % C);
+      u32x4 lo, hi;
+      widen<IO>(x[m], by[m], lo, hi);
+      const int swizzle = value ? swizzle_v<DP>(k) : swizzle_k<DP>(k);
+      const uint32_t row = to + value * kTile + k * DP * 2;
+      *lds_at<u32x4>(row + (c ^ swizzle) * 16) = lo;
+      *lds_at<u32x4>(row + ((c + 1) ^ swizzle) * 16) = hi;
+    }
+  };
+  __syncthreads();
+  if (t0 < t1) {
+    ask(t0);
+    __builtin_amdgcn_s_waitcnt(kWaitAll);
+    asm volatile("" ::: "memory");
+    put(lds, t0 + 1);
+  }
+  uint32_t buf = 0;
+  for (int t = t0; t < t1; ++t) {
+    wait_and_meet();  // tile t is written, and this wave's codes of the next one are there
+    if (t + 1 < t1) put(lds + (buf ^ (2 * kTile)), t + 2);
+    if (wave == 0) {
+      place(entry, t + 3);
+      entry = entry_of(t + 4);
+    }
+    const int start = tile_start<KT>(kr, t), end = tile_end(kr, t);
+    uint32_t valid[KT / 32], every = ~0u;
+#pragma unroll
+    for (int k = 0; k < KT / 32; ++k) every &= valid[k] = tile_rows.valid[t & 3][k];
+    const bool all = sees_all(s, kr, start, min(end, start + KT));
+    const bool whole = all && __builtin_amdgcn_readfirstlane(every) == ~0u;
+    if (!all) {
+      const uint32_t lv = lds + buf + kTile + lane * 16;
+      const int first = wave * N;
+      bool strange = false;
+#pragma unroll
+      for (int u = 0; u < N; ++u) strange |= has_not_finite<IO>(*lds_at<const u32x4>(lv + (first + u) * 1024));
+      if (strange) odd[0] = odd[1] = 1;
+      __syncthreads();
+      if (odd[0]) {
+        mark_not_finite<IO, DP, KT>(lds + buf + kTile, kr.np, s.causal ? blk.p : 0x7fffffff, s.window > 0 ? blk.p - s.window : -1,
+                                    start, end, (CB_LDS_SPACE uint32_t*)marks[0][wave], (CB_LDS_SPACE uint32_t*)marks[1][wave]);
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          CB_LDS_SPACE u32x4* at = lds_at<u32x4>(lv + (first + u) * 1024);
+          *at = finite_part<IO>(*at);
+        }
+        if (threadIdx.x == 0) odd[0] = 0;
+        __syncthreads();
+      }
+    }
+    f32x16 st[KT / 32];
+    u32x4 w[KT / 32][2];
+    const typename Block::Lanes at = Block::place(lanes, lds + buf, lds + buf + kTile);
+    blk.products(at, st);
+    blk.ready(s, kr, st, start, whole, valid);
+    typename Block::Values v = Block::first_values(at);
+    blk.weights(st, scale2, w);
+    blk.add_values(at, w, v);
+    buf ^= 2 * kTile;
+  }
+  __syncthreads();
+  if (odd[1]) blk.add_marks(marks[0][wave], marks[1][wave]);
+  blk.finish(late_args(), r, split, vector);
+}
+
+// Places of 16-byte chunks within a row of codes in LDS, exchanged so that the
+// lanes of a read hit distinct banks (K: one chunk of 16 rows; V: one of keys 0 to
+// 7 and 16 to 23, or 8 to 15 and 24 to 31).
+template <int DP>
+__device__ inline int swizzle_code_k(int key) {
+  return DP == 64 ? (key >> 2) & 3 : DP == 128 ? (key >> 1) & 7 : key & 15;
+}
+template <int DP>
+__device__ inline int swizzle_code_v(int key) {
+  return DP == 64    ? ((key >> 2) & 1) | ((key >> 3) & 2)
+         : DP == 128 ? ((key >> 1) & 3) | ((key >> 2) & 4)
+                     : (key & 7) | ((key >> 1) & 8);
+}
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+template <typename IO>
+CB_INLINE f32x4 mul16(u32x4 a, u32x4 b, f32x4 c) {
+  typedef typename Half<IO>::x8 x8;
+  if constexpr (std::is_same_v<IO, io_bf16>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+}
+
+// NB times 16 query rows of one wave over tiles of 32 keys held as codes, with
+// v_mfma_f32_16x16x32 (operands: lane l holds elements 8 (l / 16) .. + 7 of row or
+// column l % 16; result register e of lane l: row 4 (l / 16) + e, column l % 16). 16
+// rows, not the 32 of RowBlock: a step has the query heads of one KV head, mostly 8
+// or less, and what a row costs is paid for empty ones too. S^T = K Q^T leaves a
+// lane keys 16 kb + 4 g + e (g = l / 16) of query row l % 16, which are the second
+// operand of O^T += V^T P^T in the key order {4g .. 4g+3, 16+4g .. 16+4g+3}; V^T is
+// read in that order by transposing LDS reads.
+// K is widened with its scales, V without them: a value's scale goes into its
+// weight, since a lane's codes of V are of eight keys. The weights of fp16 rows
+// are kept as two bf16 terms (16 bits of each; times a scale they would leave
+// fp16's range).
+template <typename IO, int DP, int NB, bool MOD>
+struct CodeBlock {
+  typedef Half<IO> H;
+  static constexpr bool kTwo = std::is_same_v<IO, io_f16>;
+  static constexpr int DB = DP / 16, JS = DP / 64;  // result rows a column block; pairs of product steps
+  u32x4 q[NB][2 * JS];
+  f32x4 o[NB][DB];
+  float m[NB], l[NB], slope[NB];
+  int p[NB];  // cached token of this lane's query rows
+  bool live[NB];
+
+  __device__ inline void init(const ScoreArgs& s, const Request& r, int head, int row0, bool vector) {
+    const int lane = threadIdx.x & (kWave - 1), g = lane >> 4;
+    const int rows = r.n * s.group;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int row = row0 + 16 * n + (lane & 15);
+      live[n] = row < rows;
+      const int at = min(row, rows - 1), i = at / s.group, qh = head * s.group + at - i * s.group;
+      p[n] = r.length - r.n + i;
+      const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
+      // Elements 64 j + 16 g + 8 x .. + 7: those of a lane's 16 codes of K.
+#pragma unroll
+      for (int k = 0; k < 2 * JS; ++k) {
+        const char* from = qp + 2 * min(64 * (k >> 1) + 16 * g + 8 * (k & 1), s.head_dim - 8);
+        if (vector) {
+          q[n][k] = gload<u32x4>(as_global(static_cast<const void*>(from)));
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            q[n][k][w] = load_elem<uint16_t>(from + 4 * w) | static_cast<uint32_t>(load_elem<uint16_t>(from + 4 * w + 2)) << 16;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 2 * JS; ++k) q[n][k] = 64 * (k >> 1) + 16 * g < s.head_dim ? q[n][k] : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[n][d] = f32x4{0, 0, 0, 0};
+      m[n] = kNegInf;
+      l[n] = slope[n] = 0;
+      if constexpr (MOD) slope[n] = s.slopes ? s.slopes[qh] : 0.0f;
+    }
+  }
+
+  // LDS offsets within a tile that depend on the lane alone.
+  struct Lanes {
+    uint32_t k[JS];  // K chunk 4 j + g of row l % 16
+    uint32_t v[DB];  // V chunk db, this lane's half of it, of this lane's key
+  };
+  static __device__ inline Lanes lanes() {
+    Lanes a;
+    const int lane = threadIdx.x & (kWave - 1), g = lane >> 4, c = lane & 15;
+#pragma unroll
+    for (int j = 0; j < JS; ++j) a.k[j] = c * DP + ((4 * j + g) ^ swizzle_code_k<DP>(c)) * 16;
+    const int i = c >> 1, key = 4 * g + (i & 3) + 4 * (i & 4);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) a.v[d] = key * DP + (d ^ swizzle_code_v<DP>(key)) * 16 + (c & 1) * 8;
+    return a;
+  }
+
+  // Raw products with the tile at lk; ks: the scales of keys l % 16 and 16 + l % 16.
+  CB_INLINE void products(const Lanes& a, uint32_t lk, const float (&ks)[2], f32x8 (&st)[NB]) {
+    f32x4 x[NB][2];
+    u32x4 f[2][JS];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int j = 0; j < JS; ++j) f[kb][j] = *lds_at<const u32x4>(lk + a.k[j] + kb * 16 * DP);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) x[n][0] = x[n][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < JS; ++j)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        u32x4 lo, hi;
+        widen<IO>(f[kb][j], ks[kb], lo, hi);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          x[n][kb] = mul16<IO>(lo, q[n][2 * j], x[n][kb]);
+          x[n][kb] = mul16<IO>(hi, q[n][2 * j + 1], x[n][kb]);
+        }
+      }
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) st[n][e] = x[n][e >> 2][e & 3];
+  }
+
+  // Modified and masked, as RowBlock::ready.
+  CB_INLINE void ready(const ScoreArgs& s, const KeyRange& kr, f32x8 (&st)[NB], int start, bool whole, uint32_t valid) {
+    const int g = (threadIdx.x & (kWave - 1)) >> 4;
+    if constexpr (MOD) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) modify_scores<true, 8, 16>(s, st[n], kLog2e, slope[n], p[n], start, g);
+    }
+    if (!whole) {
+      asm volatile("");  // a branch, not selects that every tile would pay for
+      const uint32_t there = valid >> (4 * g);
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int k = 16 * (e >> 2) + (e & 3);
+          const bool in = sees(s, kr, p[n], start + 4 * g + k) & ((there >> k) & 1);
+          st[n][e] = in ? st[n][e] : kNegInf;
+        }
+    }
+  }
+
+  // As RowBlock's, but a weight is packed times its value's scale.
+  CB_INLINE float try_weights(int n, const f32x8& st, float scale2, const f32x4 (&vs)[2], u32x4& w, u32x4& rest) const {
+    const float mu = m[n] == kNegInf ? 0.0f : m[n];
+    float sum = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float x = exp2_fast(__builtin_fmaf(st[e], scale2, -mu)), y = exp2_fast(__builtin_fmaf(st[e + 1], scale2, -mu));
+      sum += x + y;
+      const float xs = x * vs[e >> 2][e & 3], ys = y * vs[e >> 2][(e & 3) + 1];
+      const uint32_t hi = pack_bf16(xs, ys);
+      w[e >> 1] = hi;
+      if constexpr (kTwo) rest[e >> 1] = pack_bf16(xs - lo_bf(hi), ys - hi_bf(hi));
+    }
+    return sum;
+  }
+  CB_INLINE void weights(const f32x8 (&st)[NB], float scale2, const f32x4 (&vs)[2], u32x4 (&w)[NB], u32x4 (&rest)[NB]) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      float sum = try_weights(n, st[n], scale2, vs, w[n], rest[n]);
+      if (__any(!(sum < H::kLag) | (m[n] == kNegInf))) {
+        float top = kNegInf;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, st[n][e]);
+        top = __builtin_fmaf(top, scale2, -H::kRoom);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        const float m1 = fmaxf(m[n], fmaxf(top, __shfl_xor(top, 32)));
+        const float alpha = m1 == kNegInf ? 1.0f : exp2_fast(m[n] - m1);
+        m[n] = m1;
+        l[n] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[n][d] *= alpha;
+        sum = try_weights(n, st[n], scale2, vs, w[n], rest[n]);
+      }
+      l[n] += sum;
+    }
+  }
+
+  CB_INLINE void add_values(const Lanes& a, uint32_t lv, const u32x4 (&w)[NB], const u32x4 (&rest)[NB]) {
+    i32x2 f[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) f[d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(lds_at<i32x2>(lv + a.v[d]));
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      u32x4 x;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        x[2 * k] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[d][k], 1.0f, false));
+        x[2 * k + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[d][k], 1.0f, true));
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        o[n][d] = mul16<io_bf16>(x, w[n], o[n][d]);
+        if constexpr (kTwo) o[n][d] = mul16<io_bf16>(x, rest[n], o[n][d]);
+      }
+    }
+  }
+
+  // NaN for the elements whose NaN values were taken out of the tiles.
+  CB_INLINE void add_marks(const uint32_t* marks) {
+    const int lane = threadIdx.x & (kWave - 1), g = lane >> 4;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const uint32_t bits = marks[(16 * n + (lane & 15)) * (DP / 32) + (d >> 1)] >> (16 * (d & 1) + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][d][e] += (bits >> e) & 1 ? __uint_as_float(0x7fc00000u) : 0.0f;
+      }
+  }
+
+  // The wave's sums into LDS, for join_sums.
+  template <int NW>
+  CB_INLINE void put_sums(float* sums, float (&stats)[2][NW][16 * NB], int wave) {
+    constexpr int LD = DP + 4;
+    const int lane = threadIdx.x & (kWave - 1), g = lane >> 4, c = lane & 15;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      l[n] += __shfl_xor(l[n], 16);
+      l[n] += __shfl_xor(l[n], 32);
+      if (live[n]) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(sums + (16 * n + c) * LD + 16 * d + 4 * g) = o[n][d];
+      }
+      if (g == 0) {
+        stats[0][wave][16 * n + c] = m[n];
+        stats[1][wave][16 * n + c] = l[n];
+      }
+    }
+  }
+};
+
+// One wave notes, for its rows, every NaN of the V tile of codes at lv that a row
+// sees, and takes it out of the tile: a weight of zero times it would be NaN in rows
+// that do not see it. Lane l notes for row l % 16 of column block l / 16.
+template <int DP, int NB>
+CB_INLINE void take_nan_out(uint32_t lv, int np, const int (&p)[NB], int window, int causal, int start, int end, CB_LDS_SPACE uint32_t* marks) {
+  constexpr int C = DP / 16;
+  const int lane = threadIdx.x & (kWave - 1), n = (lane >> 4) & 1;
+  const int first = p[0], last = p[NB - 1], mine = n ? last : first;
+  const int below = causal ? mine : 0x7fffffff, above = window > 0 ? mine - window : -1;
+  for (int i = 0; i < 32 * C / kWave; ++i) {
+    CB_LDS_SPACE u32x4* at = lds_at<u32x4>(lv + (i * kWave + lane) * 16);
+    u32x4 x = *at;
+    uint64_t hits = __ballot((nan_codes(x[0]) | nan_codes(x[1]) | nan_codes(x[2]) | nan_codes(x[3])) != 0);
+    if (!hits) continue;
+    while (hits) {
+      const int who = __ffsll(static_cast<unsigned long long>(hits)) - 1;
+      hits &= hits - 1;
+      const int chunk = i * kWave + who, key = chunk / C, d0 = ((chunk % C) ^ swizzle_code_v<DP>(key)) * 16, j = start + key;
+      const bool seen = (j < end) & ((j < np) | ((j <= below) & (j > above))) & (lane < 16 * NB);
+      uint32_t bits = 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t nan = nan_codes(__shfl(x[w], who)) >> 7;
+        bits |= ((nan & 1) | ((nan >> 7) & 2) | ((nan >> 14) & 4) | ((nan >> 21) & 8)) << (4 * w);
+      }
+      if (seen) marks[(lane & (16 * NB - 1)) * (DP / 32) + (d0 >> 5)] |= bits << (d0 & 31);
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) x[w] &= ~((nan_codes(x[w]) >> 7) * 0xffu);
+    *at = x;
+  }
+}
+
+// Waits for the K (else V) rows of the first of the last `left` tiles, X to S of
+// them, N instructions each for K and for V.
+template <int X, int S, int N>
+CB_INLINE void wait_last(int left, bool value) {
+  if (left == X) {
+    if (value) __builtin_amdgcn_s_waitcnt(wait_vm(2 * (X - 1) * N));
+    else __builtin_amdgcn_s_waitcnt(wait_vm((2 * X - 1) * N));
+  } else if constexpr (X < S) {
+    wait_last<X + 1, S, N>(left, value);
+  }
+}
+
+// Few query rows: attend_step_kernel's scheme on tiles of codes. Each wave
+// streams tiles of 32 keys through LDS of its own, S of them in flight.
+constexpr int kCodeTiles = 32;  // tiles a split holds at most
+constexpr int kCodeWaves = 4;
+
+template <typename IO, int DP, int NB, bool MOD>
+__global__ __launch_bounds__(kCodeWaves * kWave, DP == 256 ? 1 : 2) void step_codes_kernel(AttendArgs a, ScaledCache cache, int vector) {
+  constexpr int NW = kCodeWaves, KT = 32, kTile = KT * DP, N = kTile / 1024, C = DP / 16, S = 2;
+  constexpr int kSums = (16 * NB * (DP + 4) * 4 + 1023) / 1024 * 1024, kWaveBytes = 2 * S * kTile > kSums ? 2 * S * kTile : kSums;
+  __shared__ __align__(1024) char tiles[NW * kWaveBytes];  // a wave's K tiles, then its V tiles; at the end its sums
+  __shared__ int key_rows[kCodeTiles * KT];
+  __shared__ __align__(16) float key_scales[2][kCodeTiles * KT];
+  __shared__ uint32_t marks[NW][16 * NB * (DP / 32)];
+  __shared__ float stats[2][NW][16 * NB];
+  const ScoreArgs& s = a.s;
+  const QBatch& B = s.batch;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int head = blockIdx.x % s.kv_heads, rest = blockIdx.x / s.kv_heads;
+  const int split = rest / a.tile_slots;
+  Request r;
+  int b, tile;
+  if (!find_tile<true>(a, rest % a.tile_slots, 16 * NB, r, b, tile)) return;
+  r = uniform(r), b = uniform(b), tile = uniform(tile);
+  const int rows = r.n * s.group, row0 = tile * 16 * NB;
+  const KeyRange kr = key_range<KT>(s, r, b, row0, min(rows, row0 + 16 * NB) - 1);
+  const int per = min(split_tiles(a, kr.tiles), kCodeTiles), t0 = split * per, t1 = min(kr.tiles, t0 + per);
+  if (a.splits > 1 && t0 >= t1) return;
+
+  for (int k = threadIdx.x; k < (t1 - t0) * KT; k += NW * kWave) {
+    const int t = t0 + k / KT, j = tile_start<KT>(kr, t) + k % KT;
+    int64_t row = -1;
+    if (j < tile_end(kr, t)) {
+      row = cache_row(B, r, j);
+      if (row < 0) flag(B.err, CB_ERROR_CACHE_ROW);
+    }
+    key_rows[k] = static_cast<int>(row);
+  }
+  for (int w = threadIdx.x; w < NW * NB * DP / 2; w += NW * kWave) (&marks[0][0])[w] = 0;
+  typedef CodeBlock<IO, DP, NB, MOD> Block;
+  Block blk;
+  blk.init(s, r, head, row0, vector);
+  const typename Block::Lanes lanes = Block::lanes();
+  const float scale2 = MOD ? 1.0f : s.scale * kLog2e;
+  const int64_t off = static_cast<int64_t>(head) * s.head_dim;
+  gcptr kbase = layer_base(s.cache, 0, s.layer) + off, vbase = layer_base(s.cache, 1, s.layer) + off;
+  gcptr zero = as_global(static_cast<const void*>(g_zeros));
+  const uint32_t stride = static_cast<uint32_t>(B.row_stride_b);
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((CB_LDS_SPACE char*)tiles)) + wave * kWaveBytes;
+  wait_and_meet();
+
+  const int n = t1 - t0 > wave ? (t1 - t0 - wave + NW - 1) / NW : 0;  // this wave's tiles: t0 + wave, + NW, ...
+  auto request = [&](int i, gcptr base, uint32_t to, bool value) __attribute__((always_inline)) {
+    const int at = (wave + i * NW) * KT;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int k = u * (kWave / C) + lane / C;
+      const int row = key_rows[at + k];
+      const int c = (lane % C) ^ (value ? swizzle_code_v<DP>(k) : swizzle_code_k<DP>(k));
+      gcptr from = ((row >= 0) & (c * 16 < s.head_dim)) ? base + static_cast<uint64_t>(static_cast<uint32_t>(row)) * stride + c * 16 : zero;
+      dma16(from, to + u * 1024);
+    }
+  };
+  // Waits until the K (else V) rows of the first of `left` tiles are there.
+  auto arrived = [&](int left, bool value) __attribute__((always_inline)) {
+    // In order of asking: K and V of S tiles; V is waited for with the K of a tile S on behind it, if there is one.
+    if (!value ? left >= S : left > S) __builtin_amdgcn_s_waitcnt(wait_vm((2 * S - 1) * N));
+    else wait_last<1, S, N>(left, value);
+    asm volatile("" ::: "memory");
+  };
+  bool some_mark = false;
+#pragma unroll 1
+  for (int i = 0; i < S; ++i)
+    if (i < n) {
+      asm volatile("");
+      request(i, kbase, lds + i * kTile, false);
+      request(i, vbase, lds + (S + i) * kTile, true);
+    }
+  // The scales of keys, one without a row has no matter which.
+  const HeadScales hs(cache.scales, s.layer, head);
+  for (int k = threadIdx.x; k < (t1 - t0) * KT; k += NW * kWave) {
+    const uint32_t at = hs.at(max(key_rows[k], 0));
+    key_scales[0][k] = scale_value(hs.k[at], kMostRead<IO>);
+    key_scales[1][k] = scale_value(hs.v[at]);
+  }
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  asm volatile("s_barrier" ::: "memory");
+  uint32_t buf = 0;
+  for (int i = 0; i < n; ++i) {
+    const int t = t0 + wave + i * NW, start = tile_start<KT>(kr, t), end = tile_end(kr, t), at = (t - t0) * KT;
+    const uint32_t valid = static_cast<uint32_t>(__ballot(key_rows[at + (lane & 31)] >= 0));
+    float ks[2];
+    f32x4 vs[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      ks[kb] = key_scales[0][at + 16 * kb + (lane & 15)];
+      vs[kb] = *reinterpret_cast<const f32x4*>(&key_scales[1][at + 16 * kb + 4 * (lane >> 4)]);
+    }
+    arrived(n - i, false);
+    f32x8 st[NB];
+    u32x4 w[NB], low[NB];
+    const uint32_t lk = lds + buf, lv = lk + S * kTile;
+    blk.products(lanes, lk, ks, st);
+    if (i + S < n) {
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // the products' LDS reads
+      request(i + S, kbase, lk, false);
+    }
+    const bool all = sees_all(s, kr, start, min(end, start + KT));
+    blk.ready(s, kr, st, start, all & (valid == ~0u), valid);
+    blk.weights(st, scale2, vs, w, low);
+    arrived(n - i, true);
+    if (!all) {
+      bool strange = false;
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const u32x4 x = *lds_at<const u32x4>(lv + u * 1024 + lane * 16);
+        strange |= (nan_codes(x[0]) | nan_codes(x[1]) | nan_codes(x[2]) | nan_codes(x[3])) != 0;
+      }
+      if (__any(strange)) {
+        some_mark = true;
+        take_nan_out<DP, NB>(lv, kr.np, blk.p, s.window, s.causal, start, end, (CB_LDS_SPACE uint32_t*)marks[wave]);
+      }
+    }
+    blk.add_values(lanes, lv, w, low);
+    if (i + S < n) {
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      request(i + S, vbase, lv, true);
+    }
+    buf = buf + kTile == S * kTile ? 0 : buf + kTile;
+  }
+  if (some_mark) blk.add_marks(marks[wave]);
+  blk.put_sums(reinterpret_cast<float*>(tiles + wave * kWaveBytes), stats, wave);
+  __syncthreads();
+  join_sums<DP, NW, 16 * NB, Half<IO>>(late_args(), r, head, row0, rows, split, vector, tiles, kWaveBytes, stats);
+}
+
+// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 
@@ -388,6 +1037,7 @@ int check_scales(const cb_page_scales* scales, const cb_query_batch& batch, Page
   if (scales->pages < 0 || scales->pages > 0x7fffffff || scales->pages * scales->page_size < batch.cache.rows)
     return fail(CB_EINVAL, "the scales' pages do not cover the cache's rows");
   if (scales->page_stride < batch.cache.heads) return fail(CB_EINVAL, "page_stride below the KV heads");
+  if (scales->page_stride > 0xffffffffll / std::max<int64_t>(1, scales->pages)) return fail(CB_EINVAL, "a layer's scales above 2^32 bytes");
   if (scales->layer_stride < 0) return fail(CB_EINVAL, "negative layer_stride");
   s->k = scales->k;
   s->v = scales->v;
@@ -409,29 +1059,47 @@ int check_pages(const cb_query_batch& batch, const PageScales& s, const char* na
 
 int most_exponent(int32_t dtype) { return dtype == CB_DTYPE_F16 ? kMostExponentF16 : kMostExponent; }
 
-AttendShape quantized_shape(const ScoreArgs& s) {
-  AttendShape h{};
-  h.waves = kAnyWaves;
-  h.rows_per_tile = kAnyRows;
-  h.keys_per_tile = kAnyKeys;
-  const QBatch& B = s.batch;
-  const int per_request = std::max(1, ceil_div(static_cast<int64_t>(B.max_query) * s.group, h.rows_per_tile));
-  const int64_t by_request = static_cast<int64_t>(per_request) * B.requests;
-  const int64_t packed = ceil_div(static_cast<int64_t>(B.tokens) * s.group, h.rows_per_tile) + static_cast<int64_t>(B.requests);
-  h.request_slots = by_request <= packed ? per_request : 0;
-  h.tile_slots = std::min(by_request, packed);
-  int64_t keys = B.max_length;
-  if (s.window > 0 && s.causal && !s.prefix) keys = std::min<int64_t>(keys, static_cast<int64_t>(s.window) + std::min<int64_t>(B.max_query, h.rows_per_tile / s.group + 2));
-  const int key_tiles = std::max(1, ceil_div(keys, h.keys_per_tile) + (s.prefix ? 1 : 0));
-  const int64_t groups = h.tile_slots * s.kv_heads;
-  h.least_tiles = 2;
-  h.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(1, groups), key_tiles / h.least_tiles)));
+// Whether the kernels of 16-bit products take the call: whole 16-byte chunks of rows.
+bool takes_codes(const ScoreArgs& s, int32_t dtype, const cb_scores& scores) {
+  return !scores.fp32_weights && dtype != CB_DTYPE_F32 && s.head_dim <= kMaxDp && s.cache.row_stride_b <= 0xffffffffll &&
+         rows_aligned16(s.cache, s.head_dim);
+}
+
+AttendShape quantized_shape(const ScoreArgs& s, int32_t dtype, const cb_scores& scores) {
+  AttendShape h = attend_shape(s, takes_codes(s, dtype, scores), kCodeTiles);
+  // One block of rows a request: how many blocks there are does not change with its size.
+  if (h.step && static_cast<int64_t>(s.batch.max_query) * s.group <= 16) h.rows_per_tile = 16;
   return h;
+}
+
+template <typename IO, int DP, int KT, bool MOD>
+void launch_codes(const AttendArgs& a, const ScaledCache& cache, const AttendShape& h, unsigned grid, hipStream_t st) {
+  const int vector = aligned16(a.s.q) && aligned16(a.out);
+  if (h.step && h.rows_per_tile == 16) hipLaunchKernelGGL((step_codes_kernel<IO, DP, 1, MOD>), dim3(grid), dim3(kCodeWaves * kWave), 0, st, a, cache, vector);
+  else if (h.step) hipLaunchKernelGGL((step_codes_kernel<IO, DP, 2, MOD>), dim3(grid), dim3(kCodeWaves * kWave), 0, st, a, cache, vector);
+  else if (DP <= 128 && h.waves == 8) hipLaunchKernelGGL((attend_codes_kernel<IO, DP, KT, DP <= 128 ? 8 : 4, MOD>), dim3(grid), dim3(8 * kWave), 0, st, a, cache, vector);
+  else hipLaunchKernelGGL((attend_codes_kernel<IO, DP, KT, 4, MOD>), dim3(grid), dim3(4 * kWave), 0, st, a, cache, vector);
+  if (h.step) launch_join<IO, 32>(a, h, st);
+  else launch_join<IO, KT>(a, h, st);
 }
 
 template <typename IO>
 void launch_quantized(const AttendArgs& a, const ScaledCache& cache, const AttendShape& h, unsigned grid, hipStream_t st) {
   const int d = a.s.head_dim;
+  if constexpr (sizeof(IO) == 2) {
+    if (h.half) {
+      if (a.s.mod) {
+        if (d <= 64) launch_codes<IO, 64, 64, true>(a, cache, h, grid, st);
+        else if (d <= 128) launch_codes<IO, 128, 32, true>(a, cache, h, grid, st);
+        else launch_codes<IO, 256, 32, true>(a, cache, h, grid, st);
+      } else {
+        if (d <= 64) launch_codes<IO, 64, 64, false>(a, cache, h, grid, st);
+        else if (d <= 128) launch_codes<IO, 128, 64, false>(a, cache, h, grid, st);
+        else launch_codes<IO, 256, 32, false>(a, cache, h, grid, st);
+      }
+      return;
+    }
+  }
   if (d <= 64) launch_any<IO, 64>(a, cache, grid, st);
   else if (d <= 128) launch_any<IO, 128>(a, cache, grid, st);
   else if (d <= 256) launch_any<IO, 256>(a, cache, grid, st);
@@ -530,7 +1198,7 @@ int cb_quantized_attention_workspace_bytes(const cb_query_batch* batch, const cb
   int rc;
   if ((rc = check_scores(batch, 0, dtype, head_dim, scores, query_heads, nullptr, &s, 1)) || (rc = check_scales(scales, *batch, &p)))
     return rc;
-  *bytes = s.batch.tokens && s.batch.requests ? attend_workspace(s, quantized_shape(s)) : 0;
+  *bytes = s.batch.tokens && s.batch.requests ? attend_workspace(s, quantized_shape(s, dtype, *scores)) : 0;
   return CB_OK;
 }
 
@@ -547,9 +1215,9 @@ int cb_quantized_attention(const cb_query_batch* batch, const cb_page_scales* sc
   const int eb = elem_bytes(dtype), n = batch->num_tokens;
   if ((rc = check_heads("q", q, q->heads, eb, n, &a.s.q)) || (rc = check_output("out", out, q->heads, eb, n, head_dim, &a.out))) return rc;
   if (n == 0 || batch->num_requests == 0) return CB_OK;
-  const AttendShape h = quantized_shape(a.s);
+  const AttendShape h = quantized_shape(a.s, dtype, *scores);
   unsigned grid;
-  if ((rc = cut_attention(a, h, h.waves * kWave, lse, d_workspace, workspace_bytes, &grid))) return rc;
+  if ((rc = cut_attention(a, h, (h.step ? kCodeWaves : h.waves) * kWave, lse, d_workspace, workspace_bytes, &grid))) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == CB_DTYPE_BF16) launch_quantized<io_bf16>(a, cache, h, grid, st);
   else if (dtype == CB_DTYPE_F16) launch_quantized<io_f16>(a, cache, h, grid, st);

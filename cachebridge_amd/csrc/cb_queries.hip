@@ -139,12 +139,10 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_tile_ker
 // times the bytes (64 requests of 8192, 16 heads and 2 KV heads) 107 us, 5.0
 // TB/s, a large copy's rate. 64 ragged requests of 2550 on average (167 MB) take
 // 46 us, 3.6 TB/s: ragged lengths leave CUs without work at the end.
-constexpr int kStepTiles = 64;  // tiles a split holds at most
-
 template <typename IO, int DP, int NW, bool MOD>
 __global__ __launch_bounds__(NW * kWave, 1) void attend_step_kernel(AttendArgs a, int vector) {
-  constexpr int KT = 32, kTile = KT * DP * 2, N = kTile / 1024, C = DP / 8, LD = DP + 4;
-  static_assert(4 * kTile >= 32 * LD * 4, "a wave's sums fit its tiles");
+  constexpr int KT = 32, kTile = KT * DP * 2, N = kTile / 1024, C = DP / 8;
+  static_assert(4 * kTile >= 32 * (DP + 4) * 4, "a wave's sums fit its tiles");
   __shared__ __align__(1024) char tiles[NW * 4 * kTile];  // a wave's K, K, V, V
   __shared__ int key_rows[kStepTiles * KT];
   __shared__ uint32_t marks[2][NW][32 * (DP / 32)];
@@ -253,60 +251,7 @@ __global__ __launch_bounds__(NW * kWave, 1) void attend_step_kernel(AttendArgs a
   }
   if (some_mark) blk.add_marks(marks[0][wave], marks[1][wave]);
 
-  // The waves' sums meet in LDS, each wave's in its own tiles.
-  blk.l += __shfl_xor(blk.l, 32);
-  const int c = lane & 31, h = lane >> 5;
-  float* mine = reinterpret_cast<float*>(tiles + wave * 4 * kTile) + c * LD;
-  if (blk.live) {
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(mine + 32 * d + 8 * g + 4 * h) =
-            f32x4{blk.o[d][4 * g], blk.o[d][4 * g + 1], blk.o[d][4 * g + 2], blk.o[d][4 * g + 3]};
-  }
-  if (h == 0) {
-    stats[0][wave][c] = blk.m;
-    stats[1][wave][c] = blk.l;
-  }
-  __syncthreads();
-  const int D = s.head_dim, live = min(32, rows - row0), pairs = D / 2;
-  for (int x = threadIdx.x; x < live * pairs; x += NW * kWave) {
-    const int y = x / pairs, d = 2 * (x - y * pairs);
-    float m = kNegInf;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, stats[0][w][y]);
-    const float mu = m == kNegInf ? 0.0f : m;
-    float l = 0, o0 = 0, o1 = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float f = exp2_fast(stats[0][w][y] - mu);
-      const float* from = reinterpret_cast<const float*>(tiles + w * 4 * kTile) + y * LD + d;
-      l += f * stats[1][w][y];
-      // A wave that saw nothing of this row has nothing to add.
-      o0 += f != 0.0f ? f * from[0] : 0.0f;
-      o1 += f != 0.0f ? f * from[1] : 0.0f;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const float lse2 = l == 0.0f ? kNegInf : m + log2_fast(l);
-    const int row = row0 + y, i = row / s.group, qh = head * s.group + row - i * s.group;
-    const int64_t at = static_cast<int64_t>(r.q0 + i) * s.q_heads + qh;
-    if (a.splits > 1) {
-      const int64_t slot = static_cast<int64_t>(split) * B.tokens * s.q_heads + at;
-      *reinterpret_cast<float2*>(a.part_out + slot * D + d) = make_float2(o0 * inv, o1 * inv);
-      if (d == 0) a.part_lse[slot] = lse2;
-    } else {
-      char* op = a.out.data + static_cast<int64_t>(r.q0 + i) * a.out.token_b + qh * a.out.head_b + d * 2;
-      const uint32_t packed = Half<IO>::pack(o0 * inv, o1 * inv);
-      if (vector) {
-        gstore<uint32_t>(as_global(static_cast<void*>(op)), packed);
-      } else {
-        store_elem<uint16_t>(op, static_cast<uint16_t>(packed));
-        store_elem<uint16_t>(op + 2, static_cast<uint16_t>(packed >> 16));
-      }
-      if (a.lse && d == 0) a.lse[at] = lse2 * kLn2;
-    }
-  }
+  join_waves<DP, NW>(blk, a, r, head, row0, rows, split, vector, tiles, 4 * kTile, stats);
 }
 
 // ---------------------------------------------------------------------------
@@ -774,68 +719,9 @@ __global__ __launch_bounds__(256) void move_rows_kernel(MoveArgs a) {
 // Host side
 // ---------------------------------------------------------------------------
 
-// Workgroups of four waves that a launch is split into at least: two a CU. 512 new
-// tokens over 32768 take 262, 173 and 185 us with 256, 512 and 1024, 64 requests of
-// 8 new tokens over 2048 47, 38.5 and 39 us.
-constexpr int kTargetGroups = 512;
-
 // Whether the 16-bit kernels take the call: whole 16-byte chunks of rows.
 bool takes_half(const ScoreArgs& s, int32_t dtype) {
   return dtype != CB_DTYPE_F32 && s.head_dim % 8 == 0 && s.cache.row_stride_b <= 0xffffffffll && s.head_dim <= kMaxDp && rows_aligned16(s.cache, s.head_dim * 2);
-}
-
-// Waves of attend_tile_kernel: eight share a tile's staging among twice the
-// rows, if there are that many and a head's registers leave two waves a SIMD.
-// That pays once a launch has work for all CUs (16 query heads, 2 KV heads,
-// kernel and join, eight waves against four): 256 new tokens over 4096 cached
-// 41.1 / 37.1 us, 64 over 32768 46.1 / 49.2, 1024 over 4096 63 / 70, 256 over
-// 32768 106 / 120; 1000 of 1000 with 8 heads 39.4 / 34.1.
-constexpr int kWideRows = 512;               // query rows per KV head, and
-constexpr int64_t kWideScores = 24ll << 20;  // scores of the launch, from which eight are taken
-// Query rows per KV head up to which attend_step_kernel is taken: one block of
-// rows, so that K and V are read once. This kernel against the tile kernel, each
-// with its join, 8 query heads a KV head: 64 ragged requests of 2550 on average 52 /
-// 100 us; one request of 32768 38 / 38. Where all lengths are alike the tile
-// kernel is ahead: 64 of 2048 42 / 35, with four new tokens 57 / 40.
-constexpr int kStepRows = 32;
-// Its workgroups: one request has all its splits at work, of several requests many
-// are shorter than the bound that splits are cut by. With the join, 512, 1024
-// and 2048: 64 ragged requests 73, 52, 67 us; 64 of 2048 33, 42, 42; one request of
-// 32768 38 with 512 and 47 with 1024.
-constexpr int kStepGroups = 512, kStepGroupsRagged = 1024;
-constexpr int kStepWaves = 2;
-
-AttendShape attend_shape(const ScoreArgs& s, int32_t dtype, bool fp32_weights) {
-  AttendShape h{};
-  h.half = !fp32_weights && takes_half(s, dtype);
-  const QBatch& B = s.batch;
-  h.step = h.half && static_cast<int64_t>(B.max_query) * s.group <= kStepRows;
-  const int64_t seen = s.window > 0 && s.causal && !s.prefix ? std::min<int64_t>(B.max_length, s.window) : B.max_length;
-  h.waves = h.half && s.head_dim <= 128 && static_cast<int64_t>(B.max_query) * s.group >= kWideRows &&
-                    static_cast<int64_t>(B.tokens) * s.q_heads * seen >= kWideScores
-                ? 8 : 4;
-  h.rows_per_tile = h.step ? 32 : h.half ? 32 * h.waves : kAnyRows;
-  h.keys_per_tile = !h.half ? kAnyKeys : !h.step && s.head_dim <= (s.mod ? 64 : 128) ? 64 : 32;
-  const int per_request = std::max(1, ceil_div(static_cast<int64_t>(B.max_query) * s.group, h.rows_per_tile));
-  const int64_t by_request = static_cast<int64_t>(per_request) * B.requests;
-  const int64_t packed = ceil_div(static_cast<int64_t>(B.tokens) * s.group, h.rows_per_tile) + static_cast<int64_t>(B.requests);
-  h.request_slots = by_request <= packed ? per_request : 0;
-  h.tile_slots = std::min(by_request, packed);
-  int64_t keys = B.max_length;
-  if (s.window > 0 && s.causal && !s.prefix) keys = std::min<int64_t>(keys, static_cast<int64_t>(s.window) + std::min<int64_t>(B.max_query, h.rows_per_tile / s.group + 2));
-  const int key_tiles = std::max(1, ceil_div(keys, h.keys_per_tile) + (s.prefix ? 1 : 0));
-  const int64_t groups = h.tile_slots * s.kv_heads;
-  const int64_t target = !h.step ? kTargetGroups * 4 / h.waves : B.requests > 1 ? kStepGroupsRagged : kStepGroups;
-  h.least_tiles = h.half ? 8 : 2;
-  h.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(1, groups), key_tiles / h.least_tiles)));
-  if (h.step) {
-    // Parts of one size for all requests, cut by the bound: their workgroups end
-    // together (64 ragged requests 47 us, with parts by each one's own keys 68).
-    h.splits = std::max(h.splits, ceil_div(key_tiles, kStepTiles));
-    h.least_tiles = ceil_div(key_tiles, h.splits);
-    h.splits = ceil_div(key_tiles, h.least_tiles);
-  }
-  return h;
 }
 
 template <typename IO, int DP, int KT, bool MOD>
@@ -947,7 +833,7 @@ int cb_attention_workspace_bytes(const cb_query_batch* batch, int32_t dtype, int
   ScoreArgs s{};
   int rc;
   if ((rc = check_scores(batch, 0, dtype, head_dim, scores, query_heads, nullptr, &s))) return rc;
-  *bytes = s.batch.tokens && s.batch.requests ? attend_workspace(s, attend_shape(s, dtype, scores->fp32_weights != 0)) : 0;
+  *bytes = s.batch.tokens && s.batch.requests ? attend_workspace(s, attend_shape(s, !scores->fp32_weights && takes_half(s, dtype))) : 0;
   return CB_OK;
 }
 
@@ -961,7 +847,7 @@ int cb_paged_attention(const cb_query_batch* batch, int32_t layer, int32_t dtype
   const int eb = elem_bytes(dtype), n = batch->num_tokens;
   if ((rc = check_heads("q", q, q->heads, eb, n, &a.s.q)) || (rc = check_output("out", out, q->heads, eb, n, head_dim, &a.out))) return rc;
   if (n == 0 || batch->num_requests == 0) return CB_OK;
-  const AttendShape h = attend_shape(a.s, dtype, scores->fp32_weights != 0);
+  const AttendShape h = attend_shape(a.s, !scores->fp32_weights && takes_half(a.s, dtype));
   unsigned grid;
   if ((rc = cut_attention(a, h, (h.step ? kStepWaves : h.waves) * kWave, lse, d_workspace, workspace_bytes, &grid))) return rc;
   const bool mod = a.s.mod;

@@ -452,15 +452,15 @@ int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, i
  * Queries on an 8-bit cache. K and V rows hold e4m3 codes (the OCP format: no
  * infinities, 0x7f and 0xff are NaN), a byte an element; an element's value is
  * its code's times 2^(byte - 127), byte the scale of its layer, page and KV head
- * (1 to 254). Pages are page_size rows: row r is in page r / page_size. Such a
+ * (1 to 246; larger ones read as 246). Pages are page_size rows: row r is in page r / page_size. Such a
  * cache is described by the same cb_query_batch (strides of its cb_rows count
  * bytes) and the scales beside it; the token tensors are of `dtype`.
  *
  * Rows that are stored choose the scale: the least that holds every finite
  * element of the page's stored rows up to 448 times it (2^-126 where all are
  * zero). Codes are rounded to nearest even; infinities and NaN become NaN.
- * With dtype CB_DTYPE_F16 a scale is at most 2^7, which keeps values within that
- * type (larger elements are stored as 448 times the scale).
+ * A scale is at most 2^119, with dtype CB_DTYPE_F16 2^7, which keeps values
+ * within the type (larger elements are stored as 448 times the scale).
  * No counterpart in the reference, whose caches are 16 bits wide.
  */
 typedef struct cb_page_scales {

@@ -2,7 +2,8 @@
 
 Written from the format: 4 bits of exponent (bias 7), 3 of mantissa, no
 infinities; a page's scale is the least 2^e that keeps its finite elements
-within 448 * 2^e, e from -126 to 127 (7 for rows of half precision).
+within 448 * 2^e, e from -126 to 119 (448 * 2^119 is finite in fp32; 7 for rows
+of half precision).
 """
 
 from __future__ import annotations
@@ -39,7 +40,7 @@ def round_code(x: torch.Tensor) -> torch.Tensor:
     return (torch.round(x / s) * s).clamp(-448, 448)
 
 
-def exponent(top: float, most: int = 127) -> int:
+def exponent(top: float, most: int = 119) -> int:
     """e of the scale for finite elements up to ``top``."""
     if top == 0:
         return -126
@@ -47,7 +48,7 @@ def exponent(top: float, most: int = 127) -> int:
     return max(-126, min(most, k - 9 + (m > 0.875)))
 
 
-def store(x: torch.Tensor, most: int = 127, had: int = -126):
+def store(x: torch.Tensor, most: int = 119, had: int = -126):
     """``(values / scale, e)`` of rows ``x`` [rows, dim] that go into a page whose cached rows have exponent ``had``."""
     finite = x[torch.isfinite(x)]
     e = max(had, exponent(float(finite.abs().max()) if finite.numel() else 0.0, most))

@@ -23,7 +23,7 @@ BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 
 
 def most(dtype):
-    return 7 if dtype == FP16 else 127
+    return 7 if dtype == FP16 else 119
 
 
 def exact(got, want):

@@ -179,6 +179,7 @@ def test_oracle_codes():
     assert torch.equal(oracle.round_code(fine), fine)
     between = torch.cat([fine[:-1] + (fine[1:] - fine[:-1]) * f for f in (0.25, 0.5, 0.75)])
     assert torch.equal(oracle.round_code(between), between.float().to(torch.float8_e4m3fn).double())
-    for top, e in ((448.0, 0), (448.0001, 1), (1.75, -8), (1.8, -7), (0.0, -126), (2.0 ** -140, -126), (3e38, 120)):
+    for top, e in ((448.0, 0), (448.0001, 1), (1.75, -8), (1.8, -7), (0.0, -126), (2.0 ** -140, -126), (2.9e38, 119)):
         assert oracle.exponent(top) == e and (e == -126 or 448.0 * 2.0 ** e >= top > 448.0 * 2.0 ** (e - 1))
-    assert oracle.exponent(65504.0) == 8 and oracle.exponent(65504.0, 7) == 7
+    assert oracle.exponent(3.3e38) == 119  # 448 * 2^119 and no more: twice that is no fp32 value
+    assert oracle.exponent(65504.0, 99) == 8 and oracle.exponent(65504.0, 7) == 7
