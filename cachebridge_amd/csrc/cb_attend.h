@@ -597,19 +597,28 @@ __global__ __launch_bounds__(256) void join_few_kernel(AttendArgs a, int rows_pe
   const int D = s.head_dim, d0 = lane * E;
   float o[E] = {};
   if (d0 < D) {
-    for (int z = 0; z < n; ++z) {
-      // Read from lanes that may hold no element and are off here.
-      const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), z));
-      const float* from = a.part_out + (z * step + at) * D + d0;
-      if (f == 0.0f) continue;
-      if (D % E == 0) {
-        const vec x = *reinterpret_cast<const vec*>(from);
+    constexpr int U = 4;  // splits in flight
+    for (int z0 = 0; z0 < n; z0 += U) {
+      float x[U][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += f * x[e];
-      } else {
+      for (int u = 0; u < U; ++u) {
+        const float* from = a.part_out + (min(z0 + u, n - 1) * step + at) * D + d0;
+        if (D % E == 0) {
+          const vec y = *reinterpret_cast<const vec*>(from);
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (d0 + e < D) o[e] += f * from[e];
+          for (int e = 0; e < E; ++e) x[u][e] = y[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[u][e] = from[min(e, D - 1 - d0)];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        // Read from lanes that may hold no element and are off here. A weight of zero takes nothing, NaN included.
+        const float f = z0 + u < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), z0 + u)) : 0.0f;
+        if (f == 0.0f) continue;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += f * x[u][e];
       }
     }
   }
@@ -657,16 +666,26 @@ __global__ __launch_bounds__(kJoinThreads) void join_splits_kernel(AttendArgs a,
   const int D = s.head_dim;
   f32x4 o = {0, 0, 0, 0};
   const bool vector = D % 4 == 0;
-  for (int z = g; z < n; z += GROUPS) {
-    const float w = exp2_fast(lse[z * step] - mu);
-    if (w == 0.0f || 4 * x >= D) continue;
-    const float* from = a.part_out + (z * step + at) * D + 4 * x;
-    if (vector) {
-      o += w * *reinterpret_cast<const f32x4*>(from);
-    } else {
+  constexpr int U = 8;  // splits in flight
+  for (int z0 = g; z0 < n; z0 += U * GROUPS) {
+    f32x4 part[U];
+    float w[U];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (4 * x + e < D) o[e] += w * from[e];
+    for (int u = 0; u < U; ++u) {
+      const int z = min(z0 + u * GROUPS, n - 1);
+      w[u] = lse[z * step];
+      const float* from = a.part_out + (z * step + at) * D;
+      if (vector) {
+        part[u] = *reinterpret_cast<const f32x4*>(from + min(4 * x, D - 4));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[u][e] = from[min(4 * x + e, D - 1)];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      w[u] = z0 + u * GROUPS < n ? exp2_fast(w[u] - mu) : 0.0f;
+      o += w[u] == 0.0f ? f32x4{0, 0, 0, 0} : w[u] * part[u];  // a weight of zero takes nothing, NaN included
     }
   }
   sums[g][x] = o;

@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256) void quantize_tokens_kernel(QuantizeArgs a) {
   const int per = a.head_dim / V, total = min(ps, length - j0) * per;
   gcptr from = layer_base(a.src, kind, layer) + static_cast<int64_t>(head) * a.head_dim * static_cast<int>(sizeof(IO));
   gptr to = const_cast<gptr>(layer_base(a.dst, kind, layer)) + to_page * ps * a.dst.row_stride_b + static_cast<int64_t>(head) * a.head_dim;
-  float x[KEEP][V];
+  IO x[KEEP][V];
   bool has[KEEP];
   auto load = [&](int base) __attribute__((always_inline)) {
     int64_t row[KEEP];
@@ -216,7 +216,12 @@ __global__ __launch_bounds__(256) void quantize_tokens_kernel(QuantizeArgs a) {
       const char* p = (const char*)from + max(row[u], int64_t{0}) * a.src.row_stride_b + (at % per) * V * static_cast<int>(sizeof(IO));
       constexpr int W = V * sizeof(IO) % 16 == 0 ? 16 / sizeof(IO) : 1;
 #pragma unroll
-      for (int w = 0; w < V / W; ++w) load_vec<IO, W>(p + w * W * sizeof(IO), x[u] + w * W);
+      for (int w = 0; w < V / W; ++w) {
+        typedef IO vec __attribute__((ext_vector_type(W)));
+        const vec y = gload<vec>(as_global(static_cast<const void*>(p + w * W * sizeof(IO))));
+#pragma unroll
+        for (int e = 0; e < W; ++e) x[u][w * W + e] = y[e];
+      }
     }
   };
   float top = 0;
@@ -225,7 +230,7 @@ __global__ __launch_bounds__(256) void quantize_tokens_kernel(QuantizeArgs a) {
 #pragma unroll
     for (int u = 0; u < KEEP; ++u)
 #pragma unroll
-      for (int i = 0; i < V; ++i) top = fmaxf(top, has[u] ? finite_size(x[u][i]) : 0.0f);
+      for (int i = 0; i < V; ++i) top = fmaxf(top, has[u] ? finite_size(to_f32(x[u][i])) : 0.0f);
   }
   const int e = needed_exponent(wave_max(top), a.most);
   const float inv = inverse_scale(e);
@@ -234,7 +239,10 @@ __global__ __launch_bounds__(256) void quantize_tokens_kernel(QuantizeArgs a) {
 #pragma unroll
     for (int u = 0; u < KEEP; ++u) {
       const int at = base + u * kWave + lane;
-      if (has[u]) store_codes<V>(to + (at / per) * a.dst.row_stride_b + (at % per) * V, x[u], inv);
+      float y[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) y[i] = to_f32(x[u][i]);
+      if (has[u]) store_codes<V>(to + (at / per) * a.dst.row_stride_b + (at % per) * V, y, inv);
     }
   }
   if (lane == 0) *a.scales.at(kind, layer, to_page, head) = static_cast<uint8_t>(e + 127);
@@ -249,26 +257,29 @@ struct InstallQuantizedArgs {
   PageScales scales;
   int32_t most;
   uint32_t page_groups;
+  int32_t page_slots;  // pages of a request that its new tokens may be in, or 0: a unit for each token
 };
 
 template <int V>
 constexpr int kTurns = V == 8 ? 512 : kMaxPairs;  // pairs that 64 items turn, and those of one row at least
 
-// The new rows of one page, head and kind (0: K, 1: V): a wave. Token row t is
-// the page's first new one. Items of 2 V elements (both vectors of V pairs, or
-// two neighbours) lie one a lane in rounds of whole rows; up to KEEP rounds
-// stay in registers until the page's scale is known, more are read (and turned)
-// twice.
-template <typename IO, int V, int KEEP>
+// The new rows of one page, head and kind (0: K, 1: V): a team of TW waves, one or
+// the whole workgroup. Token row t is the page's first new one. Items of 2 V
+// elements (both vectors of V pairs, or two neighbours) lie one a lane in rounds
+// of whole rows, which the waves take in turn; up to KEEP rounds of a wave stay in
+// registers until the page's scale is known, more are read (and turned) twice.
+template <typename IO, int V, int TW, int KEEP>
 CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t, int head, int kind, turn_pair<IO>* turn) {
+  __shared__ float tops[kInstallWaves];
   const InstallArgs& a = q.i;
-  const int lane = threadIdx.x & (kWave - 1);
+  const int lane = threadIdx.x & (kWave - 1), wave = TW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) : 0;
+  const int member = wave * kWave + lane;
   const int ps = q.scales.page_size, i0 = t - r.q0, p0 = r.length - r.n + i0;
   const int page = q.scales.page_shift >= 0 ? p0 >> q.scales.page_shift : p0 / ps, slot = p0 - page * ps;
   const int rows = min(ps - slot, r.n - i0);
   const int64_t to_page = pool_page(a.batch, q.scales, r, page);
   if (to_page < 0) {
-    if (lane == 0) flag(a.batch.err, CB_ERROR_TARGET_ROW);
+    if (member == 0) flag(a.batch.err, CB_ERROR_TARGET_ROW);
     return;
   }
   CB_GLOBAL uint8_t* scale = q.scales.at(kind, a.layer, to_page, head);
@@ -281,14 +292,16 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t
   const int turned = kind ? 0 : pairs / V, straight = kind ? 0 : a.rotary_dim;
   const int plain = (D - straight) / V, items = turned + (plain + 1) / 2;
   const int per_round = max(1, kWave / items), parts = (items + kWave - 1) / kWave;
-  const int rounds = (rows + per_round - 1) / per_round * parts;
+  // This wave's rounds: groups of per_round rows, every TW-th from its own, parts each.
+  const int groups = (rows + per_round - 1) / per_round, rounds = (max(groups - wave, 0) + TW - 1) / TW * parts;
+  auto first_row = [&](int n) { return (wave + n / parts * TW) * per_round; };
   struct Item {
     int row, first, second;  // elements of the two vectors
     bool on, two;
   };
   auto item = [&](int n) __attribute__((always_inline)) {
     Item m;
-    const int row0 = n / parts * per_round, part = n - n / parts * parts;
+    const int row0 = first_row(n), part = n - n / parts * parts;
     const int in = parts == 1 ? lane / items : 0, k = parts == 1 ? lane - in * items : part * kWave + lane;
     m.row = row0 + in;
     m.on = (in < per_round) & (m.row < rows) & (k < items);
@@ -304,7 +317,7 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t
     return m;
   };
   auto load = [&](int n, float (&y)[2 * V]) __attribute__((always_inline)) {
-    const int row0 = n / parts * per_round;
+    const int row0 = first_row(n);
     if (kind == 0 && n % parts == 0) {
       const int all = min(per_round, rows - row0) * pairs;
       for (int x = lane; x < all; x += kWave) {
@@ -339,7 +352,14 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t
 #pragma unroll
         for (int i = 0; i < 2 * V; ++i) top = fmaxf(top, finite_size(y[u][i]));
       }
-  const int e = max(had, needed_exponent(wave_max(top), q.most));
+  top = wave_max(top);
+  if constexpr (TW > 1) {
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TW; ++w) top = fmaxf(top, tops[w]);
+  }
+  const int e = max(had, needed_exponent(top, q.most));
   const float inv = inverse_scale(e);
   for (int n0 = 0; n0 < rounds; n0 += KEEP)
 #pragma unroll
@@ -354,7 +374,7 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t
   if (e > had && slot > 0) {  // cached tokens of a page whose scale grows
     const float by = inverse_scale(min(e - had, 126));  // codes times 2^-126 are zeros
     const int words = D / 2;
-    for (int x = lane; x < slot * words; x += kWave) {
+    for (int x = member; x < slot * words; x += TW * kWave) {
       gptr at = to + x / words * a.cache.row_stride_b + x % words * 2;
       const uint32_t c0 = gload<uint8_t>(at), c1 = gload<uint8_t>(at + 1);
       const uint32_t c = pack_codes(__builtin_amdgcn_cvt_f32_fp8(c0, 0) * by, __builtin_amdgcn_cvt_f32_fp8(c1, 0) * by, 0, 0);
@@ -362,13 +382,15 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t
       gstore<uint8_t>(at + 1, static_cast<uint8_t>(c >> 8));
     }
   }
-  if (lane == 0 && (e > had || slot == 0)) *scale = static_cast<uint8_t>(e + 127);
+  if (member == 0 && (e > had || slot == 0)) *scale = static_cast<uint8_t>(e + 127);
 }
 
-// One launch, two kinds of workgroups: those of a wave a (token, head, K or V),
-// which store a page's new rows if the token is the first of them, and those that
-// rotate the queries (install_rows).
-template <typename IO, int V>
+// One launch, two kinds of workgroups: those whose teams of TW waves have a (page,
+// head, K or V) each and store its new rows, and those that rotate the queries
+// (install_rows). Pages are counted by request; where the bound on a request's new
+// tokens leaves more of them than there are tokens, a team goes by a token and
+// works if it is its page's first new one.
+template <typename IO, int V, int TW>
 __global__ __launch_bounds__(kInstallWaves * kWave) void install_quantized_kernel(InstallQuantizedArgs q) {
   __shared__ turn_pair<IO> turn[kInstallWaves][kTurns<V>];
   const InstallArgs& a = q.i;
@@ -378,23 +400,34 @@ __global__ __launch_bounds__(kInstallWaves * kWave) void install_quantized_kerne
       if (wave == 0) flag_requests(a.batch);
       return;
     }
-    install_rows<IO, V, false, true>(a, static_cast<int64_t>(blockIdx.x - q.page_groups) * kInstallWaves + wave, turn[wave]);
+    install_rows<IO, V, 1, false, true>(a, static_cast<int64_t>(blockIdx.x - q.page_groups) * kInstallWaves + wave, turn[wave]);
     return;
   }
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kInstallWaves + wave;
-  const int t = static_cast<int>(unit / (2 * a.kv_heads)), rest = static_cast<int>(unit % (2 * a.kv_heads));
-  if (t >= a.batch.tokens) return;
-  const int b = request_of_token(a.batch, t);
-  if (b >= a.batch.requests) return;
-  const Request r = load_request(a.batch, b);
-  if (!r.ok) return;
+  const int64_t unit = TW > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kInstallWaves + wave;
+  const int64_t place = unit / (2 * a.kv_heads);
+  const int rest = static_cast<int>(unit - place * 2 * a.kv_heads), ps = q.scales.page_size;
+  int t;
+  Request r;
+  if (q.page_slots) {
+    const int64_t b = place / q.page_slots;
+    if (b >= a.batch.requests) return;
+    r = own_request<true>(a.batch, static_cast<int>(b));
+    const int p0 = r.length - r.n, page = p0 / ps + static_cast<int>(place - b * q.page_slots);
+    t = r.q0 + max(0, page * ps - p0);
+    if (!r.ok || t >= r.q0 + r.n) return;
+  } else {
+    if (place >= a.batch.tokens) return;
+    t = static_cast<int>(place);
+    const int b = request_of_token(a.batch, t);
+    if (b >= a.batch.requests) return;
+    r = load_request(a.batch, b);
+    if (!r.ok || (t > r.q0 && (r.length - r.n + t - r.q0) % ps != 0)) return;
+  }
   if (r.rem != 0) {  // it shares a page with what lies before it
     flag(a.batch.err, CB_ERROR_REQUEST);
     return;
   }
-  const int p = r.length - r.n + (t - r.q0);
-  if (t > r.q0 && p % q.scales.page_size != 0) return;
-  store_page<IO, V, 2>(q, r, t, rest >> 1, rest & 1, turn[wave]);
+  store_page<IO, V, TW, (TW > 1 ? 4 : 2)>(q, r, t, rest >> 1, rest & 1, turn[wave]);
 }
 
 // ---------------------------------------------------------------------------
@@ -1108,14 +1141,20 @@ void launch_quantized(const AttendArgs& a, const ScaledCache& cache, const Atten
 }
 
 template <typename IO>
-void launch_store(const InstallQuantizedArgs& q, bool wide, unsigned grid, hipStream_t st) {
-  if (wide) hipLaunchKernelGGL((install_quantized_kernel<IO, 16 / sizeof(IO)>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, q);
-  else hipLaunchKernelGGL((install_quantized_kernel<IO, 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, q);
+void launch_store(const InstallQuantizedArgs& q, bool wide, bool teams, unsigned grid, hipStream_t st) {
+  constexpr int V = 16 / sizeof(IO);
+  if (wide && teams) hipLaunchKernelGGL((install_quantized_kernel<IO, V, kInstallWaves>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, q);
+  else if (wide) hipLaunchKernelGGL((install_quantized_kernel<IO, V, 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, q);
+  else if (teams) hipLaunchKernelGGL((install_quantized_kernel<IO, 1, kInstallWaves>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, q);
+  else hipLaunchKernelGGL((install_quantized_kernel<IO, 1, 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, q);
 }
 
 template <typename IO>
 void launch_quantize(const QuantizeArgs& a, int vec, dim3 grid, hipStream_t st) {
-  if (vec == 16) hipLaunchKernelGGL((quantize_tokens_kernel<IO, 16, 4>), grid, dim3(256), 0, st, a);
+  const int chunks = ceil_div(static_cast<int64_t>(a.scales.page_size) * a.head_dim, 16 * kWave);
+  if (vec == 16 && chunks <= 2) hipLaunchKernelGGL((quantize_tokens_kernel<IO, 16, 2>), grid, dim3(256), 0, st, a);
+  else if (vec == 16 && chunks > 4) hipLaunchKernelGGL((quantize_tokens_kernel<IO, 16, 8>), grid, dim3(256), 0, st, a);
+  else if (vec == 16) hipLaunchKernelGGL((quantize_tokens_kernel<IO, 16, 4>), grid, dim3(256), 0, st, a);
   else if (vec == 8) hipLaunchKernelGGL((quantize_tokens_kernel<IO, 8, 4>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((quantize_tokens_kernel<IO, 2, 4>), grid, dim3(256), 0, st, a);
 }
@@ -1138,17 +1177,24 @@ int cb_install_quantized(const cb_query_batch* batch, const cb_page_scales* scal
   const int vec = 16 / eb;
   const bool wide = (rotary_dim / 2) % vec == 0 && head_dim % vec == 0 && aligned16(a.i.q) && aligned16(a.i.q_out) &&
                     aligned16(a.i.k) && aligned16(a.i.v) && rows_aligned16(a.i.cache, 16) && head_dim % 8 == 0;
-  const int items = a.i.q_heads * (head_dim - rotary_dim / 2) / (wide ? vec : 1);
-  a.i.slices = std::max(1, std::min(64, ceil_div(items, kWave)));
+  const InstallItems each = install_items(head_dim, rotary_dim, wide ? vec : 1);
+  a.i.slices = std::max(1, std::min(64, ceil_div(a.i.q_heads * each.head, kWave)));
   a.most = most_exponent(dtype);
-  const int64_t pages = (static_cast<int64_t>(n) * 2 * a.i.kv_heads + kInstallWaves - 1) / kInstallWaves;
+  // Pages of a request that max_query tokens may be in, wherever they begin; the whole workgroup has one where a
+  // wave would go round more than twice.
+  const int64_t ps = a.scales.page_size, most = batch->max_query;
+  const int64_t slots = most < 1 ? 0 : (most + ps - 2) / ps + 1;
+  a.page_slots = slots * batch->num_requests <= n ? static_cast<int32_t>(slots) : 0;
+  const int64_t places = a.page_slots ? slots * batch->num_requests : n;
+  const bool teams = std::min(ps, most) * std::max(each.head, each.value) > 2 * kWave;
+  const int64_t units = places * 2 * a.i.kv_heads, pages = teams ? units : (units + kInstallWaves - 1) / kInstallWaves;
   const int64_t grid = pages + (static_cast<int64_t>(n) * a.i.slices + kInstallWaves - 1) / kInstallWaves + (d_error_flag ? 1 : 0);
   if (!launch_fits(grid, kInstallWaves * kWave)) return fail(CB_EINVAL, "too many tokens");
   a.page_groups = static_cast<uint32_t>(pages);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == CB_DTYPE_BF16) launch_store<io_bf16>(a, wide, static_cast<unsigned>(grid), st);
-  else if (dtype == CB_DTYPE_F16) launch_store<io_f16>(a, wide, static_cast<unsigned>(grid), st);
-  else launch_store<float>(a, wide, static_cast<unsigned>(grid), st);
+  if (dtype == CB_DTYPE_BF16) launch_store<io_bf16>(a, wide, teams, static_cast<unsigned>(grid), st);
+  else if (dtype == CB_DTYPE_F16) launch_store<io_f16>(a, wide, teams, static_cast<unsigned>(grid), st);
+  else launch_store<float>(a, wide, teams, static_cast<unsigned>(grid), st);
   CB_HIP(hipGetLastError());
   return CB_OK;
 }

@@ -7,7 +7,7 @@
 
 namespace {
 
-template <typename IO, int V>
+template <typename IO, int V, int U>
 __global__ __launch_bounds__(kInstallWaves * kWave) void install_tokens_kernel(InstallArgs a) {
   __shared__ turn_pair<IO> turn[kInstallWaves][kMaxPairs];
   const int wave = threadIdx.x / kWave;
@@ -15,7 +15,7 @@ __global__ __launch_bounds__(kInstallWaves * kWave) void install_tokens_kernel(I
     if (wave == 0) flag_requests(a.batch);
     return;
   }
-  install_rows<IO, V, true, false>(a, static_cast<int64_t>(blockIdx.x) * kInstallWaves + wave, turn[wave]);
+  install_rows<IO, V, U, true, false>(a, static_cast<int64_t>(blockIdx.x) * kInstallWaves + wave, turn[wave]);
 }
 
 // Many query rows: a workgroup's NW waves hold 32 rows each and share K and V
@@ -784,10 +784,13 @@ void launch_weights(const WeightArgs& a, bool mod, unsigned grid, hipStream_t st
   else launch_weights_any<IO, 512>(a, grid, st);
 }
 
+constexpr int kManyWaves = 8192;  // of an install, from which a lane has two items
+
 template <typename IO>
-void launch_install(const InstallArgs& a, bool wide, unsigned grid, hipStream_t st) {
-  if (wide) hipLaunchKernelGGL((install_tokens_kernel<IO, 16 / sizeof(IO)>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, a);
-  else hipLaunchKernelGGL((install_tokens_kernel<IO, 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, a);
+void launch_install(const InstallArgs& a, bool wide, int items, unsigned grid, hipStream_t st) {
+  if (wide && items == 2) hipLaunchKernelGGL((install_tokens_kernel<IO, 16 / sizeof(IO), 2>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, a);
+  else if (wide) hipLaunchKernelGGL((install_tokens_kernel<IO, 16 / sizeof(IO), 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, a);
+  else hipLaunchKernelGGL((install_tokens_kernel<IO, 1, 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, a);
 }
 
 }  // namespace
@@ -815,14 +818,17 @@ int cb_install_rotated(const cb_query_batch* batch, int32_t layer, int32_t dtype
   const int vec = 16 / eb;
   const bool wide = (rotary_dim / 2) % vec == 0 && head_dim % vec == 0 && aligned16(a.q) && aligned16(a.q_out) &&
                     aligned16(a.k) && aligned16(a.v) && rows_aligned16(a.cache, head_dim * eb);
-  const int items = (a.q_heads + kv) * (head_dim - rotary_dim / 2) / (wide ? vec : 1) + kv * head_dim / (wide ? vec : 1);
-  a.slices = std::max(1, std::min(64, ceil_div(items, kWave)));  // an item a lane: one round of memory latency
+  const InstallItems each = install_items(head_dim, rotary_dim, wide ? vec : 1);
+  const int total = (a.q_heads + kv) * each.head + kv * each.value;
+  // An item a lane: one round of memory latency; two where there are waves enough to fill the card.
+  const int items = wide && static_cast<int64_t>(n) * ceil_div(total, kWave) >= kManyWaves ? 2 : 1;
+  a.slices = std::max(1, std::min(64, ceil_div(total, items * kWave)));
   const int64_t grid = (static_cast<int64_t>(n) * a.slices + kInstallWaves - 1) / kInstallWaves + (d_error_flag ? 1 : 0);
   if (!launch_fits(grid, kInstallWaves * kWave)) return fail(CB_EINVAL, "too many tokens");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == CB_DTYPE_BF16) launch_install<io_bf16>(a, wide, static_cast<unsigned>(grid), st);
-  else if (dtype == CB_DTYPE_F16) launch_install<io_f16>(a, wide, static_cast<unsigned>(grid), st);
-  else launch_install<float>(a, wide, static_cast<unsigned>(grid), st);
+  if (dtype == CB_DTYPE_BF16) launch_install<io_bf16>(a, wide, items, static_cast<unsigned>(grid), st);
+  else if (dtype == CB_DTYPE_F16) launch_install<io_f16>(a, wide, items, static_cast<unsigned>(grid), st);
+  else launch_install<float>(a, wide, items, static_cast<unsigned>(grid), st);
   CB_HIP(hipGetLastError());
   return CB_OK;
 }

@@ -55,6 +55,16 @@ __device__ inline void sincos_turns(double turns, T* sn, T* cs) {
   *cs = (quadrant == 1 || quadrant == 2) ? -b : b;
 }
 
+// Items of two vectors of V elements in a head of q or k, of these the turned ones
+// first, and in a head of v.
+struct InstallItems {
+  int head, turned, value;
+};
+__host__ __device__ inline InstallItems install_items(int head_dim, int rotary_dim, int v) {
+  const int turned = rotary_dim / 2 / v;
+  return {turned + ((head_dim - rotary_dim) / v + 1) / 2, turned, (head_dim / v + 1) / 2};
+}
+
 // V elements as one access where V * sizeof(IO) is 16, else element by element.
 template <typename IO, int V>
 __device__ inline void load_vec(const char* p, float* out) {
@@ -126,14 +136,12 @@ CB_INLINE void turn_pairs(const float (&x)[2 * V], const PAIR* turn, bool interl
 // y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin for the pairs (a, b) of the
 // rotated part, angles position * inv_freq. One wave per (token, slice of its
 // heads' elements): lanes compute the token's angles once into LDS, then each
-// item is V pairs of a head (two vectors) or V elements that are copied; slices
-// are cut to an item a lane, so that a wave waits for memory once. Every element
-// is read once and written once. 64 tokens of 64 query and 8 KV heads of 128 in bf16
-// take 4.8 us, the latency of a launch and of three dependent loads; 2048 of 16
-// and 2 (21 MB) 9.3 us, that latency and the bytes' time at a copy's rate.
+// item is two vectors of a head: those of V pairs, or two that are copied; slices
+// are cut to U items a lane, so that a wave waits for memory once. Every element
+// is read once and written once.
 // KV: K and V rows go into the cache as they are, else queries alone are written.
 // WHOLE: requests that do not start at a page's first slot are outside the bounds.
-template <typename IO, int V, bool KV, bool WHOLE>
+template <typename IO, int V, int U, bool KV, bool WHOLE>
 CB_INLINE void install_rows(const InstallArgs& a, int64_t unit, turn_pair<IO>* turn) {
   const int lane = threadIdx.x & (kWave - 1);
   const int t = static_cast<int>(unit / a.slices), slice = static_cast<int>(unit % a.slices);
@@ -152,54 +160,58 @@ CB_INLINE void install_rows(const InstallArgs& a, int64_t unit, turn_pair<IO>* t
   for (int i = lane; i < pairs; i += kWave) turn[i] = turn_of<turn_pair<IO>, turn_t<IO>>(a, t, p, i);
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
-  const int rot_items = pairs / V, pass_items = (a.head_dim - a.rotary_dim) / V, head_items = rot_items + pass_items;
-  const int v_items = a.head_dim / V;
-  const int turned = (a.q_heads + kv_heads) * head_items;
-  const int total = turned + kv_heads * v_items;
+  const InstallItems n = install_items(a.head_dim, a.rotary_dim, V);
+  const int turned = (a.q_heads + kv_heads) * n.head, total = turned + kv_heads * n.value;
   const int per = (total + a.slices - 1) / a.slices;
   const int stop = min(total, (slice + 1) * per);
   char* krow = const_cast<char*>((const char*)layer_base(a.cache, 0, a.layer)) + row * a.cache.row_stride_b;
   char* vrow = const_cast<char*>((const char*)layer_base(a.cache, 1, a.layer)) + row * a.cache.row_stride_b;
   constexpr int E = sizeof(IO);
-  for (int idx = slice * per + lane; idx < stop; idx += kWave) {
-    const char* src;
-    char* dst;
-    int item;
-    if (idx < turned) {
-      const int head = idx / head_items;
-      item = idx - head * head_items;
-      if (head < a.q_heads) {
-        src = a.q.data + t * a.q.token_b + head * a.q.head_b;
-        dst = a.q_out.data + t * a.q_out.token_b + head * a.q_out.head_b;
+  for (int idx = slice * per + lane; idx < stop; idx += U * kWave) {
+    const char* src[U];
+    char* dst[U];
+    int oa[U], ob[U], first[U];  // the vectors, and the first pair or -1
+    bool on[U], two[U];
+    float x[U][2 * V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = min(idx + u * kWave, stop - 1);
+      on[u] = idx + u * kWave < stop;
+      const bool value = KV && at >= turned;
+      const int head = value ? (at - turned) / n.value : at / n.head;
+      const int item = value ? at - turned - head * n.value : at - head * n.head;
+      if (value) {
+        src[u] = a.v.data + t * a.v.token_b + head * a.v.head_b;
+        dst[u] = vrow + static_cast<int64_t>(head) * a.head_dim * E;
+        on[u] &= row >= 0;
+      } else if (head < a.q_heads) {
+        src[u] = a.q.data + t * a.q.token_b + head * a.q.head_b;
+        dst[u] = a.q_out.data + t * a.q_out.token_b + head * a.q_out.head_b;
       } else {
-        src = a.k.data + t * a.k.token_b + (head - a.q_heads) * a.k.head_b;
-        dst = krow + static_cast<int64_t>(head - a.q_heads) * a.head_dim * E;
-        if (row < 0) continue;
+        src[u] = a.k.data + t * a.k.token_b + (head - a.q_heads) * a.k.head_b;
+        dst[u] = krow + static_cast<int64_t>(head - a.q_heads) * a.head_dim * E;
+        on[u] &= row >= 0;
       }
-    } else {
-      if (row < 0) continue;
-      const int head = (idx - turned) / v_items;
-      const int off = (idx - turned - head * v_items) * V;
-      float x[V];
-      load_vec<IO, V>(a.v.data + t * a.v.token_b + head * a.v.head_b + off * E, x);
-      store_vec<IO, V>(vrow + (static_cast<int64_t>(head) * a.head_dim + off) * E, x);
-      continue;
+      first[u] = !value && item < n.turned ? item * V : -1;
+      const int straight = value ? 0 : a.rotary_dim, at2 = straight + 2 * (item - (value ? 0 : n.turned)) * V;
+      oa[u] = first[u] < 0 ? at2 : a.interleaved ? 2 * first[u] : first[u];
+      ob[u] = first[u] < 0 ? at2 + V : a.interleaved ? oa[u] + V : first[u] + pairs;
+      two[u] = first[u] >= 0 || at2 + V < a.head_dim;
+      if (on[u]) {
+        load_vec<IO, V>(src[u] + oa[u] * E, x[u]);
+        if (two[u]) load_vec<IO, V>(src[u] + ob[u] * E, x[u] + V);
+      }
     }
-    if (item >= rot_items) {
-      const int off = a.rotary_dim + (item - rot_items) * V;
-      float x[V];
-      load_vec<IO, V>(src + off * E, x);
-      store_vec<IO, V>(dst + off * E, x);
-      continue;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!on[u]) continue;
+      float y[2 * V];
+#pragma unroll
+      for (int i = 0; i < 2 * V; ++i) y[i] = x[u][i];
+      if (first[u] >= 0) turn_pairs<V>(x[u], turn + first[u], a.interleaved, y);
+      store_vec<IO, V>(dst[u] + oa[u] * E, y);
+      if (two[u]) store_vec<IO, V>(dst[u] + ob[u] * E, y + V);
     }
-    const int first = item * V;
-    const int oa = a.interleaved ? 2 * first : first, ob = a.interleaved ? oa + V : first + pairs;
-    float x[2 * V], y[2 * V];
-    load_vec<IO, V>(src + oa * E, x);
-    load_vec<IO, V>(src + ob * E, x + V);
-    turn_pairs<V>(x, turn + first, a.interleaved, y);
-    store_vec<IO, V>(dst + oa * E, y);
-    store_vec<IO, V>(dst + ob * E, y + V);
   }
 }
 
