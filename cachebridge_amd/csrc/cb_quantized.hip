@@ -498,19 +498,302 @@ CB_INLINE AttendArgs late_args() {
   return __builtin_bit_cast(AttendArgs, raw);
 }
 
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+template <typename IO>
+CB_INLINE f32x4 mul16(u32x4 a, u32x4 b, f32x4 c) {
+  typedef typename Half<IO>::x8 x8;
+  if constexpr (std::is_same_v<IO, io_bf16>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+}
+
+// Places of an element tile's 16-byte chunks for ElemBlock's reads: K as for RowBlock
+// (16 rows of one chunk), V eight keys of two chunks.
+__device__ inline int swizzle_v16(int key) { return (key & 7) << 1; }
+
+// 16 query rows of one wave over tiles of KT keys held as elements, with
+// v_mfma_f32_16x16x32 (operands: lane l holds elements 8 (l / 16) .. + 7 of row or
+// column l % 16; result register e of lane l: row 4 (l / 16) + e, column l % 16).
+// S^T = K Q^T leaves a lane keys 16 kb + 4 g + e (g = l / 16) of query row l % 16,
+// which for kb = 2 x and 2 x + 1 are the second operand of O^T += V^T P^T in the key
+// order {4g .. 4g+3, 16+4g .. 16+4g+3} of block x. Half of RowBlock's rows take half
+// of its registers, so that two waves share a SIMD where a head's 256 elements
+// leave RowBlock one, and twice its reads a product.
+template <typename IO, int DP, int KT, bool MOD>
+struct ElemBlock {
+  typedef Half<IO> H;
+  static constexpr int KB = KT / 32, DB = DP / 16, KS = DP / 32;
+  u32x4 q[KS];
+  f32x4 o[DB];
+  float m, l, slope;
+  int i, qh, p;  // this lane's query row
+  bool live;
+
+  __device__ inline void init(const ScoreArgs& s, const Request& r, int head, int row0, bool vector) {
+    const int lane = threadIdx.x & (kWave - 1), g = lane >> 4;
+    const int rows = r.n * s.group, row = row0 + (lane & 15);
+    live = row < rows;
+    const int at = min(row, rows - 1);
+    i = at / s.group;
+    qh = head * s.group + at - i * s.group;
+    p = r.length - r.n + i;
+    const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const char* from = qp + 2 * min(32 * k + 8 * g, s.head_dim - 8);
+      if (vector) {
+        q[k] = gload<u32x4>(as_global(static_cast<const void*>(from)));
+      } else {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          q[k][w] = load_elem<uint16_t>(from + 4 * w) | static_cast<uint32_t>(load_elem<uint16_t>(from + 4 * w + 2)) << 16;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < KS; ++k) q[k] = 32 * k + 8 * g < s.head_dim ? q[k] : u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = f32x4{0, 0, 0, 0};
+    m = kNegInf;
+    l = slope = 0;
+    if constexpr (MOD) slope = s.slopes ? s.slopes[qh] : 0.0f;
+  }
+
+  // LDS offsets within a tile that depend on the lane alone.
+  struct Lanes {
+    uint32_t k[DP == 64 ? 2 : 4];  // K chunk 4 ks + g of row l % 16; ks + 4: 256 bytes on
+    uint32_t v[DP == 64 ? 4 : 8];  // V chunks 2 db and 2 db + 1 of this lane's key; db + 8: 256 bytes on
+  };
+  static __device__ inline Lanes lanes() {
+    Lanes a;
+    const int lane = threadIdx.x & (kWave - 1), g = lane >> 4, c = lane & 15;
+#pragma unroll
+    for (int ks = 0; ks < (DP == 64 ? 2 : 4); ++ks) a.k[ks] = c * DP * 2 + ((4 * ks + g) ^ swizzle_k<DP>(c)) * 16;
+    const int key = 4 * g + (c >> 2);
+#pragma unroll
+    for (int d = 0; d < (DP == 64 ? 4 : 8); ++d) a.v[d] = key * DP * 2 + ((2 * d + ((c & 3) >> 1)) ^ place_v(key)) * 16 + (c & 1) * 8;
+    return a;
+  }
+  static __device__ inline int place_v(int key) { return DP == 64 ? ((key >> 1) & 3) << 1 : swizzle_v16(key); }
+
+  static CB_INLINE u32x4 k_frag(const Lanes& a, uint32_t lk, int kb, int ks) {
+    return *lds_at<const u32x4>(lk + a.k[ks & 3] + kb * 16 * DP * 2 + (ks >> 2) * 256);
+  }
+  static CB_INLINE u32x4 v_frag(const Lanes& a, uint32_t lv, int x, int db) {
+    const uint32_t at = lv + a.v[db & 7] + x * 32 * DP * 2 + (db >> 3) * 256;
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(at));
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(at + 16 * DP * 2));
+    const uint2 y = __builtin_bit_cast(uint2, lo), z = __builtin_bit_cast(uint2, hi);
+    return u32x4{y.x, y.y, z.x, z.y};
+  }
+
+  // Operands are read from LDS a few steps ahead of their use (as in RowBlock).
+  static constexpr int kAhead = 4;
+  CB_INLINE void products(const Lanes& a, uint32_t lk, f32x8 (&st)[KB]) {
+    constexpr int B = KT / 16, STEPS = B * KS;
+    u32x4 f[kAhead];
+    f32x4 x[B];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) f[n] = k_frag(a, lk, n % B, n / B);
+#pragma unroll
+    for (int kb = 0; kb < B; ++kb) x[kb] = f32x4{0, 0, 0, 0};
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < STEPS; ++n) {
+      x[n % B] = mul16<IO>(f[n % kAhead], q[n / B], x[n % B]);
+      if (n + kAhead < STEPS) f[n % kAhead] = k_frag(a, lk, (n + kAhead) % B, (n + kAhead) / B);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) st[kb][e] = x[2 * kb + (e >> 2)][e & 3];
+  }
+
+  // Modified and masked, as RowBlock::ready.
+  CB_INLINE void ready(const ScoreArgs& s, const KeyRange& kr, f32x8 (&st)[KB], int start, bool whole, const uint32_t* valid) {
+    const int g = (threadIdx.x & (kWave - 1)) >> 4;
+    if constexpr (MOD) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) modify_scores<true, 8, 16>(s, st[kb], kLog2e, slope, p, start + 32 * kb, g);
+    }
+    if (!whole) {
+      asm volatile("");  // a branch, not selects that every tile would pay for
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const uint32_t there = valid[kb] >> (4 * g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int k = 16 * (e >> 2) + (e & 3);
+          const bool in = sees(s, kr, p, start + 32 * kb + 4 * g + k) & ((there >> k) & 1);
+          st[kb][e] = in ? st[kb][e] : kNegInf;
+        }
+      }
+    }
+  }
+
+  CB_INLINE float try_weights(const f32x8 (&st)[KB], float scale2, u32x4 (&w)[KB]) const {
+    const float mu = m == kNegInf ? 0.0f : m;
+    float sum = 0;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float x = exp2_fast(__builtin_fmaf(st[kb][e], scale2, -mu)), y = exp2_fast(__builtin_fmaf(st[kb][e + 1], scale2, -mu));
+        sum += x + y;
+        w[kb][e >> 1] = H::pack(x, y);
+      }
+    return sum;
+  }
+  CB_INLINE void weights(const f32x8 (&st)[KB], float scale2, u32x4 (&w)[KB]) {
+    float sum = try_weights(st, scale2, w);
+    if (__any(!(sum < H::kLag) | (m == kNegInf))) {
+      float top = kNegInf;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, st[kb][e]);
+      top = __builtin_fmaf(top, scale2, -H::kRoom);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      const float m1 = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+      const float alpha = m1 == kNegInf ? 1.0f : exp2_fast(m - m1);
+      m = m1;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= alpha;
+      sum = try_weights(st, scale2, w);
+    }
+    l += sum;
+  }
+
+  struct Values {
+    u32x4 f[kAhead];
+  };
+  static CB_INLINE Values first_values(const Lanes& a, uint32_t lv) {
+    Values v;
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) v.f[n] = v_frag(a, lv, n / DB, n % DB);
+    __builtin_amdgcn_sched_barrier(0);
+    return v;
+  }
+  CB_INLINE void add_values(const Lanes& a, uint32_t lv, const u32x4 (&w)[KB], Values& v) {
+    constexpr int STEPS = KB * DB;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < STEPS; ++n) {
+      o[n % DB] = mul16<IO>(v.f[n % kAhead], w[n / DB], o[n % DB]);
+      if (n + kAhead < STEPS) v.f[n % kAhead] = v_frag(a, lv, (n + kAhead) / DB, (n + kAhead) % DB);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // One wave notes, a bit per (row, element), every NaN of the V tile at lv that its
+  // rows see (codes stand for no infinities).
+  CB_INLINE void mark_nan(uint32_t lv, const ScoreArgs& s, int np, int start, int end, CB_LDS_SPACE uint32_t* marks) const {
+    constexpr int C = DP / 8;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int below = s.causal ? p : 0x7fffffff, above = s.window > 0 ? p - s.window : -1;
+    for (int n = 0; n < KT * C / kWave; ++n) {
+      const u32x4 x = *lds_at<const u32x4>(lv + (n * kWave + lane) * 16);
+      uint64_t hits = __ballot(has_not_finite<IO>(x));
+      while (hits) {
+        const int at = __ffsll(static_cast<unsigned long long>(hits)) - 1;
+        hits &= hits - 1;
+        const int chunk = n * kWave + at, key = chunk / C, d0 = ((chunk % C) ^ place_v(key)) * 8, j = start + key;
+        const bool seen = (j < end) & ((j < np) | ((j <= below) & (j > above))) & (lane < 16);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t y = __shfl(x[w], at), c = ((y & H::kExponent) + H::kCarry) & 0x80008000u;
+          bits |= (((c >> 15) & 1) | ((c >> 30) & 2)) << (2 * w);
+        }
+        if (seen) marks[(lane & 15) * (DP / 32) + (d0 >> 5)] |= bits << (d0 & 31);
+      }
+    }
+  }
+  CB_INLINE void add_marks(const uint32_t* marks) {
+    const int lane = threadIdx.x & (kWave - 1), g = lane >> 4;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const uint32_t bits = marks[(lane & 15) * (DP / 32) + (d >> 1)] >> (16 * (d & 1) + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[d][e] += (bits >> e) & 1 ? __uint_as_float(0x7fc00000u) : 0.0f;
+    }
+  }
+
+  __device__ inline void finish(const AttendArgs& a, const Request& r, int split, bool vector) {
+    const ScoreArgs& s = a.s;
+    const int g = (threadIdx.x & (kWave - 1)) >> 4;
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float lse2 = l == 0.0f ? kNegInf : m + log2_fast(l);
+    if (!live) return;
+    const int64_t at = static_cast<int64_t>(r.q0 + i) * s.q_heads + qh;
+    if (a.splits > 1) {
+      const int64_t slot = static_cast<int64_t>(split) * s.batch.tokens * s.q_heads + at;
+      gptr po = as_global(static_cast<void*>(a.part_out + slot * s.head_dim));
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+        if (16 * d < s.head_dim) gstore<f32x4>(po + (16 * d + 4 * g) * 4, o[d] * inv);
+      if (g == 0) a.part_lse[slot] = lse2;
+      return;
+    }
+    char* op = a.out.data + static_cast<int64_t>(r.q0 + i) * a.out.token_b + qh * a.out.head_b;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+      if (16 * d < s.head_dim) {
+        char* to = op + (16 * d + 4 * g) * 2;
+        const uint2 x = make_uint2(H::pack(o[d][0] * inv, o[d][1] * inv), H::pack(o[d][2] * inv, o[d][3] * inv));
+        if (vector) {
+          gstore<uint2>(as_global(static_cast<void*>(to)), x);
+        } else {
+          store_elem<uint16_t>(to, static_cast<uint16_t>(x.x));
+          store_elem<uint16_t>(to + 2, static_cast<uint16_t>(x.x >> 16));
+          store_elem<uint16_t>(to + 4, static_cast<uint16_t>(x.y));
+          store_elem<uint16_t>(to + 6, static_cast<uint16_t>(x.y >> 16));
+        }
+      }
+    if (a.lse && g == 0) a.lse[at] = lse2 * kLn2;
+  }
+};
+
+// A tile's keys in LDS, by slot t % 4: one wave resolves rows, another fetches scales.
+template <int KT>
+struct TileCodes {
+  uint32_t off[4][KT];  // bytes from the head's first row, or the row itself where a layer has 2^32 or more; 0: no row
+  uint32_t at[4][KT];   // place of its scales
+  float scale[4][2][KT];
+  uint32_t valid[4][(KT + 31) / 32];  // keys that are there
+};
+
+// DMA of 16 bytes a lane from base + off.
+__device__ inline void dma16_at(gcptr base, uint32_t off, uint32_t lds) {
+  const uint32_t la = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :: "v"(off), "s"(reinterpret_cast<uint64_t>(base)), "s"(la) : "memory", "m0");
+}
+
+constexpr int kTileWaves = 8;
+
 // Many query rows: attend_tile_kernel's scheme on tiles that are widened once for
 // all of a workgroup's waves. A tile's codes come to LDS by DMA, each wave reads
 // the ones it asked for (16 a lane), and writes them as elements to where the
 // 16-bit kernel's DMA would have put them; the tile after that is on its way
-// while one is used.
-template <typename IO, int DP, int KT, int NW, bool MOD>
-__global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_codes_kernel(AttendArgs a, ScaledCache cache, int vector) {
-  constexpr int C = DP / 16, kTile = KT * DP * 2, kCodes = KT * DP, kHalf = kCodes / 1024, M = 2 * kHalf / NW, N = kTile / 1024 / NW;
+// while one is used. Keys without a row are read from row 0 and chunks past
+// head_dim from the last one, and made zeros when they are widened: a tile that is
+// whole pays nothing for either.
+// RB: query rows a wave, 32 (RowBlock) or 16 (ElemBlock).
+template <typename IO, int DP, int KT, int RB, bool MOD>
+__global__ __launch_bounds__(kTileWaves * kWave, 2) void attend_codes_kernel(AttendArgs a, ScaledCache cache, int vector) {
+  typedef std::conditional_t<RB == 32, RowBlock<IO, DP, KT, MOD>, ElemBlock<IO, DP, KT, MOD>> Block;
+  constexpr int NW = kTileWaves, C = DP / 16, kTile = KT * DP * 2, kCodes = KT * DP, kHalf = kCodes / 1024, M = 2 * kHalf / NW, N = kTile / 1024 / NW;
   static_assert(M >= 1 && 2 * kHalf % NW == 0 && N >= 1 && kTile % (1024 * NW) == 0, "a tile is whole DMA instructions of every wave");
   __shared__ __align__(1024) char tiles[4 * kTile];  // K, V of one buffer, K, V of the other
   __shared__ __align__(1024) char codes[2 * kCodes];
-  __shared__ TileRows<KT> tile_rows;
-  __shared__ uint32_t marks[2][NW][32 * (DP / 32)];
+  __shared__ TileCodes<KT> keys;
+  __shared__ uint32_t marks[RB / 16][NW][RB * (DP / 32)];
   __shared__ uint32_t odd[2];  // this tile holds values that are not finite; some tile did
   const ScoreArgs& s = a.s;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -518,25 +801,56 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_codes_ke
   const int split = rest / a.tile_slots;
   Request r;
   int b, tile;
-  if (!find_tile(a, rest % a.tile_slots, 32 * NW, r, b, tile)) return;
+  if (!find_tile(a, rest % a.tile_slots, RB * NW, r, b, tile)) return;
   r = uniform(r), b = uniform(b), tile = uniform(tile);
-  const int rows = r.n * s.group, row0 = tile * 32 * NW;
-  const KeyRange kr = key_range<KT>(s, r, b, row0, min(rows, row0 + 32 * NW) - 1);
+  const int rows = r.n * s.group, row0 = tile * RB * NW;
+  const KeyRange kr = key_range<KT>(s, r, b, row0, min(rows, row0 + RB * NW) - 1);
   const int per = split_tiles(a, kr.tiles), t0 = split * per, t1 = min(kr.tiles, t0 + per);
   if (a.splits > 1 && t0 >= t1) return;
 
-  typedef RowBlock<IO, DP, KT, MOD> Block;
   Block blk;
-  blk.init(s, r, head, row0 + 32 * wave, vector);
+  blk.init(s, r, head, row0 + RB * wave, vector);
   const typename Block::Lanes lanes = Block::lanes();
   const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((CB_LDS_SPACE char*)tiles));
   const uint32_t lds_codes = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((CB_LDS_SPACE char*)codes)) + wave * M * 1024;
   const float scale2 = MOD ? 1.0f : s.scale * kLog2e;
   if (threadIdx.x < 2) odd[threadIdx.x] = 0;
-  for (int w = threadIdx.x; w < 2 * NW * DP; w += NW * kWave) (&marks[0][0][0])[w] = 0;
+  for (int w = threadIdx.x; w < RB / 16 * NW * RB * (DP / 32); w += NW * kWave) (&marks[0][0][0])[w] = 0;
+  const HeadScales hs(cache.scales, s.layer, head);
+  const uint32_t stride = static_cast<uint32_t>(s.batch.row_stride_b);
+  const bool small = static_cast<uint64_t>(s.batch.rows) * stride <= 0xffffffffull;
   auto entry_of = [&](int t) { return t < t1 ? fetch_entry<KT>(s.batch, r, tile_start<KT>(kr, t), tile_end(kr, t)) : -1; };
-  auto place = [&](int64_t entry, int t) {
-    if (t < t1) place_rows(s.batch, r, entry, tile_start<KT>(kr, t), tile_end(kr, t), tile_rows, t & 3);
+  auto place = [&](int64_t entry, int t) __attribute__((always_inline)) {
+    if (t >= t1) return;
+    const int j = tile_start<KT>(kr, t) + lane, end = tile_end(kr, t);
+    int64_t row = entry;
+    if (s.batch.kind == CB_INDEX_BLOCK_TABLE) {
+      const uint32_t x = r.rem + static_cast<uint32_t>(j), ps = static_cast<uint32_t>(s.batch.page_size);
+      row = row < 0 ? -1 : row * ps + (s.batch.page_shift >= 0 ? x & (ps - 1) : x % ps);
+    }
+    const bool ok = (row >= 0) & (row < s.batch.rows) & (lane < KT) & (j < end);
+    if (__any(!ok & (j < end) & (lane < KT))) flag(s.batch.err, CB_ERROR_CACHE_ROW);
+    const uint32_t at = ok ? static_cast<uint32_t>(row) : 0u;
+    if (lane < KT) {
+      keys.off[t & 3][lane] = small ? at * stride : at;
+      keys.at[t & 3][lane] = hs.at(static_cast<int>(at));
+    }
+    const uint64_t valid = __ballot(ok);
+    if (lane < (KT + 31) / 32) keys.valid[t & 3][lane] = static_cast<uint32_t>(valid >> (32 * lane));
+  };
+  // The scales of a tile's keys, K's and then V's, 64 a step.
+  constexpr int SC = 2 * KT / kWave;
+  uint32_t byte[SC];
+  auto fetch_scales = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < SC; ++x) {
+      const int at = x * kWave + lane, value = at / KT;
+      byte[x] = (value ? hs.v : hs.k)[keys.at[t & 3][at % KT]];
+    }
+  };
+  auto keep_scales = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < SC; ++x) (&keys.scale[t & 3][0][0])[x * kWave + lane] = scale_value(byte[x], kMostRead<IO>);
   };
   int64_t entry = -1;
   if (wave == 0) {
@@ -548,64 +862,84 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_codes_ke
   }
   const int64_t off = static_cast<int64_t>(head) * s.head_dim;
   gcptr kbase = layer_base(s.cache, 0, s.layer) + off, vbase = layer_base(s.cache, 1, s.layer) + off;
-  gcptr zero = as_global(static_cast<const void*>(g_zeros));
-  const uint32_t stride = static_cast<uint32_t>(s.batch.row_stride_b);
-  // Instruction u of a tile: chunk lane % C of key (u % kHalf) * (64 / C) + lane / C, V from kHalf on.
-  const HeadScales hs(cache.scales, s.layer, head);
-  uint32_t scale[M];
+  // DMA instruction u of a tile, M a wave: chunk lane % C of key (u % kHalf) * (64 / C) + lane / C, V from kHalf on.
+  const int chunk = min(lane % C, s.head_dim / 16 - 1) * 16;
   auto ask = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      const int u = wave * M + m, value = u >= kHalf, k = (u - value * kHalf) * (kWave / C) + lane / C, c = lane % C;
-      const uint32_t row = static_cast<uint32_t>(tile_rows.row[t & 3][k]);
-      const bool ok = ((tile_rows.valid[t & 3][k >> 5] >> (k & 31)) & 1) & (c * 16 < s.head_dim);
-      gcptr at = (value ? vbase : kbase) + static_cast<uint64_t>(row) * stride + c * 16;
-      scale[m] = (value ? hs.v : hs.k)[hs.at(row)];
-      dma16(ok ? at : zero, lds_codes + m * 1024);
+      const int u = wave * M + m, value = u >= kHalf, k = (u - value * kHalf) * (kWave / C) + lane / C;
+      const uint32_t at = keys.off[t & 3][k];
+      gcptr base = value ? vbase : kbase;
+      if (small) dma16_at(base, at + chunk, lds_codes + m * 1024);
+      else dma16(base + static_cast<uint64_t>(at) * stride + chunk, lds_codes + m * 1024);
     }
   };
-  // This wave's codes of a tile, widened to the buffer at `to`.
-  auto put = [&](uint32_t to, int next) __attribute__((always_inline)) {
-    u32x4 x[M];
-    float by[M];
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-      x[m] = *lds_at<const u32x4>(lds_codes + m * 1024 + lane * 16);
-      by[m] = scale_value(scale[m], kMostRead<IO>);
-    }
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // the codes are read: others may come
+  // This wave's codes of a tile, read before the barrier that the tile's turn begins with.
+  u32x4 x[M];
+  auto take = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(wait_vm(0));
     asm volatile("" ::: "memory");
-    if (next < t1) ask(next);
+#pragma unroll
+    for (int m = 0; m < M; ++m) x[m] = *lds_at<const u32x4>(lds_codes + m * 1024 + lane * 16);
+  };
+  // Asks for the next tile's, then widens the taken ones, of tile t, to the buffer at `to`.
+  auto put = [&](uint32_t to, int t) __attribute__((always_inline)) {
+    if (t + 1 < t1) ask(t + 1);
+    uint32_t every = ~0u;
+#pragma unroll
+    for (int k = 0; k < KT / 32; ++k) every &= keys.valid[t & 3][k];
+    const bool plain = (uniform(static_cast<int>(every)) == -1) & (s.head_dim == DP);
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      const int u = wave * M + m, value = u >= kHalf, k = (u - value * kHalf) * (kWave / C) + lane / C, c = 2 * (lane % C);
+      const int u = wave * M + m, value = u >= kHalf, k = (u - value * kHalf) * (kWave / C) + lane / C;
+      if (!plain) {
+        const bool there = ((keys.valid[t & 3][k >> 5] >> (k & 31)) & 1) & (lane % C * 16 < s.head_dim);
+        x[m] = there ? x[m] : u32x4{0, 0, 0, 0};
+      }
       u32x4 lo, hi;
-      widen<IO>(x[m], by[m], lo, hi);
-      const int swizzle = value ? swizzle_v<DP>(k) : swizzle_k<DP>(k);
-      const uint32_t row = to + value * kTile + k * DP * 2;
-      *lds_at<u32x4>(row + (c ^ swizzle) * 16) = lo;
-      *lds_at<u32x4>(row + ((c + 1) ^ swizzle) * 16) = hi;
+      widen<IO>(x[m], keys.scale[t & 3][value][k], lo, hi);
+      // Chunk 2 c of the widened row, and the one after: neighbours, as the swizzles leave the lowest bit or flip it for both.
+      int swizzle = swizzle_k<DP>(k);
+      if (value) {
+        if constexpr (RB == 32) swizzle = swizzle_v<DP>(k);
+        else swizzle = Block::place_v(k);
+      }
+      const uint32_t at = to + value * kTile + k * DP * 2 + ((2 * (lane % C)) ^ swizzle) * 16;
+      *lds_at<u32x4>(at) = lo;
+      *lds_at<u32x4>(at ^ 16) = hi;
     }
   };
   __syncthreads();
+  if (wave == 1 && t0 < t1) {
+    fetch_scales(t0);
+    keep_scales(t0);
+    if (t0 + 1 < t1) {
+      fetch_scales(t0 + 1);
+      keep_scales(t0 + 1);
+    }
+  }
   if (t0 < t1) {
     ask(t0);
-    __builtin_amdgcn_s_waitcnt(kWaitAll);
-    asm volatile("" ::: "memory");
-    put(lds, t0 + 1);
+    take();
+  }
+  wait_and_meet();
+  if (t0 < t1) {
+    put(lds, t0);
+    if (t0 + 1 < t1) take();
   }
   uint32_t buf = 0;
   for (int t = t0; t < t1; ++t) {
-    wait_and_meet();  // tile t is written, and this wave's codes of the next one are there
-    if (t + 1 < t1) put(lds + (buf ^ (2 * kTile)), t + 2);
+    wait_and_meet();  // tile t is written, and this wave's codes of the next one are taken
+    if (t + 1 < t1) put(lds + (buf ^ (2 * kTile)), t + 1);
     if (wave == 0) {
       place(entry, t + 3);
       entry = entry_of(t + 4);
     }
+    if (wave == 1 && t + 2 < t1) fetch_scales(t + 2);
     const int start = tile_start<KT>(kr, t), end = tile_end(kr, t);
     uint32_t valid[KT / 32], every = ~0u;
 #pragma unroll
-    for (int k = 0; k < KT / 32; ++k) every &= valid[k] = tile_rows.valid[t & 3][k];
+    for (int k = 0; k < KT / 32; ++k) every &= valid[k] = keys.valid[t & 3][k];
     const bool all = sees_all(s, kr, start, min(end, start + KT));
     const bool whole = all && __builtin_amdgcn_readfirstlane(every) == ~0u;
     if (!all) {
@@ -617,8 +951,11 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_codes_ke
       if (strange) odd[0] = odd[1] = 1;
       __syncthreads();
       if (odd[0]) {
-        mark_not_finite<IO, DP, KT>(lds + buf + kTile, kr.np, s.causal ? blk.p : 0x7fffffff, s.window > 0 ? blk.p - s.window : -1,
-                                    start, end, (CB_LDS_SPACE uint32_t*)marks[0][wave], (CB_LDS_SPACE uint32_t*)marks[1][wave]);
+        if constexpr (RB == 32)
+          mark_not_finite<IO, DP, KT>(lds + buf + kTile, kr.np, s.causal ? blk.p : 0x7fffffff, s.window > 0 ? blk.p - s.window : -1,
+                                      start, end, (CB_LDS_SPACE uint32_t*)marks[0][wave], (CB_LDS_SPACE uint32_t*)marks[1][wave]);
+        else
+          blk.mark_nan(lds + buf + kTile, s, kr.np, start, end, (CB_LDS_SPACE uint32_t*)marks[0][wave]);
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < N; ++u) {
@@ -629,18 +966,34 @@ __global__ __launch_bounds__(NW * kWave, DP == 256 ? 1 : 2) void attend_codes_ke
         __syncthreads();
       }
     }
-    f32x16 st[KT / 32];
-    u32x4 w[KT / 32][2];
-    const typename Block::Lanes at = Block::place(lanes, lds + buf, lds + buf + kTile);
-    blk.products(at, st);
-    blk.ready(s, kr, st, start, whole, valid);
-    typename Block::Values v = Block::first_values(at);
-    blk.weights(st, scale2, w);
-    blk.add_values(at, w, v);
+    const uint32_t lk = lds + buf, lv = lk + kTile;
+    if constexpr (RB == 32) {
+      f32x16 st[KT / 32];
+      u32x4 w[KT / 32][2];
+      const typename Block::Lanes at = Block::place(lanes, lk, lv);
+      blk.products(at, st);
+      blk.ready(s, kr, st, start, whole, valid);
+      typename Block::Values v = Block::first_values(at);
+      blk.weights(st, scale2, w);
+      blk.add_values(at, w, v);
+    } else {
+      f32x8 st[KT / 32];
+      u32x4 w[KT / 32];
+      blk.products(lanes, lk, st);
+      blk.ready(s, kr, st, start, whole, valid);
+      typename Block::Values v = Block::first_values(lanes, lv);
+      blk.weights(st, scale2, w);
+      blk.add_values(lanes, lv, w, v);
+    }
+    if (wave == 1 && t + 2 < t1) keep_scales(t + 2);
+    if (t + 2 < t1) take();
     buf ^= 2 * kTile;
   }
   __syncthreads();
-  if (odd[1]) blk.add_marks(marks[0][wave], marks[1][wave]);
+  if (odd[1]) {
+    if constexpr (RB == 32) blk.add_marks(marks[0][wave], marks[1][wave]);
+    else blk.add_marks(marks[0][wave]);
+  }
   blk.finish(late_args(), r, split, vector);
 }
 
@@ -656,17 +1009,6 @@ __device__ inline int swizzle_code_v(int key) {
   return DP == 64    ? ((key >> 2) & 1) | ((key >> 3) & 2)
          : DP == 128 ? ((key >> 1) & 3) | ((key >> 2) & 4)
                      : (key & 7) | ((key >> 1) & 8);
-}
-
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-
-template <typename IO>
-CB_INLINE f32x4 mul16(u32x4 a, u32x4 b, f32x4 c) {
-  typedef typename Half<IO>::x8 x8;
-  if constexpr (std::is_same_v<IO, io_bf16>)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
 }
 
 // NB times 16 query rows of one wave over tiles of 32 keys held as codes, with
@@ -1110,8 +1452,8 @@ void launch_codes(const AttendArgs& a, const ScaledCache& cache, const AttendSha
   const int vector = aligned16(a.s.q) && aligned16(a.out);
   if (h.step && h.rows_per_tile == 16) hipLaunchKernelGGL((step_codes_kernel<IO, DP, 1, MOD>), dim3(grid), dim3(kCodeWaves * kWave), 0, st, a, cache, vector);
   else if (h.step) hipLaunchKernelGGL((step_codes_kernel<IO, DP, 2, MOD>), dim3(grid), dim3(kCodeWaves * kWave), 0, st, a, cache, vector);
-  else if (DP <= 128 && h.waves == 8) hipLaunchKernelGGL((attend_codes_kernel<IO, DP, KT, DP <= 128 ? 8 : 4, MOD>), dim3(grid), dim3(8 * kWave), 0, st, a, cache, vector);
-  else hipLaunchKernelGGL((attend_codes_kernel<IO, DP, KT, 4, MOD>), dim3(grid), dim3(4 * kWave), 0, st, a, cache, vector);
+  else if (DP <= 128 && h.rows_per_tile == 32 * kTileWaves) hipLaunchKernelGGL((attend_codes_kernel<IO, DP, KT, DP <= 128 ? 32 : 16, MOD>), dim3(grid), dim3(kTileWaves * kWave), 0, st, a, cache, vector);
+  else hipLaunchKernelGGL((attend_codes_kernel<IO, DP, KT, 16, MOD>), dim3(grid), dim3(kTileWaves * kWave), 0, st, a, cache, vector);
   if (h.step) launch_join<IO, 32>(a, h, st);
   else launch_join<IO, KT>(a, h, st);
 }
@@ -1263,7 +1605,7 @@ int cb_quantized_attention(const cb_query_batch* batch, const cb_page_scales* sc
   if (n == 0 || batch->num_requests == 0) return CB_OK;
   const AttendShape h = quantized_shape(a.s, dtype, *scores);
   unsigned grid;
-  if ((rc = cut_attention(a, h, (h.step ? kCodeWaves : h.waves) * kWave, lse, d_workspace, workspace_bytes, &grid))) return rc;
+  if ((rc = cut_attention(a, h, (h.step ? kCodeWaves : h.half ? kTileWaves : kAnyWaves) * kWave, lse, d_workspace, workspace_bytes, &grid))) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == CB_DTYPE_BF16) launch_quantized<io_bf16>(a, cache, h, grid, st);
   else if (dtype == CB_DTYPE_F16) launch_quantized<io_f16>(a, cache, h, grid, st);
