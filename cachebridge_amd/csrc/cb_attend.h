@@ -596,30 +596,36 @@ __global__ __launch_bounds__(256) void join_few_kernel(AttendArgs a, int rows_pe
   total = __shfl(total, 0);
   const int D = s.head_dim, d0 = lane * E;
   float o[E] = {};
+  // U splits from z0 on: all their loads before any is used, past the last one the last again.
+  auto add = [&](auto ahead, int z0) __attribute__((always_inline)) {
+    constexpr int U = decltype(ahead)::value;
+    float x[U][E];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float* from = a.part_out + (min(z0 + u, n - 1) * step + at) * D + d0;
+      if (D % E == 0) {
+        const vec y = *reinterpret_cast<const vec*>(from);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = y[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = from[min(e, D - 1 - d0)];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      // Read from lanes that may hold no element and are off here. A weight of zero takes nothing, NaN included.
+      const float f = z0 + u < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), z0 + u)) : 0.0f;
+      if (f == 0.0f) continue;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] += f * x[u][e];
+    }
+  };
   if (d0 < D) {
-    constexpr int U = 4;  // splits in flight
-    for (int z0 = 0; z0 < n; z0 += U) {
-      float x[U][E];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float* from = a.part_out + (min(z0 + u, n - 1) * step + at) * D + d0;
-        if (D % E == 0) {
-          const vec y = *reinterpret_cast<const vec*>(from);
-#pragma unroll
-          for (int e = 0; e < E; ++e) x[u][e] = y[e];
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e) x[u][e] = from[min(e, D - 1 - d0)];
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        // Read from lanes that may hold no element and are off here. A weight of zero takes nothing, NaN included.
-        const float f = z0 + u < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), z0 + u)) : 0.0f;
-        if (f == 0.0f) continue;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += f * x[u][e];
-      }
+    if (n <= 2) {
+      for (int z = 0; z < n; ++z) add(std::integral_constant<int, 1>{}, z);
+    } else {
+      for (int z = 0; z < n; z += 4) add(std::integral_constant<int, 4>{}, z);
     }
   }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
@@ -666,8 +672,9 @@ __global__ __launch_bounds__(kJoinThreads) void join_splits_kernel(AttendArgs a,
   const int D = s.head_dim;
   f32x4 o = {0, 0, 0, 0};
   const bool vector = D % 4 == 0;
-  constexpr int U = 8;  // splits in flight
-  for (int z0 = g; z0 < n; z0 += U * GROUPS) {
+  // U splits of this group's from z0 on, as in join_few_kernel.
+  auto add = [&](auto ahead, int z0) __attribute__((always_inline)) {
+    constexpr int U = decltype(ahead)::value;
     f32x4 part[U];
     float w[U];
 #pragma unroll
@@ -685,8 +692,13 @@ __global__ __launch_bounds__(kJoinThreads) void join_splits_kernel(AttendArgs a,
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       w[u] = z0 + u * GROUPS < n ? exp2_fast(w[u] - mu) : 0.0f;
-      o += w[u] == 0.0f ? f32x4{0, 0, 0, 0} : w[u] * part[u];  // a weight of zero takes nothing, NaN included
+      o += w[u] == 0.0f ? f32x4{0, 0, 0, 0} : w[u] * part[u];
     }
+  };
+  if (n <= 2 * GROUPS) {
+    for (int z = g; z < n; z += GROUPS) add(std::integral_constant<int, 1>{}, z);
+  } else {
+    for (int z = g; z < n; z += 8 * GROUPS) add(std::integral_constant<int, 8>{}, z);
   }
   sums[g][x] = o;
   __syncthreads();
@@ -1306,7 +1318,8 @@ constexpr int kStepGroups = 512, kStepGroupsRagged = 1024;
 constexpr int kStepWaves = 2;
 
 // half: the kernels of 16-bit products take the call.
-AttendShape attend_shape(const ScoreArgs& s, bool half, int step_tiles = kStepTiles) {
+// half_tiles: key tiles that a split of theirs has at least.
+AttendShape attend_shape(const ScoreArgs& s, bool half, int half_tiles = 8, int step_tiles = kStepTiles) {
   AttendShape h{};
   h.half = half;
   const QBatch& B = s.batch;
@@ -1327,7 +1340,7 @@ AttendShape attend_shape(const ScoreArgs& s, bool half, int step_tiles = kStepTi
   const int key_tiles = std::max(1, ceil_div(keys, h.keys_per_tile) + (s.prefix ? 1 : 0));
   const int64_t groups = h.tile_slots * s.kv_heads;
   const int64_t target = !h.step ? kTargetGroups * 4 / h.waves : B.requests > 1 ? kStepGroupsRagged : kStepGroups;
-  h.least_tiles = h.half ? 8 : 2;
+  h.least_tiles = h.half ? half_tiles : 2;
   h.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(target / std::max<int64_t>(1, groups), key_tiles / h.least_tiles)));
   if (h.step) {
     // Parts of one size for all requests, cut by the bound: their workgroups end

@@ -141,11 +141,49 @@ CB_INLINE void turn_pairs(const float (&x)[2 * V], const PAIR* turn, bool interl
 // is read once and written once.
 // KV: K and V rows go into the cache as they are, else queries alone are written.
 // WHOLE: requests that do not start at a page's first slot are outside the bounds.
+// What a wave reads of q, k and v depends on its token row alone: the loads are on
+// their way while the row's request, place and cache row are looked up.
 template <typename IO, int V, int U, bool KV, bool WHOLE>
 CB_INLINE void install_rows(const InstallArgs& a, int64_t unit, turn_pair<IO>* turn) {
   const int lane = threadIdx.x & (kWave - 1);
   const int t = static_cast<int>(unit / a.slices), slice = static_cast<int>(unit % a.slices);
   if (t >= a.batch.tokens) return;
+  const int pairs = a.rotary_dim / 2, kv_heads = KV ? a.kv_heads : 0;
+  const InstallItems n = install_items(a.head_dim, a.rotary_dim, V);
+  const int turned = (a.q_heads + kv_heads) * n.head, total = turned + kv_heads * n.value;
+  const int per = (total + a.slices - 1) / a.slices;
+  const int stop = min(total, (slice + 1) * per);
+  constexpr int E = sizeof(IO);
+  struct Item {
+    int head, oa, ob, first;  // of q's heads, then k's, then v's; the two vectors; the first pair, or -1
+    bool on, two;
+  } item[U];
+  float x[U][2 * V];
+  auto load = [&](int idx) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      Item& m = item[u];
+      const int at = min(idx + u * kWave, stop - 1);
+      m.on = idx + u * kWave < stop;
+      const bool value = KV && at >= turned;
+      const int of = value ? (at - turned) / n.value : at / n.head;
+      const int k = value ? at - turned - of * n.value : at - of * n.head;
+      m.head = value ? a.q_heads + kv_heads + of : of;
+      m.first = !value && k < n.turned ? k * V : -1;
+      const int straight = value ? 0 : a.rotary_dim, plain = straight + 2 * (k - (value ? 0 : n.turned)) * V;
+      m.oa = m.first < 0 ? plain : a.interleaved ? 2 * m.first : m.first;
+      m.ob = m.first < 0 ? plain + V : a.interleaved ? m.oa + V : m.first + pairs;
+      m.two = m.first >= 0 || plain + V < a.head_dim;
+      const Strided& from = m.head < a.q_heads ? a.q : value ? a.v : a.k;
+      const char* src = from.data + t * from.token_b + (value || m.head >= a.q_heads ? m.head - a.q_heads - (value ? kv_heads : 0) : m.head) * from.head_b;
+      if (m.on) {
+        load_vec<IO, V>(src + m.oa * E, x[u]);
+        if (m.two) load_vec<IO, V>(src + m.ob * E, x[u] + V);
+      }
+    }
+  };
+  const int first = slice * per + lane;
+  if (first < stop) load(first);
   const int b = request_of_token(a.batch, t);
   if (b >= a.batch.requests) return;
   const Request r = load_request(a.batch, b);
@@ -156,61 +194,26 @@ CB_INLINE void install_rows(const InstallArgs& a, int64_t unit, turn_pair<IO>* t
     row = cache_row(a.batch, r, p);
     if (row < 0 && lane == 0) flag(a.batch.err, CB_ERROR_TARGET_ROW);
   }
-  const int pairs = a.rotary_dim / 2, kv_heads = KV ? a.kv_heads : 0;
   for (int i = lane; i < pairs; i += kWave) turn[i] = turn_of<turn_pair<IO>, turn_t<IO>>(a, t, p, i);
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
-  const InstallItems n = install_items(a.head_dim, a.rotary_dim, V);
-  const int turned = (a.q_heads + kv_heads) * n.head, total = turned + kv_heads * n.value;
-  const int per = (total + a.slices - 1) / a.slices;
-  const int stop = min(total, (slice + 1) * per);
   char* krow = const_cast<char*>((const char*)layer_base(a.cache, 0, a.layer)) + row * a.cache.row_stride_b;
   char* vrow = const_cast<char*>((const char*)layer_base(a.cache, 1, a.layer)) + row * a.cache.row_stride_b;
-  constexpr int E = sizeof(IO);
-  for (int idx = slice * per + lane; idx < stop; idx += U * kWave) {
-    const char* src[U];
-    char* dst[U];
-    int oa[U], ob[U], first[U];  // the vectors, and the first pair or -1
-    bool on[U], two[U];
-    float x[U][2 * V];
+  for (int idx = first; idx < stop; idx += U * kWave) {
+    if (idx != first) load(idx);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int at = min(idx + u * kWave, stop - 1);
-      on[u] = idx + u * kWave < stop;
-      const bool value = KV && at >= turned;
-      const int head = value ? (at - turned) / n.value : at / n.head;
-      const int item = value ? at - turned - head * n.value : at - head * n.head;
-      if (value) {
-        src[u] = a.v.data + t * a.v.token_b + head * a.v.head_b;
-        dst[u] = vrow + static_cast<int64_t>(head) * a.head_dim * E;
-        on[u] &= row >= 0;
-      } else if (head < a.q_heads) {
-        src[u] = a.q.data + t * a.q.token_b + head * a.q.head_b;
-        dst[u] = a.q_out.data + t * a.q_out.token_b + head * a.q_out.head_b;
-      } else {
-        src[u] = a.k.data + t * a.k.token_b + (head - a.q_heads) * a.k.head_b;
-        dst[u] = krow + static_cast<int64_t>(head - a.q_heads) * a.head_dim * E;
-        on[u] &= row >= 0;
-      }
-      first[u] = !value && item < n.turned ? item * V : -1;
-      const int straight = value ? 0 : a.rotary_dim, at2 = straight + 2 * (item - (value ? 0 : n.turned)) * V;
-      oa[u] = first[u] < 0 ? at2 : a.interleaved ? 2 * first[u] : first[u];
-      ob[u] = first[u] < 0 ? at2 + V : a.interleaved ? oa[u] + V : first[u] + pairs;
-      two[u] = first[u] >= 0 || at2 + V < a.head_dim;
-      if (on[u]) {
-        load_vec<IO, V>(src[u] + oa[u] * E, x[u]);
-        if (two[u]) load_vec<IO, V>(src[u] + ob[u] * E, x[u] + V);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (!on[u]) continue;
+      const Item& m = item[u];
+      const bool query = m.head < a.q_heads, value = m.head >= a.q_heads + kv_heads;
+      if (!m.on || (!query && row < 0)) continue;
+      char* dst = query ? a.q_out.data + t * a.q_out.token_b + m.head * a.q_out.head_b
+                        : (value ? vrow : krow) + static_cast<int64_t>(m.head - a.q_heads - (value ? kv_heads : 0)) * a.head_dim * E;
       float y[2 * V];
 #pragma unroll
       for (int i = 0; i < 2 * V; ++i) y[i] = x[u][i];
-      if (first[u] >= 0) turn_pairs<V>(x[u], turn + first[u], a.interleaved, y);
-      store_vec<IO, V>(dst[u] + oa[u] * E, y);
-      if (two[u]) store_vec<IO, V>(dst[u] + ob[u] * E, y + V);
+      if (m.first >= 0) turn_pairs<V>(x[u], turn + m.first, a.interleaved, y);
+      store_vec<IO, V>(dst + m.oa * E, y);
+      if (m.two) store_vec<IO, V>(dst + m.ob * E, y + V);
     }
   }
 }
