@@ -276,7 +276,7 @@ constexpr int kTurns = V == 8 ? 512 : kMaxPairs;  // pairs that 64 items turn, a
 // registers until the page's scale is known, more are read (and turned) twice.
 template <typename IO, int V, int TW, int KEEP>
 CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t, int head, int kind, turn_pair<IO>* turn) {
-  __shared__ float tops[kInstallWaves];
+  __shared__ float tops[TW];
   const InstallArgs& a = q.i;
   const int lane = threadIdx.x & (kWave - 1), wave = TW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) : 0;
   const int member = wave * kWave + lane;
@@ -397,9 +397,12 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t
 // (install_rows). Pages are counted by request; where the bound on a request's new
 // tokens leaves more of them than there are tokens, a team goes by a token and
 // works if it is its page's first new one.
+constexpr int kTeamWaves = 8;
+
 template <typename IO, int V, int TW>
-__global__ __launch_bounds__(kInstallWaves * kWave) void install_quantized_kernel(InstallQuantizedArgs q) {
-  __shared__ turn_pair<IO> turn[kInstallWaves][kTurns<V>];
+__global__ __launch_bounds__((TW > 1 ? TW : kInstallWaves) * kWave) void install_quantized_kernel(InstallQuantizedArgs q) {
+  constexpr int W = TW > 1 ? TW : kInstallWaves;
+  __shared__ turn_pair<IO> turn[W][kTurns<V>];
   const InstallArgs& a = q.i;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   if (blockIdx.x >= q.page_groups) {
@@ -407,10 +410,10 @@ __global__ __launch_bounds__(kInstallWaves * kWave) void install_quantized_kerne
       if (wave == 0) flag_requests(a.batch);
       return;
     }
-    install_rows<IO, V, 1, false, true>(a, static_cast<int64_t>(blockIdx.x - q.page_groups) * kInstallWaves + wave, turn[wave]);
+    install_rows<IO, V, 1, false, true>(a, static_cast<int64_t>(blockIdx.x - q.page_groups) * W + wave, turn[wave]);
     return;
   }
-  const int64_t unit = TW > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kInstallWaves + wave;
+  const int64_t unit = TW > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * W + wave;
   const int64_t place = unit / (2 * a.kv_heads);
   const int rest = static_cast<int>(unit - place * 2 * a.kv_heads), ps = q.scales.page_size;
   int t;
@@ -434,7 +437,7 @@ __global__ __launch_bounds__(kInstallWaves * kWave) void install_quantized_kerne
     flag(a.batch.err, CB_ERROR_REQUEST);
     return;
   }
-  store_page<IO, V, TW, (TW > 1 ? 4 : 2)>(q, r, t, rest >> 1, rest & 1, turn[wave]);
+  store_page<IO, V, TW, 2>(q, r, t, rest >> 1, rest & 1, turn[wave]);
 }
 
 // ---------------------------------------------------------------------------
@@ -1496,9 +1499,9 @@ void launch_quantized(const AttendArgs& a, const ScaledCache& cache, const Atten
 template <typename IO>
 void launch_store(const InstallQuantizedArgs& q, bool wide, bool teams, unsigned grid, hipStream_t st) {
   constexpr int V = 16 / sizeof(IO);
-  if (wide && teams) hipLaunchKernelGGL((install_quantized_kernel<IO, V, kInstallWaves>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, q);
+  if (wide && teams) hipLaunchKernelGGL((install_quantized_kernel<IO, V, kTeamWaves>), dim3(grid), dim3(kTeamWaves * kWave), 0, st, q);
   else if (wide) hipLaunchKernelGGL((install_quantized_kernel<IO, V, 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, q);
-  else if (teams) hipLaunchKernelGGL((install_quantized_kernel<IO, 1, kInstallWaves>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, q);
+  else if (teams) hipLaunchKernelGGL((install_quantized_kernel<IO, 1, kTeamWaves>), dim3(grid), dim3(kTeamWaves * kWave), 0, st, q);
   else hipLaunchKernelGGL((install_quantized_kernel<IO, 1, 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, q);
 }
 
@@ -1540,9 +1543,10 @@ int cb_install_quantized(const cb_query_batch* batch, const cb_page_scales* scal
   a.page_slots = slots * batch->num_requests <= n ? static_cast<int32_t>(slots) : 0;
   const int64_t places = a.page_slots ? slots * batch->num_requests : n;
   const bool teams = std::min(ps, most) * std::max(each.head, each.value) > 2 * kWave;
-  const int64_t units = places * 2 * a.i.kv_heads, pages = teams ? units : (units + kInstallWaves - 1) / kInstallWaves;
-  const int64_t grid = pages + (static_cast<int64_t>(n) * a.i.slices + kInstallWaves - 1) / kInstallWaves + (d_error_flag ? 1 : 0);
-  if (!launch_fits(grid, kInstallWaves * kWave)) return fail(CB_EINVAL, "too many tokens");
+  const int waves = teams ? kTeamWaves : kInstallWaves;
+  const int64_t units = places * 2 * a.i.kv_heads, pages = teams ? units : (units + waves - 1) / waves;
+  const int64_t grid = pages + (static_cast<int64_t>(n) * a.i.slices + waves - 1) / waves + (d_error_flag ? 1 : 0);
+  if (!launch_fits(grid, waves * kWave)) return fail(CB_EINVAL, "too many tokens");
   a.page_groups = static_cast<uint32_t>(pages);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == CB_DTYPE_BF16) launch_store<io_bf16>(a, wide, teams, static_cast<unsigned>(grid), st);

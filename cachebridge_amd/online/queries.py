@@ -156,6 +156,7 @@ class QueryBatch:
         self.dtype = rows.dtype if rows.scales is None else rows.scales.dtype
         self._code = io_dtype_code(self.dtype)
         self._keep = (query_start, lengths, offsets)
+        self._by_tokens = {}
 
     @property
     def kv_heads(self) -> int:
@@ -167,13 +168,24 @@ class QueryBatch:
         return layer
 
     def _tokens(self, n: int):
-        """The C description for token tensors of ``n`` rows (a copy: calls may run side by side)."""
-        c = _lib.CbQueryBatch.from_buffer_copy(self.c)
-        c.num_tokens = n
-        c.max_query = n if self.max_query is None else min(self.max_query, n)
-        return ctypes.byref(c)
+        """The C description for token tensors of ``n`` rows (one for each ``n``, not written again: calls may run
+        side by side)."""
+        ref = self._by_tokens.get(n)
+        if ref is None:
+            c = _lib.CbQueryBatch.from_buffer_copy(self.c)
+            c.num_tokens = n
+            c.max_query = n if self.max_query is None else min(self.max_query, n)
+            if len(self._by_tokens) >= 64:
+                self._by_tokens = {}
+            ref = self._by_tokens[n] = ctypes.byref(c)
+        return ref
 
     def _heads(self, t: torch.Tensor, name: str, tokens: int | None = None, heads: int | None = None) -> _lib.CbHeads:
+        data, token_stride, head_stride, h = self._row(t, name, tokens, heads)
+        return _lib.CbHeads(data, token_stride, head_stride, h, 0)
+
+    def _row(self, t: torch.Tensor, name: str, tokens: int | None = None, heads: int | None = None):
+        """A token tensor's address, token and head stride and heads, checked: the words of a ``cb_heads``."""
         shape = t.shape
         if len(shape) != 3 or t.dtype != self.dtype or t.device != self.device:
             raise ValueError(f"{name} must be [tokens, heads, head_dim] of {self.dtype} on {self.device}")
@@ -185,7 +197,11 @@ class QueryBatch:
         st, sh, sd = t.stride()
         if sd != 1 and d > 1:
             raise ValueError(f"{name} must be contiguous in its last dimension")
-        return _lib.CbHeads(t.data_ptr(), st, sh, h, 0)
+        return t.data_ptr(), st, sh, h
+
+
+# The cb_heads of q, out, k and v, four words each (the last one heads, its upper half reserved).
+_FourHeads = ctypes.c_int64 * 16
 
 
 class Rotary(NamedTuple):
@@ -263,17 +279,17 @@ def install_tokens(batch: QueryBatch, layer: int, q: torch.Tensor, k: torch.Tens
     page size, and requests that start at a page's first slot.
     """
     n, heads, dim = q.shape if q.ndim == 3 else (0, 0, 0)
-    cq = batch._heads(q, "q")
-    ck = batch._heads(k, "k", n, batch.kv_heads)
-    cv = batch._heads(v, "v", n, batch.kv_heads)
+    rq = batch._row(q, "q")
+    rk = batch._row(k, "k", n, batch.kv_heads)
+    rv = batch._row(v, "v", n, batch.kv_heads)
     turn = _rotation(batch, rotary, positions, n)
     flag = _flag_pointer(batch, error_flag)
     with _On(batch, stream) as handle:
         if out is None:
             out = q.new_empty((n, heads, dim))
-        co = batch._heads(out, "out", n, heads)
-        how = (batch._layer(layer), batch._code, dim, ctypes.byref(cq), ctypes.byref(co), ctypes.byref(ck),
-               ctypes.byref(cv), ctypes.byref(turn), flag, handle)
+        rows = _FourHeads(*rq, *batch._row(out, "out", n, heads), *rk, *rv)
+        at = ctypes.addressof(rows)
+        how = (batch._layer(layer), batch._code, dim, at, at + 32, at + 64, at + 96, ctypes.byref(turn), flag, handle)
         lib = _lib.load()
         if batch.scales is None:
             _lib.check(lib.cb_install_rotated(batch._tokens(n), *how))

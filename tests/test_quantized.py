@@ -37,10 +37,14 @@ def rotation(**kw):
     return r
 
 
+def at(x):
+    return None if x is None else ctypes.addressof(x)
+
+
 def install(lib, b=None, s=None, layer=0, dtype=BF16, dim=128, q=None, out=None, k=None, v=None, turn=None):
+    q, out, k, v = heads() if q is None else q, heads() if out is None else out, heads(2) if k is None else k, heads(2) if v is None else v
     return lib.cb_install_quantized(ref(paged() if b is None else b), ref(scale_pages() if s is None else s), layer, dtype, dim,
-                                    ref(heads() if q is None else q), ref(heads() if out is None else out),
-                                    ref(heads(2) if k is None else k), ref(heads(2) if v is None else v),
+                                    at(q), at(out), at(k), at(v),
                                     ref(rotation() if turn is None else turn), None, None)
 
 
@@ -79,8 +83,9 @@ def test_install_refusals(lib, kw, text):  # noqa: F811
 
 def test_rotated_install_refusals(lib):  # noqa: F811
     def call(turn, b=None):
-        return lib.cb_install_rotated(ref(batch(request_stride=100) if b is None else b), 0, BF16, 128, ref(heads()), ref(heads()), ref(heads(2)),
-                                      ref(heads(2)), ref(turn), None, None)
+        many, kv = heads(), heads(2)
+        return lib.cb_install_rotated(ref(batch(request_stride=100) if b is None else b), 0, BF16, 128, at(many), at(many), at(kv),
+                                      at(kv), ref(turn), None, None)
     refused(lib, call(None), "null rotation")
     refused(lib, call(rotation(pair_axis=b"\1" * 64, axes=1)), "axis 1 of 1")
     refused(lib, call(rotation(), batch(request_stride=0)), "request_stride")
