@@ -224,13 +224,12 @@ SIGNATURES = {
         [_i32, _i64, _i32, _i32, _i32, _i32, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64,
          _c_void_p, _i64, _c_void_p],
     ),
+    # Token tensors of the three installs as addresses: the four of a call lie in one array.
     "cb_install_tokens": (
         ctypes.c_int,
-        [ctypes.POINTER(CbQueryBatch), _i32, _i32, _i32, ctypes.POINTER(CbHeads), ctypes.POINTER(CbHeads),
-         ctypes.POINTER(CbHeads), ctypes.POINTER(CbHeads), _c_void_p, _i32, _i32, ctypes.c_float, _c_void_p,
-         _i32, _c_void_p, _c_void_p],
+        [ctypes.POINTER(CbQueryBatch), _i32, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32,
+         _i32, ctypes.c_float, _c_void_p, _i32, _c_void_p, _c_void_p],
     ),
-    # Token tensors as addresses: the four of a call lie in one array.
     "cb_install_rotated": (
         ctypes.c_int,
         [ctypes.POINTER(CbQueryBatch), _i32, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p,

@@ -152,8 +152,11 @@ class QueryBatch:
         self.max_length = int(max_length)
         self.device = rows.device
         self.scales = rows.c_scales
-        self._scales = None if self.scales is None else ctypes.byref(self.scales)
-        self.dtype = rows.dtype if rows.scales is None else rows.scales.dtype
+        if rows.c_scales is None:
+            self.dtype = rows.dtype
+        else:
+            self.dtype = rows.scales.dtype
+            self._scales = ctypes.byref(rows.c_scales)
         self._code = io_dtype_code(self.dtype)
         self._keep = (query_start, lengths, offsets)
         self._by_tokens = {}
@@ -282,41 +285,51 @@ def install_tokens(batch: QueryBatch, layer: int, q: torch.Tensor, k: torch.Tens
     rq = batch._row(q, "q")
     rk = batch._row(k, "k", n, batch.kv_heads)
     rv = batch._row(v, "v", n, batch.kv_heads)
-    turn = _rotation(batch, rotary, positions, n)
+    inv = _device_vector(rotary.inv_freq, "inv_freq", (torch.float64,), batch.device, None)
+    pos, kind = _positions(batch, rotary, positions, n)
     flag = _flag_pointer(batch, error_flag)
     with _On(batch, stream) as handle:
         if out is None:
             out = q.new_empty((n, heads, dim))
         rows = _FourHeads(*rq, *batch._row(out, "out", n, heads), *rk, *rv)
         at = ctypes.addressof(rows)
-        how = (batch._layer(layer), batch._code, dim, at, at + 32, at + 64, at + 96, ctypes.byref(turn), flag, handle)
-        lib = _lib.load()
-        if batch.scales is None:
-            _lib.check(lib.cb_install_rotated(batch._tokens(n), *how))
+        lib, layer, code = _lib.load(), batch._layer(layer), batch._code
+        if batch.scales is None and rotary.axes is None:
+            _lib.check(lib.cb_install_tokens(
+                batch._tokens(n), layer, code, dim, at, at + 32, at + 64, at + 96, inv, 2 * rotary.inv_freq.numel(),
+                int(rotary.interleaved), rotary.magnitude, pos, kind, flag, handle))
         else:
-            _lib.check(lib.cb_install_quantized(batch._tokens(n), batch._scales, *how))
+            turn = ctypes.byref(_rotation(rotary, inv, pos, kind, n))
+            if batch.scales is None:
+                _lib.check(lib.cb_install_rotated(batch._tokens(n), layer, code, dim, at, at + 32, at + 64, at + 96,
+                                                  turn, flag, handle))
+            else:
+                _lib.check(lib.cb_install_quantized(batch._tokens(n), batch._scales, layer, code, dim, at, at + 32,
+                                                    at + 64, at + 96, turn, flag, handle))
         batch.rows.hold_for(stream)
     return out
 
 
-def _rotation(batch: QueryBatch, rotary: Rotary, positions: torch.Tensor | None, n: int) -> _lib.CbRotation:
-    inv, axes = rotary.inv_freq, rotary.axes
-    c = _lib.CbRotation(_device_vector(inv, "inv_freq", (torch.float64,), batch.device, None), None, None, n,
-                        2 * inv.numel(), int(rotary.interleaved), 0, 1, rotary.magnitude)
+def _positions(batch: QueryBatch, rotary: Rotary, positions: torch.Tensor | None, n: int):
+    """The positions' address and index kind, None and 0 without any; the rotation's axes checked."""
+    axes = rotary.axes
+    if axes is not None and (not isinstance(axes, bytes) or len(axes) != rotary.inv_freq.numel() or max(axes) > 7):
+        raise ValueError("axes must be bytes, 0 to 7, one for each pair of inv_freq")
+    if positions is None:
+        return None, 0
     if axes is not None:
-        if not isinstance(axes, bytes) or len(axes) != inv.numel() or max(axes) > 7:
-            raise ValueError("axes must be bytes, 0 to 7, one for each pair of inv_freq")
-        c.pair_axis, c.axes = axes, max(axes) + 1
-    if positions is not None:
-        if axes is not None:
-            if positions.ndim != 2 or positions.shape[0] < c.axes or positions.shape[1] != n:
-                raise ValueError("positions must be [axes, tokens] with one row for each of the rotation's axes")
-            # One row a axis is all that is read: the flat vector holds them one after another.
-            positions = positions.view(-1) if positions.is_contiguous() else positions
-        c.positions = _device_vector(positions, "positions", (torch.int32, torch.int64), batch.device,
-                                     n if axes is None else None)
-        c.positions_kind = _lib.CB_INDEX_I64 if positions.dtype == torch.int64 else _lib.CB_INDEX_I32
-    return c
+        if positions.ndim != 2 or positions.shape[0] <= max(axes) or positions.shape[1] != n:
+            raise ValueError("positions must be [axes, tokens] with one row for each of the rotation's axes")
+        # What is read is one row an axis; the flat vector holds them one after another.
+        positions = positions.view(-1) if positions.is_contiguous() else positions
+    at = _device_vector(positions, "positions", (torch.int32, torch.int64), batch.device, n if axes is None else None)
+    return at, _lib.CB_INDEX_I64 if positions.dtype == torch.int64 else _lib.CB_INDEX_I32
+
+
+def _rotation(rotary: Rotary, inv: int, pos: int | None, kind: int, n: int) -> _lib.CbRotation:
+    axes, dim, spin = rotary.axes, 2 * rotary.inv_freq.numel(), int(rotary.interleaved)
+    count = 1 if axes is None else max(axes) + 1
+    return _lib.CbRotation(inv, pos, axes, n, dim, spin, kind, count, rotary.magnitude)
 
 
 def _scores(batch: QueryBatch, heads: int, dim: int, scale, causal, window, cap, slopes, prefix_lengths):
