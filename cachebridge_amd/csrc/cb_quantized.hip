@@ -274,8 +274,8 @@ constexpr int kTurns = V == 8 ? 512 : kMaxPairs;  // pairs that 64 items turn, a
 // elements (both vectors of V pairs, or two neighbours) lie one a lane in rounds
 // of whole rows, which the waves take in turn; up to KEEP rounds of a wave stay in
 // registers until the page's scale is known, more are read (and turned) twice.
-template <typename IO, int V, int TW, int KEEP>
-CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t, int head, int kind, turn_pair<IO>* turn) {
+template <typename IO, int V, int TW, int KEEP, typename AXES>
+CB_INLINE void store_page(const InstallQuantizedArgs& q, const AXES& axes, const Request& r, int t, int head, int kind, turn_pair<IO>* turn) {
   __shared__ float tops[TW];
   const InstallArgs& a = q.i;
   const int lane = threadIdx.x & (kWave - 1), wave = TW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) : 0;
@@ -321,7 +321,7 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t
       const int all = min(per_round, rows - row0) * pairs;
       for (int x = lane; x < all; x += kWave) {
         const int at = row0 + x / pairs;
-        turn[x] = turn_of<turn_pair<IO>, turn_t<IO>>(a, t + at, p0 + at, x % pairs);
+        turn[x] = turn_of<turn_pair<IO>, turn_t<IO>>(a, axes, t + at, p0 + at, x % pairs);
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -399,8 +399,8 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const Request& r, int t
 // works if it is its page's first new one.
 constexpr int kTeamWaves = 8;
 
-template <typename IO, int V, int TW>
-__global__ __launch_bounds__((TW > 1 ? TW : kInstallWaves) * kWave) void install_quantized_kernel(InstallQuantizedArgs q) {
+template <typename IO, int V, int TW, typename AXES>
+__global__ __launch_bounds__((TW > 1 ? TW : kInstallWaves) * kWave) void install_quantized_kernel(InstallQuantizedArgs q, AXES axes) {
   constexpr int W = TW > 1 ? TW : kInstallWaves;
   __shared__ turn_pair<IO> turn[W][kTurns<V>];
   const InstallArgs& a = q.i;
@@ -410,7 +410,7 @@ __global__ __launch_bounds__((TW > 1 ? TW : kInstallWaves) * kWave) void install
       if (wave == 0) flag_requests(a.batch);
       return;
     }
-    install_rows<IO, V, 1, false, true>(a, static_cast<int64_t>(blockIdx.x - q.page_groups) * W + wave, turn[wave]);
+    install_rows<IO, V, 1, false, true>(a, axes, static_cast<int64_t>(blockIdx.x - q.page_groups) * W + wave, turn[wave]);
     return;
   }
   const int64_t unit = TW > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * W + wave;
@@ -428,16 +428,13 @@ __global__ __launch_bounds__((TW > 1 ? TW : kInstallWaves) * kWave) void install
   } else {
     if (place >= a.batch.tokens) return;
     t = static_cast<int>(place);
-    const int b = request_of_token(a.batch, t);
-    if (b >= a.batch.requests) return;
-    r = load_request(a.batch, b);
-    if (!r.ok || (t > r.q0 && (r.length - r.n + t - r.q0) % ps != 0)) return;
+    if (!request_of_row(a.batch, t, load_fields(a.batch, 0), r) || (t > r.q0 && (r.length - r.n + t - r.q0) % ps != 0)) return;
   }
   if (r.rem != 0) {  // it shares a page with what lies before it
     flag(a.batch.err, CB_ERROR_REQUEST);
     return;
   }
-  store_page<IO, V, TW, 2>(q, r, t, rest >> 1, rest & 1, turn[wave]);
+  store_page<IO, V, TW, 2>(q, axes, r, t, rest >> 1, rest & 1, turn[wave]);
 }
 
 // ---------------------------------------------------------------------------
@@ -1497,13 +1494,20 @@ void launch_quantized(const AttendArgs& a, const ScaledCache& cache, const Atten
   launch_join<IO, kAnyKeys>(a, h, st);
 }
 
-template <typename IO>
-void launch_store(const InstallQuantizedArgs& q, bool wide, bool teams, unsigned grid, hipStream_t st) {
+template <typename IO, typename AXES>
+void launch_store(const InstallQuantizedArgs& q, const AXES& axes, bool wide, bool teams, unsigned grid, hipStream_t st) {
   constexpr int V = 16 / sizeof(IO);
-  if (wide && teams) hipLaunchKernelGGL((install_quantized_kernel<IO, V, kTeamWaves>), dim3(grid), dim3(kTeamWaves * kWave), 0, st, q);
-  else if (wide) hipLaunchKernelGGL((install_quantized_kernel<IO, V, 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, q);
-  else if (teams) hipLaunchKernelGGL((install_quantized_kernel<IO, 1, kTeamWaves>), dim3(grid), dim3(kTeamWaves * kWave), 0, st, q);
-  else hipLaunchKernelGGL((install_quantized_kernel<IO, 1, 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, q);
+  const dim3 groups(grid), team(kTeamWaves * kWave), waves(kInstallWaves * kWave);
+  if (wide && teams) hipLaunchKernelGGL((install_quantized_kernel<IO, V, kTeamWaves, AXES>), groups, team, 0, st, q, axes);
+  else if (wide) hipLaunchKernelGGL((install_quantized_kernel<IO, V, 1, AXES>), groups, waves, 0, st, q, axes);
+  else if (teams) hipLaunchKernelGGL((install_quantized_kernel<IO, 1, kTeamWaves, AXES>), groups, team, 0, st, q, axes);
+  else hipLaunchKernelGGL((install_quantized_kernel<IO, 1, 1, AXES>), groups, waves, 0, st, q, axes);
+}
+template <typename AXES>
+void launch_store_of(int32_t dtype, const InstallQuantizedArgs& q, const AXES& axes, bool wide, bool teams, unsigned grid, hipStream_t st) {
+  if (dtype == CB_DTYPE_BF16) launch_store<io_bf16>(q, axes, wide, teams, grid, st);
+  else if (dtype == CB_DTYPE_F16) launch_store<io_f16>(q, axes, wide, teams, grid, st);
+  else launch_store<float>(q, axes, wide, teams, grid, st);
 }
 
 template <typename IO>
@@ -1524,10 +1528,12 @@ int cb_install_quantized(const cb_query_batch* batch, const cb_page_scales* scal
                          int32_t head_dim, const cb_heads* q, const cb_heads* q_out, const cb_heads* k, const cb_heads* v,
                          const cb_rotation* rotation, int32_t* d_error_flag, void* stream) {
   InstallQuantizedArgs a{};
+  PairAxes axes{};
+  bool many;
   int rc;
   if ((rc = check_batch(batch, dtype, head_dim, d_error_flag, true, &a.i.batch, &a.i.cache, 1)) ||
       (rc = check_scales(scales, *batch, &a.scales)) || (rc = check_pages(*batch, a.scales, "the batch")) ||
-      (rc = check_install(batch, layer, dtype, head_dim, q, q_out, k, v, rotation, &a.i)))
+      (rc = check_install(batch, layer, dtype, head_dim, q, q_out, k, v, rotation, &a.i, &axes, &many)))
     return rc;
   const int eb = elem_bytes(dtype), n = batch->num_tokens, rotary_dim = a.i.rotary_dim;
   if (n == 0 || batch->num_requests == 0) return CB_OK;
@@ -1550,9 +1556,8 @@ int cb_install_quantized(const cb_query_batch* batch, const cb_page_scales* scal
   if (!launch_fits(grid, waves * kWave)) return fail(CB_EINVAL, "too many tokens");
   a.page_groups = static_cast<uint32_t>(pages);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == CB_DTYPE_BF16) launch_store<io_bf16>(a, wide, teams, static_cast<unsigned>(grid), st);
-  else if (dtype == CB_DTYPE_F16) launch_store<io_f16>(a, wide, teams, static_cast<unsigned>(grid), st);
-  else launch_store<float>(a, wide, teams, static_cast<unsigned>(grid), st);
+  if (many) launch_store_of(dtype, a, axes, wide, teams, static_cast<unsigned>(grid), st);
+  else launch_store_of(dtype, a, OneAxis{}, wide, teams, static_cast<unsigned>(grid), st);
   CB_HIP(hipGetLastError());
   return CB_OK;
 }

@@ -7,15 +7,15 @@
 
 namespace {
 
-template <typename IO, int V, int U>
-__global__ __launch_bounds__(kInstallWaves * kWave) void install_tokens_kernel(InstallArgs a) {
+template <typename IO, int V, int U, typename AXES>
+__global__ __launch_bounds__(kInstallWaves * kWave) void install_tokens_kernel(InstallArgs a, AXES axes) {
   __shared__ turn_pair<IO> turn[kInstallWaves][kMaxPairs];
   const int wave = threadIdx.x / kWave;
   if (a.batch.err && blockIdx.x == gridDim.x - 1) {  // a workgroup more than there are tokens for
     if (wave == 0) flag_requests(a.batch);
     return;
   }
-  install_rows<IO, V, U, true, false>(a, static_cast<int64_t>(blockIdx.x) * kInstallWaves + wave, turn[wave]);
+  install_rows<IO, V, U, true, false>(a, axes, static_cast<int64_t>(blockIdx.x) * kInstallWaves + wave, turn[wave]);
 }
 
 // Many query rows: a workgroup's NW waves hold 32 rows each and share K and V
@@ -786,11 +786,18 @@ void launch_weights(const WeightArgs& a, bool mod, unsigned grid, hipStream_t st
 
 constexpr int kManyWaves = 8192;  // of an install, from which a lane has two items
 
-template <typename IO>
-void launch_install(const InstallArgs& a, bool wide, int items, unsigned grid, hipStream_t st) {
-  if (wide && items == 2) hipLaunchKernelGGL((install_tokens_kernel<IO, 16 / sizeof(IO), 2>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, a);
-  else if (wide) hipLaunchKernelGGL((install_tokens_kernel<IO, 16 / sizeof(IO), 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, a);
-  else hipLaunchKernelGGL((install_tokens_kernel<IO, 1, 1>), dim3(grid), dim3(kInstallWaves * kWave), 0, st, a);
+template <typename IO, typename AXES>
+void launch_install(const InstallArgs& a, const AXES& axes, bool wide, int items, unsigned grid, hipStream_t st) {
+  const dim3 groups(grid), threads(kInstallWaves * kWave);
+  if (wide && items == 2) hipLaunchKernelGGL((install_tokens_kernel<IO, 16 / sizeof(IO), 2, AXES>), groups, threads, 0, st, a, axes);
+  else if (wide) hipLaunchKernelGGL((install_tokens_kernel<IO, 16 / sizeof(IO), 1, AXES>), groups, threads, 0, st, a, axes);
+  else hipLaunchKernelGGL((install_tokens_kernel<IO, 1, 1, AXES>), groups, threads, 0, st, a, axes);
+}
+template <typename AXES>
+void launch_install_of(int32_t dtype, const InstallArgs& a, const AXES& axes, bool wide, int items, unsigned grid, hipStream_t st) {
+  if (dtype == CB_DTYPE_BF16) launch_install<io_bf16>(a, axes, wide, items, grid, st);
+  else if (dtype == CB_DTYPE_F16) launch_install<io_f16>(a, axes, wide, items, grid, st);
+  else launch_install<float>(a, axes, wide, items, grid, st);
 }
 
 }  // namespace
@@ -809,9 +816,11 @@ int cb_install_rotated(const cb_query_batch* batch, int32_t layer, int32_t dtype
                        const cb_heads* q_out, const cb_heads* k, const cb_heads* v, const cb_rotation* rotation,
                        int32_t* d_error_flag, void* stream) {
   InstallArgs a{};
+  PairAxes axes{};
+  bool many;
   int rc;
   if ((rc = check_batch(batch, dtype, head_dim, d_error_flag, true, &a.batch, &a.cache)) ||
-      (rc = check_install(batch, layer, dtype, head_dim, q, q_out, k, v, rotation, &a)))
+      (rc = check_install(batch, layer, dtype, head_dim, q, q_out, k, v, rotation, &a, &axes, &many)))
     return rc;
   const int eb = elem_bytes(dtype), kv = a.kv_heads, n = batch->num_tokens, rotary_dim = a.rotary_dim;
   if (n == 0 || batch->num_requests == 0) return CB_OK;
@@ -826,9 +835,8 @@ int cb_install_rotated(const cb_query_batch* batch, int32_t layer, int32_t dtype
   const int64_t grid = (static_cast<int64_t>(n) * a.slices + kInstallWaves - 1) / kInstallWaves + (d_error_flag ? 1 : 0);
   if (!launch_fits(grid, kInstallWaves * kWave)) return fail(CB_EINVAL, "too many tokens");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == CB_DTYPE_BF16) launch_install<io_bf16>(a, wide, items, static_cast<unsigned>(grid), st);
-  else if (dtype == CB_DTYPE_F16) launch_install<io_f16>(a, wide, items, static_cast<unsigned>(grid), st);
-  else launch_install<float>(a, wide, items, static_cast<unsigned>(grid), st);
+  if (many) launch_install_of(dtype, a, axes, wide, items, static_cast<unsigned>(grid), st);
+  else launch_install_of(dtype, a, OneAxis{}, wide, items, static_cast<unsigned>(grid), st);
   CB_HIP(hipGetLastError());
   return CB_OK;
 }

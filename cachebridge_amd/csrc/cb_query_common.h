@@ -182,6 +182,59 @@ CB_INLINE void flag_requests(const QBatch& B) {
     if (!load_requests(B, b0, top).ok) flag(B.err, CB_ERROR_REQUEST);
 }
 
+// A request of its fields, as load_request has it: its token rows, cached tokens and
+// first index token.
+CB_INLINE Request request_of(const QBatch& B, int64_t q0, int64_t q1, int length, int64_t start) {
+  Request r;
+  r.ok = start >= 0 && start <= (int64_t{1} << 61);
+  const int64_t u = r.ok ? start + B.index_offset : 0;
+  r.first = u;
+  r.rem = 0;
+  if (B.kind == CB_INDEX_BLOCK_TABLE) {
+    r.first = B.page_shift >= 0 ? u >> B.page_shift : u / B.page_size;
+    r.rem = static_cast<uint32_t>(u - r.first * B.page_size);
+  }
+  r.ok = r.ok && q0 >= 0 && q1 >= q0 && q1 <= B.tokens && q1 - q0 <= B.max_query && length <= B.max_length &&
+         q1 - q0 <= length;
+  r.q0 = static_cast<int>(q0);
+  r.n = r.ok ? static_cast<int>(q1 - q0) : 0;
+  r.length = r.ok ? length : 0;
+  return r;
+}
+
+// Requests b0 to b0 + 63, one a lane, as they stand in memory.
+struct Fields {
+  int start, end, length;
+  int64_t first;
+};
+CB_INLINE Fields load_fields(const QBatch& B, int b0) {
+  const int b = min(b0 + static_cast<int>(threadIdx.x & (kWave - 1)), B.requests - 1);
+  return {B.query_start[b], B.query_start[b + 1], B.lengths[b], B.offsets ? B.offsets[b] : b * B.request_stride};
+}
+
+// The request that token row t belongs to; false if none does. The first whose
+// rows hold t decides: if an earlier one starts behind it, so does one for any
+// later that holds t. Called by whole waves, t the same in all lanes. f: the first
+// 64 requests' fields, which a caller may have asked for ahead of other loads;
+// the request is made of its lane's, with nothing more to wait for.
+CB_INLINE bool request_of_row(const QBatch& B, int t, Fields f, Request& r) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int top = -2147483647;  // this lane's starts so far
+  for (int b0 = 0; b0 < B.requests; b0 += kWave) {
+    if (b0) f = load_fields(B, b0);
+    const uint64_t hit = __ballot((b0 + lane < B.requests) & (f.start <= t) & (t < f.end));
+    if (hit) {
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(hit)) - 1);
+      const int mine = __shfl(f.start, l);
+      if (__any((top > mine) | ((lane < l) & (f.start > mine)))) return false;
+      r = request_of(B, mine, __shfl(f.end, l), __shfl(f.length, l), static_cast<int64_t>(__shfl(static_cast<long long>(f.first), l)));
+      return r.ok;
+    }
+    top = max(top, f.start);
+  }
+  return false;
+}
+
 // The request that token row t belongs to, or `requests` if none does. The
 // first whose rows hold t decides: if an earlier one starts behind it, so does
 // one for any later that holds t. Called by whole waves, t the same in all lanes.

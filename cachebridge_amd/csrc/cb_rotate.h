@@ -25,9 +25,18 @@ struct InstallArgs {
   const void* positions;
   int32_t positions_kind;
   float magnitude;
-  int32_t axes;         // rows of positions, axis_stride entries apart
-  int64_t axis_stride;
-  uint8_t pair_axis[kMaxPairs];  // the axis of each pair
+};
+
+// Positions of one axis, or of several: rows of them, `stride` entries apart, and the
+// axis of each pair. The latter are 256 bytes of a launch's arguments, which a step of
+// 64 requests pays with 0.3 of its 5 us, so launches without axes go without.
+struct OneAxis {
+  CB_INLINE int64_t at(int, int t) const { return t; }
+};
+struct PairAxes {
+  int64_t stride;
+  uint8_t axis[kMaxPairs];
+  CB_INLINE int64_t at(int pair, int t) const { return axis[pair] * stride + t; }
 };
 
 
@@ -64,6 +73,9 @@ __host__ __device__ inline InstallItems install_items(int head_dim, int rotary_d
   const int turned = rotary_dim / 2 / v;
   return {turned + ((head_dim - rotary_dim) / v + 1) / 2, turned, (head_dim / v + 1) / 2};
 }
+
+// x / y, y the same in all lanes and mostly a power of two.
+CB_INLINE int divide(int x, int y) { return (y & (y - 1)) == 0 ? x >> __builtin_ctz(y) : x / y; }
 
 // V elements as one access where V * sizeof(IO) is 16, else element by element.
 template <typename IO, int V>
@@ -104,11 +116,11 @@ using turn_pair = turn_t<IO> __attribute__((ext_vector_type(2)));
 
 // The cosine and sine, times the magnitude, by which pair `i` of token row t at
 // place p turns.
-template <typename PAIR, typename T>
-CB_INLINE PAIR turn_of(const InstallArgs& a, int t, int p, int i) {
+template <typename PAIR, typename T, typename AXES>
+CB_INLINE PAIR turn_of(const InstallArgs& a, const AXES& axes, int t, int p, int i) {
   int64_t pos = p;
   if (a.positions) {
-    const int64_t at = a.axes > 1 ? a.pair_axis[i] * a.axis_stride + t : t;
+    const int64_t at = axes.at(i, t);
     pos = a.positions_kind == CB_INDEX_I64 ? static_cast<const int64_t*>(a.positions)[at]
                                            : static_cast<const int32_t*>(a.positions)[at];
   }
@@ -143,11 +155,12 @@ CB_INLINE void turn_pairs(const float (&x)[2 * V], const PAIR* turn, bool interl
 // WHOLE: requests that do not start at a page's first slot are outside the bounds.
 // What a wave reads of q, k and v depends on its token row alone: the loads are on
 // their way while the row's request, place and cache row are looked up.
-template <typename IO, int V, int U, bool KV, bool WHOLE>
-CB_INLINE void install_rows(const InstallArgs& a, int64_t unit, turn_pair<IO>* turn) {
+template <typename IO, int V, int U, bool KV, bool WHOLE, typename AXES>
+CB_INLINE void install_rows(const InstallArgs& a, const AXES& axes, int64_t unit, turn_pair<IO>* turn) {
   const int lane = threadIdx.x & (kWave - 1);
   const int t = static_cast<int>(unit / a.slices), slice = static_cast<int>(unit % a.slices);
   if (t >= a.batch.tokens) return;
+  const Fields fields = load_fields(a.batch, 0);
   const int pairs = a.rotary_dim / 2, kv_heads = KV ? a.kv_heads : 0;
   const InstallItems n = install_items(a.head_dim, a.rotary_dim, V);
   const int turned = (a.q_heads + kv_heads) * n.head, total = turned + kv_heads * n.value;
@@ -155,7 +168,9 @@ CB_INLINE void install_rows(const InstallArgs& a, int64_t unit, turn_pair<IO>* t
   const int stop = min(total, (slice + 1) * per);
   constexpr int E = sizeof(IO);
   struct Item {
-    int head, oa, ob, first;  // of q's heads, then k's, then v's; the two vectors; the first pair, or -1
+    int64_t to;         // where its head's elements go, from q_out, or from the cache row of K or V
+    int oa, ob, first;  // the two vectors; the first pair, or -1
+    int kind;           // 0: q, 1: K, 2: V
     bool on, two;
   } item[U];
   float x[U][2 * V];
@@ -165,17 +180,32 @@ CB_INLINE void install_rows(const InstallArgs& a, int64_t unit, turn_pair<IO>* t
       Item& m = item[u];
       const int at = min(idx + u * kWave, stop - 1);
       m.on = idx + u * kWave < stop;
-      const bool value = KV && at >= turned;
-      const int of = value ? (at - turned) / n.value : at / n.head;
-      const int k = value ? at - turned - of * n.value : at - of * n.head;
-      m.head = value ? a.q_heads + kv_heads + of : of;
-      m.first = !value && k < n.turned ? k * V : -1;
-      const int straight = value ? 0 : a.rotary_dim, plain = straight + 2 * (k - (value ? 0 : n.turned)) * V;
-      m.oa = m.first < 0 ? plain : a.interleaved ? 2 * m.first : m.first;
-      m.ob = m.first < 0 ? plain + V : a.interleaved ? m.oa + V : m.first + pairs;
-      m.two = m.first >= 0 || plain + V < a.head_dim;
-      const Strided& from = m.head < a.q_heads ? a.q : value ? a.v : a.k;
-      const char* src = from.data + t * from.token_b + (value || m.head >= a.q_heads ? m.head - a.q_heads - (value ? kv_heads : 0) : m.head) * from.head_b;
+      const char* src;
+      int k;
+      if (!KV || at < turned) {
+        const int head = divide(at, n.head);
+        k = at - head * n.head;
+        m.kind = KV && head >= a.q_heads;
+        if (m.kind) {
+          src = a.k.data + t * a.k.token_b + (head - a.q_heads) * a.k.head_b;
+          m.to = static_cast<int64_t>(head - a.q_heads) * a.head_dim * E;
+        } else {
+          src = a.q.data + t * a.q.token_b + head * a.q.head_b;
+          m.to = t * a.q_out.token_b + head * a.q_out.head_b;
+        }
+        m.first = k < n.turned ? k * V : -1;
+        m.oa = m.first < 0 ? a.rotary_dim + 2 * (k - n.turned) * V : a.interleaved ? 2 * m.first : m.first;
+      } else {
+        const int head = divide(at - turned, n.value);
+        k = at - turned - head * n.value;
+        m.kind = 2;
+        src = a.v.data + t * a.v.token_b + head * a.v.head_b;
+        m.to = static_cast<int64_t>(head) * a.head_dim * E;
+        m.first = -1;
+        m.oa = 2 * k * V;
+      }
+      m.ob = m.first < 0 || a.interleaved ? m.oa + V : m.first + pairs;
+      m.two = m.first >= 0 || m.ob < a.head_dim;
       if (m.on) {
         load_vec<IO, V>(src + m.oa * E, x[u]);
         if (m.two) load_vec<IO, V>(src + m.ob * E, x[u] + V);
@@ -184,17 +214,15 @@ CB_INLINE void install_rows(const InstallArgs& a, int64_t unit, turn_pair<IO>* t
   };
   const int first = slice * per + lane;
   if (first < stop) load(first);
-  const int b = request_of_token(a.batch, t);
-  if (b >= a.batch.requests) return;
-  const Request r = load_request(a.batch, b);
-  if (!r.ok | (WHOLE & (r.rem != 0))) return;
+  Request r;
+  if (!request_of_row(a.batch, t, fields, r) || (WHOLE & (r.rem != 0))) return;
   const int p = r.length - r.n + (t - r.q0);
   int64_t row = -1;
   if constexpr (KV) {
     row = cache_row(a.batch, r, p);
     if (row < 0 && lane == 0) flag(a.batch.err, CB_ERROR_TARGET_ROW);
   }
-  for (int i = lane; i < pairs; i += kWave) turn[i] = turn_of<turn_pair<IO>, turn_t<IO>>(a, t, p, i);
+  for (int i = lane; i < pairs; i += kWave) turn[i] = turn_of<turn_pair<IO>, turn_t<IO>>(a, axes, t, p, i);
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   char* krow = const_cast<char*>((const char*)layer_base(a.cache, 0, a.layer)) + row * a.cache.row_stride_b;
@@ -204,10 +232,8 @@ CB_INLINE void install_rows(const InstallArgs& a, int64_t unit, turn_pair<IO>* t
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const Item& m = item[u];
-      const bool query = m.head < a.q_heads, value = m.head >= a.q_heads + kv_heads;
-      if (!m.on || (!query && row < 0)) continue;
-      char* dst = query ? a.q_out.data + t * a.q_out.token_b + m.head * a.q_out.head_b
-                        : (value ? vrow : krow) + static_cast<int64_t>(m.head - a.q_heads - (value ? kv_heads : 0)) * a.head_dim * E;
+      if (!m.on || (m.kind && row < 0)) continue;
+      char* dst = (m.kind == 0 ? a.q_out.data : m.kind == 1 ? krow : vrow) + m.to;
       float y[2 * V];
 #pragma unroll
       for (int i = 0; i < 2 * V; ++i) y[i] = x[u][i];
@@ -223,9 +249,10 @@ CB_INLINE void install_rows(const InstallArgs& a, int64_t unit, turn_pair<IO>* t
 // ---------------------------------------------------------------------------
 
 // The token tensors and the rotation of an install, checked; the batch and the
-// cache are the caller's.
+// cache are the caller's. many: pairs turn by positions of several axes.
 int check_install(const cb_query_batch* batch, int32_t layer, int32_t dtype, int32_t head_dim, const cb_heads* q,
-                  const cb_heads* q_out, const cb_heads* k, const cb_heads* v, const cb_rotation* rotation, InstallArgs* a) {
+                  const cb_heads* q_out, const cb_heads* k, const cb_heads* v, const cb_rotation* rotation, InstallArgs* a,
+                  PairAxes* axes, bool* many) {
   int rc;
   if (layer < 0 || layer >= batch->cache.num_layers) return fail(CB_EINVAL, "layer %d outside the cache", layer);
   if (!q) return fail(CB_EINVAL, "null q");
@@ -242,16 +269,15 @@ int check_install(const cb_query_batch* batch, int32_t layer, int32_t dtype, int
   if (!std::isfinite(o.magnitude)) return fail(CB_EINVAL, "magnitude must be finite");
   if (o.positions && o.positions_kind != CB_INDEX_I32 && o.positions_kind != CB_INDEX_I64)
     return fail(CB_EINVAL, "positions must be int32 or int64");
-  a->axes = 1;
+  *many = o.pair_axis && o.positions && o.axes > 1;
   if (o.pair_axis) {
     if (o.axes < 1 || o.axes > kMaxAxes) return fail(CB_EINVAL, "a rotation has 1 to %d axes", kMaxAxes);
     if (o.positions && o.axis_stride < n) return fail(CB_EINVAL, "axes of positions are shorter than num_tokens");
     for (int i = 0; i < o.rotary_dim / 2; ++i) {
       if (o.pair_axis[i] >= o.axes) return fail(CB_EINVAL, "pair %d turns by axis %d of %d", i, o.pair_axis[i], o.axes);
-      a->pair_axis[i] = o.pair_axis[i];
+      axes->axis[i] = o.pair_axis[i];
     }
-    a->axes = o.axes;
-    a->axis_stride = o.axis_stride;
+    axes->stride = o.axis_stride;
   }
   if (shares_rows(*batch)) return fail(CB_EINVAL, "several requests need offsets or a request_stride");
   a->layer = layer;
