@@ -565,9 +565,10 @@ CB_INLINE int row_splits(const AttendArgs& a, int t, int qh, int rows_per_tile) 
 // Joins few splits: out = sum 2^(lse_z - lse) out_z, a wave a row. Lane z holds
 // split z's statistics, then every lane E elements of the row. Taken where
 // there are rows enough for all CUs: with 128 new tokens (2048 rows of 128) over
-// 4096 it takes 6.6 us where a workgroup a row takes 7.9, with 64 times 16
-// tokens 13.4 against 37.2, with 1000 rows of 64 5.0 against 5.8; with 37 tokens
-// (592 rows) 5.9 against 5.1, with 4 9.0 against 5.0.
+// 4096 it takes 4.9 us where a workgroup a row takes 9.5, with 64 times 16
+// tokens 13.3 against 45.7, with 1000 rows of 64 4.2 against 5.4; with 4 tokens (64
+// rows of 16 splits) 5.2 against 4.2. Between them (37 tokens, 592 rows of 8 splits:
+// 4.3 against 5.0) calls keep the order of sums that they have had.
 constexpr int kJoinFew = 16;    // splits up to which, and
 constexpr int kJoinRows = 768;  // rows from which it is taken
 
@@ -638,7 +639,9 @@ __global__ __launch_bounds__(256) void join_few_kernel(AttendArgs a, int rows_pe
 
 // Joins many splits, a workgroup a row: threads of one group of LANES hold four
 // elements each of a split's row, the groups take splits in turn and meet in
-// LDS in group order.
+// LDS in group order. Splits that are in flight together (eight a group where there
+// are many) are what it waits for: a request of 32768 tokens with 64 heads 5.4 us
+// (9.0 with splits in turn).
 constexpr int kJoinThreads = 256;
 
 template <typename IO, int KT, int LANES>

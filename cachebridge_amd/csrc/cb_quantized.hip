@@ -179,10 +179,16 @@ CB_INLINE void report_request(const QuantizeArgs& a, int b) {
   }
 }
 
-// A wave a page and head of one layer's K or V: V elements a lane and step, the
-// page's largest by an exchange among the lanes, then the codes. Pages of up
-// to 64 * KEEP vectors stay in registers between the two, longer ones are read
-// again (from L2).
+// code = round(x / 2^e), e from the largest |x| of the page. Every element is read
+// once (2 or 4 bytes) and written once (1): the copy rate bounds it. A wave a page
+// and head of one layer's K or V: V elements a lane and step, the page's largest
+// by an exchange among the lanes, then the codes. No barrier and no LDS: a page of
+// 16 tokens of 128 is two vectors a lane, and waves that are at work on other pages hide
+// its lookups. Pages of up to 64 * KEEP vectors stay in registers between
+// the two, longer ones are read again (from L2). KEEP is the least that holds the
+// page, up to 4 (64 registers of fp32 elements): 4096 tokens of 64 layers, 2 heads, 96
+// us (KEEP 2; 403 MB, 4.2 TB/s with cold caches, 86 us in a row of calls); 16 fp16
+// requests, 62 layers, pages of 32 340 us (KEEP 4; 1.5 GB, 4.5 TB/s).
 template <typename IO, int V, int KEEP>
 __global__ __launch_bounds__(256) void quantize_tokens_kernel(QuantizeArgs a) {
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -274,6 +280,8 @@ constexpr int kTurns = V == 8 ? 512 : kMaxPairs;  // pairs that 64 items turn, a
 // elements (both vectors of V pairs, or two neighbours) lie one a lane in rounds
 // of whole rows, which the waves take in turn; up to KEEP rounds of a wave stay in
 // registers until the page's scale is known, more are read (and turned) twice.
+// Cached codes of the page, where a larger scale needs them rounded again, are
+// read only then: a step in 16 meets a new page, and most others keep the scale.
 template <typename IO, int V, int TW, int KEEP, typename AXES>
 CB_INLINE void store_page(const InstallQuantizedArgs& q, const AXES& axes, const Request& r, int t, int head, int kind, turn_pair<IO>* turn) {
   __shared__ float tops[TW];
@@ -321,7 +329,7 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const AXES& axes, const
       const int all = min(per_round, rows - row0) * pairs;
       for (int x = lane; x < all; x += kWave) {
         const int at = row0 + x / pairs;
-        turn[x] = turn_of<turn_pair<IO>, turn_t<IO>>(a, axes, t + at, p0 + at, x % pairs);
+        turn[x] = turn_of<turn_pair<IO>, turn_t<IO>>(a, p0 + at, load_angle(a, axes, t + at, x % pairs));
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -397,6 +405,11 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const AXES& axes, const
 // (install_rows). Pages are counted by request; where the bound on a request's new
 // tokens leaves more of them than there are tokens, a team goes by a token and
 // works if it is its page's first new one.
+// A chunk's pages are whole: one wave a page of 64 took 93 us for 2048 tokens, a
+// workgroup of four 13.7 and of eight 10.2 (12.6 MB, 4.2 us at the rate of a copy: the
+// rest is one chain of row, largest, barrier, code). A step's pages have one new row,
+// which one wave has in one round: 64 requests, heads (64, 8) 6.4 us, launch and the
+// same chain without the barrier.
 constexpr int kTeamWaves = 8;
 
 template <typename IO, int V, int TW, typename AXES>
@@ -791,7 +804,16 @@ constexpr int kTileWaves = 8;
 // while one is used. Keys without a row are read from row 0 and chunks past
 // head_dim from the last one, and made zeros when they are widened: a tile that is
 // whole pays nothing for either.
-// RB: query rows a wave, 32 (RowBlock) or 16 (ElemBlock).
+// The matrix unit bounds it, as it does the 16-bit kernel: a chunk of 2048 over
+// 32768 with heads (16, 2) of 128 takes 540 to 625 us by the card's clock (533
+// GFLOP, 440 us at the rate of a library's product; the 16-bit kernel 529 on the
+// card where this took 537). Each wave widens an eighth of a tile, so that a tile's
+// conversions are shared by 256 rows.
+// RB: query rows a wave, 32 (RowBlock) or 16 (ElemBlock): twice the LDS reads a
+// product, half the registers. 32 where a wave's registers leave two waves a SIMD
+// (the chunk 588 us, 952 with 16). Heads of 256, where 32 rows leave one, and a head's
+// few rows take 16: windows of 1024 over 8192 with capped scores 336 us where the
+// 16-bit kernel with 32 takes 413.
 template <typename IO, int DP, int KT, int RB, bool MOD>
 __global__ __launch_bounds__(kTileWaves * kWave, 2) void attend_codes_kernel(AttendArgs a, ScaledCache cache, int vector) {
   typedef std::conditional_t<RB == 32, RowBlock<IO, DP, KT, MOD>, ElemBlock<IO, DP, KT, MOD>> Block;
@@ -1277,6 +1299,14 @@ CB_INLINE void wait_last(int left, bool value) {
 
 // Few query rows: attend_step_kernel's scheme on tiles of codes. Each wave
 // streams tiles of 32 keys through LDS of its own, S of them in flight.
+// Reading K and V bounds it: 64 requests of 8192 with one KV head's 268 MB take 56
+// to 63 us (4.3 to 4.8 TB/s, the rate of a copy). Shorter steps add 8 to 10 us for the
+// chain of lookups before the first product and the sums after the last: 64
+// ragged requests of 2550 29.5 us (17.7 at that rate), one of 32768 with 8 KV heads
+// 19.5 (14.1).
+// kCodeWaves 4, S 2: two waves take 33.7, 22.9 and 74.8 us for these three cases'
+// 29.3, 19.4 and 62; blocks of 32 rows 42, 26.7 and 81. Splits cut for 512 or 2048
+// workgroups in place of 1024 are slower, for 256 the same within noise.
 constexpr int kCodeTiles = 32;  // tiles a split holds at most
 constexpr int kCodeWaves = 4;
 

@@ -212,6 +212,13 @@ CB_INLINE Fields load_fields(const QBatch& B, int b0) {
   return {B.query_start[b], B.query_start[b + 1], B.lengths[b], B.offsets ? B.offsets[b] : b * B.request_stride};
 }
 
+// What lane `lane` (the same in all) holds.
+CB_INLINE int lane_value(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+CB_INLINE int64_t lane_value(int64_t x, int lane) {
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(lane_value(static_cast<int>(x >> 32), lane))) << 32 |
+                              static_cast<uint32_t>(lane_value(static_cast<int>(x), lane)));
+}
+
 // The request that token row t belongs to; false if none does. The first whose
 // rows hold t decides: if an earlier one starts behind it, so does one for any
 // later that holds t. Called by whole waves, t the same in all lanes. f: the first
@@ -225,9 +232,9 @@ CB_INLINE bool request_of_row(const QBatch& B, int t, Fields f, Request& r) {
     const uint64_t hit = __ballot((b0 + lane < B.requests) & (f.start <= t) & (t < f.end));
     if (hit) {
       const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(hit)) - 1);
-      const int mine = __shfl(f.start, l);
+      const int mine = lane_value(f.start, l);
       if (__any((top > mine) | ((lane < l) & (f.start > mine)))) return false;
-      r = request_of(B, mine, __shfl(f.end, l), __shfl(f.length, l), static_cast<int64_t>(__shfl(static_cast<long long>(f.first), l)));
+      r = request_of(B, mine, lane_value(f.end, l), lane_value(f.length, l), lane_value(f.first, l));
       return r.ok;
     }
     top = max(top, f.start);

@@ -114,18 +114,26 @@ using turn_t = std::conditional_t<sizeof(IO) == 4, double, float>;
 template <typename IO>
 using turn_pair = turn_t<IO> __attribute__((ext_vector_type(2)));
 
-// The cosine and sine, times the magnitude, by which pair `i` of token row t at
-// place p turns.
-template <typename PAIR, typename T, typename AXES>
-CB_INLINE PAIR turn_of(const InstallArgs& a, const AXES& axes, int t, int p, int i) {
-  int64_t pos = p;
+// What the angle of pair `i` of token row t is made of (the position where there is
+// a row of them), and its cosine and sine, times the magnitude, at place p.
+struct Angle {
+  int64_t position;
+  double inv_freq;
+};
+template <typename AXES>
+CB_INLINE Angle load_angle(const InstallArgs& a, const AXES& axes, int t, int i) {
+  Angle x{0, a.inv_freq[i]};
   if (a.positions) {
     const int64_t at = axes.at(i, t);
-    pos = a.positions_kind == CB_INDEX_I64 ? static_cast<const int64_t*>(a.positions)[at]
-                                           : static_cast<const int32_t*>(a.positions)[at];
+    x.position = a.positions_kind == CB_INDEX_I64 ? static_cast<const int64_t*>(a.positions)[at]
+                                                  : static_cast<const int32_t*>(a.positions)[at];
   }
+  return x;
+}
+template <typename PAIR, typename T>
+CB_INLINE PAIR turn_of(const InstallArgs& a, int p, const Angle& x) {
   T s, c;
-  sincos_turns(static_cast<double>(pos) * a.inv_freq[i] * 0.15915494309189533577, &s, &c);
+  sincos_turns(static_cast<double>(a.positions ? x.position : p) * x.inv_freq * 0.15915494309189533577, &s, &c);
   return PAIR{c * a.magnitude, s * a.magnitude};
 }
 
@@ -154,7 +162,13 @@ CB_INLINE void turn_pairs(const float (&x)[2 * V], const PAIR* turn, bool interl
 // KV: K and V rows go into the cache as they are, else queries alone are written.
 // WHOLE: requests that do not start at a page's first slot are outside the bounds.
 // What a wave reads of q, k and v depends on its token row alone: the loads are on
-// their way while the row's request, place and cache row are looked up.
+// their way while the row's request, place and cache row are looked up, which is
+// one load of the batch's fields by all lanes and one index entry. What is left of a
+// step is launch and that chain: 64 requests, heads (64, 8) of 128 4.9 us for 2.6 MB,
+// 2048 tokens of (16, 2) 9.1 (21 MB).
+// Above 8192 waves a lane takes two items, so that half as many waves look their
+// row up: 2048 tokens of (16, 2) heads of 256 with three axes 15.2 us for 20.3 (38
+// MB, 8.8 us at the rate of a copy; sines and cosines are 1 us of it).
 template <typename IO, int V, int U, bool KV, bool WHOLE, typename AXES>
 CB_INLINE void install_rows(const InstallArgs& a, const AXES& axes, int64_t unit, turn_pair<IO>* turn) {
   const int lane = threadIdx.x & (kWave - 1);
@@ -213,6 +227,7 @@ CB_INLINE void install_rows(const InstallArgs& a, const AXES& axes, int64_t unit
     }
   };
   const int first = slice * per + lane;
+  const Angle angle = load_angle(a, axes, t, min(lane, pairs - 1));
   if (first < stop) load(first);
   Request r;
   if (!request_of_row(a.batch, t, fields, r) || (WHOLE & (r.rem != 0))) return;
@@ -222,7 +237,7 @@ CB_INLINE void install_rows(const InstallArgs& a, const AXES& axes, int64_t unit
     row = cache_row(a.batch, r, p);
     if (row < 0 && lane == 0) flag(a.batch.err, CB_ERROR_TARGET_ROW);
   }
-  for (int i = lane; i < pairs; i += kWave) turn[i] = turn_of<turn_pair<IO>, turn_t<IO>>(a, axes, t, p, i);
+  for (int i = lane; i < pairs; i += kWave) turn[i] = turn_of<turn_pair<IO>, turn_t<IO>>(a, p, i == lane ? angle : load_angle(a, axes, t, i));
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   char* krow = const_cast<char*>((const char*)layer_base(a.cache, 0, a.layer)) + row * a.cache.row_stride_b;
