@@ -253,7 +253,7 @@ SIGNATURES = {
     "cb_quantized_attention": (
         ctypes.c_int,
         [ctypes.POINTER(CbQueryBatch), ctypes.POINTER(CbPageScales), _i32, _i32, _i32, ctypes.POINTER(CbScores),
-         ctypes.POINTER(CbHeads), ctypes.POINTER(CbHeads), _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
     ),
     "cb_attention_workspace_bytes": (
         ctypes.c_int,
@@ -261,8 +261,8 @@ SIGNATURES = {
     ),
     "cb_paged_attention": (
         ctypes.c_int,
-        [ctypes.POINTER(CbQueryBatch), _i32, _i32, _i32, ctypes.POINTER(CbScores), ctypes.POINTER(CbHeads),
-         ctypes.POINTER(CbHeads), _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
+        [ctypes.POINTER(CbQueryBatch), _i32, _i32, _i32, ctypes.POINTER(CbScores), _c_void_p, _c_void_p, _c_void_p,
+         _c_void_p, _i64, _c_void_p, _c_void_p],
     ),
     "cb_add_key_weights": (
         ctypes.c_int,

@@ -185,8 +185,8 @@ CB_INLINE void report_request(const QuantizeArgs& a, int b) {
 // by an exchange among the lanes, then the codes. No barrier and no LDS: a page of
 // 16 tokens of 128 is two vectors a lane, and waves that are at work on other pages hide
 // its lookups. Pages of up to 64 * KEEP vectors stay in registers between
-// the two, longer ones are read again (from L2). KEEP is the least that holds the
-// page, up to 4 (64 registers of fp32 elements): 4096 tokens of 64 layers, 2 heads, 96
+// the two, longer ones are read again (from L2). KEEP is the least of 2, 4 and 8
+// that holds the page: 4096 tokens of 64 layers, 2 heads, 96
 // us (KEEP 2; 403 MB, 4.2 TB/s with cold caches, 86 us in a row of calls); 16 fp16
 // requests, 62 layers, pages of 32 340 us (KEEP 4; 1.5 GB, 4.5 TB/s).
 template <typename IO, int V, int KEEP>

@@ -171,16 +171,16 @@ class QueryBatch:
         return layer
 
     def _tokens(self, n: int):
-        """The C description for token tensors of ``n`` rows (one for each ``n``, not written again: calls may run
-        side by side)."""
-        ref = self._by_tokens.get(n)
+        """The C description for token tensors of ``n`` rows (one for each ``n`` and bound, not written again: calls
+        may run side by side)."""
+        ref = self._by_tokens.get((n, self.max_query))
         if ref is None:
             c = _lib.CbQueryBatch.from_buffer_copy(self.c)
             c.num_tokens = n
             c.max_query = n if self.max_query is None else min(self.max_query, n)
             if len(self._by_tokens) >= 64:
                 self._by_tokens = {}
-            ref = self._by_tokens[n] = ctypes.byref(c)
+            ref = self._by_tokens[n, self.max_query] = ctypes.byref(c)
         return ref
 
     def _heads(self, t: torch.Tensor, name: str, tokens: int | None = None, heads: int | None = None) -> _lib.CbHeads:
@@ -203,7 +203,8 @@ class QueryBatch:
         return t.data_ptr(), st, sh, h
 
 
-# The cb_heads of q, out, k and v, four words each (the last one heads, its upper half reserved).
+# The cb_heads of q and out, or of q, out, k and v, four words each (the last one heads, its upper half reserved).
+_TwoHeads = ctypes.c_int64 * 8
 _FourHeads = ctypes.c_int64 * 16
 
 
@@ -373,7 +374,7 @@ def paged_attention(batch: QueryBatch, layer: int, q: torch.Tensor, *, scale: fl
     scales' ``dtype``.
     """
     n, heads, dim = q.shape if q.ndim == 3 else (0, 0, 0)
-    cq = batch._heads(q, "q")
+    rq = batch._row(q, "q")
     scores = _scores(batch, heads, dim, scale, causal, window, cap, slopes, prefix_lengths)
     scores.fp32_weights = bool(fp32_weights)
     flag = _flag_pointer(batch, error_flag)
@@ -381,18 +382,23 @@ def paged_attention(batch: QueryBatch, layer: int, q: torch.Tensor, *, scale: fl
     with _On(batch, stream) as handle:
         if out is None:
             out = q.new_empty((n, heads, dim))
-        co = batch._heads(out, "out", n, heads)
+        rows = _TwoHeads(*rq, *batch._row(out, "out", n, heads))
+        at = ctypes.addressof(rows)
         lse = q.new_empty((n, heads), dtype=torch.float32) if return_lse else None
         c = batch._tokens(n)
         need = ctypes.c_int64(0)
-        ask, attend, more = ((lib.cb_attention_workspace_bytes, lib.cb_paged_attention, ()) if batch.scales is None else
-                             (lib.cb_quantized_attention_workspace_bytes, lib.cb_quantized_attention, (batch._scales,)))
-        _lib.check(ask(c, *more, batch._code, dim, ctypes.byref(scores), heads, ctypes.byref(need)))
+        scored = (batch._code, dim, ctypes.byref(scores))
+        if batch.scales is None:
+            _lib.check(lib.cb_attention_workspace_bytes(c, *scored, heads, ctypes.byref(need)))
+        else:
+            _lib.check(lib.cb_quantized_attention_workspace_bytes(c, batch._scales, *scored, heads, ctypes.byref(need)))
         work = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
-        _lib.check(attend(
-            c, *more, batch._layer(layer), batch._code, dim, ctypes.byref(scores), ctypes.byref(cq), ctypes.byref(co),
-            None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), need.value, flag,
-            handle))
+        to = (at, at + 32, None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), need.value,
+              flag, handle)
+        if batch.scales is None:
+            _lib.check(lib.cb_paged_attention(c, batch._layer(layer), *scored, *to))
+        else:
+            _lib.check(lib.cb_quantized_attention(c, batch._scales, batch._layer(layer), *scored, *to))
         batch.rows.hold_for(stream)
     return (out, lse) if return_lse else out
 
@@ -533,4 +539,5 @@ def quantize_tokens(batch: QueryBatch, target: QueryBatch, *, out: torch.Tensor 
             batch._tokens(0), target._tokens(0), target._scales, batch._code, dim,
             _device_vector(out, "out", (torch.int32,), batch.device, batch.requests), flag, handle))
         batch.rows.hold_for(stream)
+        target.rows.hold_for(stream)
     return out

@@ -452,9 +452,11 @@ int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, i
  * Queries on an 8-bit cache. K and V rows hold e4m3 codes (the OCP format: no
  * infinities, 0x7f and 0xff are NaN), a byte an element; an element's value is
  * its code's times 2^(byte - 127), byte the scale of its layer, page and KV head
- * (1 to 246; larger ones read as 246). Pages are page_size rows: row r is in page r / page_size. Such a
- * cache is described by the same cb_query_batch (strides of its cb_rows count
- * bytes) and the scales beside it; the token tensors are of `dtype`.
+ * (1 to 246; larger ones read as 246; a cache that is read with dtype CB_DTYPE_F16
+ * has scales up to 134, as calls of that type store them). Pages are page_size
+ * rows: row r is in page r / page_size. Such a cache is described by the same
+ * cb_query_batch (strides of its cb_rows count bytes) and the scales beside it;
+ * the token tensors are of `dtype`.
  *
  * Rows that are stored choose the scale: the least that holds every finite
  * element of the page's stored rows up to 448 times it (2^-126 where all are
@@ -475,8 +477,8 @@ typedef struct cb_page_scales {
 
 /* cb_install_rotated into an 8-bit cache. Its index must be a block table of
    the scales' page_size and a request must start at a page's first slot (else
-   it is outside the bounds): a page then belongs to one request, and one wave
-   stores it. A page whose first slots hold cached tokens keeps its scale unless
+   it is outside the bounds): a page then belongs to one request, and one workgroup
+   stores a head of it. A page whose first slots hold cached tokens keeps its scale unless
    the new rows need a larger one: those tokens' codes are then rounded to it.
    Slots behind the new tokens keep their codes. Asynchronous. */
 int cb_install_quantized(const cb_query_batch* batch, const cb_page_scales* scales, int32_t layer,
