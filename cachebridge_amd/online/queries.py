@@ -32,6 +32,7 @@ queries (``cb/online/admission.py:466-499`` hands over after publication).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import NamedTuple
@@ -311,25 +312,36 @@ def install_tokens(batch: QueryBatch, layer: int, q: torch.Tensor, k: torch.Tens
     return out
 
 
+@functools.lru_cache(maxsize=64)
+def _axis_count(axes: bytes) -> int:
+    """The axes that pairs turn by: a step of many layers asks at every one."""
+    return max(axes, default=0) + 1
+
+
 def _positions(batch: QueryBatch, rotary: Rotary, positions: torch.Tensor | None, n: int):
     """The positions' address and index kind, None and 0 without any; the rotation's axes checked."""
     axes = rotary.axes
-    if axes is not None and (not isinstance(axes, bytes) or len(axes) != rotary.inv_freq.numel() or max(axes) > 7):
-        raise ValueError("axes must be bytes, 0 to 7, one for each pair of inv_freq")
-    if positions is None:
-        return None, 0
-    if axes is not None:
-        if positions.ndim != 2 or positions.shape[0] <= max(axes) or positions.shape[1] != n:
+    if axes is None:
+        if positions is None:
+            return None, 0
+        at = _device_vector(positions, "positions", (torch.int32, torch.int64), batch.device, n)
+    else:
+        if not isinstance(axes, bytes) or len(axes) != rotary.inv_freq.numel() or _axis_count(axes) > 8:
+            raise ValueError("axes must be bytes, 0 to 7, one for each pair of inv_freq")
+        if positions is None:
+            return None, 0
+        shape = positions.shape
+        if len(shape) != 2 or shape[0] < _axis_count(axes) or shape[1] != n:
             raise ValueError("positions must be [axes, tokens] with one row for each of the rotation's axes")
-        # What is read is one row an axis; the flat vector holds them one after another.
-        positions = positions.view(-1) if positions.is_contiguous() else positions
-    at = _device_vector(positions, "positions", (torch.int32, torch.int64), batch.device, n if axes is None else None)
+        if positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous() or positions.device != batch.device:
+            raise ValueError(f"positions must be a contiguous tensor of torch.int32 or torch.int64 on {batch.device}")
+        at = positions.data_ptr()
     return at, _lib.CB_INDEX_I64 if positions.dtype == torch.int64 else _lib.CB_INDEX_I32
 
 
 def _rotation(rotary: Rotary, inv: int, pos: int | None, kind: int, n: int) -> _lib.CbRotation:
     axes, dim, spin = rotary.axes, 2 * rotary.inv_freq.numel(), int(rotary.interleaved)
-    count = 1 if axes is None else max(axes) + 1
+    count = 1 if axes is None else _axis_count(axes)
     return _lib.CbRotation(inv, pos, axes, n, dim, spin, kind, count, rotary.magnitude)
 
 
