@@ -345,7 +345,7 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const AXES& axes, const
     for (int i = 0; i < 2 * V; ++i) y[i] = x[i];
     if (kind == 0) {
       const int k = a.interleaved ? m.first / 2 : m.first;
-      if (m.on & (m.first < straight)) turn_pairs<V>(x, turn + (m.row - row0) * pairs + k, a.interleaved, y);
+      if (m.on & (m.first < straight)) turn_pairs<V>(y, turn + (m.row - row0) * pairs + k, a.interleaved);
       __builtin_amdgcn_wave_barrier();  // before the next round's angles
     }
   };

@@ -329,3 +329,37 @@ def test_long_pages_and_shared_heads(dtype):
     assert ((values - want).abs() <= 2.0 ** -4 * want.abs() + 2.0 ** -10 * max(float(want.abs().max()), 0.2) / 224).all()
 
 
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("sections", [None, (24, 20, 20)])
+def test_long_prompts_store_what_their_chunks_do(sections, quantized, dtype):
+    """A prompt of 2500 tokens at once, its queries rotated in place, against chunks of 160 (whole pages): the same bits."""
+    heads, kv, dim, n, page = 16, 2, 256, 2500, 32
+    fused = torch.randn(n, heads + 2 * kv, dim, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+    spin = Rotary.build(128, 1e4, sections=sections)
+    places = torch.randint(0, 5000, (n,) if sections is None else (3, n), generator=torch.Generator().manual_seed(4)).cuda()
+    got = []
+    for step in (n, 160):
+        case = (make if quantized else query_cases.make)([n], [n], heads=heads, kv_heads=kv, dim=dim, dtype=dtype, page=page, seed=5)
+        rows = case.batch.rows
+        x = fused.clone()
+        for t in range(0, n, step):
+            part = x[t:t + step]
+            m = len(part)
+            batch = QueryBatch(rows, torch.tensor([0, m], dtype=torch.int32).cuda(),
+                               torch.tensor([t + m], dtype=torch.int32).cuda(), request_stride=n, max_length=n)
+            flag = torch.zeros(1, dtype=torch.int32).cuda()
+            install_tokens(batch, 0, part[:, :heads], part[:, heads:heads + kv], part[:, heads + kv:], spin,
+                           positions=places[..., t:t + m].contiguous(), out=part[:, :heads], error_flag=flag)
+            assert int(flag) == 0
+        assert torch.equal(x[:, heads:], fused[:, heads:])
+        got.append([x, *(rows.keep[:2] if not quantized else [codes_of(y) for y in (*case.pool, *case.scales)])])
+    for a, b in zip(*got):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    # A turn keeps the lengths: an element is off by half a step, its square by twice that share, all else by far less.
+    before, after = (x[:, :heads].double().cpu() for x in (fused, got[0][0]))
+    assert not torch.equal(before, after)
+    size = before.square().sum(-1)
+    assert ((after.square().sum(-1) - size).abs() <= 1.01 * torch.finfo(dtype).eps * size).all()
