@@ -1175,10 +1175,10 @@ CB_INLINE void mark_not_finite(uint32_t lv, int np, int below, int above, int st
 
 // Sums of NW waves that lie in LDS, each wave's of its own keys (ROWS rows of DP + 4
 // floats, `stride` bytes a wave, with their maxima and totals in stats), become the
-// rows of the result or of a part.
+// rows of the result or of a part. up: the power of two that sums lack.
 template <int DP, int NW, int ROWS, typename H>
 CB_INLINE void join_sums(const AttendArgs& a, const Request& r, int head, int row0, int rows, int split, int vector, const char* sums,
-                         int stride, const float (&stats)[2][NW][ROWS]) {
+                         int stride, const float (&stats)[2][NW][ROWS], int up = 0) {
   constexpr int LD = DP + 4;
   const ScoreArgs& s = a.s;
   const int D = s.head_dim, live = min(ROWS, rows - row0), pairs = D / 2;
@@ -1200,15 +1200,17 @@ CB_INLINE void join_sums(const AttendArgs& a, const Request& r, int head, int ro
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const float lse2 = l == 0.0f ? kNegInf : m + log2_fast(l);
+    o0 = __builtin_amdgcn_ldexpf(o0 * inv, up);
+    o1 = __builtin_amdgcn_ldexpf(o1 * inv, up);
     const int row = row0 + y, i = row / s.group, qh = head * s.group + row - i * s.group;
     const int64_t at = static_cast<int64_t>(r.q0 + i) * s.q_heads + qh;
     if (a.splits > 1) {
       const int64_t slot = static_cast<int64_t>(split) * s.batch.tokens * s.q_heads + at;
-      *reinterpret_cast<float2*>(a.part_out + slot * D + d) = make_float2(o0 * inv, o1 * inv);
+      *reinterpret_cast<float2*>(a.part_out + slot * D + d) = make_float2(o0, o1);
       if (d == 0) a.part_lse[slot] = lse2;
     } else {
       char* op = a.out.data + static_cast<int64_t>(r.q0 + i) * a.out.token_b + qh * a.out.head_b + d * 2;
-      const uint32_t packed = H::pack(o0 * inv, o1 * inv);
+      const uint32_t packed = H::pack(o0, o1);
       if (vector) {
         gstore<uint32_t>(as_global(static_cast<void*>(op)), packed);
       } else {

@@ -1309,6 +1309,12 @@ CB_INLINE void wait_last(int left, bool value) {
 // workgroups in place of 1024 are slower, for 256 the same within noise.
 constexpr int kCodeTiles = 32;  // tiles a split holds at most
 constexpr int kCodeWaves = 4;
+// Weights times scales, and their low terms, have to stay normal in bf16, and their
+// sums finite: weights reach 2^15 (H::kLag), codes 2^9, a split 2^10 keys. Scales
+// of V beyond 2^+-80 are taken relative to the split's largest, which becomes 2^80,
+// and the result is set right at its end: powers of two change no digit of what is
+// within 2^190 of the largest. Looking for such scales takes 0.2 us of a step's 19.5.
+constexpr int kFarScale = 80;
 
 template <typename IO, int DP, int NB, bool MOD>
 __global__ __launch_bounds__(kCodeWaves * kWave, DP == 256 ? 1 : 2) void step_codes_kernel(AttendArgs a, ScaledCache cache, int vector) {
@@ -1319,6 +1325,7 @@ __global__ __launch_bounds__(kCodeWaves * kWave, DP == 256 ? 1 : 2) void step_co
   __shared__ __align__(16) float key_scales[2][kCodeTiles * KT];
   __shared__ uint32_t marks[NW][16 * NB * (DP / 32)];
   __shared__ float stats[2][NW][16 * NB];
+  __shared__ int far_scale, top_scale;  // some scale of V is beyond 2^+-kFarScale; then the largest, a float's bits
   const ScoreArgs& s = a.s;
   const QBatch& B = s.batch;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -1342,6 +1349,7 @@ __global__ __launch_bounds__(kCodeWaves * kWave, DP == 256 ? 1 : 2) void step_co
     }
     key_rows[k] = static_cast<int>(row);
   }
+  if (threadIdx.x == 0) far_scale = top_scale = 0;
   for (int w = threadIdx.x; w < NW * NB * DP / 2; w += NW * kWave) (&marks[0][0])[w] = 0;
   typedef CodeBlock<IO, DP, NB, MOD> Block;
   Block blk;
@@ -1385,12 +1393,25 @@ __global__ __launch_bounds__(kCodeWaves * kWave, DP == 256 ? 1 : 2) void step_co
   // The scales of keys, one without a row has no matter which.
   const HeadScales hs(cache.scales, s.layer, head);
   for (int k = threadIdx.x; k < (t1 - t0) * KT; k += NW * kWave) {
-    const uint32_t at = hs.at(max(key_rows[k], 0));
+    const int row = key_rows[k];
+    const uint32_t at = hs.at(max(row, 0)), value = hs.v[at];
     key_scales[0][k] = scale_value(hs.k[at], kMostRead<IO>);
-    key_scales[1][k] = scale_value(hs.v[at]);
+    key_scales[1][k] = scale_value(value);
+    if ((row >= 0) & (value - (127 - kFarScale) > 2u * kFarScale)) far_scale = 1;
   }
   __builtin_amdgcn_s_waitcnt(0xc07f);
   asm volatile("s_barrier" ::: "memory");
+  auto scaled_down = [&]() { return uniform(far_scale) ? (uniform(top_scale) >> 23) - 127 - kFarScale : 0; };
+  if (uniform(far_scale)) {
+    auto each = [&](auto f) __attribute__((always_inline)) {
+      for (int k = threadIdx.x; k < (t1 - t0) * KT; k += NW * kWave)
+        if (key_rows[k] >= 0) f(key_scales[1][k]);
+      __syncthreads();
+    };
+    each([&](float x) { atomicMax(&top_scale, __float_as_int(x)); });
+    const int down = scaled_down();
+    each([&](float& x) { x = __builtin_amdgcn_ldexpf(x, -down); });
+  }
   uint32_t buf = 0;
   for (int i = 0; i < n; ++i) {
     const int t = t0 + wave + i * NW, start = tile_start<KT>(kr, t), end = tile_end(kr, t), at = (t - t0) * KT;
@@ -1437,7 +1458,7 @@ __global__ __launch_bounds__(kCodeWaves * kWave, DP == 256 ? 1 : 2) void step_co
   if (some_mark) blk.add_marks(marks[wave]);
   blk.put_sums(reinterpret_cast<float*>(tiles + wave * kWaveBytes), stats, wave);
   __syncthreads();
-  join_sums<DP, NW, 16 * NB, Half<IO>>(late_args(), r, head, row0, rows, split, vector, tiles, kWaveBytes, stats);
+  join_sums<DP, NW, 16 * NB, Half<IO>>(late_args(), r, head, row0, rows, split, vector, tiles, kWaveBytes, stats, scaled_down());
 }
 
 // ---------------------------------------------------------------------------

@@ -463,6 +463,9 @@ int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, i
  * zero). Codes are rounded to nearest even; infinities and NaN become NaN.
  * A scale is at most 2^119, with dtype CB_DTYPE_F16 2^7, which keeps values
  * within the type (larger elements are stored as 448 times the scale).
+ * Attention sums weights (up to 2^10 with bf16 tokens) times values in fp32, as
+ * over a 16-bit cache: values that a token sees should stay below 2^90. What it
+ * does not see changes nothing, whatever its scale.
  * No counterpart in the reference, whose caches are 16 bits wide.
  */
 typedef struct cb_page_scales {
