@@ -209,7 +209,13 @@ _TwoHeads = ctypes.c_int64 * 8
 _FourHeads = ctypes.c_int64 * 16
 
 
-class Rotary(NamedTuple):
+class _Rotation(NamedTuple):
+    inv_freq: torch.Tensor
+    magnitude: float = 1.0
+    interleaved: bool = False
+
+
+class Rotary(_Rotation):
     """Rotation of new tokens: radians per position of each pair (float64, on
     the batch's device), the magnitude of scaled contexts, and whether pairs
     are neighbours instead of halves of the rotated part. The rotated part is
@@ -217,12 +223,36 @@ class Rotary(NamedTuple):
 
     ``axes`` (bytes, one per pair) makes positions of several axes, such as time,
     height and width of image patches: pair ``i`` turns by the position along
-    axis ``axes[i]``."""
+    axis ``axes[i]``. It is an attribute beside the tuple's three fields, which
+    unpack as those of a rotation of one axis.
+    """
 
-    inv_freq: torch.Tensor
-    magnitude: float = 1.0
-    interleaved: bool = False
     axes: bytes | None = None
+
+    def __new__(cls, inv_freq: torch.Tensor, magnitude: float = 1.0, interleaved: bool = False,
+                axes: bytes | None = None) -> "Rotary":
+        self = super().__new__(cls, inv_freq, magnitude, interleaved)
+        self.axes = axes
+        return self
+
+    def __getnewargs__(self):
+        return (*self, self.axes)
+
+    def _replace(self, **fields) -> "Rotary":
+        axes = fields.pop("axes", self.axes)
+        return type(self)(*super()._replace(**fields), axes)
+
+    def __eq__(self, other):
+        return self.axes == getattr(other, "axes", None) and super().__eq__(other)
+
+    def __ne__(self, other):
+        return not self == other
+
+    def __hash__(self):
+        return hash((*self, self.axes))
+
+    def __repr__(self):
+        return f"Rotary({', '.join(f'{k}={v!r}' for k, v in self._asdict().items())}, axes={self.axes!r})"
 
     @staticmethod
     def axis_of_pairs(sections, *, cyclic: bool = False) -> bytes:
