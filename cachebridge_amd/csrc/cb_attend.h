@@ -865,14 +865,12 @@ __device__ inline u32x4 finite_part(u32x4 x) {
 
 // The operands of one row of `dim` elements: chunks 2 k + h of 16 bytes, zeros
 // past dim. Loads are at clamped places and selected after: as branches each
-// would wait for the one before. WIDE: a lane's chunks 2 k and 2 k + 1 are
-// neighbours, as 16 codes of an 8-bit row are (dim a multiple of 16).
-template <int KS, bool WIDE = false>
+// would wait for the one before.
+template <int KS>
 CB_INLINE void load_operands(const char* row, int dim, int h, bool vector, u32x4 (&x)[KS]) {
 #pragma unroll
   for (int k = 0; k < KS; ++k) {
-    const int first = WIDE ? 32 * (k >> 1) + 16 * h + 8 * (k & 1) : 16 * k + 8 * h;
-    const char* at = row + 2 * min(first, dim - 8);
+    const char* at = row + 2 * min(16 * k + 8 * h, dim - 8);
     if (vector) {
       x[k] = gload<u32x4>(as_global(static_cast<const void*>(at)));
     } else {
@@ -882,7 +880,7 @@ CB_INLINE void load_operands(const char* row, int dim, int h, bool vector, u32x4
     }
   }
 #pragma unroll
-  for (int k = 0; k < KS; ++k) x[k] = (WIDE ? 32 * (k >> 1) + 16 * h : 16 * k + 8 * h) < dim ? x[k] : u32x4{0, 0, 0, 0};
+  for (int k = 0; k < KS; ++k) x[k] = 16 * k + 8 * h < dim ? x[k] : u32x4{0, 0, 0, 0};
 }
 
 // 32 query rows of one wave: their operands, statistics and sums.
@@ -897,7 +895,6 @@ struct RowBlock {
   int row, i, qh, p;  // this lane's query row
   bool live;
 
-  template <bool WIDE = false>
   __device__ inline void init(const ScoreArgs& s, const Request& r, int head, int row0, bool vector) {
     const int lane = threadIdx.x & (kWave - 1), h = lane >> 5;
     const int rows = r.n * s.group;
@@ -908,7 +905,7 @@ struct RowBlock {
     qh = head * s.group + at - i * s.group;
     p = r.length - r.n + i;
     const char* qp = s.q.data + static_cast<int64_t>(r.q0 + i) * s.q.token_b + qh * s.q.head_b;
-    load_operands<KS, WIDE>(qp, s.head_dim, h, vector, q);
+    load_operands<KS>(qp, s.head_dim, h, vector, q);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
