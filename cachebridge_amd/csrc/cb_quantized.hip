@@ -406,7 +406,7 @@ CB_INLINE void store_page(const InstallQuantizedArgs& q, const AXES& axes, const
 // tokens leaves more of them than there are tokens, a team goes by a token and
 // works if it is its page's first new one.
 // A chunk's pages are whole: one wave a page of 64 took 93 us for 2048 tokens, a
-// workgroup of four 13.7 and of eight 10.2 (12.6 MB, 4.2 us at the rate of a copy: the
+// workgroup of four 13.7 and of eight 10.2 to 11.3 (20 MB, 4.2 us at the rate of a copy: the
 // rest is one chain of row, largest, barrier, code). A step's pages have one new row,
 // which one wave has in one round: 64 requests, heads (64, 8) 6.4 us, launch and the
 // same chain without the barrier.
@@ -1299,21 +1299,26 @@ CB_INLINE void wait_last(int left, bool value) {
 
 // Few query rows: attend_step_kernel's scheme on tiles of codes. Each wave
 // streams tiles of 32 keys through LDS of its own, S of them in flight.
-// Reading K and V bounds it: 64 requests of 8192 with one KV head's 268 MB take 56
-// to 63 us (4.3 to 4.8 TB/s, the rate of a copy). Shorter steps add 8 to 10 us for the
+// Reading K and V bounds it: 64 requests of 8192 with 268 MB take 56 to 66 us by
+// card (4.1 to 4.8 TB/s, the rate of a copy). Shorter steps add 8 to 10 us for the
 // chain of lookups before the first product and the sums after the last: 64
-// ragged requests of 2550 29.5 us (17.7 at that rate), one of 32768 with 8 KV heads
-// 19.5 (14.1).
+// ragged requests of 2550 28.9 us (17.7 at that rate), one of 32768 with 8 KV heads
+// 19.3 (14.1).
+// Two blocks of rows (17 to 32) of 128 elements hold 85,000 bytes of LDS, so one
+// workgroup has the CU, one wave a SIMD and half as many bytes in flight: calls of 64
+// requests of 2048 with heads (16, 2) take 29.5, 34.3, 65.7 and 72.9 us for one to four
+// new tokens (8 to 32 rows), where a 16-bit pool takes 43.5, 48.8, 54.9 and 59.4.
 // kCodeWaves 4, S 2: two waves take 33.7, 22.9 and 74.8 us for these three cases'
-// 29.3, 19.4 and 62; blocks of 32 rows 42, 26.7 and 81. Splits cut for 512 or 2048
-// workgroups in place of 1024 are slower, for 256 the same within noise.
+// 29.3, 19.4 and 62; blocks of 32 rows, with the LDS that they take, 42, 26.7 and 81.
+// Splits cut for 512 or 2048 workgroups in place of 1024 are slower, for 256 the same
+// within noise.
 constexpr int kCodeTiles = 32;  // tiles a split holds at most
 constexpr int kCodeWaves = 4;
 // Weights times scales, and their low terms, have to stay normal in bf16, and their
 // sums finite: weights reach 2^15 (H::kLag), codes 2^9, a split 2^10 keys. Scales
 // of V beyond 2^+-80 are taken relative to the split's largest, which becomes 2^80,
 // and the result is set right at its end: powers of two change no digit of what is
-// within 2^190 of the largest. Looking for such scales takes 0.2 us of a step's 19.5.
+// within 2^190 of the largest. Looking for such scales takes 0.2 us of a step's 19.3.
 constexpr int kFarScale = 80;
 
 template <typename IO, int DP, int NB, bool MOD>
@@ -1500,9 +1505,12 @@ bool takes_codes(const ScoreArgs& s, int32_t dtype, const cb_scores& scores) {
 }
 
 // Key tiles of 64 that a split has at least: 37 tokens over 4133 take 25.5, 19.8 and 17.6
-// us with 8, 4 and 2 (the join 5.8, 5.8 and 6.1).
+// us with 8, 4 and 2 (the join 5.8, 5.8 and 6.1); with 1 the call takes 30.8 for 23.2.
 constexpr int kCodeLeast = 2;
 
+// attend_shape's waves are the 16-bit tile kernel's. Here a workgroup always has
+// kTileWaves; they say which rows a wave has (8: 32, 4: 16), and launches of 16 rows a
+// wave are cut for 512 workgroups, two a CU, where one has the CU.
 AttendShape quantized_shape(const ScoreArgs& s, int32_t dtype, const cb_scores& scores) {
   AttendShape h = attend_shape(s, takes_codes(s, dtype, scores), kCodeLeast, kCodeTiles);
   // One block of rows a request: how many blocks there are does not change with its size.

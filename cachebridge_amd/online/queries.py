@@ -408,12 +408,15 @@ def paged_attention(batch: QueryBatch, layer: int, q: torch.Tensor, *, scale: fl
     exponentials. A token that sees nothing gets zeros and ``-inf``; rows of no
     request are not written. What a token does not see never reaches its row,
     NaN and infinities in the cache included. Scores, statistics and sums are
-    fp32; the weights of a 16-bit pool are rounded to its type for their product
-    with V, which adds about as much error as the result's own rounding, unless
-    ``fp32_weights``, which takes fp32 products (8 to 13 times as long for
-    prompts, 2 to 4 times for steps and short questions). Over an 8-bit pool the
-    cached values are codes times scales, and ``q`` and the result are of the
-    scales' ``dtype``.
+    fp32; with 16-bit tokens the weights are rounded to their type for their
+    product with V, which adds about as much error as the result's own rounding,
+    unless ``fp32_weights``, which takes fp32 products (6 to 14 times as long for
+    prompts, 2 to 10 times for steps and short questions). Over an 8-bit pool the
+    cached values are codes times scales, ``q`` and the result are of the scales'
+    ``dtype``, calls of up to 32 query rows a KV head keep 16 bits of a weight in
+    any case, and ``fp32_weights`` takes 7 to 16 times as long for prompts, 2 to 18
+    times for steps and short questions. fp32 tokens, and head sizes that are no
+    multiple of 16 (on 16-bit pools: of 8) or above 256, go to that kernel too.
     """
     n, heads, dim = q.shape if q.ndim == 3 else (0, 0, 0)
     rq = batch._row(q, "q")

@@ -357,7 +357,8 @@ typedef struct cb_scores {
   const float* slopes;           /* device, one per query head, or NULL */
   const int32_t* prefix_lengths; /* device, one per request, or NULL */
   int32_t fp32_weights; /* cb_paged_attention: softmax weights keep fp32 for their product with V;
-                           0: they are rounded to the type of a 16-bit cache */
+                           0: with 16-bit tokens they are rounded to their type (steps over an
+                           8-bit cache keep 16 bits) */
   int32_t reserved;
 } cb_scores;
 
@@ -465,7 +466,7 @@ int cb_evict_tokens(const cb_query_batch* batch, const cb_query_batch* target, i
  * within the type (larger elements are stored as 448 times the scale).
  * Attention sums weights (up to 2^10 with bf16 tokens) times values in fp32, as
  * over a 16-bit cache: values that a token sees should stay below 2^90. What it
- * does not see changes nothing, whatever its scale.
+ * does not see is not counted, whatever its scale.
  * No counterpart in the reference, whose caches are 16 bits wide.
  */
 typedef struct cb_page_scales {
